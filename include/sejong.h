@@ -340,6 +340,97 @@ int sj_copy_rows(const void* src, size_t ld_src_bytes, void* dst, size_t ld_dst_
 int sj_rows_sum_f32(const void* x, int ldx, int rows, int d, float* acc, int reset, void* stream);
 int sj_scale_to_bf16(const float* x, int n, float alpha, void* y, void* stream);
 
+/* ------------------------------------------------------------------ batched decoding on a paged KV cache
+ * No counterpart in the reference, whose cache serves one sequence (architecture.rs:395-533).  A cache of
+ * one layer is `pages` pages of `page` slots in a K and a V buffer (bf16): slot s is row s % page of page
+ * s / page, and element (page p, KV head h, row r, dim d) lies at p*page_stride + h*head_stride +
+ * r*token_stride + d elements, so the storage order is the caller's.  Strides are multiples of 8, buffers
+ * 16-byte aligned and up to 64 GiB each, head_dim 64 or 128, pages*page < 2^31.  Request b's tokens fill the
+ * pages block_table[b][0], block_table[b][1], ... (int32 [requests, ld_table]) in order.  One block table
+ * serves every layer.
+ *
+ *   sj_paged_plan    the maps of a step that adds added[b] >= 0 tokens to the cached[b] of each request (int32
+ *                    [batch], batch <= 4096).  New pages come from the top of a stack: the i-th, requests in
+ *                    order, is free_pages[*free_count - 1 - i], entered into block_table.  lengths[b] =
+ *                    cached[b] + added[b]; row r (requests in order, tokens in order) of the step has
+ *                    request[r], position[r] and slot[r]; rows past the step's last, up to `rows` (<= 2^19),
+ *                    get -1 in all three, so a captured graph of fixed size can run a step of any size.
+ *                    summary (int32 [4]) = {rows, pages taken, status, pages left}.  status 0: planned; 1:
+ *                    more than `rows` rows; 2: too few free pages; 3: ld_table too small; 4: a negative or
+ *                    overflowing count.  With a status other than 0 nothing is planned: lengths = cached,
+ *                    every row -1, block_table untouched.  cached, added and the stack are only read, so a
+ *                    repeated call writes the same.
+ *   sj_paged_commit  ends the step: *free_count -= pages taken, cached = lengths; requests with release[b] !=
+ *                    0 (release may be null) give their pages back to the stack and get length 0.  `pages` is
+ *                    the stack's capacity; a stack that would leave [0, pages] stays as it is and records
+ *                    SJ_DEV_BAD_INDEX.  summary's first two entries are zeroed, so a second call does nothing.
+ *   sj_paged_append  qkv bf16 [rows, ld] with the heads [hq q | hk k | hk v]: the first rope_dim (a multiple of
+ *                    16, or 0) dims of q and k are rotated by position[r]'s row of rope_table (rope_len rows of
+ *                    rope_dim / 2 (cos, sin) pairs: sj_rope_table or sj_rope_table_scaled), pairs (2i, 2i+1),
+ *                    or (i, i + rope_dim/2) when half != 0, in f32 and rounded once; q to q [rows, ldq], k and v
+ *                    to slot[r].  A row with slot -1 gets a zero q and writes no cache; so does one whose slot
+ *                    or position is out of range, which records SJ_DEV_BAD_INDEX.  q may be the q part of qkv
+ *                    itself (same pointer and stride).
+ *   sj_attn_paged    o[r] = softmax(q[r] K^T / sqrt(head_dim)) V per head over the first position[r] + 1 tokens of
+ *                    request[r] (request null: request r), or the last `window` of them (window > 0); hq / hk
+ *                    query heads share a KV head.  A row with request or position -1 sees nothing: o = 0 and
+ *                    lse = -inf.  lse (f32 [rows, hq], optional) is the natural log of the softmax sum.  A
+ *                    request, position or page id out of range records SJ_DEV_BAD_INDEX; the row sees nothing,
+ *                    or not that page.  Slots past the length are never read.  workspace:
+ *                    sj_attn_paged_workspace bytes, zero before its first use (each call leaves it ready for
+ *                    the next); one per stream. */
+int sj_paged_plan(const int32_t* cached, const int32_t* added, int batch, int page, const int32_t* free_pages,
+                  const int32_t* free_count, int32_t* block_table, int ld_table, int32_t* lengths, int32_t* request,
+                  int32_t* position, int32_t* slot, int rows, int32_t* summary, void* stream);
+int sj_paged_commit(int32_t* cached, int32_t* lengths, const int32_t* release, int batch, int page,
+                    const int32_t* block_table, int ld_table, int32_t* free_pages, int32_t* free_count, int pages,
+                    int32_t* summary, void* stream);
+/* table[p*rope_dim/2 + i] = amplitude * (cos, sin) of (p + offset) * f_i for p < t, evaluated in f64 and
+ * rounded once, with f_i = theta^(-2i/rope_dim) and
+ *   SJ_ROPE_PLAIN   amplitude 1
+ *   SJ_ROPE_LINEAR  f_i / factor (position interpolation)
+ *   SJ_ROPE_BASE    theta * factor^(rope_dim / (rope_dim - 2)) for theta (the lowest frequency is divided by factor)
+ *   SJ_ROPE_RAMP    by turns T_i = original * f_i / 2 pi over the original context: w f_i + (1 - w) f_i / factor,
+ *                   w = clamp((T_i - slow) / (fast - slow), 0, 1), amplitude 0.1 ln(factor) + 1 (the "NTK-by-parts"
+ *                   rule of the YaRN paper, arXiv 2309.00071)
+ * factor >= 1.  original, fast and slow matter to SJ_ROPE_RAMP only. */
+enum { SJ_ROPE_PLAIN = 0, SJ_ROPE_LINEAR = 1, SJ_ROPE_BASE = 2, SJ_ROPE_RAMP = 3 };
+int sj_rope_table_scaled(float* table, int t, int rope_dim, int offset, float theta, int scaling, float factor,
+                         int original, float fast, float slow, void* stream);
+int sj_paged_append(const void* qkv, int ld, const int32_t* position, const int32_t* slot, int rows, int hq, int hk,
+                    int head_dim, const float* rope_table, int rope_len, int rope_dim, int half, void* q, int ldq,
+                    void* k_cache, void* v_cache, int pages, int page, int64_t page_stride, int64_t head_stride,
+                    int64_t token_stride, void* stream);
+size_t sj_attn_paged_workspace(int rows, int hq, int hk, int head_dim);
+int sj_attn_paged(const void* q, int ldq, const void* k_cache, const void* v_cache, int pages, int page,
+                  int64_t page_stride, int64_t head_stride, int64_t token_stride, const int32_t* block_table,
+                  int ld_table, int requests, const int32_t* request, const int32_t* position, int rows, int hq, int hk,
+                  int head_dim, int window, void* o, int ldo, float* lse, void* workspace, size_t workspace_bytes,
+                  void* stream);
+
+/* ------------------------------------------------------------------ token scores
+ * No counterpart in the reference, which trains by cross entropy only (kernels.py:176-191).
+ *   sj_token_scores      per row of logits (f32 or bf16 by dtype, [rows, ld], the first vocab columns):
+ *                        logp[r] = log softmax(logits[r])[target[r]], entropy[r] = -sum p log p (0 log 0 = 0), lse[r],
+ *                        and the `top` <= min(32, vocab) largest logits in order (the lowest index first among
+ *                        equal ones, NaN last): top_id int32 and top_logp f32 [rows, top].  Each of logp, entropy
+ *                        and lse may be null.  target -1: logp 0.  A target outside [-1, vocab) counts as -1 and
+ *                        records SJ_DEV_BAD_INDEX.  Logits of -inf are forbidden tokens (log probability -inf);
+ *                        a row of nothing else has lse -inf, entropy 0.  workspace:
+ *                        sj_token_scores_workspace bytes, zero before its first use (each call leaves it ready for
+ *                        the next); one per stream.
+ *   sj_token_scores_bwd  d_logits [rows, ldd] (the logits' type; columns vocab..ldd zeroed) = d_logp (1[target] - p)
+ *                        - d_entropy p (log p + entropy) with p = e^(logits - lse); d_logp or d_entropy may be null
+ *                        (zero), entropy when d_entropy is.  A target of -1 takes no d_logp.  d_logits may be the
+ *                        logits themselves when ldd == ld.  The alternatives are not differentiated. */
+size_t sj_token_scores_workspace(int rows, int vocab, int top);
+int sj_token_scores(const void* logits, int dtype, int ld, const int32_t* target, int rows, int vocab, int top,
+                    float* logp, float* entropy, float* lse, int32_t* top_id, float* top_logp, void* workspace,
+                    size_t workspace_bytes, void* stream);
+int sj_token_scores_bwd(const void* logits, int dtype, int ld, const int32_t* target, int rows, int vocab,
+                        const float* lse, const float* entropy, const float* d_logp, const float* d_entropy,
+                        void* d_logits, int ldd, void* stream);
+
 /* ------------------------------------------------------------------ NativeValue head */
 /* The categorical value head of NativeValue::forward_batch (crates/sejong-model/src/native/value.rs:
  * 111-160) with its loss (Engine::cross_entropy, lib.rs:524-543) and backward.  hidden bf16 [rows,

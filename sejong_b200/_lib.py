@@ -10,6 +10,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsejong_b200.so")
 
 c_int, c_float, c_double, c_size_t, c_void_p = ctypes.c_int, ctypes.c_float, ctypes.c_double, ctypes.c_size_t, ctypes.c_void_p
+c_i64 = ctypes.c_int64
 c_u64, c_u64p = ctypes.c_uint64, ctypes.POINTER(ctypes.c_uint64)
 
 # name -> (restype, argtypes)
@@ -61,6 +62,24 @@ SIGNATURES = {
     "sj_attn_cached": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int,
                                c_int, c_int, c_int, c_void_p]),
     "sj_copy_rows": (c_int, [c_void_p, c_size_t, c_void_p, c_size_t, c_int, c_size_t, c_void_p]),
+    "sj_paged_plan": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+                              c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    "sj_paged_commit": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p,
+                                c_int, c_void_p, c_void_p]),
+    "sj_rope_table_scaled": (c_int, [c_void_p, c_int, c_int, c_int, c_float, c_int, c_float, c_int, c_float,
+                                     c_float, c_void_p]),
+    "sj_paged_append": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int,
+                                c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_i64, c_i64,
+                                c_i64, c_void_p]),
+    "sj_attn_paged_workspace": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "sj_attn_paged": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_i64, c_i64, c_i64, c_void_p,
+                              c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int,
+                              c_void_p, c_void_p, c_size_t, c_void_p]),
+    "sj_token_scores_workspace": (c_size_t, [c_int, c_int, c_int]),
+    "sj_token_scores": (c_int, [c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
+                                c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "sj_token_scores_bwd": (c_int, [c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p,
+                                    c_void_p, c_void_p, c_int, c_void_p]),
     "sj_rows_sum_f32": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p]),
     "sj_scale_to_bf16": (c_int, [c_void_p, c_int, c_float, c_void_p, c_void_p]),
     "sj_value_head_fwd": (c_int, [c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p,
@@ -154,6 +173,7 @@ SIGNATURES = {
 # status codes (include/sejong.h)
 SJ_OK, SJ_ERR_SHAPE, SJ_ERR_CAPACITY, SJ_ERR_CUDA, SJ_ERR_NCCL, SJ_ERR_TIMEOUT, SJ_ERR_ARGUMENT, SJ_ERR_UNSUPPORTED = range(8)
 SJ_F32, SJ_F64, SJ_F16, SJ_I32, SJ_BF16 = range(5)
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_RAMP = range(4)
 EPI_STORE, EPI_ACCUM, EPI_RESIDUAL, EPI_SWIGLU, EPI_ROPE, EPI_BIAS, EPI_BIAS_GELU, EPI_BIAS_RESIDUAL = range(8)
 
 

@@ -54,6 +54,10 @@ inline int ensure_max_smem(KernelAttrOnce& once, const void* kernel, int bytes, 
 // Zero `bytes` bytes at `ptr` on `stream` with a kernel (elementwise.cu).
 int zero_async(void* ptr, size_t bytes, cudaStream_t stream);
 
+// What sj_paged_append and sj_attn_paged (`who`) ask of a paged K/V cache (paged.cu).
+int check_paged_cache(const char* who, const void* k, const void* v, int pages, int page, int64_t page_stride,
+                      int64_t head_stride, int64_t token_stride, int hk, int head_dim);
+
 // Whether kernels are launched with programmatic stream serialization (default on; SJ_PDL=0 in the
 // environment turns it off, read once per process).
 bool pdl_enabled();

@@ -1,12 +1,10 @@
 // Batched decoding on a paged key-value cache: the step's block tables and slot maps, the rotated
-// queries and the keys and values written to their slots, and each row's attention over its
-// request's pages.
+// queries, and the keys and values written to their slots (attention_paged.cu reads them).
 //
 //   paged_plan_kernel     lengths -> new block-table entries, row maps, new lengths (idempotent)
 //   paged_commit_kernel   makes a planned step final and takes back the pages of finished requests
 //   rope_scaled_kernel    (cos, sin) tables of scaled rotary positions, angles in f64
 //   paged_append_kernel   rotary positions of q and k, k and v into their cache slots
-//   attn_paged_kernel     one row's attention over its request's pages
 //
 // A cache of one layer is `pages` pages of `page` slots; slot s is row s % page of page s / page.
 // Element (page p, head h, row r, dim d) lies at p * page_stride + h * head_stride + r *
@@ -276,78 +274,23 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const __nv_bfloat16* 
   *reinterpret_cast<uint4*>(dst + second) = y;
 }
 
-// ---------------------------------------------------------------- attention over the pages
-// One CTA per (row, query head), four warps over the keys, lanes over the dims; each warp keeps the
-// running maximum, sum and output of its keys and the CTA joins them at the end:
-//   m = max m_w,  o = sum_w e^(m_w - m) o_w / sum_w e^(m_w - m) l_w.
-constexpr int kPagedWarps = 4;
-
-template <int DIM>
-__global__ void __launch_bounds__(kPagedWarps * 32)
-    attn_paged_kernel(const __nv_bfloat16* q, int ldq, const __nv_bfloat16* kc, const __nv_bfloat16* vc, int pages,
-                      int page, int64_t page_stride, int64_t head_stride, int64_t token_stride, const int32_t* table,
-                      int ld_table, int requests, const int32_t* request, const int32_t* position, int hq, int hk,
-                      int window, __nv_bfloat16* o, int ldo, float* lse) {
-  pdl_wait();
-  constexpr int PER = DIM / 32;
-  __shared__ float sm[kPagedWarps], sl[kPagedWarps], so[kPagedWarps][DIM];
-  const int r = blockIdx.x, h = blockIdx.y, kvh = h / (hq / hk);
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const int b = request ? request[r] : r;
-  const int pos = position[r];
-  int n = b == -1 || pos == INT_MAX ? 0 : pos + 1;
-  if (b < -1 || b >= requests || pos < -1 || pos == INT_MAX || static_cast<int64_t>(n) > static_cast<int64_t>(ld_table) * page) {
-    record_error(SJ_DEV_BAD_INDEX);
-    n = 0;
-  }
-  const int lo = window > 0 ? max(0, n - window) : 0;
-  const float scale = rsqrtf(static_cast<float>(DIM));
-  float qv[PER], acc[PER], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    qv[i] = n > 0 ? bf2f(q[static_cast<size_t>(r) * ldq + h * DIM + PER * lane + i]) * scale : 0.f;
-    acc[i] = 0.f;
-  }
-  for (int j = lo + warp; j < n; j += kPagedWarps) {
-    const int id = table[static_cast<size_t>(b) * ld_table + j / page];
-    if (id < 0 || id >= pages) {
-      record_error(SJ_DEV_BAD_INDEX);
-      continue;
-    }
-    const int64_t at = id * page_stride + kvh * head_stride + j % page * token_stride + PER * lane;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) s = fmaf(qv[i], bf2f(kc[at + i]), s);
-    s = warp_sum(s);
-    const float top = fmaxf(m, s);
-    const float base = top == -INFINITY ? 0.f : top;  // every score so far -inf: all weights 0, not NaN
-    const float keep = expf(m - base), p = expf(s - base);
-    m = top;
-    l = l * keep + p;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] = acc[i] * keep + p * bf2f(vc[at + i]);
-  }
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
-  }
-#pragma unroll
-  for (int i = 0; i < PER; ++i) so[warp][PER * lane + i] = acc[i];
-  __syncthreads();
-  float top = -INFINITY, total = 0.f, out = 0.f;
-  for (int w = 0; w < kPagedWarps; ++w) top = fmaxf(top, sm[w]);
-  const float base = top == -INFINITY ? 0.f : top;
-  if (t < DIM) {
-    for (int w = 0; w < kPagedWarps; ++w) {
-      const float f = expf(sm[w] - base);
-      total += f * sl[w];
-      out += f * so[w][t];
-    }
-    o[static_cast<size_t>(r) * ldo + h * DIM + t] = f2bf(total == 0.f ? 0.f : out / total);
-    if (t == 0 && lse) lse[static_cast<size_t>(r) * hq + h] = total == 0.f ? -INFINITY : base + logf(total);
-  }
+// ---------------------------------------------------------------- host
+int check_paged_cache(const char* who, const void* k, const void* v, int pages, int page, int64_t page_stride,
+                int64_t head_stride, int64_t token_stride, int hk, int head_dim) {
+  if (head_dim != 64 && head_dim != 128)
+    return fail(SJ_ERR_UNSUPPORTED, "%s: head_dim %d (this build: 64 or 128)", who, head_dim);
+  if (pages <= 0 || page <= 0 || static_cast<int64_t>(pages) * page > INT_MAX)
+    return fail(SJ_ERR_SHAPE, "%s: pages=%d page=%d (below 2^31 slots)", who, pages, page);
+  if (!k || !v || !aligned16(k) || !aligned16(v) || page_stride < 0 || head_stride < 0 || token_stride < 0 ||
+      (page_stride | head_stride | token_stride) % 8)
+    return fail(SJ_ERR_ARGUMENT, "%s: the cache takes 16-byte aligned buffers and strides that are multiples of 8",
+                who);
+  const int64_t limit = int64_t{1} << 35;
+  if (page_stride > limit / pages || head_stride > limit / hk || token_stride > limit / page ||
+      (pages - 1) * page_stride + (hk - 1) * head_stride + (page - 1) * token_stride + head_dim > limit)
+    return fail(SJ_ERR_SHAPE, "%s: a cache buffer of more than 64 GiB", who);
+  return SJ_OK;
 }
-
 }  // namespace sj
 
 using namespace sj;
@@ -403,36 +346,17 @@ extern "C" int sj_rope_table_scaled(float* table, int t, int rope_dim, int offse
   return SJ_OK;
 }
 
-namespace {
-// What sj_paged_append and sj_attn_paged ask of a cache.
-int check_cache(const char* who, const void* k, const void* v, int pages, int page, int64_t page_stride,
-                int64_t head_stride, int64_t token_stride, int hk, int head_dim) {
-  if (head_dim != 64 && head_dim != 128)
-    return fail(SJ_ERR_UNSUPPORTED, "%s: head_dim %d (this build: 64 or 128)", who, head_dim);
-  if (pages <= 0 || page <= 0 || static_cast<int64_t>(pages) * page > INT_MAX)
-    return fail(SJ_ERR_SHAPE, "%s: pages=%d page=%d (below 2^31 slots)", who, pages, page);
-  if (!k || !v || !aligned16(k) || !aligned16(v) || page_stride < 0 || head_stride < 0 || token_stride < 0 ||
-      (page_stride | head_stride | token_stride) % 8)
-    return fail(SJ_ERR_ARGUMENT, "%s: the cache takes 16-byte aligned buffers and strides that are multiples of 8", who);
-  const int64_t limit = int64_t{1} << 35;
-  if (page_stride > limit / pages || head_stride > limit / hk || token_stride > limit / page ||
-      (pages - 1) * page_stride + (hk - 1) * head_stride + (page - 1) * token_stride + head_dim > limit)
-    return fail(SJ_ERR_SHAPE, "%s: a cache buffer of more than 64 GiB", who);
-  return SJ_OK;
-}
-}  // namespace
-
 extern "C" int sj_paged_append(const void* qkv, int ld, const int32_t* position, const int32_t* slot, int rows, int hq,
                                int hk, int head_dim, const float* rope_table, int rope_len, int rope_dim, int half,
                                void* q, int ldq, void* k_cache, void* v_cache, int pages, int page,
                                int64_t page_stride, int64_t head_stride, int64_t token_stride, void* stream) {
   if (rows < 0 || hq < 0 || hk <= 0 || hq > 4096 || hk > 4096)
     return fail(SJ_ERR_SHAPE, "sj_paged_append: rows=%d hq=%d hk=%d", rows, hq, hk);
-  const int rc = check_cache("sj_paged_append", k_cache, v_cache, pages, page, page_stride, head_stride, token_stride,
-                             hk, head_dim);
+  const int rc = check_paged_cache("sj_paged_append", k_cache, v_cache, pages, page, page_stride, head_stride,
+                                   token_stride, hk, head_dim);
   if (rc != SJ_OK) return rc;
-  if (rope_dim < 0 || rope_dim > head_dim || rope_dim % 16 || (rope_dim > 0 && rope_len <= 0) || ld < (hq + 2 * hk) * head_dim ||
-      ldq < hq * head_dim)
+  if (rope_dim < 0 || rope_dim > head_dim || rope_dim % 16 || (rope_dim > 0 && rope_len <= 0) ||
+      ld < (hq + 2 * hk) * head_dim || ldq < hq * head_dim)
     return fail(SJ_ERR_SHAPE, "sj_paged_append: rope_dim=%d (a multiple of 16) rope_len=%d ld=%d ldq=%d", rope_dim,
                 rope_len, ld, ldq);
   if (rows == 0) return SJ_OK;
@@ -446,37 +370,5 @@ extern "C" int sj_paged_append(const void* qkv, int ld, const int32_t* position,
          rope_dim, half, static_cast<__nv_bfloat16*>(q), ldq, static_cast<__nv_bfloat16*>(k_cache),
          static_cast<__nv_bfloat16*>(v_cache), pages, page, page_stride, head_stride, token_stride);
   SJ_LAUNCH_CHECK("paged_append");
-  return SJ_OK;
-}
-
-extern "C" size_t sj_attn_paged_workspace(int rows, int hq, int hk, int head_dim) {
-  if (rows < 0 || hq <= 0 || hk <= 0 || hq % hk || head_dim <= 0) return 0;
-  return 16;
-}
-
-extern "C" int sj_attn_paged(const void* q, int ldq, const void* k_cache, const void* v_cache, int pages, int page,
-                             int64_t page_stride, int64_t head_stride, int64_t token_stride,
-                             const int32_t* block_table, int ld_table, int requests, const int32_t* request,
-                             const int32_t* position, int rows, int hq, int hk, int head_dim, int window, void* o,
-                             int ldo, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
-  if (rows < 0 || requests <= 0 || ld_table <= 0 || hq <= 0 || hk <= 0 || hq % hk || hq > 4096 || window < 0 ||
-      (!request && rows > requests))
-    return fail(SJ_ERR_SHAPE, "sj_attn_paged: rows=%d requests=%d ld_table=%d hq=%d hk=%d window=%d", rows, requests,
-                ld_table, hq, hk, window);
-  const int rc = check_cache("sj_attn_paged", k_cache, v_cache, pages, page, page_stride, head_stride, token_stride, hk,
-                             head_dim);
-  if (rc != SJ_OK) return rc;
-  if (ldq < hq * head_dim || ldo < hq * head_dim)
-    return fail(SJ_ERR_SHAPE, "sj_attn_paged: ldq=%d ldo=%d", ldq, ldo);
-  if (rows == 0) return SJ_OK;
-  if (!q || !o || !block_table || !position || !aligned16(q) || !aligned16(o) || ldq % 8 || ldo % 8)
-    return fail(SJ_ERR_ARGUMENT, "sj_attn_paged: null or unaligned operand, or a row stride not a multiple of 8");
-  if (!workspace || !aligned16(workspace) || workspace_bytes < sj_attn_paged_workspace(rows, hq, hk, head_dim))
-    return fail(SJ_ERR_CAPACITY, "sj_attn_paged: workspace of %zu bytes", workspace_bytes);
-  launch(head_dim == 64 ? attn_paged_kernel<64> : attn_paged_kernel<128>, dim3(rows, hq), kPagedWarps * 32, 0,
-         as_stream(stream), static_cast<const __nv_bfloat16*>(q), ldq, static_cast<const __nv_bfloat16*>(k_cache),
-         static_cast<const __nv_bfloat16*>(v_cache), pages, page, page_stride, head_stride, token_stride, block_table,
-         ld_table, requests, request, position, hq, hk, window, static_cast<__nv_bfloat16*>(o), ldo, lse);
-  SJ_LAUNCH_CHECK("attn_paged");
   return SJ_OK;
 }

@@ -19,6 +19,7 @@ namespace {
 constexpr int kScoreMaxTop = 32;
 constexpr int kScoreNarrow = 1024;    // rows of at most this many logits are held by one warp
 constexpr int kScoreThreads = 256;    // of the kernel for wider rows
+constexpr int kScoreCtas = 3, kScoreStages = 3;  // of an SM, of a CTA's ring of 16 KB chunks
 constexpr int kScoreMaxSplits = 16;
 constexpr int kScoreHeld = kScoreMaxTop * 32 + kScoreMaxTop;  // candidates: the best of 32 threads' 32, and the list
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -31,6 +32,34 @@ SJ_DEVICE float score_load(const __nv_bfloat16* x) { return bf2f(*x); }
 SJ_DEVICE float exp2_flush(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two f32 at a time: sm_100 adds, multiplies and fuses a register pair in one instruction.
+SJ_DEVICE uint64_t pair2(float a, float b) {
+  return static_cast<uint64_t>(__float_as_uint(b)) << 32 | __float_as_uint(a);
+}
+SJ_DEVICE float low2(uint64_t p) { return __uint_as_float(static_cast<uint32_t>(p)); }
+SJ_DEVICE float high2(uint64_t p) { return __uint_as_float(static_cast<uint32_t>(p >> 32)); }
+SJ_DEVICE uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t y;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+  return y;
+}
+SJ_DEVICE uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t y;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+  return y;
+}
+SJ_DEVICE uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t y;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
+  return y;
+}
+// The floor keeps 0 * -inf out of products with 2^x (2^-150 is 0 as well) and lets a NaN pass.
+SJ_DEVICE float floor_exponent(float x) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(-150.f));
   return y;
 }
 
@@ -75,13 +104,13 @@ SJ_DEVICE ScoreSum score_warp_join(ScoreSum a) {
                                __shfl_xor_sync(0xffffffffu, a.u, o)});
   return a;
 }
-// One logit into s and u.  The floor keeps 0 * -inf out of u (2^-150 is 0 as well) and lets a NaN pass.
-SJ_DEVICE void score_add(float x, float base, float& s, float& u) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"((x - base) * kLog2e), "f"(-150.f));
-  const float e = exp2_flush(d);
-  s += e;
-  u = fmaf(e, d, u);
+// Two logits into pairs of partial s and u: d = (x - base) log2(e), s += 2^d, u += 2^d d.
+SJ_DEVICE void score_add2(uint64_t x, uint64_t minus_base, uint64_t& s, uint64_t& u) {
+  uint64_t d = mul2(add2(x, minus_base), pair2(kLog2e, kLog2e));
+  d = pair2(floor_exponent(low2(d)), floor_exponent(high2(d)));
+  const uint64_t e = pair2(exp2_flush(low2(d)), exp2_flush(high2(d)));
+  s = add2(s, e);
+  u = fma2(e, d, u);
 }
 
 // Floats of a part in the workspace: m, s, u, the number of keys, the keys.
@@ -109,32 +138,74 @@ SJ_DEVICE void score_write_row(const ScoreOut& out, const T* x, int r, const Sco
 }
 
 // ---------------------------------------------------------------- narrow rows
-// A warp holds a row in R registers a lane: one read, maximum, sums, then each alternative by two warp
-// reductions (value, then lowest index) and the lane's own next best.
+// A warp holds a row in R registers a lane: one read, maximum, sums.  Alternatives: the `top`-th largest of the
+// lanes' maxima is a bar that at least `top` logits reach; the few that do (31 are expected at top = 20) are
+// listed and ranked by counting.  Where more than 64 do (ties), each alternative is found by two warp
+// reductions instead (value, then lowest index).
 template <typename T, int R>
 __global__ void __launch_bounds__(128) token_scores_narrow_kernel(const T* logits, int ld, int rows, ScoreOut out) {
   pdl_wait();
-  const int lane = threadIdx.x & 31, r = blockIdx.x * 4 + (threadIdx.x >> 5);
+  __shared__ uint64_t listed[4][64];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = blockIdx.x * 4 + warp;
   if (r >= rows) return;
   const T* x = logits + static_cast<size_t>(r) * ld;
-  float v[R];
+  float v[R + (R & 1)];
   ScoreSum a{-INFINITY, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < R; ++i) v[i] = i * 32 + lane < out.vocab ? score_load(x + i * 32 + lane) : -INFINITY;
+  if (R & 1) v[R] = -INFINITY;
 #pragma unroll
   for (int i = 0; i < R; ++i) a.m = fmaxf(a.m, v[i]);
+  const float lane_max = a.m;
   a.m = warp_max(a.m);
   const float base = a.m == -INFINITY ? 0.f : a.m;
+  uint64_t s = 0, u = 0;
 #pragma unroll
-  for (int i = 0; i < R; ++i) score_add(v[i], base, a.s, a.u);
-  a.s = warp_sum(a.s);
-  a.u = warp_sum(a.u);
+  for (int i = 0; i < R; i += 2) score_add2(pair2(v[i], v[i + 1]), pair2(-base, -base), s, u);
+  a.s = warp_sum(low2(s) + high2(s));
+  a.u = warp_sum(low2(u) + high2(u));
   if (lane == 0) score_write_row(out, x, r, a);
   if (out.top == 0) return;
   const float log_s = logf(a.s);
-  uint32_t order[R];
+  auto write = [&](int k, uint64_t key) {
+    out.top_id[static_cast<size_t>(r) * out.top + k] = static_cast<int32_t>(~static_cast<uint32_t>(key));
+    out.top_logp[static_cast<size_t>(r) * out.top + k] =
+        score_logp(score_value(static_cast<uint32_t>(key >> 32)), a, base, log_s);
+  };
+
+  uint32_t bar = score_order(lane_max);
 #pragma unroll
-  for (int i = 0; i < R; ++i) order[i] = score_order(v[i]);
+  for (int size = 2; size <= 32; size *= 2)  // a bitonic sort of the lanes' maxima, the largest first
+#pragma unroll
+    for (int step = size / 2; step > 0; step /= 2) {
+      const uint32_t o = __shfl_xor_sync(0xffffffffu, bar, step);
+      const bool larger = ((lane & step) == 0) == ((lane & size) == 0);
+      bar = larger ? max(bar, o) : min(bar, o);
+    }
+  bar = __shfl_sync(0xffffffffu, bar, out.top - 1);
+  if (bar <= kForbidden) bar = 0;  // fewer than `top` lanes hold more than forbidden tokens
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const bool hit = i * 32 + lane < out.vocab && score_order(v[i]) >= bar;
+    const uint32_t hits = __ballot_sync(0xffffffffu, hit);
+    const int at = n + __popc(hits & ((1u << lane) - 1));
+    if (hit && at < 64) listed[warp][at] = score_key(v[i], i * 32 + lane);
+    n += __popc(hits);
+  }
+  __syncwarp();
+  if (n <= 64) {
+    const uint64_t first = lane < n ? listed[warp][lane] : 0, second = lane + 32 < n ? listed[warp][lane + 32] : 0;
+    int rank = 0, rank2 = 0;
+    for (int k = 0; k < n; ++k) {
+      const uint64_t o = listed[warp][k];
+      rank += o > first ? 1 : 0;
+      rank2 += o > second ? 1 : 0;
+    }
+    if (lane < n && rank < out.top) write(rank, first);
+    if (lane + 32 < n && rank2 < out.top) write(rank2, second);
+    return;
+  }
   uint32_t bound = 0xffffffffu;  // the last alternative's order and index
   int bound_at = -1;
   for (int k = 0; k < out.top; ++k) {
@@ -143,7 +214,7 @@ __global__ void __launch_bounds__(128) token_scores_narrow_kernel(const T* logit
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int at = i * 32 + lane;
-      const uint32_t up = order[i];
+      const uint32_t up = score_order(v[i]);
       const bool left = at < out.vocab && (up < bound || (up == bound && at > bound_at));
       if (left && (up > best || best_at == 0x7fffffff)) {
         best = up;
@@ -153,55 +224,109 @@ __global__ void __launch_bounds__(128) token_scores_narrow_kernel(const T* logit
     bound = __reduce_max_sync(0xffffffffu, best_at == 0x7fffffff ? 0u : best);
     bound_at = static_cast<int>(
         __reduce_min_sync(0xffffffffu, best == bound ? static_cast<unsigned>(best_at) : 0x7fffffffu));
-    if (lane == 0) {
-      out.top_id[static_cast<size_t>(r) * out.top + k] = bound_at;
-      out.top_logp[static_cast<size_t>(r) * out.top + k] = score_logp(score_value(bound), a, base, log_s);
-    }
+    if (lane == 0) write(k, static_cast<uint64_t>(bound) << 32 | static_cast<uint32_t>(~bound_at));
   }
 }
 
 // ---------------------------------------------------------------- wide rows
-// Sixteen 4-byte (32 2-byte) logits of a thread's chunk as they are stored.
+// 64 bytes of a row a thread, in pieces of 16 that lie side by side across the CTA: 16 KB of the row.
 template <typename T>
 struct ScoreChunk {
   static constexpr int PER = 16 / sizeof(T), N = 4 * PER, SIZE = kScoreThreads * N;
   uint4 raw[4];
-  SJ_DEVICE static int index(int base, int i) {  // of element i: sixteen bytes of each thread side by side
+  SJ_DEVICE static int index(int base, int i) {  // column of the thread's element i; base: of the chunk
     return base + (i / PER * kScoreThreads + static_cast<int>(threadIdx.x)) * PER + i % PER;
   }
+  SJ_DEVICE static uint32_t word(const uint4& q, int i) { return i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w; }
   SJ_DEVICE float at(int i) const {
     const uint4& q = raw[i / PER];
-    if (sizeof(T) == 4) return __uint_as_float(i % 4 == 0 ? q.x : i % 4 == 1 ? q.y : i % 4 == 2 ? q.z : q.w);
-    const int w = i % PER / 2;
-    const uint32_t pair = w == 0 ? q.x : w == 1 ? q.y : w == 2 ? q.z : q.w;
-    return __uint_as_float(i % 2 ? pair & 0xffff0000u : pair << 16);
+    if (sizeof(T) == 4) return __uint_as_float(word(q, i % 4));
+    const uint32_t w = word(q, i % PER / 2);
+    return __uint_as_float(i % 2 ? w & 0xffff0000u : w << 16);
   }
-  // Elements outside [0, vocab) are -inf.  base is a 16-byte boundary.
-  SJ_DEVICE void load(const T* x, int base, int vocab) {
+  SJ_DEVICE float largest() const {  // NaN left out, -inf where there is nothing else
+    float m = -INFINITY;
+    if (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) m = fmaxf(m, at(i));
+      return m;
+    }
+    uint32_t p = 0xff80ff80u;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) asm("max.bf16x2 %0, %0, %1;" : "+r"(p) : "r"(word(raw[i / 4], i % 4)));
+    return fmaxf(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u));
+  }
+  // The chunk's pieces that lie in the row, on their way to `stage` (16 KB of shared memory).
+  SJ_DEVICE static void fetch(const T* x, int base, int vocab, uint32_t stage) {
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
-      const int j = base + (v * kScoreThreads + static_cast<int>(threadIdx.x)) * PER;
-      if (j >= 0 && j + PER <= vocab) {
-        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(raw[v].x), "=r"(raw[v].y), "=r"(raw[v].z), "=r"(raw[v].w)
-                     : "l"(x + j)
+      const int j = index(base, v * PER);
+      if (j >= 0 && j + PER <= vocab)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(stage + (v * kScoreThreads + threadIdx.x) * 16),
+                     "l"(x + j)
                      : "memory");
-      } else {
-        uint32_t w[4];
+    }
+  }
+  // The thread's own pieces from `stage`, the row's ends from memory; -inf outside [0, vocab).
+  SJ_DEVICE void read(const T* x, int base, int vocab, uint32_t stage) {
+    constexpr uint32_t NONE = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (sizeof(T) == 4) {
-            w[e] = __float_as_uint(j + e >= 0 && j + e < vocab ? score_load(x + j + e) : -INFINITY);
-          } else {
-            const int a = j + 2 * e;
-            const float lo = a >= 0 && a < vocab ? score_load(x + a) : -INFINITY;
-            const float hi = a + 1 >= 0 && a + 1 < vocab ? score_load(x + a + 1) : -INFINITY;
-            w[e] = __float_as_uint(lo) >> 16 | (__float_as_uint(hi) & 0xffff0000u);
-          }
+    for (int v = 0; v < 4; ++v) {
+      const int j = index(base, v * PER);
+      raw[v] = make_uint4(NONE, NONE, NONE, NONE);
+      if (j >= 0 && j + PER <= vocab) {
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(raw[v].x), "=r"(raw[v].y), "=r"(raw[v].z), "=r"(raw[v].w)
+                     : "r"(stage + (v * kScoreThreads + threadIdx.x) * 16)
+                     : "memory");
+      } else if (j < vocab) {
+        uint32_t w[4] = {NONE, NONE, NONE, NONE};
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+          if (j + e < 0 || j + e >= vocab) continue;
+          const uint32_t bits = __float_as_uint(score_load(x + j + e));
+          if (sizeof(T) == 4)
+            w[e % 4] = bits;
+          else
+            w[e / 2] = e % 2 ? (w[e / 2] & 0xffffu) | (bits & 0xffff0000u) : (w[e / 2] & 0xffff0000u) | bits >> 16;
         }
         raw[v] = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
+  }
+};
+
+// The chunks of the parts that a CTA takes: part blockIdx.x, + gridDim.x, ...; part p is the (p % splits)-th of
+// equal numbers of chunks of row p / splits.  Columns are counted from the 16-byte boundary at or before the row.
+template <typename T>
+struct ScoreWalk {
+  const T *logits, *x;
+  int ld, vocab, splits, parts, part, origin, c, c1;
+  SJ_DEVICE ScoreWalk(const T* all, int ld_, int vocab_, int splits_, int parts_)
+      : logits(all), ld(ld_), vocab(vocab_), splits(splits_), parts(parts_), part(blockIdx.x) {
+    enter();
+  }
+  SJ_DEVICE void enter() {
+    if (part >= parts) return;
+    const int r = part / splits, k = part - r * splits;
+    x = logits + static_cast<size_t>(r) * ld;
+    origin = -static_cast<int>(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
+    const int chunks = (vocab - origin + ScoreChunk<T>::SIZE - 1) / ScoreChunk<T>::SIZE;
+    c = static_cast<int>(static_cast<int64_t>(chunks) * k / splits);
+    c1 = static_cast<int>(static_cast<int64_t>(chunks) * (k + 1) / splits);
+  }
+  SJ_DEVICE void leave() {
+    part += gridDim.x;
+    enter();
+  }
+  SJ_DEVICE int base() const { return origin + c * ScoreChunk<T>::SIZE; }
+  SJ_DEVICE void fetch(uint32_t stage) {  // the next chunk, whichever part it is of
+    while (part < parts && c >= c1) leave();
+    if (part < parts) {
+      ScoreChunk<T>::fetch(x, base(), vocab, stage);
+      ++c;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   }
 };
 
@@ -222,7 +347,8 @@ SJ_DEVICE int score_compact(ScoreBest& b, int top, int before) {
   for (int i = threadIdx.x; i < n; i += kScoreThreads) {
     const uint64_t key = b.held[i];
     int rank = static_cast<int>(~static_cast<uint32_t>(key)) < before ? 0 : top;
-    for (int k = 0; k < n && rank < top; ++k) {
+#pragma unroll 8
+    for (int k = 0; k < n; ++k) {
       const uint64_t other = b.held[k];
       rank += other > key && static_cast<int>(~static_cast<uint32_t>(other)) < before ? 1 : 0;
     }
@@ -244,160 +370,187 @@ SJ_DEVICE int score_compact(ScoreBest& b, int top, int before) {
   return kept;
 }
 
-// One CTA for a part of a row (splits > 1: as many parts of equal numbers of chunks), 16 KB at a time with the
-// next chunk's loads in flight.  The sums are each thread's own until the part's end.  Alternatives: the
-// `top`-th largest of 64 groups' maxima of the first chunk is a bar that at least `top` logits reach; what
-// reaches it (of later chunks, exceeds it) goes to a list in shared memory that is ranked once at the end: about
-// 24 candidates a chunk at top = 20.  A list that fills up is ranked at once, which raises the bar; a chunk with more
-// candidates than the list holds (equal or rising logits) takes those of the `top` threads with the best maxima.
+// Persistent CTAs over the parts of rows, 16 KB at a time; the next two chunks, of the next part too, are on their way
+// to shared memory meanwhile (cp.async; a thread reads back only what it copied, so copies need no barrier).  The
+// sums are each thread's own until the part's end.  Alternatives: the `top`-th largest of 64 groups' maxima of the
+// first chunk is a bar that at least `top` logits reach; what reaches it (of later chunks, exceeds it)
+// goes to a list that is ranked once at the end: about 24 candidates a chunk at top = 20.  A list that fills up
+// is ranked at once, which raises the bar; a chunk with more candidates than the list holds (equal or rising
+// logits) takes those of the `top` threads with the best maxima.
 template <typename T>
-__global__ void __launch_bounds__(kScoreThreads, 4)
-    token_scores_wide_kernel(const T* logits, int ld, int splits, int* counters, float* partial, ScoreOut out) {
+__global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
+    token_scores_wide_kernel(const T* logits, int ld, int splits, int parts, int* counters, float* partial,
+                             ScoreOut out) {
   pdl_wait();
   using Chunk = ScoreChunk<T>;
+  extern __shared__ __align__(16) uint8_t ring[];
   __shared__ ScoreBest best;
   __shared__ ScoreSum sums[kScoreThreads / 32];
   __shared__ int s_last;
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const int r = blockIdx.x / splits, split = blockIdx.x % splits, top = out.top, vocab = out.vocab;
-  const T* x = logits + static_cast<size_t>(r) * ld;
-  const int origin = -static_cast<int>(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
-  const int chunks = (vocab - origin + Chunk::SIZE - 1) / Chunk::SIZE;
-  const int c0 = static_cast<int>(static_cast<int64_t>(chunks) * split / splits);
-  const int c1 = static_cast<int>(static_cast<int64_t>(chunks) * (split + 1) / splits);
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, top = out.top, vocab = out.vocab;
+  const uint32_t stages = smem_u32(ring);
+  ScoreWalk<T> ahead(logits, ld, vocab, splits, parts);
+  for (int i = 0; i < kScoreStages - 1; ++i) ahead.fetch(stages + i * 16384);
+  int stage = 0;
   if (t == 0) best.count = 0;
-  ScoreSum a{-INFINITY, 0.f, 0.f};
-  uint32_t bar = 0;    // order to exceed, once `raised`
-  bool raised = false;
-  Chunk now, next;
-  if (c0 < c1) next.load(x, origin + c0 * Chunk::SIZE, vocab);
-  for (int c = c0; c < c1; ++c) {
-    const int first = origin + c * Chunk::SIZE;
-    now = next;
-    if (c + 1 < c1) next.load(x, first + Chunk::SIZE, vocab);
-    float m = -INFINITY;
+  __syncthreads();
+  for (ScoreWalk<T> here(logits, ld, vocab, splits, parts); here.part < parts; here.leave()) {
+    const T* x = here.x;
+    const int r = here.part / splits;
+    ScoreSum a{-INFINITY, 0.f, 0.f};
+    uint32_t bar = 0;  // order to exceed, once `raised`
+    bool raised = false;
+    for (; here.c < here.c1; ++here.c) {
+      const int first = here.base();
+      asm volatile("cp.async.wait_group %0;" ::"n"(kScoreStages - 2) : "memory");
+      Chunk now;
+      now.read(x, first, vocab, stages + stage * 16384);
+      ahead.fetch(stages + (stage == 0 ? kScoreStages - 1 : stage - 1) * 16384);
+      stage = stage == kScoreStages - 1 ? 0 : stage + 1;
+      const float m = now.largest();
+      if (m > a.m) a = score_join(ScoreSum{m, 0.f, 0.f}, a);
+      const float base = a.m == -INFINITY ? 0.f : a.m;
+      uint64_t s = pair2(a.s, 0.f), u = pair2(a.u, 0.f);
 #pragma unroll
-    for (int i = 0; i < Chunk::N; ++i) m = fmaxf(m, now.at(i));
-    if (m > a.m) a = score_join(ScoreSum{m, 0.f, 0.f}, a);
-    const float base = a.m == -INFINITY ? 0.f : a.m;
-#pragma unroll
-    for (int i = 0; i < Chunk::N; ++i) score_add(now.at(i), base, a.s, a.u);
-    if (top == 0) continue;
+      for (int i = 0; i < Chunk::N; i += 2) score_add2(pair2(now.at(i), now.at(i + 1)), pair2(-base, -base), s, u);
+      a.s = low2(s) + high2(s);
+      a.u = low2(u) + high2(u);
+      if (top == 0) continue;
 
-    const bool any = Chunk::index(first, 0) < vocab;  // a thread's first element is its lowest
-    const uint32_t order = any ? score_order(m) : 0u;
-    uint32_t reach = raised ? bar + 1 : 0;
-    if (!raised) {  // the first chunk: 64 groups of four threads
-      uint32_t g = max(order, __shfl_xor_sync(0xffffffffu, order, 1));
-      g = max(g, __shfl_xor_sync(0xffffffffu, g, 2));
-      if ((lane & 3) == 0) best.group[t >> 2] = g;
-      __syncthreads();
-      int rank = 0;
-      for (int i = 0; i < 16; ++i) {
-        const int k = (t & 3) * 16 + i;
-        const uint32_t o = best.group[k];
-        rank += o > g || (o == g && k < t >> 2) ? 1 : 0;
-      }
-      rank += __shfl_xor_sync(0xffffffffu, rank, 1);
-      rank += __shfl_xor_sync(0xffffffffu, rank, 2);
-      if ((lane & 3) == 0 && rank == top - 1) best.bar = g;
-      __syncthreads();
-      bar = best.bar;
-      raised = bar > kForbidden;  // fewer than `top` groups hold more than forbidden tokens: all are candidates
-      reach = raised ? bar : 0;
-    }
-    int held = 0;
-    if (any && order >= reach) {
+      const bool any = Chunk::index(first, 0) < vocab;  // a thread's first element is its lowest
+      const uint32_t order = any ? score_order(m) : 0u;
+      uint32_t reach = raised ? bar + 1 : 0;
+      if (!raised) {  // the first chunk: 64 groups of four threads
+        uint32_t g = max(order, __shfl_xor_sync(0xffffffffu, order, 1));
+        g = max(g, __shfl_xor_sync(0xffffffffu, g, 2));
+        if ((lane & 3) == 0) best.group[t >> 2] = g;
+        __syncthreads();
+        int rank = 0;
 #pragma unroll
-      for (int i = 0; i < Chunk::N; ++i) {
-        const float v = now.at(i);
-        const int j = Chunk::index(first, i);
-        if (j >= 0 && j < vocab && score_order(v) >= reach) {
+        for (int i = 0; i < 16; ++i) {
+          const int k = i * 4 + (t & 3);
+          const uint32_t o = best.group[k];
+          rank += o > g || (o == g && k < t >> 2) ? 1 : 0;
+        }
+        rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+        rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+        if ((lane & 3) == 0 && rank == top - 1) best.bar = g;
+        __syncthreads();
+        bar = best.bar;
+        raised = bar > kForbidden;  // fewer than `top` groups hold more than forbidden tokens: all are candidates
+        reach = raised ? bar : 0;
+      }
+      int held = 0;
+      if (any && order >= reach) {
+        // which of the thread's logits reach the bar; they are few, and are read again
+        uint32_t hits = Chunk::N == 32 ? 0xffffffffu : (1u << Chunk::N) - 1;
+        if (reach > kForbidden) {
+          const float least = score_value(reach);
+          hits = 0;
+#pragma unroll
+          for (int i = 0; i < Chunk::N; ++i) hits |= now.at(i) >= least ? 1u << i : 0u;
+        }
+        while (hits) {
+          const int i = __ffs(hits) - 1, j = Chunk::index(first, i);
+          hits &= hits - 1;
+          if (j < 0 || j >= vocab) continue;
+          const float v = score_load(x + j);
+          if (score_order(v) < reach) continue;
           held = atomicAdd(&best.count, 1) + 1;
           if (held <= kScoreHeld) best.held[held - 1] = score_key(v, j);
         }
       }
-    }
-    if (__syncthreads_or(held > kScoreHeld)) {
-      score_compact(best, top, first);
-      uint64_t mine = 0;
-      if (any && order >= reach) {
+      const int full = __syncthreads_or(held > kScoreHeld / 2);
+      if (!full) continue;
+      if (__syncthreads_or(held > kScoreHeld)) {
+        score_compact(best, top, first);
+        uint64_t mine = 0;
+        if (any && order >= reach) {
 #pragma unroll
-        for (int i = 0; i < Chunk::N; ++i) {
-          const int j = Chunk::index(first, i);
-          if (j >= 0 && j < vocab) mine = max(mine, score_key(now.at(i), j));
+          for (int i = 0; i < Chunk::N; ++i) {
+            const int j = Chunk::index(first, i);
+            if (j >= 0 && j < vocab) mine = max(mine, score_key(now.at(i), j));
+          }
+        }
+        best.thread_best[t] = mine;
+        __syncthreads();
+        int rank = 0;
+        for (int k = 0; k < kScoreThreads; ++k) rank += best.thread_best[k] > mine ? 1 : 0;
+        if (mine && rank < top) {
+#pragma unroll
+          for (int i = 0; i < Chunk::N; ++i) {
+            const float v = now.at(i);
+            const int j = Chunk::index(first, i);
+            if (j >= 0 && j < vocab && score_order(v) >= reach)
+              best.held[atomicAdd(&best.count, 1)] = score_key(v, j);
+          }
         }
       }
-      best.thread_best[t] = mine;
-      __syncthreads();
-      int rank = 0;
-      for (int k = 0; k < kScoreThreads; ++k) rank += best.thread_best[k] > mine ? 1 : 0;
-      if (mine && rank < top) {
-#pragma unroll
-        for (int i = 0; i < Chunk::N; ++i) {
-          const float v = now.at(i);
-          const int j = Chunk::index(first, i);
-          if (j >= 0 && j < vocab && score_order(v) >= reach)
-            best.held[atomicAdd(&best.count, 1)] = score_key(v, j);
-        }
-      }
-      held = kScoreHeld;
-      __syncthreads();
-    }
-    if (__syncthreads_or(held > kScoreHeld / 2)) {
       if (score_compact(best, top, INT_MAX) == top) {
         bar = static_cast<uint32_t>(best.list[top - 1] >> 32);
         raised = true;
       }
     }
-  }
 
-  // ---- the part's sums and alternatives
-  a = score_warp_join(a);
-  if (lane == 0) sums[warp] = a;
-  __syncthreads();
-  a = sums[0];
-  for (int w = 1; w < kScoreThreads / 32; ++w) a = score_join(a, sums[w]);
-  int n = top > 0 ? score_compact(best, top, INT_MAX) : 0;
-  if (splits > 1) {
-    const int size = score_part(top);
-    float* mine = partial + static_cast<size_t>(blockIdx.x) * size;
-    if (t < n) reinterpret_cast<uint64_t*>(mine + 4)[t] = best.list[t];
-    if (t == 0) *reinterpret_cast<float4*>(mine) = make_float4(a.m, a.s, a.u, __int_as_float(n));
-    __syncthreads();
-    if (t == 0) {
-      __threadfence();
-      s_last = atomicAdd(counters + r, 1) == splits - 1;
-      if (s_last) counters[r] = 0;
-      __threadfence();
-    }
-    __syncthreads();
-    if (!s_last) return;
-    // the parts in order
-    const float* row = partial + static_cast<size_t>(r) * splits * size;
-    a = ScoreSum{-INFINITY, 0.f, 0.f};
-    for (int k = 0; k < splits; ++k) {
-      const float4 p = __ldcg(reinterpret_cast<const float4*>(row + static_cast<size_t>(k) * size));
-      a = score_join(a, ScoreSum{p.x, p.y, p.z});
-    }
-    if (top > 0) {
-      if (t == 0) best.count = 0;
-      __syncthreads();
-      for (int i = t; i < splits * top; i += kScoreThreads) {
-        const float* p = row + static_cast<size_t>(i / top) * size;
-        if (i % top < __float_as_int(__ldcg(p + 3)))
-          best.held[atomicAdd(&best.count, 1)] = __ldcg(reinterpret_cast<const unsigned long long*>(p + 4) + i % top);
-      }
+    // ---- the part's sums and alternatives
+    a = score_warp_join(a);
+    if (lane == 0) sums[warp] = a;
+    int n = 0;
+    if (top > 0)
       n = score_compact(best, top, INT_MAX);
+    else
+      __syncthreads();
+    a = sums[lane & 7];
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1)
+      a = score_join(a, ScoreSum{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o),
+                                 __shfl_xor_sync(0xffffffffu, a.u, o)});
+    bool writes = true;
+    if (splits > 1) {
+      const int size = score_part(top);
+      float* mine = partial + static_cast<size_t>(here.part) * size;
+      if (t < n) reinterpret_cast<uint64_t*>(mine + 4)[t] = best.list[t];
+      if (t == 0) *reinterpret_cast<float4*>(mine) = make_float4(a.m, a.s, a.u, __int_as_float(n));
+      __syncthreads();
+      if (t == 0) {
+        __threadfence();
+        s_last = atomicAdd(counters + r, 1) == splits - 1;
+        if (s_last) counters[r] = 0;
+        __threadfence();
+      }
+      __syncthreads();
+      writes = s_last != 0;
+      if (writes) {  // the row's parts, in order
+        const float* row = partial + static_cast<size_t>(r) * splits * size;
+        a = ScoreSum{-INFINITY, 0.f, 0.f};
+        for (int k = 0; k < splits; ++k) {
+          const float4 p = __ldcg(reinterpret_cast<const float4*>(row + static_cast<size_t>(k) * size));
+          a = score_join(a, ScoreSum{p.x, p.y, p.z});
+        }
+        if (top > 0) {
+          if (t == 0) best.count = 0;
+          __syncthreads();
+          for (int i = t; i < splits * top; i += kScoreThreads) {
+            const float* p = row + static_cast<size_t>(i / top) * size;
+            if (i % top < __float_as_int(__ldcg(p + 3)))
+              best.held[atomicAdd(&best.count, 1)] =
+                  __ldcg(reinterpret_cast<const unsigned long long*>(p + 4) + i % top);
+          }
+          n = score_compact(best, top, INT_MAX);
+        }
+      }
     }
-  }
-  if (t == 0) score_write_row(out, x, r, a);
-  if (t < top) {  // top <= vocab: the list is full
-    const float base = a.m == -INFINITY ? 0.f : a.m;
-    const uint64_t key = best.list[t];
-    out.top_id[static_cast<size_t>(r) * top + t] = static_cast<int32_t>(~static_cast<uint32_t>(key));
-    out.top_logp[static_cast<size_t>(r) * top + t] =
-        score_logp(score_value(static_cast<uint32_t>(key >> 32)), a, base, logf(a.s));
+    if (writes && warp == 1 && lane == 0) score_write_row(out, x, r, a);
+    if (writes && t < top) {  // top <= vocab: the list is full
+      const float base = a.m == -INFINITY ? 0.f : a.m;
+      const uint64_t key = best.list[t];
+      out.top_id[static_cast<size_t>(r) * top + t] = static_cast<int32_t>(~static_cast<uint32_t>(key));
+      out.top_logp[static_cast<size_t>(r) * top + t] =
+          score_logp(score_value(static_cast<uint32_t>(key >> 32)), a, base, logf(a.s));
+    }
+    __syncthreads();
+    if (t == 0) best.count = 0;
+    __syncthreads();
   }
 }
 
@@ -407,9 +560,9 @@ struct ScoreGrad {
   const float *lse, *entropy, *d_logp, *d_entropy;
   int vocab;
 };
-// A row's part of the gradient: g = -p (a + b (log p + h)), + a at the target.
+// A row's part of the gradient: with d = (x - z) log2(e), g = 2^d (-(a + b h) - b ln(2) d), and + a at the target.
 struct ScoreRow {
-  float a, b, z, h;
+  float minus_z, c, b2, a;
   int at;
   SJ_DEVICE ScoreRow(const ScoreGrad& in, int r, bool reports) {
     at = in.target ? in.target[r] : -1;
@@ -417,82 +570,104 @@ struct ScoreRow {
       if (reports) record_error(SJ_DEV_BAD_INDEX);
       at = -1;
     }
+    const float z = in.lse[r], b = in.d_entropy ? in.d_entropy[r] : 0.f;
     a = in.d_logp && at >= 0 ? in.d_logp[r] : 0.f;
-    b = in.d_entropy ? in.d_entropy[r] : 0.f;
-    z = in.lse[r];
-    h = in.d_entropy ? in.entropy[r] : 0.f;
+    if (z == -INFINITY) at = -1;  // a row of forbidden tokens only: no gradient
+    minus_z = z == -INFINITY ? z : -z;
+    c = z == -INFINITY ? 0.f : in.d_entropy ? -fmaf(b, in.entropy[r], a) : -a;
+    b2 = z == -INFINITY ? 0.f : -b * kLn2;
+  }
+  SJ_DEVICE uint64_t grad2(uint64_t x) const {
+    uint64_t d = mul2(add2(x, pair2(minus_z, minus_z)), pair2(kLog2e, kLog2e));
+    d = pair2(floor_exponent(low2(d)), floor_exponent(high2(d)));
+    const uint64_t p = pair2(exp2_flush(low2(d)), exp2_flush(high2(d)));
+    return mul2(p, fma2(pair2(b2, b2), d, pair2(c, c)));
   }
   SJ_DEVICE float grad(float x, int j) const {
-    const float lp = x - z, p = exp2_flush(lp * kLog2e);
-    float g = -p * fmaf(b, fmaxf(lp, -1e30f) + h, a);  // a forbidden token: p = 0, and no 0 * -inf
-    if (z == -INFINITY) g = 0.f;                       // a row of nothing else
-    if (j == at && z != -INFINITY) g += a;
-    return g;
+    const float g = low2(grad2(pair2(x, x)));
+    return j == at ? g + a : g;
   }
 };
 
 SJ_DEVICE void score_store(float* d, float g) { *d = g; }
 SJ_DEVICE void score_store(__nv_bfloat16* d, float g) { *d = f2bf(g); }
 
+// Sixteen bytes of logits, x's columns j and up, to sixteen bytes of gradient.
 template <typename T>
-SJ_DEVICE uint4 score_grad16(const ScoreRow& row, const uint4& q, int j) {
+SJ_DEVICE void score_grad16(const ScoreRow& row, const uint4& q, const T* x, int j, T* d) {
+  constexpr int PER = 16 / sizeof(T);
   uint4 y;
   if (sizeof(T) == 4) {
-    y.x = __float_as_uint(row.grad(__uint_as_float(q.x), j));
-    y.y = __float_as_uint(row.grad(__uint_as_float(q.y), j + 1));
-    y.z = __float_as_uint(row.grad(__uint_as_float(q.z), j + 2));
-    y.w = __float_as_uint(row.grad(__uint_as_float(q.w), j + 3));
+    const uint64_t a = row.grad2(pair2(__uint_as_float(q.x), __uint_as_float(q.y)));
+    const uint64_t b = row.grad2(pair2(__uint_as_float(q.z), __uint_as_float(q.w)));
+    y = make_uint4(static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32), static_cast<uint32_t>(b),
+                   static_cast<uint32_t>(b >> 32));
   } else {
-    auto pair = [&](uint32_t w, int at) {
-      return pack_bf16x2(row.grad(__uint_as_float(w << 16), at), row.grad(__uint_as_float(w & 0xffff0000u), at + 1));
+    auto two = [&](uint32_t w) {
+      const uint64_t g = row.grad2(pair2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)));
+      return pack_bf16x2(low2(g), high2(g));
     };
-    y.x = pair(q.x, j);
-    y.y = pair(q.y, j + 2);
-    y.z = pair(q.z, j + 4);
-    y.w = pair(q.w, j + 6);
+    y = make_uint4(two(q.x), two(q.y), two(q.z), two(q.w));
   }
-  return y;
+  const unsigned hit = static_cast<unsigned>(row.at - j);
+  const float own = hit < PER ? row.grad(score_load(x + row.at), row.at) : 0.f;  // read before an in-place write
+  *reinterpret_cast<uint4*>(d + j) = y;
+  if (hit < PER) score_store(d + row.at, own);
 }
 
-// Sixteen bytes of logits in, sixteen bytes of gradient out: rows on 16-byte boundaries.  The 16-byte pieces of
-// all rows, one after the other, four to a thread (a CTA's side by side), so that narrow rows leave no
-// thread idle; a piece that holds the row's end goes element by element.
-template <typename T>
-__global__ void __launch_bounds__(256) token_scores_bwd_kernel(const T* logits, int ld, T* d_logits, int ldd,
-                                                               int64_t pieces, int per_row, ScoreGrad in) {
-  pdl_wait();
+// Pieces k, k + STEP, ... below `end` of row r, four in flight; the first ones on their way before the row's scalars.
+template <typename T, int STEP>
+SJ_DEVICE void score_grad_pieces(const T* x, T* d, int k, int end, bool reports, int r, const ScoreGrad& in) {
   constexpr int PER = 16 / sizeof(T);
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * 1024;
-  const int r0 = static_cast<int>(first / per_row), j0 = static_cast<int>(first - static_cast<int64_t>(r0) * per_row);
   uint4 raw[4];
-  int r[4], j[4];
+  auto load = [&](int at) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int k = i * 256 + static_cast<int>(threadIdx.x);
-    raw[i] = make_uint4(0, 0, 0, 0);
-    r[i] = -1;
-    if (first + k < pieces) {
-      const int down = (j0 + k) / per_row;
-      r[i] = r0 + down;
-      j[i] = (j0 + k - down * per_row) * PER;
-      if (j[i] + PER <= in.vocab)
-        raw[i] = *reinterpret_cast<const uint4*>(logits + static_cast<size_t>(r[i]) * ld + j[i]);
+    for (int i = 0; i < 4; ++i) {
+      const int j = (at + i * STEP) * PER;
+      raw[i] = make_uint4(0, 0, 0, 0);
+      if (at + i * STEP < end && j + PER <= in.vocab) raw[i] = *reinterpret_cast<const uint4*>(x + j);
     }
-  }
+  };
+  load(k);
+  const ScoreRow row(in, r, reports);
+  for (; k < end; k += 4 * STEP) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (r[i] < 0) continue;
-    const ScoreRow row(in, r[i], j[i] == 0);
-    T* d = d_logits + static_cast<size_t>(r[i]) * ldd + j[i];
-    if (j[i] + PER <= in.vocab) {
-      *reinterpret_cast<uint4*>(d) = score_grad16<T>(row, raw[i], j[i]);
-    } else {
-      for (int e = 0; e < PER; ++e) {
-        const int at = j[i] + e;
-        score_store(d + e, at < in.vocab ? row.grad(score_load(logits + static_cast<size_t>(r[i]) * ld + at), at) : 0.f);
+    for (int i = 0; i < 4; ++i) {
+      const int j = (k + i * STEP) * PER;
+      if (k + i * STEP >= end) continue;
+      if (j + PER <= in.vocab) {
+        score_grad16<T>(row, raw[i], x, j, d);
+      } else {
+        for (int at = j; at < j + PER; ++at)
+          score_store(d + at, at < in.vocab ? row.grad(score_load(x + at), at) : 0.f);
       }
     }
+    load(k + 4 * STEP);
   }
+}
+
+// Narrow rows on 16-byte boundaries: a warp for a row, four 16-byte pieces a lane in flight; a piece that holds the row's
+// end goes element by element.
+template <typename T>
+__global__ void __launch_bounds__(128, 8) token_scores_bwd_narrow_kernel(const T* logits, int ld, T* d_logits, int ldd,
+                                                                         int rows, int per_row, ScoreGrad in) {
+  pdl_wait();
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (r >= rows) return;
+  score_grad_pieces<T, 32>(logits + static_cast<size_t>(r) * ld, d_logits + static_cast<size_t>(r) * ldd, lane,
+                           per_row, lane == 0, r, in);
+}
+
+// Wide rows on 16-byte boundaries: a CTA for an equal part of a row's pieces.
+template <typename T>
+__global__ void __launch_bounds__(256, 4) token_scores_bwd_wide_kernel(const T* logits, int ld, T* d_logits, int ldd,
+                                                                       int parts, int per_row, ScoreGrad in) {
+  pdl_wait();
+  const int r = blockIdx.x / parts, part = blockIdx.x % parts;
+  const int k0 = static_cast<int>(static_cast<int64_t>(per_row) * part / parts);
+  const int k1 = static_cast<int>(static_cast<int64_t>(per_row) * (part + 1) / parts);
+  score_grad_pieces<T, 256>(logits + static_cast<size_t>(r) * ld, d_logits + static_cast<size_t>(r) * ldd,
+                            k0 + static_cast<int>(threadIdx.x), k1, part == 0 && threadIdx.x == 0, r, in);
 }
 
 // Any strides and alignments: a CTA for 2048 elements of a row, side by side.
@@ -516,11 +691,17 @@ __global__ void __launch_bounds__(256) token_scores_bwd_any_kernel(const T* logi
 using namespace sj;
 
 namespace {
-// Parts of a row: enough CTAs for the GPU when the rows are few (4 fit an SM), of at least 4096 logits.
+int score_ctas() { return kScoreCtas * sm_count(); }
+// Parts of a row, of at least 4096 logits: 1 when the rows keep every CTA busy, or nearly, to the end; else the fewest
+// that do.
 int score_splits(int rows, int vocab) {
   if (vocab <= kScoreNarrow || rows <= 0) return 1;
-  const int fill = (4 * sm_count() + rows - 1) / rows, parts = (vocab + 4095) / 4096;
-  return std::max(1, std::min({fill, parts, kScoreMaxSplits}));
+  const int ctas = score_ctas(), most = std::min((vocab + 4095) / 4096, kScoreMaxSplits);
+  for (int s = 1; s < most; ++s) {
+    const int64_t parts = static_cast<int64_t>(rows) * s, rounds = (parts + ctas - 1) / ctas;
+    if (parts * 100 >= rounds * ctas * 85) return s;
+  }
+  return most;
 }
 size_t score_counter_bytes(int rows) { return (static_cast<size_t>(rows) * sizeof(int) + 255) / 256 * 256; }
 
@@ -534,10 +715,16 @@ int scores(const T* logits, int ld, int rows, const ScoreOut& out, void* workspa
                         : token_scores_narrow_kernel<T, 32>,
            grid, 128, 0, stream, logits, ld, rows, out);
   } else {
-    const int splits = score_splits(rows, out.vocab);
-    launch(token_scores_wide_kernel<T>, rows * splits, kScoreThreads, 0, stream, logits, ld, splits,
-           static_cast<int*>(workspace), reinterpret_cast<float*>(static_cast<char*>(workspace) + score_counter_bytes(rows)),
-           out);
+    const int splits = score_splits(rows, out.vocab), smem = kScoreStages * 16384;
+    if (static_cast<int64_t>(rows) * splits > INT_MAX - score_ctas())
+      return fail(SJ_ERR_SHAPE, "sj_token_scores: rows=%d vocab=%d", rows, out.vocab);
+    static KernelAttrOnce once;
+    const int rc = ensure_max_smem(once, reinterpret_cast<const void*>(token_scores_wide_kernel<T>), smem,
+                                   "sj_token_scores: shared memory");
+    if (rc != SJ_OK) return rc;
+    launch(token_scores_wide_kernel<T>, std::min(rows * splits, score_ctas()), kScoreThreads, smem, stream, logits, ld,
+           splits, rows * splits, static_cast<int*>(workspace),
+           reinterpret_cast<float*>(static_cast<char*>(workspace) + score_counter_bytes(rows)), out);
   }
   SJ_LAUNCH_CHECK("token_scores");
   return SJ_OK;
@@ -548,9 +735,16 @@ int scores_bwd(const T* logits, int ld, T* d_logits, int ldd, int rows, const Sc
   constexpr int PER = 16 / sizeof(T);
   if (aligned16(logits) && aligned16(d_logits) && ld % PER == 0 && ldd % PER == 0) {
     const int per_row = ldd / PER;
-    const int64_t pieces = static_cast<int64_t>(rows) * per_row;
-    launch(token_scores_bwd_kernel<T>, static_cast<unsigned>((pieces + 1023) / 1024), 256, 0, stream, logits, ld,
-           d_logits, ldd, pieces, per_row, in);
+    if (per_row <= 256) {
+      launch(token_scores_bwd_narrow_kernel<T>, (rows + 3) / 4, 128, 0, stream, logits, ld, d_logits, ldd, rows,
+             per_row, in);
+    } else {
+      const int parts = (per_row + 2047) / 2048;
+      if (static_cast<int64_t>(rows) * parts > INT_MAX)
+        return fail(SJ_ERR_SHAPE, "sj_token_scores_bwd: rows=%d ldd=%d", rows, ldd);
+      launch(token_scores_bwd_wide_kernel<T>, static_cast<unsigned>(rows) * parts, 256, 0, stream, logits, ld, d_logits,
+             ldd, parts, per_row, in);
+    }
   } else {
     const int parts = (ldd + 2047) / 2048;
     if (static_cast<int64_t>(rows) * parts > INT_MAX)

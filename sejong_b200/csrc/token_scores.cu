@@ -97,13 +97,27 @@ SJ_DEVICE ScoreSum score_join(ScoreSum a, ScoreSum b) {
   a.s += f * b.s;
   return a;
 }
-SJ_DEVICE ScoreSum score_warp_join(ScoreSum a) {
+// The same part with a maximum of at least m.
+SJ_DEVICE ScoreSum score_raise(ScoreSum a, float m) {
+  const float top = fmaxf(a.m, m);
+  const float d = a.m == top ? 0.f : fmaxf((a.m - top) * kLog2e, -150.f), f = exp2_flush(d);
+  return ScoreSum{top, f * a.s, f * fmaf(d, a.s, a.u)};
+}
+// The parts of WIDTH lanes: the maximum first, then each part raised to it once.
+template <int WIDTH>
+SJ_DEVICE ScoreSum score_lanes_join(ScoreSum a) {
+  float m = a.m;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    a = score_join(a, ScoreSum{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o),
-                               __shfl_xor_sync(0xffffffffu, a.u, o)});
+  for (int o = WIDTH / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  a = score_raise(a, m);
+#pragma unroll
+  for (int o = WIDTH / 2; o > 0; o >>= 1) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+    a.u += __shfl_xor_sync(0xffffffffu, a.u, o);
+  }
   return a;
 }
+
 // Two logits into pairs of partial s and u: d = (x - base) log2(e), s += 2^d, u += 2^d d.
 SJ_DEVICE void score_add2(uint64_t x, uint64_t minus_base, uint64_t& s, uint64_t& u) {
   uint64_t d = mul2(add2(x, minus_base), pair2(kLog2e, kLog2e));
@@ -244,41 +258,56 @@ struct ScoreChunk {
     const uint32_t w = word(q, i % PER / 2);
     return __uint_as_float(i % 2 ? w & 0xffff0000u : w << 16);
   }
-  SJ_DEVICE float largest() const {  // NaN left out, -inf where there is nothing else
-    float m = -INFINITY;
-    if (sizeof(T) == 4) {
+  // The maxima of the four pieces: NaN left out, -inf where there is nothing else.
+  SJ_DEVICE void largest(float (&m)[4]) const {
 #pragma unroll
-      for (int i = 0; i < N; ++i) m = fmaxf(m, at(i));
-      return m;
+    for (int v = 0; v < 4; ++v) {
+      if (sizeof(T) == 4) {
+        m[v] = fmaxf(fmaxf(at(4 * v), at(4 * v + 1)), fmaxf(at(4 * v + 2), at(4 * v + 3)));
+      } else {
+        uint32_t p = 0xff80ff80u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) asm("max.bf16x2 %0, %0, %1;" : "+r"(p) : "r"(word(raw[v], i)));
+        m[v] = fmaxf(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u));
+      }
     }
-    uint32_t p = 0xff80ff80u;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) asm("max.bf16x2 %0, %0, %1;" : "+r"(p) : "r"(word(raw[i / 4], i % 4)));
-    return fmaxf(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u));
   }
-  // The chunk's pieces that lie in the row, on their way to `stage` (16 KB of shared memory).
-  SJ_DEVICE static void fetch(const T* x, int base, int vocab, uint32_t stage) {
+  // The chunk's pieces that lie in the row, on their way to `own`, the thread's place in a stage of shared memory.
+  // A chunk inside the row needs no look at its pieces.
+  SJ_DEVICE static void fetch(const T* x, int base, int vocab, uint32_t own) {
+    const T* src = x + index(base, 0);
+    const bool inside = base >= 0 && base + SIZE <= vocab;
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
       const int j = index(base, v * PER);
-      if (j >= 0 && j + PER <= vocab)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(stage + (v * kScoreThreads + threadIdx.x) * 16),
-                     "l"(x + j)
+      if (inside || (j >= 0 && j + PER <= vocab))
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(own + v * (16 * kScoreThreads)),
+                     "l"(src + v * (PER * kScoreThreads))
                      : "memory");
     }
   }
-  // The thread's own pieces from `stage`, the row's ends from memory; -inf outside [0, vocab).
-  SJ_DEVICE void read(const T* x, int base, int vocab, uint32_t stage) {
+  SJ_DEVICE static uint4 piece(uint32_t own, int v) {
+    uint4 q;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
+                 : "r"(own + v * (16 * kScoreThreads))
+                 : "memory");
+    return q;
+  }
+  // The thread's pieces from its place in a stage, the row's ends from memory; -inf outside [0, vocab).
+  SJ_DEVICE void read(const T* x, int base, int vocab, uint32_t own) {
+    if (base >= 0 && base + SIZE <= vocab) {
+#pragma unroll
+      for (int v = 0; v < 4; ++v) raw[v] = piece(own, v);
+      return;
+    }
     constexpr uint32_t NONE = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
       const int j = index(base, v * PER);
       raw[v] = make_uint4(NONE, NONE, NONE, NONE);
       if (j >= 0 && j + PER <= vocab) {
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(raw[v].x), "=r"(raw[v].y), "=r"(raw[v].z), "=r"(raw[v].w)
-                     : "r"(stage + (v * kScoreThreads + threadIdx.x) * 16)
-                     : "memory");
+        raw[v] = piece(own, v);
       } else if (j < vocab) {
         uint32_t w[4] = {NONE, NONE, NONE, NONE};
 #pragma unroll
@@ -308,22 +337,22 @@ struct ScoreWalk {
   }
   SJ_DEVICE void enter() {
     if (part >= parts) return;
-    const int r = part / splits, k = part - r * splits;
+    const int r = splits == 1 ? part : part / splits, k = part - r * splits;
     x = logits + static_cast<size_t>(r) * ld;
     origin = -static_cast<int>(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
     const int chunks = (vocab - origin + ScoreChunk<T>::SIZE - 1) / ScoreChunk<T>::SIZE;
-    c = static_cast<int>(static_cast<int64_t>(chunks) * k / splits);
-    c1 = static_cast<int>(static_cast<int64_t>(chunks) * (k + 1) / splits);
+    c = splits == 1 ? 0 : chunks * k / splits;  // at most 2^19 chunks, 16 splits
+    c1 = splits == 1 ? chunks : chunks * (k + 1) / splits;
   }
   SJ_DEVICE void leave() {
     part += gridDim.x;
     enter();
   }
   SJ_DEVICE int base() const { return origin + c * ScoreChunk<T>::SIZE; }
-  SJ_DEVICE void fetch(uint32_t stage) {  // the next chunk, whichever part it is of
+  SJ_DEVICE void fetch(uint32_t own) {  // the next chunk, whichever part it is of
     while (part < parts && c >= c1) leave();
     if (part < parts) {
-      ScoreChunk<T>::fetch(x, base(), vocab, stage);
+      ScoreChunk<T>::fetch(x, base(), vocab, own);
       ++c;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -340,30 +369,34 @@ struct ScoreBest {
   int count;     // of held
 };
 
-// held[0, n) cut down to the `top` largest keys, in order, among those whose index is below `before`.
-SJ_DEVICE int score_compact(ScoreBest& b, int top, int before) {
+// held[0, n) cut down to the `top` largest keys, in order; !ALL: among those whose index is below `before`.
+template <bool ALL>
+SJ_DEVICE int score_compact(ScoreBest& b, int top, int before = 0) {
+  auto counts = [&](uint64_t key) { return ALL || static_cast<int>(~static_cast<uint32_t>(key)) < before; };
   __syncthreads();
   const int n = min(b.count, kScoreHeld);
   for (int i = threadIdx.x; i < n; i += kScoreThreads) {
     const uint64_t key = b.held[i];
-    int rank = static_cast<int>(~static_cast<uint32_t>(key)) < before ? 0 : top;
+    int rank = 0;
 #pragma unroll 8
     for (int k = 0; k < n; ++k) {
       const uint64_t other = b.held[k];
-      rank += other > key && static_cast<int>(~static_cast<uint32_t>(other)) < before ? 1 : 0;
+      rank += other > key && counts(other) ? 1 : 0;
     }
-    if (rank < top) b.list[rank] = key;
+    if (rank < top && counts(key)) b.list[rank] = key;
   }
-  int kept = 0;
-  for (int i = threadIdx.x; i < n; i += kScoreThreads)
-    kept += static_cast<int>(~static_cast<uint32_t>(b.held[i])) < before ? 1 : 0;
+  int kept = min(n, top);
   __syncthreads();
-  if (threadIdx.x == 0) b.count = 0;
-  __syncthreads();
-  if (kept) atomicAdd(&b.count, kept);
-  __syncthreads();
-  kept = min(b.count, top);
-  __syncthreads();
+  if (!ALL) {
+    kept = 0;
+    for (int i = threadIdx.x; i < n; i += kScoreThreads) kept += counts(b.held[i]) ? 1 : 0;
+    if (threadIdx.x == 0) b.count = 0;
+    __syncthreads();
+    if (kept) atomicAdd(&b.count, kept);
+    __syncthreads();
+    kept = min(b.count, top);
+    __syncthreads();
+  }
   if (threadIdx.x < kept) b.held[threadIdx.x] = b.list[threadIdx.x];
   if (threadIdx.x == 0) b.count = kept;
   __syncthreads();
@@ -388,7 +421,7 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
   __shared__ ScoreSum sums[kScoreThreads / 32];
   __shared__ int s_last;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, top = out.top, vocab = out.vocab;
-  const uint32_t stages = smem_u32(ring);
+  const uint32_t stages = smem_u32(ring) + t * 16;
   ScoreWalk<T> ahead(logits, ld, vocab, splits, parts);
   for (int i = 0; i < kScoreStages - 1; ++i) ahead.fetch(stages + i * 16384);
   int stage = 0;
@@ -396,19 +429,22 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
   __syncthreads();
   for (ScoreWalk<T> here(logits, ld, vocab, splits, parts); here.part < parts; here.leave()) {
     const T* x = here.x;
-    const int r = here.part / splits;
+    const int r = splits == 1 ? here.part : here.part / splits;
     ScoreSum a{-INFINITY, 0.f, 0.f};
     uint32_t bar = 0;  // order to exceed, once `raised`
     bool raised = false;
     for (; here.c < here.c1; ++here.c) {
       const int first = here.base();
       asm volatile("cp.async.wait_group %0;" ::"n"(kScoreStages - 2) : "memory");
+      const uint32_t own = stages + stage * 16384;
       Chunk now;
-      now.read(x, first, vocab, stages + stage * 16384);
+      now.read(x, first, vocab, own);
       ahead.fetch(stages + (stage == 0 ? kScoreStages - 1 : stage - 1) * 16384);
       stage = stage == kScoreStages - 1 ? 0 : stage + 1;
-      const float m = now.largest();
-      if (m > a.m) a = score_join(ScoreSum{m, 0.f, 0.f}, a);
+      float most[4];
+      now.largest(most);
+      const float m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+      if (__any_sync(0xffffffffu, m > a.m)) a = score_raise(a, m);
       const float base = a.m == -INFINITY ? 0.f : a.m;
       uint64_t s = pair2(a.s, 0.f), u = pair2(a.u, 0.f);
 #pragma unroll
@@ -442,28 +478,39 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
       }
       int held = 0;
       if (any && order >= reach) {
-        // which of the thread's logits reach the bar; they are few, and are read again
-        uint32_t hits = Chunk::N == 32 ? 0xffffffffu : (1u << Chunk::N) - 1;
-        if (reach > kForbidden) {
-          const float least = score_value(reach);
-          hits = 0;
+        // the pieces whose maximum reaches the bar are few: their logits are looked at one by one
+        const float least = reach > kForbidden ? score_value(reach) : -INFINITY;
+        unsigned hot = 0;
 #pragma unroll
-          for (int i = 0; i < Chunk::N; ++i) hits |= now.at(i) >= least ? 1u << i : 0u;
-        }
-        while (hits) {
-          const int i = __ffs(hits) - 1, j = Chunk::index(first, i);
-          hits &= hits - 1;
-          if (j < 0 || j >= vocab) continue;
-          const float v = score_load(x + j);
-          if (score_order(v) < reach) continue;
+        for (int v = 0; v < 4; ++v) hot |= most[v] >= least ? 1u << v : 0u;
+        auto push = [&](float y, int j) {
           held = atomicAdd(&best.count, 1) + 1;
-          if (held <= kScoreHeld) best.held[held - 1] = score_key(v, j);
+          if (held <= kScoreHeld) best.held[held - 1] = score_key(y, j);
+        };
+        while (hot) {
+          const int v = __ffs(hot) - 1, j0 = Chunk::index(first, v * Chunk::PER);
+          hot &= hot - 1;
+          if (reach > kForbidden && j0 >= 0 && j0 + Chunk::PER <= vocab) {
+            const uint4 q = Chunk::piece(own, v);
+#pragma unroll
+            for (int e = 0; e < Chunk::PER; ++e) {
+              const uint32_t w = Chunk::word(q, e * static_cast<int>(sizeof(T)) / 4);
+              const float y = __uint_as_float(sizeof(T) == 4 ? w : e % 2 ? w & 0xffff0000u : w << 16);
+              if (y >= least) push(y, j0 + e);
+            }
+          } else {
+#pragma unroll 1
+            for (int j = max(j0, 0); j < min(j0 + Chunk::PER, vocab); ++j) {
+              const float y = score_load(x + j);
+              if (score_order(y) >= reach) push(y, j);
+            }
+          }
         }
       }
       const int full = __syncthreads_or(held > kScoreHeld / 2);
       if (!full) continue;
       if (__syncthreads_or(held > kScoreHeld)) {
-        score_compact(best, top, first);
+        score_compact<false>(best, top, first);
         uint64_t mine = 0;
         if (any && order >= reach) {
 #pragma unroll
@@ -486,25 +533,21 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
           }
         }
       }
-      if (score_compact(best, top, INT_MAX) == top) {
+      if (score_compact<true>(best, top) == top) {
         bar = static_cast<uint32_t>(best.list[top - 1] >> 32);
         raised = true;
       }
     }
 
     // ---- the part's sums and alternatives
-    a = score_warp_join(a);
+    a = score_lanes_join<32>(a);
     if (lane == 0) sums[warp] = a;
     int n = 0;
     if (top > 0)
-      n = score_compact(best, top, INT_MAX);
+      n = score_compact<true>(best, top);
     else
       __syncthreads();
-    a = sums[lane & 7];
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1)
-      a = score_join(a, ScoreSum{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o),
-                                 __shfl_xor_sync(0xffffffffu, a.u, o)});
+    if (warp == 0) a = score_lanes_join<8>(sums[lane & 7]);  // what follows is warp 0's
     bool writes = true;
     if (splits > 1) {
       const int size = score_part(top);
@@ -536,11 +579,11 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
               best.held[atomicAdd(&best.count, 1)] =
                   __ldcg(reinterpret_cast<const unsigned long long*>(p + 4) + i % top);
           }
-          n = score_compact(best, top, INT_MAX);
+          n = score_compact<true>(best, top);
         }
       }
     }
-    if (writes && warp == 1 && lane == 0) score_write_row(out, x, r, a);
+    if (writes && t == 0) score_write_row(out, x, r, a);
     if (writes && t < top) {  // top <= vocab: the list is full
       const float base = a.m == -INFINITY ? 0.f : a.m;
       const uint64_t key = best.list[t];
@@ -699,7 +742,7 @@ int score_splits(int rows, int vocab) {
   const int ctas = score_ctas(), most = std::min((vocab + 4095) / 4096, kScoreMaxSplits);
   for (int s = 1; s < most; ++s) {
     const int64_t parts = static_cast<int64_t>(rows) * s, rounds = (parts + ctas - 1) / ctas;
-    if (parts * 100 >= rounds * ctas * 85) return s;
+    if (parts * 100 >= rounds * ctas * 70) return s;
   }
   return most;
 }

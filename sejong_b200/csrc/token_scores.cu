@@ -330,7 +330,7 @@ struct ScoreChunk {
 template <typename T>
 struct ScoreWalk {
   const T *logits, *x;
-  int ld, vocab, splits, parts, part, origin, c, c1;
+  int ld, vocab, splits, parts, part, origin, c, c1, start;
   SJ_DEVICE ScoreWalk(const T* all, int ld_, int vocab_, int splits_, int parts_)
       : logits(all), ld(ld_), vocab(vocab_), splits(splits_), parts(parts_), part(blockIdx.x) {
     enter();
@@ -343,6 +343,7 @@ struct ScoreWalk {
     const int chunks = (vocab - origin + ScoreChunk<T>::SIZE - 1) / ScoreChunk<T>::SIZE;
     c = splits == 1 ? 0 : chunks * k / splits;  // at most 2^19 chunks, 16 splits
     c1 = splits == 1 ? chunks : chunks * (k + 1) / splits;
+    start = base();
   }
   SJ_DEVICE void leave() {
     part += gridDim.x;
@@ -364,52 +365,118 @@ struct ScoreBest {
   uint64_t held[kScoreHeld];
   uint64_t list[kScoreMaxTop];
   uint64_t thread_best[kScoreThreads];
-  uint32_t group[64];
-  uint32_t bar;  // order that a group of the first chunk reaches `top` times
+  __align__(16) uint32_t group[64];
+  uint32_t bar;
+  int kept;
   int count;     // of held
 };
 
-// held[0, n) cut down to the `top` largest keys, in order; !ALL: among those whose index is below `before`.
-template <bool ALL>
-SJ_DEVICE int score_compact(ScoreBest& b, int top, int before = 0) {
-  auto counts = [&](uint64_t key) { return ALL || static_cast<int>(~static_cast<uint32_t>(key)) < before; };
+// An order that at least `top` of the CTA's logits reach (a thread gives the largest of its own): the `top`-th
+// largest of 64 groups of four threads, but for its last six bits, which make the groups' values distinct.
+// 0 when fewer than `top` groups hold more than forbidden tokens.
+SJ_DEVICE uint32_t score_bar(ScoreBest& b, uint32_t order, int top) {
+  const int t = threadIdx.x;
+  uint32_t g = max(order, __shfl_xor_sync(0xffffffffu, order, 1));
+  g = max(g, __shfl_xor_sync(0xffffffffu, g, 2));
+  g = (g & ~63u) | static_cast<uint32_t>(t >> 2);
+  if ((t & 3) == 0) b.group[t >> 2] = g;
   __syncthreads();
-  const int n = min(b.count, kScoreHeld);
+  int rank = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint4 o = reinterpret_cast<const uint4*>(b.group)[i * 4 + (t & 3)];
+    rank += (o.x > g) + (o.y > g) + (o.z > g) + (o.w > g);
+  }
+  rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+  rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+  if ((t & 3) == 0 && rank == top - 1) b.bar = (g & ~63u) > kForbidden ? g & ~63u : 0u;
+  __syncthreads();
+  return b.bar;
+}
+
+// held cut down to its `top` largest keys, in order, which are in list, too; returns how many there are.
+SJ_DEVICE int score_rank(ScoreBest& b, int top) {
+  __syncthreads();
+  const int n = b.count;
+#pragma unroll 1
   for (int i = threadIdx.x; i < n; i += kScoreThreads) {
     const uint64_t key = b.held[i];
     int rank = 0;
 #pragma unroll 8
-    for (int k = 0; k < n; ++k) {
-      const uint64_t other = b.held[k];
-      rank += other > key && counts(other) ? 1 : 0;
-    }
-    if (rank < top && counts(key)) b.list[rank] = key;
+    for (int k = 0; k < n; ++k) rank += b.held[k] > key ? 1 : 0;
+    if (rank < top) b.list[rank] = key;
   }
-  int kept = min(n, top);
   __syncthreads();
-  if (!ALL) {
-    kept = 0;
-    for (int i = threadIdx.x; i < n; i += kScoreThreads) kept += counts(b.held[i]) ? 1 : 0;
-    if (threadIdx.x == 0) b.count = 0;
-    __syncthreads();
-    if (kept) atomicAdd(&b.count, kept);
-    __syncthreads();
-    kept = min(b.count, top);
-    __syncthreads();
-  }
+  const int kept = min(n, top);
   if (threadIdx.x < kept) b.held[threadIdx.x] = b.list[threadIdx.x];
   if (threadIdx.x == 0) b.count = kept;
   __syncthreads();
   return kept;
 }
 
+// held without what lies below the bar of the whole part, which is higher than its first chunk's: ranking takes the
+// square of its length.  Left as it is where many are equal.
+SJ_DEVICE void score_sift(ScoreBest& b, uint32_t bar) {
+  const int n = b.count;
+  if (threadIdx.x == 0) b.kept = 0;
+  __syncthreads();
+#pragma unroll 1
+  for (int i = threadIdx.x; i < n; i += kScoreThreads) {
+    const uint64_t key = b.held[i];
+    if (static_cast<uint32_t>(key >> 32) < bar) continue;
+    const int at = atomicAdd(&b.kept, 1);
+    if (at < kScoreThreads) b.thread_best[at] = key;
+  }
+  __syncthreads();
+  const int kept = b.kept;
+  if (kept > kScoreThreads) return;
+  if (threadIdx.x < kept) b.held[threadIdx.x] = b.thread_best[threadIdx.x];
+  if (threadIdx.x == 0) b.count = kept;
+}
+
+// The same where more logits reach the bar than the list holds (equal or rising logits): chunk by chunk, the logits of
+// the `top` threads with the best maxima join the list, which is ranked each time.  Leaves best.list; returns
+// its length.
+template <typename T>
+SJ_DEVICE int score_rank_all(ScoreBest& best, const T* x, int base, int end, int vocab, int top) {
+  __syncthreads();
+  if (threadIdx.x == 0) best.count = 0;
+  int n = 0;
+  for (; base < end; base += ScoreChunk<T>::SIZE) {
+    const uint32_t reach = n == top ? static_cast<uint32_t>(best.list[top - 1] >> 32) + 1 : 0u;
+    uint64_t mine = 0;
+#pragma unroll 1
+    for (int i = 0; i < ScoreChunk<T>::N; ++i) {
+      const int j = ScoreChunk<T>::index(base, i);
+      if (j < 0 || j >= vocab) continue;
+      const uint64_t key = score_key(score_load(x + j), j);
+      if (static_cast<uint32_t>(key >> 32) >= reach) mine = max(mine, key);
+    }
+    __syncthreads();
+    best.thread_best[threadIdx.x] = mine;
+    __syncthreads();
+    int rank = 0;
+    for (int k = 0; k < kScoreThreads; ++k) rank += best.thread_best[k] > mine ? 1 : 0;
+    if (mine && rank < top) {
+#pragma unroll 1
+      for (int i = 0; i < ScoreChunk<T>::N; ++i) {
+        const int j = ScoreChunk<T>::index(base, i);
+        if (j < 0 || j >= vocab) continue;
+        const uint64_t key = score_key(score_load(x + j), j);
+        if (static_cast<uint32_t>(key >> 32) >= reach) best.held[atomicAdd(&best.count, 1)] = key;
+      }
+    }
+    n = score_rank(best, top);
+  }
+  return n;
+}
+
 // Persistent CTAs over the parts of rows, 16 KB at a time; the next two chunks, of the next part too, are on their way
 // to shared memory meanwhile (cp.async; a thread reads back only what it copied, so copies need no barrier).  The
 // sums are each thread's own until the part's end.  Alternatives: the `top`-th largest of 64 groups' maxima of the
 // first chunk is a bar that at least `top` logits reach; what reaches it (of later chunks, exceeds it)
-// goes to a list that is ranked once at the end: about 24 candidates a chunk at top = 20.  A list that fills up
-// is ranked at once, which raises the bar; a chunk with more candidates than the list holds (equal or rising
-// logits) takes those of the `top` threads with the best maxima.
+// goes to a list that is ranked once at the end: about 24 candidates a chunk at top = 20.  So a part takes
+// two barriers in its first chunk and none in the others.
 template <typename T>
 __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
     token_scores_wide_kernel(const T* logits, int ld, int splits, int parts, int* counters, float* partial,
@@ -421,7 +488,7 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
   __shared__ ScoreSum sums[kScoreThreads / 32];
   __shared__ int s_last;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, top = out.top, vocab = out.vocab;
-  const uint32_t stages = smem_u32(ring) + t * 16;
+  const uint32_t stages = smem_u32(ring) + t * 16, count_at = smem_u32(&best.count);
   ScoreWalk<T> ahead(logits, ld, vocab, splits, parts);
   for (int i = 0; i < kScoreStages - 1; ++i) ahead.fetch(stages + i * 16384);
   int stage = 0;
@@ -456,27 +523,10 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
       const bool any = Chunk::index(first, 0) < vocab;  // a thread's first element is its lowest
       const uint32_t order = any ? score_order(m) : 0u;
       uint32_t reach = raised ? bar + 1 : 0;
-      if (!raised) {  // the first chunk: 64 groups of four threads
-        uint32_t g = max(order, __shfl_xor_sync(0xffffffffu, order, 1));
-        g = max(g, __shfl_xor_sync(0xffffffffu, g, 2));
-        if ((lane & 3) == 0) best.group[t >> 2] = g;
-        __syncthreads();
-        int rank = 0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int k = i * 4 + (t & 3);
-          const uint32_t o = best.group[k];
-          rank += o > g || (o == g && k < t >> 2) ? 1 : 0;
-        }
-        rank += __shfl_xor_sync(0xffffffffu, rank, 1);
-        rank += __shfl_xor_sync(0xffffffffu, rank, 2);
-        if ((lane & 3) == 0 && rank == top - 1) best.bar = g;
-        __syncthreads();
-        bar = best.bar;
-        raised = bar > kForbidden;  // fewer than `top` groups hold more than forbidden tokens: all are candidates
-        reach = raised ? bar : 0;
+      if (!raised) {
+        reach = bar = score_bar(best, order, top);
+        raised = bar > 0;
       }
-      int held = 0;
       if (any && order >= reach) {
         // the pieces whose maximum reaches the bar are few: their logits are looked at one by one
         const float least = reach > kForbidden ? score_value(reach) : -INFINITY;
@@ -484,8 +534,9 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
 #pragma unroll
         for (int v = 0; v < 4; ++v) hot |= most[v] >= least ? 1u << v : 0u;
         auto push = [&](float y, int j) {
-          held = atomicAdd(&best.count, 1) + 1;
-          if (held <= kScoreHeld) best.held[held - 1] = score_key(y, j);
+          int at;
+          asm volatile("atom.shared.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(count_at) : "memory");
+          if (at < kScoreHeld) best.held[at] = score_key(y, j);
         };
         while (hot) {
           const int v = __ffs(hot) - 1, j0 = Chunk::index(first, v * Chunk::PER);
@@ -507,46 +558,20 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
           }
         }
       }
-      const int full = __syncthreads_or(held > kScoreHeld / 2);
-      if (!full) continue;
-      if (__syncthreads_or(held > kScoreHeld)) {
-        score_compact<false>(best, top, first);
-        uint64_t mine = 0;
-        if (any && order >= reach) {
-#pragma unroll
-          for (int i = 0; i < Chunk::N; ++i) {
-            const int j = Chunk::index(first, i);
-            if (j >= 0 && j < vocab) mine = max(mine, score_key(now.at(i), j));
-          }
-        }
-        best.thread_best[t] = mine;
-        __syncthreads();
-        int rank = 0;
-        for (int k = 0; k < kScoreThreads; ++k) rank += best.thread_best[k] > mine ? 1 : 0;
-        if (mine && rank < top) {
-#pragma unroll
-          for (int i = 0; i < Chunk::N; ++i) {
-            const float v = now.at(i);
-            const int j = Chunk::index(first, i);
-            if (j >= 0 && j < vocab && score_order(v) >= reach)
-              best.held[atomicAdd(&best.count, 1)] = score_key(v, j);
-          }
-        }
-      }
-      if (score_compact<true>(best, top) == top) {
-        bar = static_cast<uint32_t>(best.list[top - 1] >> 32);
-        raised = true;
-      }
     }
 
     // ---- the part's sums and alternatives
+    const uint32_t order = score_order(a.m);
     a = score_lanes_join<32>(a);
     if (lane == 0) sums[warp] = a;
     int n = 0;
-    if (top > 0)
-      n = score_compact<true>(best, top);
-    else
-      __syncthreads();
+    __syncthreads();
+    if (top > 0 && best.count > kScoreHeld) {
+      n = score_rank_all(best, x, here.start, here.origin + here.c1 * Chunk::SIZE, vocab, top);
+    } else if (top > 0) {
+      if (best.count > 64) score_sift(best, score_bar(best, order, top));
+      n = score_rank(best, top);
+    }
     if (warp == 0) a = score_lanes_join<8>(sums[lane & 7]);  // what follows is warp 0's
     bool writes = true;
     if (splits > 1) {
@@ -579,7 +604,7 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
               best.held[atomicAdd(&best.count, 1)] =
                   __ldcg(reinterpret_cast<const unsigned long long*>(p + 4) + i % top);
           }
-          n = score_compact<true>(best, top);
+          n = score_rank(best, top);
         }
       }
     }
@@ -639,19 +664,22 @@ SJ_DEVICE void score_store(__nv_bfloat16* d, float g) { *d = f2bf(g); }
 template <typename T>
 SJ_DEVICE void score_grad16(const ScoreRow& row, const uint4& q, const T* x, int j, T* d) {
   constexpr int PER = 16 / sizeof(T);
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  auto logits2 = [&](int i) {
+    if (sizeof(T) == 4) return pair2(__uint_as_float(w[2 * i % 4]), __uint_as_float(w[(2 * i + 1) % 4]));
+    return pair2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+  };
+  uint64_t g[PER / 2];
+#pragma unroll
+  for (int i = 0; i < PER / 2; ++i) g[i] = row.grad2(logits2(i));
   uint4 y;
-  if (sizeof(T) == 4) {
-    const uint64_t a = row.grad2(pair2(__uint_as_float(q.x), __uint_as_float(q.y)));
-    const uint64_t b = row.grad2(pair2(__uint_as_float(q.z), __uint_as_float(q.w)));
-    y = make_uint4(static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32), static_cast<uint32_t>(b),
-                   static_cast<uint32_t>(b >> 32));
-  } else {
-    auto two = [&](uint32_t w) {
-      const uint64_t g = row.grad2(pair2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)));
-      return pack_bf16x2(low2(g), high2(g));
-    };
-    y = make_uint4(two(q.x), two(q.y), two(q.z), two(q.w));
-  }
+  if (sizeof(T) == 4)
+    y = make_uint4(static_cast<uint32_t>(g[0]), static_cast<uint32_t>(g[0] >> 32), static_cast<uint32_t>(g[1]),
+                   static_cast<uint32_t>(g[1] >> 32));
+  else
+    y = make_uint4(pack_bf16x2(low2(g[0]), high2(g[0])), pack_bf16x2(low2(g[1]), high2(g[1])),
+                   pack_bf16x2(low2(g[2 % (PER / 2)]), high2(g[2 % (PER / 2)])),
+                   pack_bf16x2(low2(g[3 % (PER / 2)]), high2(g[3 % (PER / 2)])));
   const unsigned hit = static_cast<unsigned>(row.at - j);
   const float own = hit < PER ? row.grad(score_load(x + row.at), row.at) : 0.f;  // read before an in-place write
   *reinterpret_cast<uint4*>(d + j) = y;

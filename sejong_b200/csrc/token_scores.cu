@@ -19,7 +19,7 @@ namespace {
 constexpr int kScoreMaxTop = 32;
 constexpr int kScoreNarrow = 1024;    // rows of at most this many logits are held by one warp
 constexpr int kScoreThreads = 256;    // of the kernel for wider rows
-constexpr int kScoreCtas = 3, kScoreStages = 3;  // of an SM, of a CTA's ring of 16 KB chunks
+constexpr int kScoreCtas = 4, kScoreStages = 2;  // of an SM, of a CTA's ring of 16 KB chunks
 constexpr int kScoreMaxSplits = 16;
 constexpr int kScoreHeld = kScoreMaxTop * 32 + kScoreMaxTop;  // candidates: the best of 32 threads' 32, and the list
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -367,31 +367,60 @@ struct ScoreBest {
   uint64_t thread_best[kScoreThreads];
   __align__(16) uint32_t group[64];
   uint32_t bar;
-  int kept;
   int count;     // of held
 };
 
-// An order that at least `top` of the CTA's logits reach (a thread gives the largest of its own): the `top`-th
-// largest of 64 groups of four threads, but for its last six bits, which make the groups' values distinct.
-// 0 when fewer than `top` groups hold more than forbidden tokens.
-SJ_DEVICE uint32_t score_bar(ScoreBest& b, uint32_t order, int top) {
-  const int t = threadIdx.x;
+// The bar: an order that at least `top` of the part's logits reach.  64 groups of four threads keep the largest order
+// they have met (its last six bits make the groups' values distinct); the `top`-th largest of them is one.  It
+// only rises, so one that is out of date still holds.  0 when fewer than `top` groups hold more than
+// forbidden tokens.
+SJ_DEVICE uint32_t score_group(ScoreBest& b, uint32_t order) {
   uint32_t g = max(order, __shfl_xor_sync(0xffffffffu, order, 1));
   g = max(g, __shfl_xor_sync(0xffffffffu, g, 2));
-  g = (g & ~63u) | static_cast<uint32_t>(t >> 2);
-  if ((t & 3) == 0) b.group[t >> 2] = g;
+  g = (g & ~63u) | (threadIdx.x >> 2);
+  if ((threadIdx.x & 3) == 0) b.group[threadIdx.x >> 2] = g;
+  return g;
+}
+SJ_DEVICE uint32_t score_bar_of(uint32_t g) { return (g & ~63u) > kForbidden ? g & ~63u : 0u; }
+// By the whole CTA, for a part's first chunk.
+SJ_DEVICE void score_first_bar(ScoreBest& b, uint32_t order, int top) {
+  const uint32_t g = score_group(b, order);
   __syncthreads();
   int rank = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint4 o = reinterpret_cast<const uint4*>(b.group)[i * 4 + (t & 3)];
+    const uint4 o = reinterpret_cast<const uint4*>(b.group)[i * 4 + (threadIdx.x & 3)];
     rank += (o.x > g) + (o.y > g) + (o.z > g) + (o.w > g);
   }
   rank += __shfl_xor_sync(0xffffffffu, rank, 1);
   rank += __shfl_xor_sync(0xffffffffu, rank, 2);
-  if ((t & 3) == 0 && rank == top - 1) b.bar = (g & ~63u) > kForbidden ? g & ~63u : 0u;
+  if ((threadIdx.x & 3) == 0 && rank == top - 1) b.bar = score_bar_of(g);
   __syncthreads();
-  return b.bar;
+}
+// By one warp, whatever the others have come to: a bitonic sort of the groups, two a lane, the largest first.
+SJ_DEVICE void score_raise_bar(ScoreBest& b, int top) {
+  const int lane = threadIdx.x & 31;
+  uint32_t v[2] = {b.group[lane], b.group[lane + 32]};
+#pragma unroll
+  for (int size = 2; size <= 64; size *= 2)
+#pragma unroll
+    for (int step = size / 2; step > 0; step /= 2) {
+      if (step == 32) {
+        const uint32_t high = max(v[0], v[1]);
+        v[1] = min(v[0], v[1]);
+        v[0] = high;
+        continue;
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int at = lane + 32 * r;
+        const uint32_t o = __shfl_xor_sync(0xffffffffu, v[r], step);
+        const bool larger = ((at & step) == 0) == ((at & size) == 0);
+        v[r] = larger ? max(v[r], o) : min(v[r], o);
+      }
+    }
+  const uint32_t g = __shfl_sync(0xffffffffu, v[0], top - 1);
+  if (lane == 0) atomicMax(&b.bar, score_bar_of(g));
 }
 
 // held cut down to its `top` largest keys, in order, which are in list, too; returns how many there are.
@@ -412,26 +441,6 @@ SJ_DEVICE int score_rank(ScoreBest& b, int top) {
   if (threadIdx.x == 0) b.count = kept;
   __syncthreads();
   return kept;
-}
-
-// held without what lies below the bar of the whole part, which is higher than its first chunk's: ranking takes the
-// square of its length.  Left as it is where many are equal.
-SJ_DEVICE void score_sift(ScoreBest& b, uint32_t bar) {
-  const int n = b.count;
-  if (threadIdx.x == 0) b.kept = 0;
-  __syncthreads();
-#pragma unroll 1
-  for (int i = threadIdx.x; i < n; i += kScoreThreads) {
-    const uint64_t key = b.held[i];
-    if (static_cast<uint32_t>(key >> 32) < bar) continue;
-    const int at = atomicAdd(&b.kept, 1);
-    if (at < kScoreThreads) b.thread_best[at] = key;
-  }
-  __syncthreads();
-  const int kept = b.kept;
-  if (kept > kScoreThreads) return;
-  if (threadIdx.x < kept) b.held[threadIdx.x] = b.thread_best[threadIdx.x];
-  if (threadIdx.x == 0) b.count = kept;
 }
 
 // The same where more logits reach the bar than the list holds (equal or rising logits): chunk by chunk, the logits of
@@ -471,12 +480,11 @@ SJ_DEVICE int score_rank_all(ScoreBest& best, const T* x, int base, int end, int
   return n;
 }
 
-// Persistent CTAs over the parts of rows, 16 KB at a time; the next two chunks, of the next part too, are on their way
+// Persistent CTAs over the parts of rows, 16 KB at a time; the next chunk, be it of the next part, is on its way
 // to shared memory meanwhile (cp.async; a thread reads back only what it copied, so copies need no barrier).  The
-// sums are each thread's own until the part's end.  Alternatives: the `top`-th largest of 64 groups' maxima of the
-// first chunk is a bar that at least `top` logits reach; what reaches it (of later chunks, exceeds it)
-// goes to a list that is ranked once at the end: about 24 candidates a chunk at top = 20.  So a part takes
-// two barriers in its first chunk and none in the others.
+// sums are each thread's own until the part's end.  What reaches the bar of the alternatives goes to a list that
+// is ranked at the end (of 50001 logits at top = 20 about 60).  After the two barriers of a part's first bar
+// the warps go on without any; in turn, they raise the bar chunk by chunk.
 template <typename T>
 __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
     token_scores_wide_kernel(const T* logits, int ld, int splits, int parts, int* counters, float* partial,
@@ -489,6 +497,8 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
   __shared__ int s_last;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, top = out.top, vocab = out.vocab;
   const uint32_t stages = smem_u32(ring) + t * 16, count_at = smem_u32(&best.count);
+  uint32_t one;  // not a constant that the compiler sees: it would gather a warp's additions, at more cost than they have
+  asm volatile("mov.u32 %0, 1;" : "=r"(one));
   ScoreWalk<T> ahead(logits, ld, vocab, splits, parts);
   for (int i = 0; i < kScoreStages - 1; ++i) ahead.fetch(stages + i * 16384);
   int stage = 0;
@@ -498,36 +508,38 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
     const T* x = here.x;
     const int r = splits == 1 ? here.part : here.part / splits;
     ScoreSum a{-INFINITY, 0.f, 0.f};
-    uint32_t bar = 0;  // order to exceed, once `raised`
-    bool raised = false;
     for (; here.c < here.c1; ++here.c) {
       const int first = here.base();
       asm volatile("cp.async.wait_group %0;" ::"n"(kScoreStages - 2) : "memory");
       const uint32_t own = stages + stage * 16384;
-      Chunk now;
-      now.read(x, first, vocab, own);
       ahead.fetch(stages + (stage == 0 ? kScoreStages - 1 : stage - 1) * 16384);
       stage = stage == kScoreStages - 1 ? 0 : stage + 1;
-      float most[4];
-      now.largest(most);
-      const float m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-      if (__any_sync(0xffffffffu, m > a.m)) a = score_raise(a, m);
-      const float base = a.m == -INFINITY ? 0.f : a.m;
-      uint64_t s = pair2(a.s, 0.f), u = pair2(a.u, 0.f);
+      float m = -INFINITY, most[4];
+      if (first + warp * 32 * Chunk::PER < vocab) {  // not past the row's end
+        Chunk now;
+        now.read(x, first, vocab, own);
+        now.largest(most);
+        m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+        if (__any_sync(0xffffffffu, m > a.m)) a = score_raise(a, m);
+        const float base = a.m == -INFINITY ? 0.f : a.m;
+        uint64_t s = pair2(a.s, 0.f), u = pair2(a.u, 0.f);
 #pragma unroll
-      for (int i = 0; i < Chunk::N; i += 2) score_add2(pair2(now.at(i), now.at(i + 1)), pair2(-base, -base), s, u);
-      a.s = low2(s) + high2(s);
-      a.u = low2(u) + high2(u);
+        for (int i = 0; i < Chunk::N; i += 2) score_add2(pair2(now.at(i), now.at(i + 1)), pair2(-base, -base), s, u);
+        a.s = low2(s) + high2(s);
+        a.u = low2(u) + high2(u);
+      }
       if (top == 0) continue;
 
       const bool any = Chunk::index(first, 0) < vocab;  // a thread's first element is its lowest
-      const uint32_t order = any ? score_order(m) : 0u;
-      uint32_t reach = raised ? bar + 1 : 0;
-      if (!raised) {
-        reach = bar = score_bar(best, order, top);
-        raised = bar > 0;
+      const uint32_t met = score_order(a.m);  // -inf from nothing: no more than kForbidden
+      if (first == here.start) {
+        score_first_bar(best, met, top);
+      } else {
+        score_group(best, met);
+        if (warp == (here.c & 7)) score_raise_bar(best, top);
       }
-      if (any && order >= reach) {
+      const uint32_t reach = *const_cast<volatile uint32_t*>(&best.bar);
+      if (any && score_order(m) >= reach) {
         // the pieces whose maximum reaches the bar are few: their logits are looked at one by one
         const float least = reach > kForbidden ? score_value(reach) : -INFINITY;
         unsigned hot = 0;
@@ -535,7 +547,7 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
         for (int v = 0; v < 4; ++v) hot |= most[v] >= least ? 1u << v : 0u;
         auto push = [&](float y, int j) {
           int at;
-          asm volatile("atom.shared.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(count_at) : "memory");
+          asm volatile("atom.shared.add.u32 %0, [%1], %2;" : "=r"(at) : "r"(count_at), "r"(one) : "memory");
           if (at < kScoreHeld) best.held[at] = score_key(y, j);
         };
         while (hot) {
@@ -561,7 +573,6 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
     }
 
     // ---- the part's sums and alternatives
-    const uint32_t order = score_order(a.m);
     a = score_lanes_join<32>(a);
     if (lane == 0) sums[warp] = a;
     int n = 0;
@@ -569,7 +580,6 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
     if (top > 0 && best.count > kScoreHeld) {
       n = score_rank_all(best, x, here.start, here.origin + here.c1 * Chunk::SIZE, vocab, top);
     } else if (top > 0) {
-      if (best.count > 64) score_sift(best, score_bar(best, order, top));
       n = score_rank(best, top);
     }
     if (warp == 0) a = score_lanes_join<8>(sums[lane & 7]);  // what follows is warp 0's

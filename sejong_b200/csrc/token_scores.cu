@@ -21,6 +21,8 @@ constexpr int kScoreNarrow = 1024;    // rows of at most this many logits are he
 constexpr int kScoreThreads = 256;    // of the kernel for wider rows
 constexpr int kScoreCtas = 4, kScoreStages = 2;  // of an SM, of a CTA's ring of 16 KB chunks
 constexpr int kScoreMaxSplits = 16;
+constexpr int kGradRows = 4, kGradNarrowCtas = 8, kGradNarrow = 1024;
+constexpr int kGradCtas = 4;          // of an SM, of the gradient's kernel for wide rows
 constexpr int kScoreHeld = kScoreMaxTop * 32 + kScoreMaxTop;  // candidates: the best of 32 threads' 32, and the list
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 }  // namespace
@@ -154,7 +156,7 @@ SJ_DEVICE void score_write_row(const ScoreOut& out, const T* x, int r, const Sco
 // ---------------------------------------------------------------- narrow rows
 // A warp holds a row in R registers a lane: one read, maximum, sums.  Alternatives: the `top`-th largest of the
 // lanes' maxima is a bar that at least `top` logits reach; the few that do (31 are expected at top = 20) are
-// listed and ranked by counting.  Where more than 64 do (ties), each alternative is found by two warp
+// listed and ranked by counting.  Where more than 64 do (ties), or too few are not forbidden, each alternative is found by two warp
 // reductions instead (value, then lowest index).
 template <typename T, int R>
 __global__ void __launch_bounds__(128) token_scores_narrow_kernel(const T* logits, int ld, int rows, ScoreOut out) {
@@ -197,25 +199,26 @@ __global__ void __launch_bounds__(128) token_scores_narrow_kernel(const T* logit
       bar = larger ? max(bar, o) : min(bar, o);
     }
   bar = __shfl_sync(0xffffffffu, bar, out.top - 1);
-  if (bar <= kForbidden) bar = 0;  // fewer than `top` lanes hold more than forbidden tokens
   int n = 0;
+  if (bar > kForbidden) {  // else fewer than `top` lanes hold more than forbidden tokens
+    const float least = score_value(bar);
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const bool hit = i * 32 + lane < out.vocab && score_order(v[i]) >= bar;
-    const uint32_t hits = __ballot_sync(0xffffffffu, hit);
-    const int at = n + __popc(hits & ((1u << lane) - 1));
-    if (hit && at < 64) listed[warp][at] = score_key(v[i], i * 32 + lane);
-    n += __popc(hits);
+    for (int i = 0; i < R; ++i) {
+      const bool hit = v[i] >= least;
+      const uint32_t hits = __ballot_sync(0xffffffffu, hit);
+      if (hits == 0) continue;
+      const int at = n + __popc(hits & ((1u << lane) - 1));
+      if (hit && at < 64) listed[warp][at] = score_key(v[i], i * 32 + lane);
+      n += __popc(hits);
+    }
+    __syncwarp();
   }
-  __syncwarp();
-  if (n <= 64) {
+  if (n > 0 && n <= 64) {
     const uint64_t first = lane < n ? listed[warp][lane] : 0, second = lane + 32 < n ? listed[warp][lane + 32] : 0;
     int rank = 0, rank2 = 0;
-    for (int k = 0; k < n; ++k) {
-      const uint64_t o = listed[warp][k];
-      rank += o > first ? 1 : 0;
-      rank2 += o > second ? 1 : 0;
-    }
+    for (int k = 0; k < n; ++k) rank += listed[warp][k] > first ? 1 : 0;
+    if (n > 32)
+      for (int k = 0; k < n; ++k) rank2 += listed[warp][k] > second ? 1 : 0;
     if (lane < n && rank < out.top) write(rank, first);
     if (lane + 32 < n && rank2 < out.top) write(rank2, second);
     return;
@@ -655,6 +658,16 @@ struct ScoreRow {
     c = z == -INFINITY ? 0.f : in.d_entropy ? -fmaf(b, in.entropy[r], a) : -a;
     b2 = z == -INFINITY ? 0.f : -b * kLn2;
   }
+  SJ_DEVICE ScoreRow() {}
+  SJ_DEVICE ScoreRow of_lane(int i) const {
+    ScoreRow row;
+    row.minus_z = __shfl_sync(0xffffffffu, minus_z, i);
+    row.c = __shfl_sync(0xffffffffu, c, i);
+    row.b2 = __shfl_sync(0xffffffffu, b2, i);
+    row.a = __shfl_sync(0xffffffffu, a, i);
+    row.at = __shfl_sync(0xffffffffu, at, i);
+    return row;
+  }
   SJ_DEVICE uint64_t grad2(uint64_t x) const {
     uint64_t d = mul2(add2(x, pair2(minus_z, minus_z)), pair2(kLog2e, kLog2e));
     d = pair2(floor_exponent(low2(d)), floor_exponent(high2(d)));
@@ -670,85 +683,122 @@ struct ScoreRow {
 SJ_DEVICE void score_store(float* d, float g) { *d = g; }
 SJ_DEVICE void score_store(__nv_bfloat16* d, float g) { *d = f2bf(g); }
 
-// Sixteen bytes of logits, x's columns j and up, to sixteen bytes of gradient.
+// Sixteen bytes of logits to sixteen bytes of gradient, but for the target's own.
 template <typename T>
-SJ_DEVICE void score_grad16(const ScoreRow& row, const uint4& q, const T* x, int j, T* d) {
-  constexpr int PER = 16 / sizeof(T);
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-  auto logits2 = [&](int i) {
-    if (sizeof(T) == 4) return pair2(__uint_as_float(w[2 * i % 4]), __uint_as_float(w[(2 * i + 1) % 4]));
-    return pair2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
-  };
-  uint64_t g[PER / 2];
-#pragma unroll
-  for (int i = 0; i < PER / 2; ++i) g[i] = row.grad2(logits2(i));
-  uint4 y;
-  if (sizeof(T) == 4)
-    y = make_uint4(static_cast<uint32_t>(g[0]), static_cast<uint32_t>(g[0] >> 32), static_cast<uint32_t>(g[1]),
-                   static_cast<uint32_t>(g[1] >> 32));
-  else
-    y = make_uint4(pack_bf16x2(low2(g[0]), high2(g[0])), pack_bf16x2(low2(g[1]), high2(g[1])),
-                   pack_bf16x2(low2(g[2 % (PER / 2)]), high2(g[2 % (PER / 2)])),
-                   pack_bf16x2(low2(g[3 % (PER / 2)]), high2(g[3 % (PER / 2)])));
-  const unsigned hit = static_cast<unsigned>(row.at - j);
-  const float own = hit < PER ? row.grad(score_load(x + row.at), row.at) : 0.f;  // read before an in-place write
-  *reinterpret_cast<uint4*>(d + j) = y;
-  if (hit < PER) score_store(d + row.at, own);
-}
-
-// Pieces k, k + STEP, ... below `end` of row r, four in flight; the first ones on their way before the row's scalars.
-template <typename T, int STEP>
-SJ_DEVICE void score_grad_pieces(const T* x, T* d, int k, int end, bool reports, int r, const ScoreGrad& in) {
-  constexpr int PER = 16 / sizeof(T);
-  uint4 raw[4];
-  auto load = [&](int at) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int j = (at + i * STEP) * PER;
-      raw[i] = make_uint4(0, 0, 0, 0);
-      if (at + i * STEP < end && j + PER <= in.vocab) raw[i] = *reinterpret_cast<const uint4*>(x + j);
-    }
-  };
-  load(k);
-  const ScoreRow row(in, r, reports);
-  for (; k < end; k += 4 * STEP) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int j = (k + i * STEP) * PER;
-      if (k + i * STEP >= end) continue;
-      if (j + PER <= in.vocab) {
-        score_grad16<T>(row, raw[i], x, j, d);
-      } else {
-        for (int at = j; at < j + PER; ++at)
-          score_store(d + at, at < in.vocab ? row.grad(score_load(x + at), at) : 0.f);
-      }
-    }
-    load(k + 4 * STEP);
+SJ_DEVICE uint4 score_grad16(const ScoreRow& row, const uint4& q) {
+  if (sizeof(T) == 4) {
+    const uint64_t a = row.grad2(pair2(__uint_as_float(q.x), __uint_as_float(q.y)));
+    const uint64_t b = row.grad2(pair2(__uint_as_float(q.z), __uint_as_float(q.w)));
+    return make_uint4(static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32), static_cast<uint32_t>(b),
+                      static_cast<uint32_t>(b >> 32));
   }
+  auto two = [&](uint32_t w) {
+    const uint64_t g = row.grad2(pair2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)));
+    return pack_bf16x2(low2(g), high2(g));
+  };
+  return make_uint4(two(q.x), two(q.y), two(q.z), two(q.w));
 }
 
-// Narrow rows on 16-byte boundaries: a warp for a row, four 16-byte pieces a lane in flight; a piece that holds the row's
-// end goes element by element.
+// The two kernels for rows on 16-byte boundaries take the pieces that lie whole in the row as such, and the columns
+// after them one by one.  The target's gradient is computed before anything is written (d may be x) and written
+// last.
+
+// Narrow rows: a warp for four rows, their loads in flight together; lane i looks up row i's scalars.
 template <typename T>
-__global__ void __launch_bounds__(128, 8) token_scores_bwd_narrow_kernel(const T* logits, int ld, T* d_logits, int ldd,
-                                                                         int rows, int per_row, ScoreGrad in) {
+__global__ void __launch_bounds__(128, kGradNarrowCtas) token_scores_bwd_narrow_kernel(const T* logits, int ld, T* d_logits, int ldd,
+                                                                         int rows, ScoreGrad in) {
   pdl_wait();
-  const int r = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (r >= rows) return;
-  score_grad_pieces<T, 32>(logits + static_cast<size_t>(r) * ld, d_logits + static_cast<size_t>(r) * ldd, lane,
-                           per_row, lane == 0, r, in);
+  constexpr int PER = 16 / sizeof(T), ROWS = kGradRows;
+  const int lane = threadIdx.x & 31, r0 = (blockIdx.x * 4 + (threadIdx.x >> 5)) * ROWS, live = min(ROWS, rows - r0);
+  if (live <= 0) return;
+  const int whole = in.vocab / PER;
+  const T* x = logits + static_cast<size_t>(r0) * ld;
+  T* d = d_logits + static_cast<size_t>(r0) * ldd;
+  uint4 raw[ROWS][2];
+  auto load = [&](int k) {
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        raw[i][e] = make_uint4(0, 0, 0, 0);
+        if (i < live && k + e * 32 < whole)
+          raw[i][e] = reinterpret_cast<const uint4*>(x + static_cast<size_t>(i) * ld)[k + e * 32];
+      }
+  };
+  load(lane);
+  const int mine = min(lane, live - 1);
+  const ScoreRow all(in, r0 + mine, lane < live);
+  const T* own_x = x + static_cast<size_t>(mine) * ld;
+  const float own = all.at >= 0 ? all.grad(score_load(own_x + all.at), all.at) : 0.f;
+  __syncwarp();
+  for (int k0 = 0; k0 < whole; k0 += 64) {  // the same for every lane: they exchange the rows' scalars
+    const int k = k0 + lane;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const ScoreRow row = all.of_lane(i);
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (i < live && k + e * 32 < whole)
+          reinterpret_cast<uint4*>(d + static_cast<size_t>(i) * ldd)[k + e * 32] = score_grad16<T>(row, raw[i][e]);
+    }
+    load(k + 64);
+  }
+  for (int i = 0; i < live; ++i) {
+    const ScoreRow row = all.of_lane(i);
+    for (int j = whole * PER + lane; j < ldd; j += 32)
+      score_store(d + static_cast<size_t>(i) * ldd + j,
+                  j < in.vocab ? row.grad(score_load(x + static_cast<size_t>(i) * ld + j), j) : 0.f);
+  }
+  __syncwarp();
+  if (lane < live && all.at >= 0) score_store(d + static_cast<size_t>(lane) * ldd + all.at, own);
 }
 
-// Wide rows on 16-byte boundaries: a CTA for an equal part of a row's pieces.
+// Wide rows: persistent CTAs over parts of 1024 pieces, four pieces a thread; the next part's loads in flight.
 template <typename T>
-__global__ void __launch_bounds__(256, 4) token_scores_bwd_wide_kernel(const T* logits, int ld, T* d_logits, int ldd,
-                                                                       int parts, int per_row, ScoreGrad in) {
+struct ScorePart {
+  static constexpr int PER = 16 / sizeof(T);
+  int r, k;  // row; this thread's first piece
+  uint4 raw[4];
+  SJ_DEVICE void load(const T* logits, int ld, int part, int per_row, int whole) {
+    r = part / per_row;
+    k = (part - r * per_row) * 1024 + static_cast<int>(threadIdx.x);
+    const uint4* src = reinterpret_cast<const uint4*>(logits + static_cast<size_t>(r) * ld) + k;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (k + i * 256 < whole) raw[i] = src[i * 256];
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256, kGradCtas) token_scores_bwd_wide_kernel(const T* logits, int ld, T* d_logits,
+                                                                               int ldd, int parts, int per_row,
+                                                                               ScoreGrad in) {
   pdl_wait();
-  const int r = blockIdx.x / parts, part = blockIdx.x % parts;
-  const int k0 = static_cast<int>(static_cast<int64_t>(per_row) * part / parts);
-  const int k1 = static_cast<int>(static_cast<int64_t>(per_row) * (part + 1) / parts);
-  score_grad_pieces<T, 256>(logits + static_cast<size_t>(r) * ld, d_logits + static_cast<size_t>(r) * ldd,
-                            k0 + static_cast<int>(threadIdx.x), k1, part == 0 && threadIdx.x == 0, r, in);
+  constexpr int PER = 16 / sizeof(T);
+  const int whole = in.vocab / PER;
+  ScorePart<T> next;
+  next.load(logits, ld, blockIdx.x, per_row, whole);
+  for (int part = blockIdx.x; part < parts;) {
+    const ScorePart<T> now = next;
+    part += gridDim.x;
+    const ScoreRow row(in, now.r, now.k == 0);
+    if (part < parts) next.load(logits, ld, part, per_row, whole);
+    const T* x = logits + static_cast<size_t>(now.r) * ld;
+    T* d = d_logits + static_cast<size_t>(now.r) * ldd;
+    const int home = row.at / PER - now.k;  // the target's piece is this thread's
+    const bool owner = row.at >= 0 && row.at < whole * PER && home >= 0 && home < 1024 && home % 256 == 0;
+    const float own = owner ? row.grad(score_load(x + row.at), row.at) : 0.f;
+    uint4* dst = reinterpret_cast<uint4*>(d) + now.k;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (now.k + i * 256 < whole) dst[i * 256] = score_grad16<T>(row, now.raw[i]);
+    if (now.k - static_cast<int>(threadIdx.x) + 1024 >= whole) {  // the row's end
+      const int done = max(now.k - static_cast<int>(threadIdx.x), whole) * PER;
+      for (int j = done + static_cast<int>(threadIdx.x); j < ldd && j < done + 1024 * PER; j += 256)
+        score_store(d + j, j < in.vocab ? row.grad(score_load(x + j), j) : 0.f);
+    }
+    if (owner) score_store(d + row.at, own);
+  }
 }
 
 // Any strides and alignments: a CTA for 2048 elements of a row, side by side.
@@ -760,10 +810,21 @@ __global__ void __launch_bounds__(256) token_scores_bwd_any_kernel(const T* logi
   const ScoreRow row(in, r, j0 == 0 && threadIdx.x == 0);
   const T* x = logits + static_cast<size_t>(r) * ld;
   T* d = d_logits + static_cast<size_t>(r) * ldd;
+  float v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int j = j0 + i * 256 + threadIdx.x;
-    if (j < ldd) score_store(d + j, j < in.vocab ? row.grad(score_load(x + j), j) : 0.f);
+    const int j = j0 + i * 256 + static_cast<int>(threadIdx.x);
+    v[i] = j < in.vocab ? score_load(x + j) : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const uint64_t g = row.grad2(pair2(v[i], v[i + 1]));
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int j = j0 + (i + e) * 256 + static_cast<int>(threadIdx.x);
+      const float y = e ? high2(g) : low2(g);
+      if (j < ldd) score_store(d + j, j < in.vocab ? (j == row.at ? y + row.a : y) : 0.f);
+    }
   }
 }
 
@@ -814,17 +875,18 @@ int scores(const T* logits, int ld, int rows, const ScoreOut& out, void* workspa
 template <typename T>
 int scores_bwd(const T* logits, int ld, T* d_logits, int ldd, int rows, const ScoreGrad& in, cudaStream_t stream) {
   constexpr int PER = 16 / sizeof(T);
+  const int vocab_pieces = in.vocab / PER;
   if (aligned16(logits) && aligned16(d_logits) && ld % PER == 0 && ldd % PER == 0) {
-    const int per_row = ldd / PER;
-    if (per_row <= 256) {
-      launch(token_scores_bwd_narrow_kernel<T>, (rows + 3) / 4, 128, 0, stream, logits, ld, d_logits, ldd, rows,
-             per_row, in);
+    if (vocab_pieces <= kGradNarrow) {
+      launch(token_scores_bwd_narrow_kernel<T>, (rows - 1) / (4 * kGradRows) + 1, 128, 0, stream, logits, ld, d_logits, ldd, rows,
+             in);
     } else {
-      const int parts = (per_row + 2047) / 2048;
-      if (static_cast<int64_t>(rows) * parts > INT_MAX)
+      const int per_row = (ldd / PER + 1023) / 1024;
+      if (static_cast<int64_t>(rows) * per_row > INT_MAX / 2)
         return fail(SJ_ERR_SHAPE, "sj_token_scores_bwd: rows=%d ldd=%d", rows, ldd);
-      launch(token_scores_bwd_wide_kernel<T>, static_cast<unsigned>(rows) * parts, 256, 0, stream, logits, ld, d_logits,
-             ldd, parts, per_row, in);
+      const int parts = rows * per_row;
+      launch(token_scores_bwd_wide_kernel<T>, std::min(parts, kGradCtas * sm_count()), 256, 0, stream, logits, ld,
+             d_logits, ldd, parts, per_row, in);
     }
   } else {
     const int parts = (ldd + 2047) / 2048;

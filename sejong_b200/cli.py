@@ -13,6 +13,9 @@ training step (crates/sejong-cli/src/main.rs:20-164 commands, 165-407 dispatch).
                (crates/sejong-cli/src/benchmark.rs:173-353): out/run-XXX/ and out/benchmark.json.
   init         Initialise a model and save its weights (main.rs:306-318).
   generate     Generate bytes with the KV cache (main.rs:334-390).
+  generate-batch  Generate for every line of a file at once on a paged KV cache; one JSON line each, with the
+               log probabilities of the bytes and their best alternatives if asked for.
+  score        Log probability, entropy and alternatives of every byte of a text file, as JSON.
   inspect      Print a model artifact's configuration and provenance (main.rs:391-405).
 
 Every step runs on the GPU through libsejong_b200.so (ByteTrainer); the host loop only draws batches,
@@ -731,6 +734,44 @@ def generate(model, prompt, max_bytes, temperature, top_k, top_p, seed, raw=Fals
         print(text.decode(errors="replace"))
 
 
+def _score_record(scores):
+    return {"logp": scores.logp, "entropy": scores.entropy,
+            "alternatives": [[[t, p] for t, p in row] for row in scores.alternatives]}
+
+
+def generate_batch(model, prompts, max_bytes, temperature, top_k, top_p, seed, batch, page, pages, top, device=0,
+                   out=None):
+    """Generate for each line of the file `prompts` together; the i-th prompt draws with seed + i."""
+    from . import checkpoint
+    from .generate import Sampling
+    from .serve import BatchGenerator
+    config, params, _, _ = checkpoint.load(model)
+    with open(prompts, "rb") as fh:
+        lines = fh.read().splitlines()
+    gen = BatchGenerator(config, params=params, device=device, batch=batch, page=page, pages=pages)
+    options = [Sampling(temperature=temperature, top_k=top_k, top_p=top_p, seed=seed + i, max_bytes=max_bytes)
+               for i in range(len(lines))]
+    for line, done in zip(lines, gen.generate(lines, options, top=top)):
+        record = {"prompt": line.decode(errors="replace"), "text": done.text.decode(errors="replace"),
+                  "ended": done.ended}
+        if done.scores is not None:
+            record["scores"] = _score_record(done.scores)
+        print(json.dumps(record), file=out or sys.stdout)
+
+
+def score(model, data, top, device=0, out=None):
+    """Scores of the bytes of the file `data`."""
+    from . import checkpoint
+    from .serve import BatchGenerator
+    config, params, _, _ = checkpoint.load(model)
+    with open(data, "rb") as fh:
+        text = fh.read()
+    scores = BatchGenerator(config, params=params, device=device, batch=1, pages=1).score(text, top)
+    total = -sum(scores.logp)
+    print(json.dumps({"bytes": len(text), "bits_per_byte": total / np.log(2.0) / max(len(text), 1),
+                      **_score_record(scores)}), file=out or sys.stdout)
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser(prog="python -m sejong_b200", description="Sejong byte-model training on B200")
     sub = ap.add_subparsers(dest="command", required=True)
@@ -767,6 +808,22 @@ def main(argv=None):
     p.add_argument("--top-p", type=float, default=0.95)
     p.add_argument("--seed", type=int, default=42)
     p.add_argument("--raw", action="store_true")
+    p = sub.add_parser("generate-batch", help="generate for every line of a file together, on a paged KV cache")
+    p.add_argument("--model", required=True)
+    p.add_argument("--prompts", required=True)
+    p.add_argument("--max-bytes", type=int, default=512)
+    p.add_argument("--temperature", type=float, default=0.8)
+    p.add_argument("--top-k", type=int, default=0)
+    p.add_argument("--top-p", type=float, default=0.95)
+    p.add_argument("--seed", type=int, default=42)
+    p.add_argument("--batch", type=int, default=32)
+    p.add_argument("--page", type=int, default=16)
+    p.add_argument("--pages", type=int, default=None)
+    p.add_argument("--alternatives", type=int, default=None, help="score the drawn bytes, with this many alternatives")
+    p = sub.add_parser("score", help="log probabilities of the bytes of a text file")
+    p.add_argument("--model", required=True)
+    p.add_argument("--data", required=True)
+    p.add_argument("--alternatives", type=int, default=0)
     a = ap.parse_args(argv)
     from . import config as cfgmod
     if a.command == "train":
@@ -788,4 +845,9 @@ def main(argv=None):
         inspect(a.model)
     elif a.command == "generate":
         generate(a.model, a.prompt, a.max_bytes, a.temperature, a.top_k, a.top_p, a.seed, a.raw)
+    elif a.command == "generate-batch":
+        generate_batch(a.model, a.prompts, a.max_bytes, a.temperature, a.top_k, a.top_p, a.seed, a.batch, a.page, a.pages,
+                       a.alternatives)
+    elif a.command == "score":
+        score(a.model, a.data, a.alternatives)
     return 0

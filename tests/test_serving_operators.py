@@ -174,3 +174,31 @@ def test_restated_scaled_tables():
     f, _ = opaged.frequencies(64, 10000.0, scaling="base", factor=8.0)
     f0, _ = opaged.frequencies(64, 10000.0)
     assert abs(f[-1] * 8 / f0[-1] - 1) < 1e-12 and f[0] == f0[0]
+
+
+# ---------------------------------------------------------------- the Python layer's own refusals
+def test_batch_generator_refuses_models_it_does_not_serve():
+    from sejong_b200 import model as pm
+    from sejong_b200.serve import BatchGenerator, RopeScaling
+    with pytest.raises(ValueError, match="dense"):
+        BatchGenerator(pm.small_hierarchy())
+    with pytest.raises(ValueError, match="dense"):
+        BatchGenerator(pm.with_(pm.config_c5(), hierarchy=None))
+    for kw in (dict(batch=0), dict(batch=5000), dict(page=0)):
+        with pytest.raises(ValueError, match="batch"):
+            BatchGenerator(pm.config_c1(), **kw)
+    with pytest.raises(ValueError, match="rope scaling"):
+        RopeScaling("cubic", 2.0).code()
+
+
+def test_token_scores_refuses(lib):
+    from sejong_b200.scores import token_scores
+    x, t = torch.zeros(3, 5), torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(ValueError, match="rows"):
+        token_scores(x, t[:2])
+    with pytest.raises(ValueError, match="rows"):
+        token_scores(x[0], t)
+    with pytest.raises(ValueError, match="float32 or bfloat16"):
+        token_scores(x.half(), t)
+    with pytest.raises(ValueError, match="GPU"):
+        token_scores(x, t)

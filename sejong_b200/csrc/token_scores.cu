@@ -511,13 +511,45 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
     const T* x = here.x;
     const int r = splits == 1 ? here.part : here.part / splits;
     ScoreSum a{-INFINITY, 0.f, 0.f};
+    uint32_t noted = 0;  // pieces of up to eight chunks
+    int room = 0;
+    // Files the logits that reach the bar in the noted pieces of the chunk at `base` and the `before` ones before it.
+    auto look = [&](int base, int before, uint32_t pieces) {
+      const uint32_t reach = *const_cast<volatile uint32_t*>(&best.bar);
+      const float least = reach > kForbidden ? score_value(reach) : -INFINITY;
+      auto push = [&](float y, int j) {
+        int at;
+        asm volatile("atom.shared.add.u32 %0, [%1], %2;" : "=r"(at) : "r"(count_at), "r"(one) : "memory");
+        if (at < kScoreHeld) best.held[at] = score_key(y, j);
+      };
+      while (pieces) {
+        const int bit = __ffs(pieces) - 1;
+        pieces &= pieces - 1;
+        const int j0 = Chunk::index(base + (bit / 4 - before) * Chunk::SIZE, bit % 4 * Chunk::PER);
+        if (reach > kForbidden && j0 >= 0 && j0 + Chunk::PER <= vocab) {
+          const uint4 q = *reinterpret_cast<const uint4*>(x + j0);
+#pragma unroll
+          for (int e = 0; e < Chunk::PER; ++e) {
+            const uint32_t w = Chunk::word(q, e * static_cast<int>(sizeof(T)) / 4);
+            const float y = __uint_as_float(sizeof(T) == 4 ? w : e % 2 ? w & 0xffff0000u : w << 16);
+            if (y >= least) push(y, j0 + e);
+          }
+        } else {
+#pragma unroll 1
+          for (int j = max(j0, 0); j < min(j0 + Chunk::PER, vocab); ++j) {
+            const float y = score_load(x + j);
+            if (score_order(y) >= reach) push(y, j);
+          }
+        }
+      }
+    };
     for (; here.c < here.c1; ++here.c) {
       const int first = here.base();
       asm volatile("cp.async.wait_group %0;" ::"n"(kScoreStages - 2) : "memory");
       const uint32_t own = stages + stage * 16384;
       ahead.fetch(stages + (stage == 0 ? kScoreStages - 1 : stage - 1) * 16384);
       stage = stage == kScoreStages - 1 ? 0 : stage + 1;
-      float m = -INFINITY, most[4];
+      float m = -INFINITY, most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       if (first + warp * 32 * Chunk::PER < vocab) {  // not past the row's end
         Chunk now;
         now.read(x, first, vocab, own);
@@ -541,37 +573,18 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
         score_group(best, met);
         if (warp == (here.c & 7)) score_raise_bar(best, top);
       }
+      // the pieces whose maximum reaches the bar are few: they are noted, and looked at once the bar has risen
       const uint32_t reach = *const_cast<volatile uint32_t*>(&best.bar);
-      if (any && score_order(m) >= reach) {
-        // the pieces whose maximum reaches the bar are few: their logits are looked at one by one
-        const float least = reach > kForbidden ? score_value(reach) : -INFINITY;
-        unsigned hot = 0;
+      const float least = reach > kForbidden ? score_value(reach) : -INFINITY;
+      uint32_t hot = 0;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) hot |= most[v] >= least ? 1u << v : 0u;
-        auto push = [&](float y, int j) {
-          int at;
-          asm volatile("atom.shared.add.u32 %0, [%1], %2;" : "=r"(at) : "r"(count_at), "r"(one) : "memory");
-          if (at < kScoreHeld) best.held[at] = score_key(y, j);
-        };
-        while (hot) {
-          const int v = __ffs(hot) - 1, j0 = Chunk::index(first, v * Chunk::PER);
-          hot &= hot - 1;
-          if (reach > kForbidden && j0 >= 0 && j0 + Chunk::PER <= vocab) {
-            const uint4 q = Chunk::piece(own, v);
-#pragma unroll
-            for (int e = 0; e < Chunk::PER; ++e) {
-              const uint32_t w = Chunk::word(q, e * static_cast<int>(sizeof(T)) / 4);
-              const float y = __uint_as_float(sizeof(T) == 4 ? w : e % 2 ? w & 0xffff0000u : w << 16);
-              if (y >= least) push(y, j0 + e);
-            }
-          } else {
-#pragma unroll 1
-            for (int j = max(j0, 0); j < min(j0 + Chunk::PER, vocab); ++j) {
-              const float y = score_load(x + j);
-              if (score_order(y) >= reach) push(y, j);
-            }
-          }
-        }
+      for (int v = 0; v < 4; ++v) hot |= most[v] >= least ? 1u << v : 0u;
+      noted |= (any ? hot : 0u) << room;
+      room += 4;
+      if (room == 32 || here.c + 1 == here.c1) {
+        look(first, room / 4 - 1, noted);
+        noted = 0;
+        room = 0;
       }
     }
 

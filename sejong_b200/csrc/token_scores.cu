@@ -805,7 +805,7 @@ __global__ void __launch_bounds__(256, kGradCtas) token_scores_bwd_wide_kernel(c
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (now.k + i * 256 < whole) dst[i * 256] = score_grad16<T>(row, now.raw[i]);
-    if (now.k - static_cast<int>(threadIdx.x) + 1024 >= whole) {  // the row's end
+    if (now.k - static_cast<int>(threadIdx.x) + 1024 > whole) {  // the row's end, which one part takes
       const int done = max(now.k - static_cast<int>(threadIdx.x), whole) * PER;
       for (int j = done + static_cast<int>(threadIdx.x); j < ldd && j < done + 1024 * PER; j += 256)
         score_store(d + j, j < in.vocab ? row.grad(score_load(x + j), j) : 0.f);

@@ -221,6 +221,19 @@ def test_gradient_matches_the_restatement(rows, vocab, ld, ldd, kind):
         check_gradient(x, target, vocab, ldd, a, b, in_place=True)
 
 
+@pytest.mark.parametrize("kind,vocab", [(torch.float32, 8193), (torch.float32, 12291), (torch.bfloat16, 16385),
+                                        (torch.float32, 4097), (torch.bfloat16, 8195)])
+def test_gradient_in_place_where_a_part_ends_with_the_whole_pieces(kind, vocab):
+    """The columns after the last whole 16 bytes are read and written by one CTA alone."""
+    ld = -(-vocab // 8) * 8 + 8
+    x, target = logits(40, vocab, ld, kind, vocab)
+    target[:20] = vocab - 1
+    gen = torch.Generator().manual_seed(vocab)
+    a, b = (torch.randn(40, generator=gen).to(DEV) for _ in range(2))
+    for _ in range(5):
+        check_gradient(x, target, vocab, ld, a, b, in_place=True)
+
+
 @pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
 def test_gradient_of_masked_rows(kind):
     gen = torch.Generator().manual_seed(2)

@@ -846,8 +846,8 @@ def main(argv=None):
     elif a.command == "generate":
         generate(a.model, a.prompt, a.max_bytes, a.temperature, a.top_k, a.top_p, a.seed, a.raw)
     elif a.command == "generate-batch":
-        generate_batch(a.model, a.prompts, a.max_bytes, a.temperature, a.top_k, a.top_p, a.seed, a.batch, a.page, a.pages,
-                       a.alternatives)
+        generate_batch(a.model, a.prompts, a.max_bytes, a.temperature, a.top_k, a.top_p, a.seed, a.batch, a.page,
+                       a.pages, a.alternatives)
     elif a.command == "score":
         score(a.model, a.data, a.alternatives)
     return 0

@@ -22,8 +22,8 @@
 //
 // Measured on B200 (graph replays; the caches are larger than L2): 256 rows of 512 to 16384 keys, 12 / 4 heads of 64:
 // 189 us, 6.35 TB/s of 1.2 GB (97% of the measured copy rate); two rows of 150 and 200 thousand keys, 16 / 4 heads:
-// 64 us, 5.6 TB/s; 64 rows of 4 to 9 thousand keys, 16 / 2 heads of 128: 72 us, 5.6 TB/s.  The first simple kernel (a CTA
-// for each row and query head) took 4730 us and 49200 us on the first two; K and V loaded straight into
+// 64 us, 5.6 TB/s; 64 rows of 4 to 9 thousand keys, 16 / 2 heads of 128: 72 us, 5.6 TB/s.  The first simple kernel
+// (a CTA for each row and query head) took 4730 us and 49200 us on the first two; K and V loaded straight into
 // registers, 203 and 71 us (no copies in flight while a warp computes); 16- and 24-warp CTAs, one an SM, 10 to
 // 20% more (all wait for the slowest warp at a unit's end); a last fifth of the tiles dealt to whoever is
 // done first: the same.

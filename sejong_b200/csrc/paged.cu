@@ -90,7 +90,8 @@ SJ_DEVICE int owner_of(const int* start, int n, int i) {
 // Request b holds H_b = ceil(cached_b / page) pages and needs N_b = ceil((cached_b + added_b) / page);
 // the i-th new page, requests in order, is the i-th from the top of the free stack.  Every CTA scans
 // the batch for itself (a few KB out of L2) and writes its share of the rows and new table entries,
-// so one launch does it all without a grid-wide wait.
+// so one launch does it all without a grid-wide wait.  Bound by latency: a launch, three dependent look-ups and the
+// scan (64 requests 4.3 us, 1021 requests with 50000 rows 5.3; graph replays).
 __global__ void __launch_bounds__(1024) paged_plan_kernel(const int32_t* cached, const int32_t* added, int batch,
                                                           int page, const int32_t* free_pages,
                                                           const int32_t* free_count, int32_t* table, int ld_table,

@@ -6,6 +6,13 @@
 //
 // The alternatives are the `top` largest logits, the lowest index first among equal ones: a key of
 // (value, ~index) orders them without ties.
+//
+// Each logit is read once from memory.  Measured on B200 (graph replays): 2048 x 50001 bf16 with 20 alternatives 71 us
+// (2.9 TB/s; without alternatives 50), where the exponentials (the special-function unit takes a warp's in 8
+// cycles), the unpacking and the alternatives bound it, not memory: 470 instructions a warp and 1024 logits; 1024 x
+// 50001 f32 37.6 us without alternatives (5.4 TB/s).  The first simple kernel (a pass for the maximum, one for the
+// sums, one for each alternative) took 1629.  Gradient: 2048 x 65537 bf16 91 us (5.9 TB/s), 1024 x 50001 f32 69 us
+// (6.0).
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -19,10 +26,17 @@ namespace {
 constexpr int kScoreMaxTop = 32;
 constexpr int kScoreNarrow = 1024;    // rows of at most this many logits are held by one warp
 constexpr int kScoreThreads = 256;    // of the kernel for wider rows
-constexpr int kScoreCtas = 4, kScoreStages = 2;  // of an SM, of a CTA's ring of 16 KB chunks
+// CTAs of an SM, stages of a CTA's ring of 16 KB chunks: 2048 x 50001 bf16, 20 alternatives, 89 us with three CTAs of
+// three stages, 79 with four of two, 90 with five of two (48 registers spill); then 71 by other steps.
+constexpr int kScoreCtas = 4, kScoreStages = 2;
 constexpr int kScoreMaxSplits = 16;
+// The gradient of rows of at most 1024 pieces of 16 bytes: four rows a warp (32768 x 257 f32 16.3 us with eight CTAs of
+// four warps an SM, 18.4 with six; 8192 x 2000 f32 25.8 us, 36.7 by the kernel for wide rows).
 constexpr int kGradRows = 4, kGradNarrowCtas = 8, kGradNarrow = 1024;
-constexpr int kGradCtas = 4;          // of an SM, of the gradient's kernel for wide rows
+// CTAs of an SM, of the gradient's kernel for wide rows: 2048 x 65537 bf16 94.3 us with four, 90.9 with five, 95.8 with
+// six; 1024 x 50001 f32 68.9, 70.9, 72.7.
+template <typename T>
+constexpr int kGradCtas = sizeof(T) == 2 ? 5 : 4;
 constexpr int kScoreHeld = kScoreMaxTop * 32 + kScoreMaxTop;  // candidates: the best of 32 threads' 32, and the list
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 }  // namespace
@@ -156,8 +170,8 @@ SJ_DEVICE void score_write_row(const ScoreOut& out, const T* x, int r, const Sco
 // ---------------------------------------------------------------- narrow rows
 // A warp holds a row in R registers a lane: one read, maximum, sums.  Alternatives: the `top`-th largest of the
 // lanes' maxima is a bar that at least `top` logits reach; the few that do (31 are expected at top = 20) are
-// listed and ranked by counting.  Where more than 64 do (ties), or too few are not forbidden, each alternative is found by two warp
-// reductions instead (value, then lowest index).
+// listed and ranked by counting.  Where more than 64 do (ties), or too few are not forbidden, each alternative
+// is found by two warp reductions instead (value, then lowest index).
 template <typename T, int R>
 __global__ void __launch_bounds__(128) token_scores_narrow_kernel(const T* logits, int ld, int rows, ScoreOut out) {
   pdl_wait();
@@ -500,7 +514,7 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
   __shared__ int s_last;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, top = out.top, vocab = out.vocab;
   const uint32_t stages = smem_u32(ring) + t * 16, count_at = smem_u32(&best.count);
-  uint32_t one;  // not a constant that the compiler sees: it would gather a warp's additions, at more cost than they have
+  uint32_t one;  // not a constant that the compiler sees: gathering a warp's additions costs more than they do
   asm volatile("mov.u32 %0, 1;" : "=r"(one));
   ScoreWalk<T> ahead(logits, ld, vocab, splits, parts);
   for (int i = 0; i < kScoreStages - 1; ++i) ahead.fetch(stages + i * 16384);
@@ -718,8 +732,8 @@ SJ_DEVICE uint4 score_grad16(const ScoreRow& row, const uint4& q) {
 
 // Narrow rows: a warp for four rows, their loads in flight together; lane i looks up row i's scalars.
 template <typename T>
-__global__ void __launch_bounds__(128, kGradNarrowCtas) token_scores_bwd_narrow_kernel(const T* logits, int ld, T* d_logits, int ldd,
-                                                                         int rows, ScoreGrad in) {
+__global__ void __launch_bounds__(128, kGradNarrowCtas)
+    token_scores_bwd_narrow_kernel(const T* logits, int ld, T* d_logits, int ldd, int rows, ScoreGrad in) {
   pdl_wait();
   constexpr int PER = 16 / sizeof(T), ROWS = kGradRows;
   const int lane = threadIdx.x & 31, r0 = (blockIdx.x * 4 + (threadIdx.x >> 5)) * ROWS, live = min(ROWS, rows - r0);
@@ -783,9 +797,8 @@ struct ScorePart {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(256, kGradCtas) token_scores_bwd_wide_kernel(const T* logits, int ld, T* d_logits,
-                                                                               int ldd, int parts, int per_row,
-                                                                               ScoreGrad in) {
+__global__ void __launch_bounds__(256, kGradCtas<T>)
+    token_scores_bwd_wide_kernel(const T* logits, int ld, T* d_logits, int ldd, int parts, int per_row, ScoreGrad in) {
   pdl_wait();
   constexpr int PER = 16 / sizeof(T);
   const int whole = in.vocab / PER;
@@ -891,14 +904,14 @@ int scores_bwd(const T* logits, int ld, T* d_logits, int ldd, int rows, const Sc
   const int vocab_pieces = in.vocab / PER;
   if (aligned16(logits) && aligned16(d_logits) && ld % PER == 0 && ldd % PER == 0) {
     if (vocab_pieces <= kGradNarrow) {
-      launch(token_scores_bwd_narrow_kernel<T>, (rows - 1) / (4 * kGradRows) + 1, 128, 0, stream, logits, ld, d_logits, ldd, rows,
-             in);
+      launch(token_scores_bwd_narrow_kernel<T>, (rows - 1) / (4 * kGradRows) + 1, 128, 0, stream, logits, ld, d_logits,
+             ldd, rows, in);
     } else {
       const int per_row = (ldd / PER + 1023) / 1024;
       if (static_cast<int64_t>(rows) * per_row > INT_MAX / 2)
         return fail(SJ_ERR_SHAPE, "sj_token_scores_bwd: rows=%d ldd=%d", rows, ldd);
       const int parts = rows * per_row;
-      launch(token_scores_bwd_wide_kernel<T>, std::min(parts, kGradCtas * sm_count()), 256, 0, stream, logits, ld,
+      launch(token_scores_bwd_wide_kernel<T>, std::min(parts, kGradCtas<T> * sm_count()), 256, 0, stream, logits, ld,
              d_logits, ldd, parts, per_row, in);
     }
   } else {

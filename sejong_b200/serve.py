@@ -191,7 +191,8 @@ class BatchGenerator:
 
     def _head(self, first, rows, out):
         d = self.s.width
-        self._gemm(_ptr(self.z, first * d), d, self._wb("output"), VOCAB_PAD, _ptr(out), VOCAB_PAD, SJ_F32, rows, VOCAB, d)
+        self._gemm(_ptr(self.z, first * d), d, self._wb("output"), VOCAB_PAD, _ptr(out), VOCAB_PAD, SJ_F32, rows, VOCAB,
+                   d)
 
     def _prompt(self, n, file):
         """Rows 0 .. n - 1 at positions 0 .. n - 1 through the blocks; their keys and values filed when `file`."""

@@ -2,8 +2,8 @@
 (exact), scaled rotary tables, the rotary append and the attention over pages.
 
 Bounds, from the arithmetic.  A bf16 has 8 significant bits, so a rounding to it is at most 2^-8 of the
-value.  Append: two f32 products, a sum and one bf16 rounding.  Attention: products of bf16 are exact in f32 and a score sums `dim` of them, so
-it is off by at most (dim + 8) 2^-24 sum |q_i k_i| / sqrt(dim) (the eight covers the scaling and the shift by
+value.  Append: two f32 products, a sum and one bf16 rounding.  Attention: products of bf16 are exact in f32
+and a score sums `dim` of them, so it is off by at most (dim + 8) 2^-24 sum |q_i k_i| / sqrt(dim) (the eight covers the scaling and the shift by
 the maximum); the probabilities are rounded to bf16 for the product with V (2^-8 of each weight, and
 another 2^-9 for the f32 exponentials, sums and the scores' error at the sizes here) and the result
 once more.

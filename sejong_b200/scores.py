@@ -45,8 +45,8 @@ class _Scores(torch.autograd.Function):
         d_logp, d_entropy = d_logp.float().contiguous(), d_entropy.float().contiguous()
         out = torch.empty(rows, vocab, dtype=logits.dtype, device=logits.device)
         call("sj_token_scores_bwd", logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), targets.data_ptr(),
-             rows, vocab, lse.data_ptr(), entropy.data_ptr(), d_logp.data_ptr(), d_entropy.data_ptr(), out.data_ptr(), vocab,
-             _stream(logits))
+             rows, vocab, lse.data_ptr(), entropy.data_ptr(), d_logp.data_ptr(), d_entropy.data_ptr(), out.data_ptr(),
+             vocab, _stream(logits))
         return out, None, None
 
 

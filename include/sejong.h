@@ -353,7 +353,7 @@ int sj_scale_to_bf16(const float* x, int n, float alpha, void* y, void* stream);
  *                    [batch], batch <= 4096).  New pages come from the top of a stack: the i-th, requests in
  *                    order, is free_pages[*free_count - 1 - i], entered into block_table.  lengths[b] =
  *                    cached[b] + added[b]; row r (requests in order, tokens in order) of the step has
- *                    request[r], position[r] and slot[r]; rows past the step's last, up to `rows` (<= 2^19),
+ *                    request[r], position[r] and slot[r]; rows past the step's last, up to `rows` (< 2^19),
  *                    get -1 in all three, so a captured graph of fixed size can run a step of any size.
  *                    summary (int32 [4]) = {rows, pages taken, status, pages left}.  status 0: planned; 1:
  *                    more than `rows` rows; 2: too few free pages; 3: ld_table too small; 4: a negative or

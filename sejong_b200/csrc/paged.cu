@@ -20,7 +20,7 @@
 namespace sj {
 
 namespace {
-constexpr int kPlanMaxBatch = 4096, kPlanMaxRows = 1 << 19;
+constexpr int kPlanMaxBatch = 4096, kPlanMaxRows = (1 << 19) - 1;  // their product fits 31 bits, so sums do
 constexpr int kPlanRowsOver = 1, kPlanNoPages = 2, kPlanTableNarrow = 3, kPlanBadCount = 4;
 }  // namespace
 

@@ -91,8 +91,8 @@ class BatchGenerator:
         self.lib = _lib.load()
         call("sj_device_init", self.dev.index)
         self.context, self.batch, self.page = L, B, P = int(context or c.context), int(batch), int(page)
-        if not 0 < L <= 1 << 19:
-            raise ValueError("the context must be 1 to 524288")
+        if not 0 < L < 1 << 19:
+            raise ValueError("the context must be 1 to 524287")
         self.width = -(-L // P)
         self.pages = int(pages or B * self.width)
         if self.pages < 1:

@@ -144,6 +144,15 @@ def test_plan_refuses_as_a_whole(cached, added, rows, width, spare, status):
     assert p.summary.tolist() == [0, 0, status, len(p.free0)]
 
 
+def test_plan_of_the_largest_counts():
+    """4096 requests that each ask for as many rows as a plan can have: refused, although the sum fills 31 bits."""
+    most = (1 << 19) - 1
+    p = Planner(np.zeros(4096), np.full(4096, most), 1, 4, 2, most)
+    p.plan()
+    assert p.summary.tolist() == [0, 0, 1, 4]
+    assert (p.maps[0] == -1).all() and (p.lengths == 0).all()
+
+
 def test_commit_takes_and_returns_pages():
     """Steps with growing and finishing requests: no page is ever held twice or lost."""
     rng = np.random.default_rng(4)

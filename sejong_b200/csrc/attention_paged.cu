@@ -42,8 +42,9 @@ constexpr int kTile = 128;                   // keys of a tile
 // short rows: 8.0 against 5.2 us).
 constexpr int kWhole = 2;
 // More parts than kGroup are joined in groups of about their square root: 444 parts of one unit by one CTA took 80 us,
-// in two levels 9; 14 parts of 32 units took 2 us more in two levels than in one.
-constexpr int kGroup = 20;
+// in two levels 9; 14 parts of 32 units took 2 us more in two levels than in one.  A group has at most kGroupMost
+// parts: 1024 CTAs would be 32 groups of 32.
+constexpr int kGroup = 20, kGroupMost = 64;
 constexpr int kWarps = 4, kCtas = 3, kStages = 2;  // of a CTA, of an SM, of a warp's ring
 constexpr int kLastPosition = INT_MAX - 4096;  // key indices step past the end by less than this
 constexpr uint32_t kNoKey = 0xffffffffu;     // past any offset: buffers hold at most 2^32 16-byte chunks
@@ -124,48 +125,65 @@ struct Cut {
 };
 SJ_DEVICE int span_tiles(int lo, int n) { return max(1, (n - lo + kTile - 1) / kTile); }
 
-// Parts first, first + stride, ... (count <= 32 of them) of a unit added in that order by the whole CTA, left
+// Parts first, first + stride, ... (count <= kGroupMost of them) of a unit added in that order by the whole CTA, left
 // unnormalised in shared memory: sm[q] the maxima, sl[q] the sums, and the outputs as float4 [heads * DIM /
-// 4] in `sums`.  Each lane of a query's warp takes one part's maximum and sum; then a thread adds four
-// dims of one query over every `shares`-th part, the loads of four parts in flight at a time.
+// 4] in `sums`.  A query's warp takes its maxima and sums, one or two parts a lane; a thread adds four dims of one
+// query over every `shares`-th part, eight parts' loads in flight, the first ones before the weights are known.  Not
+// inlined: its registers would push the main loop's into memory (193 instead of 187 us at 256 ragged rows, 135 instead of 81 at 16 heads of 128).
 template <int DIM, int Q, int WARPS>
-SJ_DEVICE void join_parts(const float* partial, int from, int first, int count, int stride, int heads, float* sm,
-                          float* sl, float (*weight)[Q], float4* sums) {
+__device__ __noinline__ void join_parts(const float* partial, int from, int first, int count, int stride, int heads,
+                                        float* sm, float* sl, float (*weight)[Q], float4* sums) {
   constexpr int SLOT = Q * (DIM + 2), THREADS = WARPS * 32;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  auto slot_of = [&](int i) {
-    const int w = first + i * stride;
-    return partial + (static_cast<size_t>(w) * 2 + (w == from ? 1 : 0)) * SLOT;
+  const int items = heads * (DIM / 4), shares = max(1, min(count, THREADS / items));
+  auto slot_of = [&](int k) {
+    const int at = first + k * stride;
+    return partial + (at * 2 + (at == from ? 1 : 0)) * static_cast<size_t>(SLOT);
   };
+  float4 x[8];
+  auto fetch = [&](int i, int w) {
+    const int item = i % items, at = 2 * Q + item / (DIM / 4) * DIM + item % (DIM / 4) * 4;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int k = min(w + e * shares, count - 1);
+      x[e] = __ldcg(reinterpret_cast<const float4*>(slot_of(k) + at));
+    }
+  };
+  int i = t;
+  if (i < items * shares) fetch(i, i / items);
 #pragma unroll 1
   for (int qi = warp; qi < heads; qi += WARPS) {
-    const float m = lane < count ? __ldcg(slot_of(lane) + qi) : -INFINITY;
-    const float l = lane < count ? __ldcg(slot_of(lane) + Q + qi) : 0.f;
-    const float top = warp_max(m), f = exp2_fast(m - (top == -INFINITY ? 0.f : top));
-    const float sum = warp_sum(f * l);
-    weight[lane][qi] = f;
+    float m[2], l[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const bool is = lane + 32 * e < count;
+      m[e] = is ? __ldcg(slot_of(lane + 32 * e) + qi) : -INFINITY;
+      l[e] = is ? __ldcg(slot_of(lane + 32 * e) + Q + qi) : 0.f;
+    }
+    const float top = warp_max(fmaxf(m[0], m[1])), ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float f = exp2_fast(m[e] - ref);
+      sum += f * l[e];
+      if (lane + 32 * e < kGroupMost) weight[lane + 32 * e][qi] = f;
+    }
+    sum = warp_sum(sum);
     if (lane == 0) {
       sm[qi] = top;
       sl[qi] = sum;
     }
   }
   __syncthreads();
-  const int items = heads * (DIM / 4), shares = max(1, min(count, THREADS / items));
 #pragma unroll 1
-  for (int i = t; i < items * shares; i += THREADS) {
-    const int item = i % items, qi = item / (DIM / 4), d = item % (DIM / 4) * 4;
+  while (i < items * shares) {
+    const int qi = i % items / (DIM / 4);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    const float4* src = reinterpret_cast<const float4*>(partial + 2 * Q + qi * DIM + d);
 #pragma unroll 1
-    for (int w = i / items; w < count; w += 4 * shares) {
-      float4 x[4];
+    for (int w = i / items; w < count; w += 8 * shares) {
+      if (w >= shares) fetch(i, w);  // the first eight are here
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int k = min(w + e * shares, count - 1), at = first + k * stride;
-        x[e] = __ldcg(src + (at * 2 + (at == from ? 1 : 0)) * (SLOT / 4));
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < 8; ++e) {
         const float f = w + e * shares < count ? weight[w + e * shares][qi] : 0.f;
         if (f != 0.f) {
           acc.x += f * x[e].x;
@@ -176,24 +194,34 @@ SJ_DEVICE void join_parts(const float* partial, int from, int first, int count, 
       }
     }
     sums[i] = acc;
+    i += THREADS;
+    if (i < items * shares) fetch(i, i / items);
   }
   __syncthreads();
   if (shares > 1) {
 #pragma unroll 1
-    for (int i = t; i < items; i += THREADS) {
-      float4 out = sums[i];
+    for (int k = t; k < items; k += THREADS) {
+      float4 out = sums[k];
 #pragma unroll 1
       for (int w = 1; w < shares; ++w) {
-        const float4 x = sums[w * items + i];
-        out.x += x.x;
-        out.y += x.y;
-        out.z += x.z;
-        out.w += x.w;
+        const float4 y = sums[w * items + k];
+        out.x += y.x;
+        out.y += y.y;
+        out.z += y.z;
+        out.w += y.w;
       }
-      sums[i] = out;
+      sums[k] = out;
     }
     __syncthreads();
   }
+}
+
+// One more on a counter, after what the CTA's threads have written (and a barrier has passed on to this one), and before
+// what they read from others.
+SJ_DEVICE int arrive(int* counter) {
+  int before;
+  asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+  return before;
 }
 
 // DIM: head_dim; NQ: query tiles of 8 that a unit holds (a query's columns of S^T; 2 above 8 heads a KV head).
@@ -210,7 +238,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attn_paged_kernel(const Pa
   extern __shared__ uint8_t unaligned[];
   uint8_t* smem = unaligned + (-smem_u32(unaligned) & 127);
   float* so = reinterpret_cast<float*>(smem);  // [WARPS][Q][LD], once a unit's stages are read
-  __shared__ float sm[WARPS][Q], sl[WARPS][Q], weight[32][Q];
+  __shared__ float sm[WARPS][Q], sl[WARPS][Q], weight[kGroupMost][Q];
   __shared__ unsigned long long scan[WARPS], s_base;
   __shared__ int s_row, s_last;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = lane >> 2, c = lane & 3;
@@ -535,10 +563,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attn_paged_kernel(const Pa
         auto last_of = [&](int* counter, int expected) {
           __syncthreads();
           if (t == 0) {
-            __threadfence();
-            s_last = atomicAdd(counter, 1) == expected - 1;
+            s_last = arrive(counter) == expected - 1;
             if (s_last) *counter = 0;
-            __threadfence();
           }
           __syncthreads();
           return s_last != 0;

@@ -44,7 +44,7 @@ constexpr int kWhole = 2;
 // More parts than kGroup are joined in groups of about their square root: 444 parts of one unit by one CTA took 80 us,
 // in two levels 9; 14 parts of 32 units took 2 us more in two levels than in one.  A group has at most kGroupMost
 // parts: 1024 CTAs would be 32 groups of 32.
-constexpr int kGroup = 20, kGroupMost = 64;
+constexpr int kGroup = 20, kGroupMost = 32;
 constexpr int kWarps = 4, kCtas = 3, kStages = 2;  // of a CTA, of an SM, of a warp's ring
 constexpr int kLastPosition = INT_MAX - 4096;  // key indices step past the end by less than this
 constexpr uint32_t kNoKey = 0xffffffffu;     // past any offset: buffers hold at most 2^32 16-byte chunks
@@ -126,15 +126,16 @@ struct Cut {
 SJ_DEVICE int span_tiles(int lo, int n) { return max(1, (n - lo + kTile - 1) / kTile); }
 
 // Parts first, first + stride, ... (count <= kGroupMost of them) of a unit added in that order by the whole CTA, left
-// unnormalised in shared memory: sm[q] the maxima, sl[q] the sums, and the outputs as float4 [heads * DIM /
-// 4] in `sums`.  A query's warp takes its maxima and sums, one or two parts a lane; a thread adds four dims of one
-// query over every `shares`-th part, eight parts' loads in flight, the first ones before the weights are known.  Not
-// inlined: its registers would push the main loop's into memory (193 instead of 187 us at 256 ragged rows, 135 instead of 81 at 16 heads of 128).
+// unnormalised in shared memory: sm[q] the maxima, sl[q] the sums, and the outputs as float4 [heads * DIM / 4] in
+// `sums`.  Eight threads take a query's maxima and sums; a thread adds four dims of one query over every
+// `shares`-th part, eight parts' loads in flight, the first ones before the weights are known.  Not inlined: its
+// registers would push the main loop's into memory (193 instead of 187 us at 256 ragged rows, 135 instead of 81 at
+// 16 heads of 128).
 template <int DIM, int Q, int WARPS>
 __device__ __noinline__ void join_parts(const float* partial, int from, int first, int count, int stride, int heads,
                                         float* sm, float* sl, float (*weight)[Q], float4* sums) {
   constexpr int SLOT = Q * (DIM + 2), THREADS = WARPS * 32;
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int t = threadIdx.x;
   const int items = heads * (DIM / 4), shares = max(1, min(count, THREADS / items));
   auto slot_of = [&](int k) {
     const int at = first + k * stride;
@@ -151,25 +152,30 @@ __device__ __noinline__ void join_parts(const float* partial, int from, int firs
   };
   int i = t;
   if (i < items * shares) fetch(i, i / items);
-#pragma unroll 1
-  for (int qi = warp; qi < heads; qi += WARPS) {
-    float m[2], l[2];
+  static_assert(THREADS >= Q * 8 && kGroupMost == 32, "eight threads a query, four parts a thread");
+  {
+    const int qi = t >> 3;
+    float m[4], l[4], top = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const bool is = lane + 32 * e < count;
-      m[e] = is ? __ldcg(slot_of(lane + 32 * e) + qi) : -INFINITY;
-      l[e] = is ? __ldcg(slot_of(lane + 32 * e) + Q + qi) : 0.f;
+    for (int e = 0; e < 4; ++e) {
+      const int k = (t & 7) + 8 * e;
+      const bool is = qi < heads && k < count;
+      m[e] = is ? __ldcg(slot_of(k) + qi) : -INFINITY;
+      l[e] = is ? __ldcg(slot_of(k) + Q + qi) : 0.f;
+      top = fmaxf(top, m[e]);
     }
-    const float top = warp_max(fmaxf(m[0], m[1])), ref = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
       const float f = exp2_fast(m[e] - ref);
       sum += f * l[e];
-      if (lane + 32 * e < kGroupMost) weight[lane + 32 * e][qi] = f;
+      if (qi < heads) weight[(t & 7) + 8 * e][qi] = f;
     }
-    sum = warp_sum(sum);
-    if (lane == 0) {
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (qi < heads && (t & 7) == 0) {
       sm[qi] = top;
       sl[qi] = sum;
     }
@@ -216,7 +222,7 @@ __device__ __noinline__ void join_parts(const float* partial, int from, int firs
   }
 }
 
-// One more on a counter, after what the CTA's threads have written (and a barrier has passed on to this one), and before
+// One more on a counter, after what the CTA's threads have written (a barrier has passed it on to this one) and before
 // what they read from others.
 SJ_DEVICE int arrive(int* counter) {
   int before;

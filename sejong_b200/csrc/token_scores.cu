@@ -7,10 +7,10 @@
 // The alternatives are the `top` largest logits, the lowest index first among equal ones: a key of
 // (value, ~index) orders them without ties.
 //
-// Each logit is read once from memory.  Measured on B200 (graph replays): 2048 x 50001 bf16 with 20 alternatives 71 us
-// (2.9 TB/s; without alternatives 50), where the exponentials (the special-function unit takes a warp's in 8
-// cycles), the unpacking and the alternatives bound it, not memory: 470 instructions a warp and 1024 logits; 1024 x
-// 50001 f32 37.6 us without alternatives (5.4 TB/s).  The first simple kernel (a pass for the maximum, one for the
+// Each logit is read once from memory.  Measured on B200 (graph replays): 2048 x 50001 bf16 with 20 alternatives 67 us
+// (3.1 TB/s; without alternatives 45), where the exponentials (the special-function unit takes a warp's in 8
+// cycles), the unpacking and the alternatives bound it, not memory: about 450 instructions a warp and 1024 logits;
+// 1024 x 50001 f32 47 us (4.4 TB/s).  The first simple kernel (a pass for the maximum, one for the
 // sums, one for each alternative) took 1629.  Gradient: 2048 x 65537 bf16 91 us (5.9 TB/s), 1024 x 50001 f32 69 us
 // (6.0).
 #include <algorithm>
@@ -25,10 +25,14 @@ namespace sj {
 namespace {
 constexpr int kScoreMaxTop = 32;
 constexpr int kScoreNarrow = 1024;    // rows of at most this many logits are held by one warp
-constexpr int kScoreThreads = 256;    // of the kernel for wider rows
-// CTAs of an SM, stages of a CTA's ring of 16 KB chunks: 2048 x 50001 bf16, 20 alternatives, 89 us with three CTAs of
-// three stages, 79 with four of two, 90 with five of two (48 registers spill); then 71 by other steps.
-constexpr int kScoreCtas = 4, kScoreStages = 2;
+constexpr int kScoreThreads = 128, kScoreWarps = kScoreThreads / 32;  // of the kernel for wider rows
+constexpr int kScorePieces = 5;       // 16-byte pieces of a chunk that a thread takes
+constexpr int kScoreStage = kScoreThreads * kScorePieces * 16;
+// CTAs of an SM, stages of a CTA's ring.  Small CTAs and small chunks waste less of a row's last chunk, many pieces a
+// thread spread a chunk's fixed cost: with 128 threads, five pieces and seven CTAs, 2048 x 50001 bf16 with 20
+// alternatives takes 66.8 us and 8000 x 2000 f32 45.6; with 256, four and four, 71.2 and 71.8; 128, four and eight,
+// 73.8 and 42.3; 128, eight and five, 73.8; 64, eight and nine, 78.9.
+constexpr int kScoreCtas = 7, kScoreStages = 2;
 constexpr int kScoreMaxSplits = 16;
 // The gradient of rows of at most 1024 pieces of 16 bytes: four rows a warp (32768 x 257 f32 16.3 us with eight CTAs of
 // four warps an SM, 18.4 with six; 8192 x 2000 f32 25.8 us, 36.7 by the kernel for wide rows).
@@ -260,11 +264,11 @@ __global__ void __launch_bounds__(128) token_scores_narrow_kernel(const T* logit
 }
 
 // ---------------------------------------------------------------- wide rows
-// 64 bytes of a row a thread, in pieces of 16 that lie side by side across the CTA: 16 KB of the row.
+// A thread's pieces of a chunk of 10 KB of a row: each lies side by side with the other threads'.
 template <typename T>
 struct ScoreChunk {
-  static constexpr int PER = 16 / sizeof(T), N = 4 * PER, SIZE = kScoreThreads * N;
-  uint4 raw[4];
+  static constexpr int PER = 16 / sizeof(T), N = kScorePieces * PER, SIZE = kScoreThreads * N;
+  uint4 raw[kScorePieces];
   SJ_DEVICE static int index(int base, int i) {  // column of the thread's element i; base: of the chunk
     return base + (i / PER * kScoreThreads + static_cast<int>(threadIdx.x)) * PER + i % PER;
   }
@@ -275,10 +279,10 @@ struct ScoreChunk {
     const uint32_t w = word(q, i % PER / 2);
     return __uint_as_float(i % 2 ? w & 0xffff0000u : w << 16);
   }
-  // The maxima of the four pieces: NaN left out, -inf where there is nothing else.
-  SJ_DEVICE void largest(float (&m)[4]) const {
+  // The maxima of the pieces: NaN left out, -inf where there is nothing else.
+  SJ_DEVICE void largest(float (&m)[kScorePieces]) const {
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
+    for (int v = 0; v < kScorePieces; ++v) {
       if (sizeof(T) == 4) {
         m[v] = fmaxf(fmaxf(at(4 * v), at(4 * v + 1)), fmaxf(at(4 * v + 2), at(4 * v + 3)));
       } else {
@@ -295,7 +299,7 @@ struct ScoreChunk {
     const T* src = x + index(base, 0);
     const bool inside = base >= 0 && base + SIZE <= vocab;
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
+    for (int v = 0; v < kScorePieces; ++v) {
       const int j = index(base, v * PER);
       if (inside || (j >= 0 && j + PER <= vocab))
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(own + v * (16 * kScoreThreads)),
@@ -315,12 +319,12 @@ struct ScoreChunk {
   SJ_DEVICE void read(const T* x, int base, int vocab, uint32_t own) {
     if (base >= 0 && base + SIZE <= vocab) {
 #pragma unroll
-      for (int v = 0; v < 4; ++v) raw[v] = piece(own, v);
+      for (int v = 0; v < kScorePieces; ++v) raw[v] = piece(own, v);
       return;
     }
     constexpr uint32_t NONE = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
+    for (int v = 0; v < kScorePieces; ++v) {
       const int j = index(base, v * PER);
       raw[v] = make_uint4(NONE, NONE, NONE, NONE);
       if (j >= 0 && j + PER <= vocab) {
@@ -387,31 +391,34 @@ struct ScoreBest {
   int count;     // of held
 };
 
-// The bar: an order that at least `top` of the part's logits reach.  64 groups of four threads keep the largest order
+// The bar: an order that at least `top` of the part's logits reach.  64 groups of threads keep the largest order
 // they have met (its last six bits make the groups' values distinct); the `top`-th largest of them is one.  It
 // only rises, so one that is out of date still holds.  0 when fewer than `top` groups hold more than
 // forbidden tokens.
 SJ_DEVICE uint32_t score_group(ScoreBest& b, uint32_t order) {
-  uint32_t g = max(order, __shfl_xor_sync(0xffffffffu, order, 1));
-  g = max(g, __shfl_xor_sync(0xffffffffu, g, 2));
-  g = (g & ~63u) | (threadIdx.x >> 2);
-  if ((threadIdx.x & 3) == 0) b.group[threadIdx.x >> 2] = g;
+  constexpr int OF = kScoreThreads / 64;  // threads of a group
+  uint32_t g = order;
+#pragma unroll
+  for (int o = 1; o < OF; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+  g = (g & ~63u) | (threadIdx.x / OF);
+  if (threadIdx.x % OF == 0) b.group[threadIdx.x / OF] = g;
   return g;
 }
 SJ_DEVICE uint32_t score_bar_of(uint32_t g) { return (g & ~63u) > kForbidden ? g & ~63u : 0u; }
 // By the whole CTA, for a part's first chunk.
 SJ_DEVICE void score_first_bar(ScoreBest& b, uint32_t order, int top) {
+  constexpr int OF = kScoreThreads / 64;
   const uint32_t g = score_group(b, order);
   __syncthreads();
   int rank = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint4 o = reinterpret_cast<const uint4*>(b.group)[i * 4 + (threadIdx.x & 3)];
+  for (int i = 0; i < 16 / OF; ++i) {
+    const uint4 o = reinterpret_cast<const uint4*>(b.group)[i * OF + threadIdx.x % OF];
     rank += (o.x > g) + (o.y > g) + (o.z > g) + (o.w > g);
   }
-  rank += __shfl_xor_sync(0xffffffffu, rank, 1);
-  rank += __shfl_xor_sync(0xffffffffu, rank, 2);
-  if ((threadIdx.x & 3) == 0 && rank == top - 1) b.bar = score_bar_of(g);
+#pragma unroll
+  for (int o = 1; o < OF; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+  if (threadIdx.x % OF == 0 && rank == top - 1) b.bar = score_bar_of(g);
   __syncthreads();
 }
 // By one warp, whatever the others have come to: a bitonic sort of the groups, two a lane, the largest first.
@@ -460,21 +467,22 @@ SJ_DEVICE int score_rank(ScoreBest& b, int top) {
   return kept;
 }
 
-// The same where more logits reach the bar than the list holds (equal or rising logits): chunk by chunk, the logits of
-// the `top` threads with the best maxima join the list, which is ranked each time.  Leaves best.list; returns
-// its length.
+// The same where more logits reach the bar than the list holds (equal or rising logits): columns [base, end) once
+// more, 4096 at a time, of which those of the `top` threads with the best maxima join the list; it is ranked each
+// time.  Leaves best.list; returns its length.
 template <typename T>
-SJ_DEVICE int score_rank_all(ScoreBest& best, const T* x, int base, int end, int vocab, int top) {
+SJ_DEVICE int score_rank_all(ScoreBest& best, const T* x, int base, int end, int top) {
+  constexpr int N = 32;  // logits of a thread at a time
   __syncthreads();
   if (threadIdx.x == 0) best.count = 0;
   int n = 0;
-  for (; base < end; base += ScoreChunk<T>::SIZE) {
+  for (; base < end; base += kScoreThreads * N) {
     const uint32_t reach = n == top ? static_cast<uint32_t>(best.list[top - 1] >> 32) + 1 : 0u;
     uint64_t mine = 0;
 #pragma unroll 1
-    for (int i = 0; i < ScoreChunk<T>::N; ++i) {
-      const int j = ScoreChunk<T>::index(base, i);
-      if (j < 0 || j >= vocab) continue;
+    for (int i = 0; i < N; ++i) {
+      const int j = base + i * kScoreThreads + static_cast<int>(threadIdx.x);
+      if (j < 0 || j >= end) continue;
       const uint64_t key = score_key(score_load(x + j), j);
       if (static_cast<uint32_t>(key >> 32) >= reach) mine = max(mine, key);
     }
@@ -485,9 +493,9 @@ SJ_DEVICE int score_rank_all(ScoreBest& best, const T* x, int base, int end, int
     for (int k = 0; k < kScoreThreads; ++k) rank += best.thread_best[k] > mine ? 1 : 0;
     if (mine && rank < top) {
 #pragma unroll 1
-      for (int i = 0; i < ScoreChunk<T>::N; ++i) {
-        const int j = ScoreChunk<T>::index(base, i);
-        if (j < 0 || j >= vocab) continue;
+      for (int i = 0; i < N; ++i) {
+        const int j = base + i * kScoreThreads + static_cast<int>(threadIdx.x);
+        if (j < 0 || j >= end) continue;
         const uint64_t key = score_key(score_load(x + j), j);
         if (static_cast<uint32_t>(key >> 32) >= reach) best.held[atomicAdd(&best.count, 1)] = key;
       }
@@ -497,7 +505,7 @@ SJ_DEVICE int score_rank_all(ScoreBest& best, const T* x, int base, int end, int
   return n;
 }
 
-// Persistent CTAs over the parts of rows, 16 KB at a time; the next chunk, be it of the next part, is on its way
+// Persistent CTAs over the parts of rows, 10 KB at a time; the next chunk, be it of the next part, is on its way
 // to shared memory meanwhile (cp.async; a thread reads back only what it copied, so copies need no barrier).  The
 // sums are each thread's own until the part's end.  What reaches the bar of the alternatives goes to a list that
 // is ranked at the end (of 50001 logits at top = 20 about 60).  After the two barriers of a part's first bar
@@ -510,14 +518,14 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
   using Chunk = ScoreChunk<T>;
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ ScoreBest best;
-  __shared__ ScoreSum sums[kScoreThreads / 32];
+  __shared__ ScoreSum sums[kScoreWarps];
   __shared__ int s_last;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, top = out.top, vocab = out.vocab;
   const uint32_t stages = smem_u32(ring) + t * 16, count_at = smem_u32(&best.count);
   uint32_t one;  // not a constant that the compiler sees: gathering a warp's additions costs more than they do
   asm volatile("mov.u32 %0, 1;" : "=r"(one));
   ScoreWalk<T> ahead(logits, ld, vocab, splits, parts);
-  for (int i = 0; i < kScoreStages - 1; ++i) ahead.fetch(stages + i * 16384);
+  for (int i = 0; i < kScoreStages - 1; ++i) ahead.fetch(stages + i * kScoreStage);
   int stage = 0;
   if (t == 0) best.count = 0;
   __syncthreads();
@@ -525,7 +533,7 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
     const T* x = here.x;
     const int r = splits == 1 ? here.part : here.part / splits;
     ScoreSum a{-INFINITY, 0.f, 0.f};
-    uint32_t noted = 0;  // pieces of up to eight chunks
+    uint32_t noted = 0;  // pieces of up to 32 / kScorePieces chunks
     int room = 0;
     // Files the logits that reach the bar in the noted pieces of the chunk at `base` and the `before` ones before it.
     auto look = [&](int base, int before, uint32_t pieces) {
@@ -539,7 +547,8 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
       while (pieces) {
         const int bit = __ffs(pieces) - 1;
         pieces &= pieces - 1;
-        const int j0 = Chunk::index(base + (bit / 4 - before) * Chunk::SIZE, bit % 4 * Chunk::PER);
+        const int j0 =
+            Chunk::index(base + (bit / kScorePieces - before) * Chunk::SIZE, bit % kScorePieces * Chunk::PER);
         if (reach > kForbidden && j0 >= 0 && j0 + Chunk::PER <= vocab) {
           const uint4 q = *reinterpret_cast<const uint4*>(x + j0);
 #pragma unroll
@@ -560,15 +569,18 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
     for (; here.c < here.c1; ++here.c) {
       const int first = here.base();
       asm volatile("cp.async.wait_group %0;" ::"n"(kScoreStages - 2) : "memory");
-      const uint32_t own = stages + stage * 16384;
-      ahead.fetch(stages + (stage == 0 ? kScoreStages - 1 : stage - 1) * 16384);
+      const uint32_t own = stages + stage * kScoreStage;
+      ahead.fetch(stages + (stage == 0 ? kScoreStages - 1 : stage - 1) * kScoreStage);
       stage = stage == kScoreStages - 1 ? 0 : stage + 1;
-      float m = -INFINITY, most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      float m = -INFINITY, most[kScorePieces];
+#pragma unroll
+      for (int v = 0; v < kScorePieces; ++v) most[v] = -INFINITY;
       if (first + warp * 32 * Chunk::PER < vocab) {  // not past the row's end
         Chunk now;
         now.read(x, first, vocab, own);
         now.largest(most);
-        m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+#pragma unroll
+        for (int v = 0; v < kScorePieces; ++v) m = fmaxf(m, most[v]);
         if (__any_sync(0xffffffffu, m > a.m)) a = score_raise(a, m);
         const float base = a.m == -INFINITY ? 0.f : a.m;
         uint64_t s = pair2(a.s, 0.f), u = pair2(a.u, 0.f);
@@ -585,18 +597,18 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
         score_first_bar(best, met, top);
       } else {
         score_group(best, met);
-        if (warp == (here.c & 7)) score_raise_bar(best, top);
+        if (warp == here.c % kScoreWarps) score_raise_bar(best, top);
       }
       // the pieces whose maximum reaches the bar are few: they are noted, and looked at once the bar has risen
       const uint32_t reach = *const_cast<volatile uint32_t*>(&best.bar);
       const float least = reach > kForbidden ? score_value(reach) : -INFINITY;
       uint32_t hot = 0;
 #pragma unroll
-      for (int v = 0; v < 4; ++v) hot |= most[v] >= least ? 1u << v : 0u;
+      for (int v = 0; v < kScorePieces; ++v) hot |= most[v] >= least ? 1u << v : 0u;
       noted |= (any ? hot : 0u) << room;
-      room += 4;
-      if (room == 32 || here.c + 1 == here.c1) {
-        look(first, room / 4 - 1, noted);
+      room += kScorePieces;
+      if (room + kScorePieces > 32 || here.c + 1 == here.c1) {
+        look(first, room / kScorePieces - 1, noted);
         noted = 0;
         room = 0;
       }
@@ -608,11 +620,11 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
     int n = 0;
     __syncthreads();
     if (top > 0 && best.count > kScoreHeld) {
-      n = score_rank_all(best, x, here.start, here.origin + here.c1 * Chunk::SIZE, vocab, top);
+      n = score_rank_all(best, x, here.start, min(vocab, here.origin + here.c1 * Chunk::SIZE), top);
     } else if (top > 0) {
       n = score_rank(best, top);
     }
-    if (warp == 0) a = score_lanes_join<8>(sums[lane & 7]);  // what follows is warp 0's
+    if (warp == 0) a = score_lanes_join<kScoreWarps>(sums[lane % kScoreWarps]);  // what follows is warp 0's
     bool writes = true;
     if (splits > 1) {
       const int size = score_part(top);
@@ -860,10 +872,10 @@ using namespace sj;
 
 namespace {
 int score_ctas() { return kScoreCtas * sm_count(); }
-// Parts of a row, of at least 4096 logits: the fewest that give two CTAs of five one, since a CTA that has its SM to itself
-// runs faster and a part costs its own ranking and a share of a join (64 x 131072 f32: 16.6 us with 4 parts, 19 to
-// 21 with 2, 3, 5 or 7; 300 x 50001 bf16: 18.5 whole, 25.9 in two).  For the same reason a partly filled last round of
-// whole rows is left as it is (2048 rows on 592 CTAs: 71 us, 80 with the last 272 split in two).
+// Parts of a row, of at least 4096 logits: the fewest that give two CTAs of five one, since a CTA that has its SM to
+// itself runs faster and a part costs its own ranking and a share of a join (400 x 32000 f32: 19.0 us whole, 20.7 in
+// two, 26.6 in three; 128 x 130000 f32: 32.5 us in two, 24.8 in four, 24.1 in seven).  For the same reason a partly
+// filled last round of whole rows is left as it is.
 int score_splits(int rows, int vocab) {
   if (vocab <= kScoreNarrow || rows <= 0) return 1;
   const int fill = (score_ctas() * 2 / 5 + rows - 1) / rows;
@@ -881,7 +893,7 @@ int scores(const T* logits, int ld, int rows, const ScoreOut& out, void* workspa
                         : token_scores_narrow_kernel<T, 32>,
            grid, 128, 0, stream, logits, ld, rows, out);
   } else {
-    const int splits = score_splits(rows, out.vocab), smem = kScoreStages * 16384;
+    const int splits = score_splits(rows, out.vocab), smem = kScoreStages * kScoreStage;
     if (static_cast<int64_t>(rows) * splits > INT_MAX - score_ctas())
       return fail(SJ_ERR_SHAPE, "sj_token_scores: rows=%d vocab=%d", rows, out.vocab);
     static KernelAttrOnce once;

@@ -114,6 +114,19 @@ def test_scores_of_ties_and_orders(vocab, kind):
         check_scores(x, target, vocab, top)
 
 
+@pytest.mark.parametrize("vocab", [5001, 40000])
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+def test_scores_of_peaks_anywhere(vocab, kind):
+    """Smooth peaks: the best logits lie side by side, many equal after rounding, at and around the ends of chunks and of a
+    row's parts; each is found once."""
+    step = torch.arange(vocab, dtype=torch.float32)
+    at = list(range(0, vocab, 977)) + [2559, 2560, 4095, 4096, 5119, vocab - 1]
+    x = torch.stack([-(step - p).abs() / 50 for p in at if p < vocab]).to(kind).to(DEV)
+    target = torch.zeros(len(x), dtype=torch.int32, device=DEV)
+    check_scores(x, target, vocab, 32)
+    check_scores(x[:3], target[:3], vocab, 32)
+
+
 @pytest.mark.parametrize("vocab", [257, 9001])
 @pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
 def test_scores_of_masked_rows(vocab, kind):

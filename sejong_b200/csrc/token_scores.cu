@@ -7,12 +7,11 @@
 // The alternatives are the `top` largest logits, the lowest index first among equal ones: a key of
 // (value, ~index) orders them without ties.
 //
-// Each logit is read once from memory.  Measured on B200 (graph replays): 2048 x 50001 bf16 with 20 alternatives 67 us
-// (3.1 TB/s; without alternatives 45), where the exponentials (the special-function unit takes a warp's in 8
-// cycles), the unpacking and the alternatives bound it, not memory: about 450 instructions a warp and 1024 logits;
-// 1024 x 50001 f32 47 us (4.4 TB/s).  The first simple kernel (a pass for the maximum, one for the
-// sums, one for each alternative) took 1629.  Gradient: 2048 x 65537 bf16 91 us (5.9 TB/s), 1024 x 50001 f32 69 us
-// (6.0).
+// Each logit is read once from memory.  Measured on B200 (graph replays): 2048 x 50001 bf16 with 20 alternatives 60 us
+// (3.4 TB/s; without alternatives 43.5, 4.7 TB/s), where instructions bound it, not memory: of a warp's 430 for 1024
+// logits, the exponentials' unit takes 32 (8 cycles each), floors and unpacking 64, the alternatives 110.
+// 1024 x 50001 f32 42 us (4.8 TB/s).  The first simple kernel (a pass for the maximum, one for the sums, one for each
+// alternative) took 1629.  Gradient: 2048 x 65537 bf16 91 us (5.9 TB/s), 1024 x 50001 f32 69 us (6.0).
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -30,8 +29,9 @@ constexpr int kScorePieces = 5;       // 16-byte pieces of a chunk that a thread
 constexpr int kScoreStage = kScoreThreads * kScorePieces * 16;
 // CTAs of an SM, stages of a CTA's ring.  Small CTAs and small chunks waste less of a row's last chunk, many pieces a
 // thread spread a chunk's fixed cost: with 128 threads, five pieces and seven CTAs, 2048 x 50001 bf16 with 20
-// alternatives takes 66.8 us and 8000 x 2000 f32 45.6; with 256, four and four, 71.2 and 71.8; 128, four and eight,
-// 73.8 and 42.3; 128, eight and five, 73.8; 64, eight and nine, 78.9.
+// alternatives takes 60.2 us and 8000 x 2000 f32 47.8; with 256, four and four, 71.4 and 82.3; 128, four and eight,
+// 67.6 and 42.3; 128, six and six, 61.8 and 54.2; 64, eight and nine, 63.5 and 38.6.  A third stage leaves room for
+// five CTAs: 66.9 and 60.8.
 constexpr int kScoreCtas = 7, kScoreStages = 2;
 constexpr int kScoreMaxSplits = 16;
 // The gradient of rows of at most 1024 pieces of 16 bytes: four rows a warp (32768 x 257 f32 16.3 us with eight CTAs of
@@ -41,7 +41,8 @@ constexpr int kGradRows = 4, kGradNarrowCtas = 8, kGradNarrow = 1024;
 // six; 1024 x 50001 f32 68.9, 70.9, 72.7.
 template <typename T>
 constexpr int kGradCtas = sizeof(T) == 2 ? 5 : 4;
-constexpr int kScoreHeld = kScoreMaxTop * 32 + kScoreMaxTop;  // candidates: the best of 32 threads' 32, and the list
+constexpr int kScoreHeld = kScoreMaxTop * 16 + kScoreMaxTop;  // candidates: the best of 32 threads' 16, and the list
+constexpr int kScoreNoted = 512;  // pieces with candidates (128 are expected of 2^20 logits)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 }  // namespace
 
@@ -161,12 +162,21 @@ struct ScoreOut {
 SJ_DEVICE float score_logp(float x, const ScoreSum& a, float base, float log_s) {
   return x == -INFINITY && a.s == a.s ? -INFINITY : (x - base) - log_s;
 }
-template <typename T>
-SJ_DEVICE void score_write_row(const ScoreOut& out, const T* x, int r, const ScoreSum& a) {
+// A row's target and its logit.
+struct ScoreTarget {
+  int at;
+  float x;
+  SJ_DEVICE explicit ScoreTarget(int at_) : at(at_), x(0.f) {}
+  template <typename T>
+  SJ_DEVICE void load(const T* row, int vocab) {
+    if (at >= 0 && at < vocab) x = score_load(row + at);
+  }
+};
+SJ_DEVICE void score_write_row(const ScoreOut& out, const ScoreTarget& target, int r, const ScoreSum& a) {
   const float base = a.m == -INFINITY ? 0.f : a.m, log_s = logf(a.s);
-  const int at = out.target ? out.target[r] : -1;
+  const int at = target.at;
   if (at >= out.vocab || at < -1) record_error(SJ_DEV_BAD_INDEX);
-  if (out.logp) out.logp[r] = at < 0 || at >= out.vocab ? 0.f : score_logp(score_load(x + at), a, base, log_s);
+  if (out.logp) out.logp[r] = at < 0 || at >= out.vocab ? 0.f : score_logp(target.x, a, base, log_s);
   if (out.entropy) out.entropy[r] = a.s == 0.f ? 0.f : log_s - a.u / a.s * kLn2;
   if (out.lse) out.lse[r] = base + log_s;
 }
@@ -198,7 +208,11 @@ __global__ void __launch_bounds__(128) token_scores_narrow_kernel(const T* logit
   for (int i = 0; i < R; i += 2) score_add2(pair2(v[i], v[i + 1]), pair2(-base, -base), s, u);
   a.s = warp_sum(low2(s) + high2(s));
   a.u = warp_sum(low2(u) + high2(u));
-  if (lane == 0) score_write_row(out, x, r, a);
+  if (lane == 0) {
+    ScoreTarget target(out.target ? out.target[r] : -1);
+    target.load(x, out.vocab);
+    score_write_row(out, target, r, a);
+  }
   if (out.top == 0) return;
   const float log_s = logf(a.s);
   auto write = [&](int k, uint64_t key) {
@@ -268,6 +282,7 @@ __global__ void __launch_bounds__(128) token_scores_narrow_kernel(const T* logit
 template <typename T>
 struct ScoreChunk {
   static constexpr int PER = 16 / sizeof(T), N = kScorePieces * PER, SIZE = kScoreThreads * N;
+  static constexpr uint32_t NONE = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;  // -inf
   uint4 raw[kScorePieces];
   SJ_DEVICE static int index(int base, int i) {  // column of the thread's element i; base: of the chunk
     return base + (i / PER * kScoreThreads + static_cast<int>(threadIdx.x)) * PER + i % PER;
@@ -279,19 +294,31 @@ struct ScoreChunk {
     const uint32_t w = word(q, i % PER / 2);
     return __uint_as_float(i % 2 ? w & 0xffff0000u : w << 16);
   }
-  // The maxima of the pieces: NaN left out, -inf where there is nothing else.
-  SJ_DEVICE void largest(float (&m)[kScorePieces]) const {
+  // The maximum, and those of the pieces, of which bf16 keeps two halves: NaN left out, -inf where there is nothing
+  // else.
+  SJ_DEVICE float largest(uint32_t (&most)[kScorePieces]) const {
+    if (sizeof(T) == 4) {
+      float m = -INFINITY;
+#pragma unroll
+      for (int v = 0; v < kScorePieces; ++v) {
+        most[v] = __float_as_uint(fmaxf(fmaxf(at(4 * v), at(4 * v + 1)), fmaxf(at(4 * v + 2), at(4 * v + 3))));
+        m = fmaxf(m, __uint_as_float(most[v]));
+      }
+      return m;
+    }
+    uint32_t m = NONE;
 #pragma unroll
     for (int v = 0; v < kScorePieces; ++v) {
-      if (sizeof(T) == 4) {
-        m[v] = fmaxf(fmaxf(at(4 * v), at(4 * v + 1)), fmaxf(at(4 * v + 2), at(4 * v + 3)));
-      } else {
-        uint32_t p = 0xff80ff80u;
+      most[v] = NONE;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) asm("max.bf16x2 %0, %0, %1;" : "+r"(p) : "r"(word(raw[v], i)));
-        m[v] = fmaxf(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u));
-      }
+      for (int i = 0; i < 4; ++i) asm("max.bf16x2 %0, %0, %1;" : "+r"(most[v]) : "r"(word(raw[v], i)));
+      asm("max.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(most[v]));
     }
+    return of(m);
+  }
+  SJ_DEVICE static float of(uint32_t most) {
+    if (sizeof(T) == 4) return __uint_as_float(most);
+    return fmaxf(__uint_as_float(most << 16), __uint_as_float(most & 0xffff0000u));
   }
   // The chunk's pieces that lie in the row, on their way to `own`, the thread's place in a stage of shared memory.
   // A chunk inside the row needs no look at its pieces.
@@ -322,7 +349,6 @@ struct ScoreChunk {
       for (int v = 0; v < kScorePieces; ++v) raw[v] = piece(own, v);
       return;
     }
-    constexpr uint32_t NONE = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
 #pragma unroll
     for (int v = 0; v < kScorePieces; ++v) {
       const int j = index(base, v * PER);
@@ -386,70 +412,47 @@ struct ScoreBest {
   uint64_t held[kScoreHeld];
   uint64_t list[kScoreMaxTop];
   uint64_t thread_best[kScoreThreads];
-  __align__(16) uint32_t group[64];
+  __align__(4) uint16_t group[64];
+  int piece[kScoreNoted];  // columns of the pieces that reached the bar
   uint32_t bar;
-  int count;     // of held
+  int count, pieces;  // of held, of piece
+  SJ_DEVICE void clear() {
+    bar = 0;
+    count = pieces = 0;
+  }
 };
 
 // The bar: an order that at least `top` of the part's logits reach.  64 groups of threads keep the largest order
-// they have met (its last six bits make the groups' values distinct); the `top`-th largest of them is one.  It
-// only rises, so one that is out of date still holds.  0 when fewer than `top` groups hold more than
-// forbidden tokens.
-SJ_DEVICE uint32_t score_group(ScoreBest& b, uint32_t order) {
+// they have met, of which 16 bits make the bar no higher than it may be; the `top`-th largest of them is one.  It
+// only rises, so one that is out of date still holds.  0 when fewer than `top` groups hold more than forbidden
+// tokens.
+SJ_DEVICE void score_group(ScoreBest& b, uint32_t order) {
   constexpr int OF = kScoreThreads / 64;  // threads of a group
-  uint32_t g = order;
 #pragma unroll
-  for (int o = 1; o < OF; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
-  g = (g & ~63u) | (threadIdx.x / OF);
-  if (threadIdx.x % OF == 0) b.group[threadIdx.x / OF] = g;
-  return g;
+  for (int o = 1; o < OF; o <<= 1) order = max(order, __shfl_xor_sync(0xffffffffu, order, o));
+  if (threadIdx.x % OF == 0) b.group[threadIdx.x / OF] = static_cast<uint16_t>(order >> 16);
 }
-SJ_DEVICE uint32_t score_bar_of(uint32_t g) { return (g & ~63u) > kForbidden ? g & ~63u : 0u; }
-// By the whole CTA, for a part's first chunk.
-SJ_DEVICE void score_first_bar(ScoreBest& b, uint32_t order, int top) {
-  constexpr int OF = kScoreThreads / 64;
-  const uint32_t g = score_group(b, order);
-  __syncthreads();
-  int rank = 0;
-#pragma unroll
-  for (int i = 0; i < 16 / OF; ++i) {
-    const uint4 o = reinterpret_cast<const uint4*>(b.group)[i * OF + threadIdx.x % OF];
-    rank += (o.x > g) + (o.y > g) + (o.z > g) + (o.w > g);
-  }
-#pragma unroll
-  for (int o = 1; o < OF; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
-  if (threadIdx.x % OF == 0 && rank == top - 1) b.bar = score_bar_of(g);
-  __syncthreads();
-}
-// By one warp, whatever the others have come to: a bitonic sort of the groups, two a lane, the largest first.
+// By one warp, whatever the others have come to: bitonic sorts of the low and of the high half of each lane, the
+// largest first; of sorted a and b the k-th largest is the largest min(a_j, b_(k-j)).
 SJ_DEVICE void score_raise_bar(ScoreBest& b, int top) {
   const int lane = threadIdx.x & 31;
-  uint32_t v[2] = {b.group[lane], b.group[lane + 32]};
+  uint32_t v = reinterpret_cast<const volatile uint32_t*>(b.group)[lane];
 #pragma unroll
-  for (int size = 2; size <= 64; size *= 2)
+  for (int size = 2; size <= 32; size *= 2)
 #pragma unroll
     for (int step = size / 2; step > 0; step /= 2) {
-      if (step == 32) {
-        const uint32_t high = max(v[0], v[1]);
-        v[1] = min(v[0], v[1]);
-        v[0] = high;
-        continue;
-      }
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int at = lane + 32 * r;
-        const uint32_t o = __shfl_xor_sync(0xffffffffu, v[r], step);
-        const bool larger = ((at & step) == 0) == ((at & size) == 0);
-        v[r] = larger ? max(v[r], o) : min(v[r], o);
-      }
+      const uint32_t o = __shfl_xor_sync(0xffffffffu, v, step);
+      const bool larger = ((lane & step) == 0) == ((lane & size) == 0);
+      v = larger ? __vmaxu2(v, o) : __vminu2(v, o);
     }
-  const uint32_t g = __shfl_sync(0xffffffffu, v[0], top - 1);
-  if (lane == 0) atomicMax(&b.bar, score_bar_of(g));
+  const uint32_t other = __shfl_sync(0xffffffffu, v, (top - 2 - lane) & 31) >> 16, low = v & 0xffffu;
+  const uint32_t mine = lane < top - 1 ? min(low, other) : lane == top - 1 ? max(low, v >> 16) : 0u;
+  const uint32_t bar = __reduce_max_sync(0xffffffffu, mine);
+  if (lane == 0 && bar > kForbidden >> 16) atomicMax(&b.bar, bar << 16);
 }
 
-// held cut down to its `top` largest keys, in order, which are in list, too; returns how many there are.
+// The `top` largest keys of held, which all threads see, in order into list; returns how many there are.
 SJ_DEVICE int score_rank(ScoreBest& b, int top) {
-  __syncthreads();
   const int n = b.count;
 #pragma unroll 1
   for (int i = threadIdx.x; i < n; i += kScoreThreads) {
@@ -460,19 +463,15 @@ SJ_DEVICE int score_rank(ScoreBest& b, int top) {
     if (rank < top) b.list[rank] = key;
   }
   __syncthreads();
-  const int kept = min(n, top);
-  if (threadIdx.x < kept) b.held[threadIdx.x] = b.list[threadIdx.x];
-  if (threadIdx.x == 0) b.count = kept;
-  __syncthreads();
-  return kept;
+  return min(n, top);
 }
 
 // The same where more logits reach the bar than the list holds (equal or rising logits): columns [base, end) once
-// more, 4096 at a time, of which those of the `top` threads with the best maxima join the list; it is ranked each
+// more, 2048 at a time, of which those of the `top` threads with the best maxima join the list; it is ranked each
 // time.  Leaves best.list; returns its length.
 template <typename T>
 SJ_DEVICE int score_rank_all(ScoreBest& best, const T* x, int base, int end, int top) {
-  constexpr int N = 32;  // logits of a thread at a time
+  constexpr int N = 16;  // logits of a thread at a time
   __syncthreads();
   if (threadIdx.x == 0) best.count = 0;
   int n = 0;
@@ -500,16 +499,21 @@ SJ_DEVICE int score_rank_all(ScoreBest& best, const T* x, int base, int end, int
         if (static_cast<uint32_t>(key >> 32) >= reach) best.held[atomicAdd(&best.count, 1)] = key;
       }
     }
+    __syncthreads();
     n = score_rank(best, top);
+    if (threadIdx.x < n) best.held[threadIdx.x] = best.list[threadIdx.x];
+    if (threadIdx.x == 0) best.count = n;
+    __syncthreads();
   }
   return n;
 }
 
 // Persistent CTAs over the parts of rows, 10 KB at a time; the next chunk, be it of the next part, is on its way
 // to shared memory meanwhile (cp.async; a thread reads back only what it copied, so copies need no barrier).  The
-// sums are each thread's own until the part's end.  What reaches the bar of the alternatives goes to a list that
-// is ranked at the end (of 50001 logits at top = 20 about 60).  After the two barriers of a part's first bar
-// the warps go on without any; in turn, they raise the bar chunk by chunk.
+// sums are each thread's own until the part's end.  Pieces of 16 bytes that reach the bar of the alternatives are
+// noted (of 50001 logits at top = 20 about 70); at the end, each is looked at by a thread of its own and what
+// reaches the bar now is ranked.  After the two barriers of a part's first bar the warps go on without any; in
+// turn, they raise the bar at every other chunk (60.2 us; at every one 61.0).
 template <typename T>
 __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
     token_scores_wide_kernel(const T* logits, int ld, int splits, int parts, int* counters, float* partial,
@@ -518,113 +522,120 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
   using Chunk = ScoreChunk<T>;
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ ScoreBest best;
-  __shared__ ScoreSum sums[kScoreWarps];
+  __shared__ ScoreSum sums[2][kScoreWarps];
   __shared__ int s_last;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, top = out.top, vocab = out.vocab;
-  const uint32_t stages = smem_u32(ring) + t * 16, count_at = smem_u32(&best.count);
-  uint32_t one;  // not a constant that the compiler sees: gathering a warp's additions costs more than they do
+  const uint32_t stages = smem_u32(ring) + t * 16;
+  int one;  // not a constant that the compiler sees: gathering a warp's additions costs more than they do
   asm volatile("mov.u32 %0, 1;" : "=r"(one));
+  auto next = [&](int* count, int n) {
+    int at;
+    asm volatile("atom.shared.add.u32 %0, [%1], %2;" : "=r"(at) : "r"(smem_u32(count)), "r"(n) : "memory");
+    return at;
+  };
+  // Files the logits of the piece at column j0 that reach the bar.
+  auto look = [&](const T* x, int j0) {
+    const float least = best.bar > kForbidden ? score_value(best.bar) : -INFINITY;
+    auto push = [&](float y, int j) {
+      const int at = next(&best.count, one);
+      if (at < kScoreHeld) best.held[at] = score_key(y, j);
+    };
+    if (best.bar > kForbidden && j0 >= 0 && j0 + Chunk::PER <= vocab) {
+      const uint4 q = *reinterpret_cast<const uint4*>(x + j0);
+      auto value = [&](int e) {
+        const uint32_t w = Chunk::word(q, e * static_cast<int>(sizeof(T)) / 4);
+        return __uint_as_float(sizeof(T) == 4 ? w : e % 2 ? w & 0xffff0000u : w << 16);
+      };
+      uint32_t hits = 0;
+#pragma unroll
+      for (int e = 0; e < Chunk::PER; ++e) hits |= value(e) >= least ? 1u << e : 0u;
+      for (; hits; hits &= hits - 1) push(value(__ffs(hits) - 1), j0 + __ffs(hits) - 1);
+      return;
+    }
+#pragma unroll 1
+    for (int j = max(j0, 0); j < min(j0 + Chunk::PER, vocab); ++j) {
+      const float y = score_load(x + j);
+      if (score_order(y) >= best.bar) push(y, j);
+    }
+  };
   ScoreWalk<T> ahead(logits, ld, vocab, splits, parts);
   for (int i = 0; i < kScoreStages - 1; ++i) ahead.fetch(stages + i * kScoreStage);
-  int stage = 0;
-  if (t == 0) best.count = 0;
+  int stage = 0, turn = 0;
+  if (t == 0) best.clear();
   __syncthreads();
   for (ScoreWalk<T> here(logits, ld, vocab, splits, parts); here.part < parts; here.leave()) {
     const T* x = here.x;
     const int r = splits == 1 ? here.part : here.part / splits;
-    ScoreSum a{-INFINITY, 0.f, 0.f};
-    uint32_t noted = 0;  // pieces of up to 32 / kScorePieces chunks
-    int room = 0;
-    // Files the logits that reach the bar in the noted pieces of the chunk at `base` and the `before` ones before it.
-    auto look = [&](int base, int before, uint32_t pieces) {
-      const uint32_t reach = *const_cast<volatile uint32_t*>(&best.bar);
-      const float least = reach > kForbidden ? score_value(reach) : -INFINITY;
-      auto push = [&](float y, int j) {
-        int at;
-        asm volatile("atom.shared.add.u32 %0, [%1], %2;" : "=r"(at) : "r"(count_at), "r"(one) : "memory");
-        if (at < kScoreHeld) best.held[at] = score_key(y, j);
-      };
-      while (pieces) {
-        const int bit = __ffs(pieces) - 1;
-        pieces &= pieces - 1;
-        const int j0 =
-            Chunk::index(base + (bit / kScorePieces - before) * Chunk::SIZE, bit % kScorePieces * Chunk::PER);
-        if (reach > kForbidden && j0 >= 0 && j0 + Chunk::PER <= vocab) {
-          const uint4 q = *reinterpret_cast<const uint4*>(x + j0);
-#pragma unroll
-          for (int e = 0; e < Chunk::PER; ++e) {
-            const uint32_t w = Chunk::word(q, e * static_cast<int>(sizeof(T)) / 4);
-            const float y = __uint_as_float(sizeof(T) == 4 ? w : e % 2 ? w & 0xffff0000u : w << 16);
-            if (y >= least) push(y, j0 + e);
-          }
-        } else {
-#pragma unroll 1
-          for (int j = max(j0, 0); j < min(j0 + Chunk::PER, vocab); ++j) {
-            const float y = score_load(x + j);
-            if (score_order(y) >= reach) push(y, j);
-          }
-        }
-      }
-    };
+    ScoreTarget target(t == 0 && out.target ? out.target[r] : -1);
+    float m = -INFINITY;  // the thread's maximum; s, u: its sums, in two halves
+    uint64_t s = 0, u = 0;
     for (; here.c < here.c1; ++here.c) {
       const int first = here.base();
       asm volatile("cp.async.wait_group %0;" ::"n"(kScoreStages - 2) : "memory");
       const uint32_t own = stages + stage * kScoreStage;
       ahead.fetch(stages + (stage == 0 ? kScoreStages - 1 : stage - 1) * kScoreStage);
       stage = stage == kScoreStages - 1 ? 0 : stage + 1;
-      float m = -INFINITY, most[kScorePieces];
+      if (t == 0 && here.c + 1 == here.c1) target.load(x, vocab);
+      float here_m = -INFINITY;
+      uint32_t most[kScorePieces];
 #pragma unroll
-      for (int v = 0; v < kScorePieces; ++v) most[v] = -INFINITY;
+      for (int v = 0; v < kScorePieces; ++v) most[v] = Chunk::NONE;
       if (first + warp * 32 * Chunk::PER < vocab) {  // not past the row's end
         Chunk now;
         now.read(x, first, vocab, own);
-        now.largest(most);
+        here_m = now.largest(most);
+        if (__any_sync(0xffffffffu, here_m > m)) {  // as score_raise
+          const float raised = fmaxf(m, here_m);
+          const float d = m == raised ? 0.f : fmaxf((m - raised) * kLog2e, -150.f), f = exp2_flush(d);
+          u = mul2(pair2(f, f), fma2(pair2(d, d), s, u));
+          s = mul2(pair2(f, f), s);
+          m = raised;
+        }
+        const float minus_base = m == -INFINITY ? 0.f : -m;
 #pragma unroll
-        for (int v = 0; v < kScorePieces; ++v) m = fmaxf(m, most[v]);
-        if (__any_sync(0xffffffffu, m > a.m)) a = score_raise(a, m);
-        const float base = a.m == -INFINITY ? 0.f : a.m;
-        uint64_t s = pair2(a.s, 0.f), u = pair2(a.u, 0.f);
-#pragma unroll
-        for (int i = 0; i < Chunk::N; i += 2) score_add2(pair2(now.at(i), now.at(i + 1)), pair2(-base, -base), s, u);
-        a.s = low2(s) + high2(s);
-        a.u = low2(u) + high2(u);
+        for (int i = 0; i < Chunk::N; i += 2)
+          score_add2(pair2(now.at(i), now.at(i + 1)), pair2(minus_base, minus_base), s, u);
       }
       if (top == 0) continue;
 
-      const bool any = Chunk::index(first, 0) < vocab;  // a thread's first element is its lowest
-      const uint32_t met = score_order(a.m);  // -inf from nothing: no more than kForbidden
+      score_group(best, score_order(m));  // -inf from nothing: no more than kForbidden
       if (first == here.start) {
-        score_first_bar(best, met, top);
-      } else {
-        score_group(best, met);
-        if (warp == here.c % kScoreWarps) score_raise_bar(best, top);
+        __syncthreads();
+        if (warp == 0) score_raise_bar(best, top);
+        __syncthreads();
+      } else if (here.c % 2 == 1 && warp == here.c / 2 % kScoreWarps) {
+        score_raise_bar(best, top);
       }
       // the pieces whose maximum reaches the bar are few: they are noted, and looked at once the bar has risen
       const uint32_t reach = *const_cast<volatile uint32_t*>(&best.bar);
       const float least = reach > kForbidden ? score_value(reach) : -INFINITY;
-      uint32_t hot = 0;
+      if (here_m >= least && Chunk::index(first, 0) < vocab) {  // a thread's first element is its lowest
+        uint32_t hot = 0;
 #pragma unroll
-      for (int v = 0; v < kScorePieces; ++v) hot |= most[v] >= least ? 1u << v : 0u;
-      noted |= (any ? hot : 0u) << room;
-      room += kScorePieces;
-      if (room + kScorePieces > 32 || here.c + 1 == here.c1) {
-        look(first, room / kScorePieces - 1, noted);
-        noted = 0;
-        room = 0;
+        for (int v = 0; v < kScorePieces; ++v) hot |= Chunk::of(most[v]) >= least ? 1u << v : 0u;
+        for (int at = next(&best.pieces, __popc(hot)); hot && at < kScoreNoted; hot &= hot - 1)
+          best.piece[at++] = Chunk::index(first, (__ffs(hot) - 1) * Chunk::PER);
       }
     }
 
     // ---- the part's sums and alternatives
-    a = score_lanes_join<32>(a);
-    if (lane == 0) sums[warp] = a;
+    ScoreSum a = score_lanes_join<32>(ScoreSum{m, low2(s) + high2(s), low2(u) + high2(u)});
+    if (lane == 0) sums[turn][warp] = a;
     int n = 0;
     __syncthreads();
-    if (top > 0 && best.count > kScoreHeld) {
-      n = score_rank_all(best, x, here.start, min(vocab, here.origin + here.c1 * Chunk::SIZE), top);
-    } else if (top > 0) {
-      n = score_rank(best, top);
+    if (top > 0) {
+      const int pieces = best.pieces;
+      if (pieces <= kScoreNoted)
+        for (int i = t; i < pieces; i += kScoreThreads) look(x, best.piece[i]);
+      __syncthreads();
+      n = pieces > kScoreNoted || best.count > kScoreHeld
+              ? score_rank_all(best, x, here.start, min(vocab, here.origin + here.c1 * Chunk::SIZE), top)
+              : score_rank(best, top);
+      if (t == 0) best.clear();  // seen by all after the next part's first barrier
     }
-    if (warp == 0) a = score_lanes_join<kScoreWarps>(sums[lane % kScoreWarps]);  // what follows is warp 0's
+    // What follows is warp 0's; the others go on.  Sums have two turns, since warp 0 may still read these.
+    if (warp == 0) a = score_lanes_join<kScoreWarps>(sums[turn][lane % kScoreWarps]);
+    turn ^= 1;
     bool writes = true;
     if (splits > 1) {
       const int size = score_part(top);
@@ -648,19 +659,19 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
           a = score_join(a, ScoreSum{p.x, p.y, p.z});
         }
         if (top > 0) {
-          if (t == 0) best.count = 0;
-          __syncthreads();
           for (int i = t; i < splits * top; i += kScoreThreads) {
             const float* p = row + static_cast<size_t>(i / top) * size;
             if (i % top < __float_as_int(__ldcg(p + 3)))
               best.held[atomicAdd(&best.count, 1)] =
                   __ldcg(reinterpret_cast<const unsigned long long*>(p + 4) + i % top);
           }
+          __syncthreads();
           n = score_rank(best, top);
+          if (t == 0) best.clear();
         }
       }
     }
-    if (writes && t == 0) score_write_row(out, x, r, a);
+    if (writes && t == 0) score_write_row(out, target, r, a);
     if (writes && t < top) {  // top <= vocab: the list is full
       const float base = a.m == -INFINITY ? 0.f : a.m;
       const uint64_t key = best.list[t];
@@ -668,9 +679,6 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
       out.top_logp[static_cast<size_t>(r) * top + t] =
           score_logp(score_value(static_cast<uint32_t>(key >> 32)), a, base, logf(a.s));
     }
-    __syncthreads();
-    if (t == 0) best.count = 0;
-    __syncthreads();
   }
 }
 

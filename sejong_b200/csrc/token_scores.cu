@@ -11,7 +11,7 @@
 // (3.4 TB/s; without alternatives 43.5, 4.7 TB/s), where instructions bound it, not memory: of a warp's 430 for 1024
 // logits, the exponentials' unit takes 32 (8 cycles each), floors and unpacking 64, the alternatives 110.
 // 1024 x 50001 f32 42 us (4.8 TB/s).  The first simple kernel (a pass for the maximum, one for the sums, one for each
-// alternative) took 1629.  Gradient: 2048 x 65537 bf16 91 us (5.9 TB/s), 1024 x 50001 f32 69 us (6.0).
+// alternative) took 1629.  Gradient: 2048 x 65537 bf16 85 us (6.3 TB/s), 1024 x 50001 f32 63 us (6.5).
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -34,11 +34,12 @@ constexpr int kScoreStage = kScoreThreads * kScorePieces * 16;
 // five CTAs: 66.9 and 60.8.
 constexpr int kScoreCtas = 7, kScoreStages = 2;
 constexpr int kScoreMaxSplits = 16;
-// The gradient of rows of at most 1024 pieces of 16 bytes: four rows a warp (32768 x 257 f32 16.3 us with eight CTAs of
-// four warps an SM, 18.4 with six; 8192 x 2000 f32 25.8 us, 36.7 by the kernel for wide rows).
+// The gradient of rows of at most 1024 pieces of 16 bytes: four rows a warp (32768 x 257 f32 13.0 us with eight CTAs of
+// four warps an SM, 13.6 with nine; three rows and nine CTAs 15.3, two and eleven 17.1; 8192 x 2000 f32 25.4, 36.7 by
+// the kernel for wide rows).
 constexpr int kGradRows = 4, kGradNarrowCtas = 8, kGradNarrow = 1024;
-// CTAs of an SM, of the gradient's kernel for wide rows: 2048 x 65537 bf16 94.3 us with four, 90.9 with five, 95.8 with
-// six; 1024 x 50001 f32 68.9, 70.9, 72.7.
+// CTAs of an SM, of the gradient's kernel for wide rows: 2048 x 65537 bf16 85.6 us with four, 84.8 with five, 98.6 with
+// six; 1024 x 50001 f32 65.6 with three, 62.9 with four, 68.7 with five.
 template <typename T>
 constexpr int kGradCtas = sizeof(T) == 2 ? 5 : 4;
 constexpr int kScoreHeld = kScoreMaxTop * 16 + kScoreMaxTop;  // candidates: the best of 32 threads' 16, and the list
@@ -688,23 +689,31 @@ struct ScoreGrad {
   const float *lse, *entropy, *d_logp, *d_entropy;
   int vocab;
 };
+// A row's scalars, none of whose loads waits for another.
+struct ScoreScalars {
+  int at;
+  float z, h, a, b;
+  SJ_DEVICE ScoreScalars(const ScoreGrad& in, int r)
+      : at(in.target ? in.target[r] : -1), z(in.lse[r]), h(in.d_entropy ? in.entropy[r] : 0.f),
+        a(in.d_logp ? in.d_logp[r] : 0.f), b(in.d_entropy ? in.d_entropy[r] : 0.f) {}
+};
 // A row's part of the gradient: with d = (x - z) log2(e), g = 2^d (-(a + b h) - b ln(2) d), and + a at the target.
 struct ScoreRow {
   float minus_z, c, b2, a;
   int at;
-  SJ_DEVICE ScoreRow(const ScoreGrad& in, int r, bool reports) {
-    at = in.target ? in.target[r] : -1;
+  SJ_DEVICE ScoreRow(const ScoreGrad& in, const ScoreScalars& row, bool reports) {
+    at = row.at;
     if (at >= in.vocab || at < -1) {
       if (reports) record_error(SJ_DEV_BAD_INDEX);
       at = -1;
     }
-    const float z = in.lse[r], b = in.d_entropy ? in.d_entropy[r] : 0.f;
-    a = in.d_logp && at >= 0 ? in.d_logp[r] : 0.f;
-    if (z == -INFINITY) at = -1;  // a row of forbidden tokens only: no gradient
-    minus_z = z == -INFINITY ? z : -z;
-    c = z == -INFINITY ? 0.f : in.d_entropy ? -fmaf(b, in.entropy[r], a) : -a;
-    b2 = z == -INFINITY ? 0.f : -b * kLn2;
+    a = at >= 0 ? row.a : 0.f;
+    if (row.z == -INFINITY) at = -1;  // a row of forbidden tokens only: no gradient
+    minus_z = row.z == -INFINITY ? row.z : -row.z;
+    c = row.z == -INFINITY ? 0.f : in.d_entropy ? -fmaf(row.b, row.h, a) : -a;
+    b2 = row.z == -INFINITY ? 0.f : -row.b * kLn2;
   }
+  SJ_DEVICE ScoreRow(const ScoreGrad& in, int r, bool reports) : ScoreRow(in, ScoreScalars(in, r), reports) {}
   SJ_DEVICE ScoreRow() {}
   SJ_DEVICE ScoreRow of_lane(int i) const {
     ScoreRow row;
@@ -758,7 +767,7 @@ __global__ void __launch_bounds__(128, kGradNarrowCtas)
   constexpr int PER = 16 / sizeof(T), ROWS = kGradRows;
   const int lane = threadIdx.x & 31, r0 = (blockIdx.x * 4 + (threadIdx.x >> 5)) * ROWS, live = min(ROWS, rows - r0);
   if (live <= 0) return;
-  const int whole = in.vocab / PER;
+  const int whole = in.vocab / PER, tail = ldd - whole * PER;  // columns after the whole pieces, with the padding
   const T* x = logits + static_cast<size_t>(r0) * ld;
   T* d = d_logits + static_cast<size_t>(r0) * ldd;
   uint4 raw[ROWS][2];
@@ -772,11 +781,17 @@ __global__ void __launch_bounds__(128, kGradNarrowCtas)
           raw[i][e] = reinterpret_cast<const uint4*>(x + static_cast<size_t>(i) * ld)[k + e * 32];
       }
   };
+  // Element e of the rows' tails.
+  auto load_tail = [&](int e) {
+    const int i = e / tail, j = whole * PER + e % tail;
+    return i < live && j < in.vocab ? score_load(x + static_cast<size_t>(i) * ld + j) : 0.f;
+  };
   load(lane);
+  const float last = tail > 0 ? load_tail(lane) : 0.f;
   const int mine = min(lane, live - 1);
   const ScoreRow all(in, r0 + mine, lane < live);
-  const T* own_x = x + static_cast<size_t>(mine) * ld;
-  const float own = all.at >= 0 ? all.grad(score_load(own_x + all.at), all.at) : 0.f;
+  const float own =
+      all.at >= 0 ? all.grad(score_load(x + static_cast<size_t>(mine) * ld + all.at), all.at) : 0.f;
   __syncwarp();
   for (int k0 = 0; k0 < whole; k0 += 64) {  // the same for every lane: they exchange the rows' scalars
     const int k = k0 + lane;
@@ -790,11 +805,12 @@ __global__ void __launch_bounds__(128, kGradNarrowCtas)
     }
     load(k + 64);
   }
-  for (int i = 0; i < live; ++i) {
+  for (int e0 = 0; e0 < live * tail; e0 += 32) {
+    const int e = e0 + lane, i = min(e / tail, live - 1), j = whole * PER + e % tail;
     const ScoreRow row = all.of_lane(i);
-    for (int j = whole * PER + lane; j < ldd; j += 32)
+    if (e < live * tail)
       score_store(d + static_cast<size_t>(i) * ldd + j,
-                  j < in.vocab ? row.grad(score_load(x + static_cast<size_t>(i) * ld + j), j) : 0.f);
+                  j < in.vocab ? row.grad(e0 == 0 ? last : load_tail(e), j) : 0.f);
   }
   __syncwarp();
   if (lane < live && all.at >= 0) score_store(d + static_cast<size_t>(lane) * ldd + all.at, own);
@@ -919,9 +935,8 @@ int scores(const T* logits, int ld, int rows, const ScoreOut& out, void* workspa
 template <typename T>
 int scores_bwd(const T* logits, int ld, T* d_logits, int ldd, int rows, const ScoreGrad& in, cudaStream_t stream) {
   constexpr int PER = 16 / sizeof(T);
-  const int vocab_pieces = in.vocab / PER;
   if (aligned16(logits) && aligned16(d_logits) && ld % PER == 0 && ldd % PER == 0) {
-    if (vocab_pieces <= kGradNarrow) {
+    if (ldd / PER <= kGradNarrow) {
       launch(token_scores_bwd_narrow_kernel<T>, (rows - 1) / (4 * kGradRows) + 1, 128, 0, stream, logits, ld, d_logits,
              ldd, rows, in);
     } else {

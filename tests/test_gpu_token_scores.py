@@ -234,6 +234,19 @@ def test_gradient_matches_the_restatement(rows, vocab, ld, ldd, kind):
         check_gradient(x, target, vocab, ldd, a, b, in_place=True)
 
 
+@pytest.mark.parametrize("vocab,ld", [(1, 8), (3, 8), (3, 800), (257, 320), (259, 4096), (100, 8200), (2049, 9000)])
+@pytest.mark.parametrize("rows", [1, 3, 6, 9])
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+def test_gradient_of_rows_with_padding(vocab, ld, rows, kind):
+    """Columns after the last whole 16 bytes: fewer and many more than a warp's lanes, in rows of one to nine."""
+    x, target = logits(rows, vocab, ld, kind, rows + ld)
+    target[-1] = vocab - 1
+    gen = torch.Generator().manual_seed(ld)
+    a, b = (torch.randn(rows, generator=gen).to(DEV) for _ in range(2))
+    check_gradient(x, target, vocab, ld, a, b)
+    check_gradient(x, target, vocab, ld, a, b, in_place=True)
+
+
 @pytest.mark.parametrize("kind,vocab", [(torch.float32, 8193), (torch.float32, 12291), (torch.bfloat16, 16385),
                                         (torch.float32, 4097), (torch.bfloat16, 8195)])
 def test_gradient_in_place_where_a_part_ends_with_the_whole_pieces(kind, vocab):

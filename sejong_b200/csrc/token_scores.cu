@@ -24,6 +24,14 @@ namespace sj {
 namespace {
 constexpr int kScoreMaxTop = 32;
 constexpr int kScoreNarrow = 1024;    // rows of at most this many logits are held by one warp
+// CTAs of an SM, of the kernel that holds R logits a lane: 32768 x 257 f32 with 5 alternatives 21.9 us with ten, 22.5
+// with nine, 23.1 with twelve; 32768 x 500 27.9 with nine, 27.3 with ten; 32768 x 1000 42.5 with seven, 40.5 with eight
+// (some spills), 63.9 without a limit on registers.
+template <int R>
+constexpr int kScoreNarrowCtas = R <= 16 ? 10 : 8;
+// Alternatives up to which their bar is found one by one, not by a sort: at 32768 x 257 one alternative takes 17.2 us,
+// not 20.1, five 21.9, not 22.9, and ten the same either way.
+constexpr int kScoreRounds = 8;
 constexpr int kScoreThreads = 128, kScoreWarps = kScoreThreads / 32;  // of the kernel for wider rows
 constexpr int kScorePieces = 5;       // 16-byte pieces of a chunk that a thread takes
 constexpr int kScoreStage = kScoreThreads * kScorePieces * 16;
@@ -54,6 +62,13 @@ SJ_DEVICE float score_load(const __nv_bfloat16* x) { return bf2f(*x); }
 SJ_DEVICE float exp2_flush(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The largest x of a warp's lanes, none a NaN.
+SJ_DEVICE float warp_largest(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -188,32 +203,31 @@ SJ_DEVICE void score_write_row(const ScoreOut& out, const ScoreTarget& target, i
 // listed and ranked by counting.  Where more than 64 do (ties), or too few are not forbidden, each alternative
 // is found by two warp reductions instead (value, then lowest index).
 template <typename T, int R>
-__global__ void __launch_bounds__(128) token_scores_narrow_kernel(const T* logits, int ld, int rows, ScoreOut out) {
+__global__ void __launch_bounds__(128, kScoreNarrowCtas<R>)
+    token_scores_narrow_kernel(const T* logits, int ld, int rows, ScoreOut out) {
   pdl_wait();
   __shared__ uint64_t listed[4][64];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = blockIdx.x * 4 + warp;
   if (r >= rows) return;
   const T* x = logits + static_cast<size_t>(r) * ld;
+  ScoreTarget target(lane == 0 && out.target ? out.target[r] : -1);
   float v[R + (R & 1)];
   ScoreSum a{-INFINITY, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < R; ++i) v[i] = i * 32 + lane < out.vocab ? score_load(x + i * 32 + lane) : -INFINITY;
   if (R & 1) v[R] = -INFINITY;
+  target.load(x, out.vocab);
 #pragma unroll
   for (int i = 0; i < R; ++i) a.m = fmaxf(a.m, v[i]);
   const float lane_max = a.m;
-  a.m = warp_max(a.m);
+  a.m = warp_largest(a.m);
   const float base = a.m == -INFINITY ? 0.f : a.m;
   uint64_t s = 0, u = 0;
 #pragma unroll
   for (int i = 0; i < R; i += 2) score_add2(pair2(v[i], v[i + 1]), pair2(-base, -base), s, u);
   a.s = warp_sum(low2(s) + high2(s));
   a.u = warp_sum(low2(u) + high2(u));
-  if (lane == 0) {
-    ScoreTarget target(out.target ? out.target[r] : -1);
-    target.load(x, out.vocab);
-    score_write_row(out, target, r, a);
-  }
+  if (lane == 0) score_write_row(out, target, r, a);
   if (out.top == 0) return;
   const float log_s = logf(a.s);
   auto write = [&](int k, uint64_t key) {
@@ -222,22 +236,32 @@ __global__ void __launch_bounds__(128) token_scores_narrow_kernel(const T* logit
         score_logp(score_value(static_cast<uint32_t>(key >> 32)), a, base, log_s);
   };
 
-  uint32_t bar = score_order(lane_max);
-#pragma unroll
-  for (int size = 2; size <= 32; size *= 2)  // a bitonic sort of the lanes' maxima, the largest first
-#pragma unroll
-    for (int step = size / 2; step > 0; step /= 2) {
-      const uint32_t o = __shfl_xor_sync(0xffffffffu, bar, step);
-      const bool larger = ((lane & step) == 0) == ((lane & size) == 0);
-      bar = larger ? max(bar, o) : min(bar, o);
+  float bar = a.m;  // -inf: fewer than `top` lanes hold more than forbidden tokens
+  if (out.top <= kScoreRounds) {
+    float left = lane_max;
+    for (int above = 0;;) {
+      const bool is = left == bar;
+      above += __popc(__ballot_sync(0xffffffffu, is));
+      if (above >= out.top || bar == -INFINITY) break;
+      if (is) left = -INFINITY;
+      bar = warp_largest(left);
     }
-  bar = __shfl_sync(0xffffffffu, bar, out.top - 1);
+  } else {
+    bar = lane_max;
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2)  // a bitonic sort, the largest first
+#pragma unroll
+      for (int step = size / 2; step > 0; step /= 2) {
+        const float o = __shfl_xor_sync(0xffffffffu, bar, step);
+        bar = ((lane & step) == 0) == ((lane & size) == 0) ? fmaxf(bar, o) : fminf(bar, o);
+      }
+    bar = __shfl_sync(0xffffffffu, bar, out.top - 1);
+  }
   int n = 0;
-  if (bar > kForbidden) {  // else fewer than `top` lanes hold more than forbidden tokens
-    const float least = score_value(bar);
+  if (bar > -INFINITY) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const bool hit = v[i] >= least;
+      const bool hit = v[i] >= bar;
       const uint32_t hits = __ballot_sync(0xffffffffu, hit);
       if (hits == 0) continue;
       const int at = n + __popc(hits & ((1u << lane) - 1));

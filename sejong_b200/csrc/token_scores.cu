@@ -8,8 +8,8 @@
 // (value, ~index) orders them without ties.
 //
 // Each logit is read once from memory.  Measured on B200 (graph replays): 2048 x 50001 bf16 with 20 alternatives 60 us
-// (3.4 TB/s; without alternatives 43.5, 4.7 TB/s), where instructions bound it, not memory: of a warp's 430 for 1024
-// logits, the exponentials' unit takes 32 (8 cycles each), floors and unpacking 64, the alternatives 110.
+// (3.4 TB/s; without alternatives 43.5, 4.7 TB/s), where instructions bound it, not memory: of a warp's 440 for 1024
+// logits, the exponentials' unit takes 32 (8 cycles each), floors and unpacking 64, the alternatives 115.
 // 1024 x 50001 f32 42 us (4.8 TB/s).  The first simple kernel (a pass for the maximum, one for the sums, one for each
 // alternative) took 1629.  Gradient: 2048 x 65537 bf16 85 us (6.3 TB/s), 1024 x 50001 f32 63 us (6.5).
 #include <algorithm>

@@ -7,10 +7,10 @@
 // The alternatives are the `top` largest logits, the lowest index first among equal ones: a key of
 // (value, ~index) orders them without ties.
 //
-// Each logit is read once from memory.  Measured on B200 (graph replays): 2048 x 50001 bf16 with 20 alternatives 60 us
-// (3.4 TB/s; without alternatives 43.5, 4.7 TB/s), where instructions bound it, not memory: of a warp's 440 for 1024
-// logits, the exponentials' unit takes 32 (8 cycles each), floors and unpacking 64, the alternatives 115.
-// 1024 x 50001 f32 42 us (4.8 TB/s).  The first simple kernel (a pass for the maximum, one for the sums, one for each
+// Each logit is read once from memory.  Measured on B200 (graph replays): 2048 x 50001 bf16 with 20 alternatives 56 us
+// (3.7 TB/s; without alternatives 43, 4.8 TB/s), where instructions bound it, not memory: of a warp's 400 for 1024
+// logits, the exponentials' unit takes 32 (8 cycles each), floors and unpacking 64, the alternatives 80.
+// 1024 x 50001 f32 40 us (5.1 TB/s).  The first simple kernel (a pass for the maximum, one for the sums, one for each
 // alternative) took 1629.  Gradient: 2048 x 65537 bf16 85 us (6.3 TB/s), 1024 x 50001 f32 63 us (6.5).
 #include <algorithm>
 #include <climits>
@@ -37,9 +37,9 @@ constexpr int kScorePieces = 5;       // 16-byte pieces of a chunk that a thread
 constexpr int kScoreStage = kScoreThreads * kScorePieces * 16;
 // CTAs of an SM, stages of a CTA's ring.  Small CTAs and small chunks waste less of a row's last chunk, many pieces a
 // thread spread a chunk's fixed cost: with 128 threads, five pieces and seven CTAs, 2048 x 50001 bf16 with 20
-// alternatives takes 60.2 us and 8000 x 2000 f32 47.8; with 256, four and four, 71.4 and 82.3; 128, four and eight,
-// 67.6 and 42.3; 128, six and six, 61.8 and 54.2; 64, eight and nine, 63.5 and 38.6.  A third stage leaves room for
-// five CTAs: 66.9 and 60.8.
+// alternatives takes 55.7 us and 8000 x 2000 f32 48.4; with 256, four and four, 68.2 and 83.5; 128, four and eight,
+// 62.2 and 43.5; 128, six and six, 59.9 and 58.5; 64, eight and nine, 61.7 and 73.2.  A third stage leaves room for
+// five CTAs: 63.0 and 62.3.
 constexpr int kScoreCtas = 7, kScoreStages = 2;
 constexpr int kScoreMaxSplits = 16;
 // The gradient of rows of at most 1024 pieces of 16 bytes: four rows a warp (32768 x 257 f32 13.0 us with eight CTAs of
@@ -51,7 +51,7 @@ constexpr int kGradRows = 4, kGradNarrowCtas = 8, kGradNarrow = 1024;
 template <typename T>
 constexpr int kGradCtas = sizeof(T) == 2 ? 5 : 4;
 constexpr int kScoreHeld = kScoreMaxTop * 16 + kScoreMaxTop;  // candidates: the best of 32 threads' 16, and the list
-constexpr int kScoreNoted = 512;  // pieces with candidates (128 are expected of 2^20 logits)
+constexpr int kScoreNoted = 512, kScoreKept = 128;  // shares of chunks with candidates (of 2^20 logits, 128 noted)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 }  // namespace
 
@@ -100,12 +100,13 @@ SJ_DEVICE float floor_exponent(float x) {
   return y;
 }
 
-// Order-preserving integer of a logit; NaN last.
-SJ_DEVICE uint32_t score_order(float v) {
-  v += 0.f;  // -0 and +0 are equal
+// Order-preserving integer of a logit that is no NaN.
+SJ_DEVICE uint32_t score_up(float v) {
   const uint32_t bits = __float_as_uint(v);
-  return v != v ? 0u : bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+  return bits ^ (static_cast<uint32_t>(static_cast<int32_t>(bits) >> 31) | 0x80000000u);
 }
+// The same where -0 and +0 are equal; NaN last.
+SJ_DEVICE uint32_t score_order(float v) { return v != v ? 0u : score_up(v + 0.f); }
 SJ_DEVICE float score_value(uint32_t up) {
   return __uint_as_float(up == 0u ? 0x7fc00000u : up & 0x80000000u ? up & 0x7fffffffu : ~up);
 }
@@ -312,6 +313,7 @@ struct ScoreChunk {
   SJ_DEVICE static int index(int base, int i) {  // column of the thread's element i; base: of the chunk
     return base + (i / PER * kScoreThreads + static_cast<int>(threadIdx.x)) * PER + i % PER;
   }
+  SJ_DEVICE static uint4 nothing() { return make_uint4(NONE, NONE, NONE, NONE); }
   SJ_DEVICE static uint32_t word(const uint4& q, int i) { return i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w; }
   SJ_DEVICE float at(int i) const {
     const uint4& q = raw[i / PER];
@@ -319,31 +321,20 @@ struct ScoreChunk {
     const uint32_t w = word(q, i % PER / 2);
     return __uint_as_float(i % 2 ? w & 0xffff0000u : w << 16);
   }
-  // The maximum, and those of the pieces, of which bf16 keeps two halves: NaN left out, -inf where there is nothing
-  // else.
-  SJ_DEVICE float largest(uint32_t (&most)[kScorePieces]) const {
+  // The maximum: NaN left out, -inf where there is nothing else.
+  SJ_DEVICE float largest() const {
     if (sizeof(T) == 4) {
       float m = -INFINITY;
 #pragma unroll
-      for (int v = 0; v < kScorePieces; ++v) {
-        most[v] = __float_as_uint(fmaxf(fmaxf(at(4 * v), at(4 * v + 1)), fmaxf(at(4 * v + 2), at(4 * v + 3))));
-        m = fmaxf(m, __uint_as_float(most[v]));
-      }
+      for (int i = 0; i < N; ++i) m = fmaxf(m, at(i));
       return m;
     }
     uint32_t m = NONE;
 #pragma unroll
-    for (int v = 0; v < kScorePieces; ++v) {
-      most[v] = NONE;
+    for (int v = 0; v < kScorePieces; ++v)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) asm("max.bf16x2 %0, %0, %1;" : "+r"(most[v]) : "r"(word(raw[v], i)));
-      asm("max.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(most[v]));
-    }
-    return of(m);
-  }
-  SJ_DEVICE static float of(uint32_t most) {
-    if (sizeof(T) == 4) return __uint_as_float(most);
-    return fmaxf(__uint_as_float(most << 16), __uint_as_float(most & 0xffff0000u));
+      for (int i = 0; i < 4; ++i) asm("max.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(word(raw[v], i)));
+    return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
   }
   // The chunk's pieces that lie in the row, on their way to `own`, the thread's place in a stage of shared memory.
   // A chunk inside the row needs no look at its pieces.
@@ -377,7 +368,7 @@ struct ScoreChunk {
 #pragma unroll
     for (int v = 0; v < kScorePieces; ++v) {
       const int j = index(base, v * PER);
-      raw[v] = make_uint4(NONE, NONE, NONE, NONE);
+      raw[v] = nothing();
       if (j >= 0 && j + PER <= vocab) {
         raw[v] = piece(own, v);
       } else if (j < vocab) {
@@ -438,19 +429,20 @@ struct ScoreBest {
   uint64_t list[kScoreMaxTop];
   uint64_t thread_best[kScoreThreads];
   __align__(4) uint16_t group[64];
-  int piece[kScoreNoted];  // columns of the pieces that reached the bar
-  uint32_t bar;
-  int count, pieces;  // of held, of piece
+  int noted[kScoreNoted];  // first columns of the threads' shares of chunks that reached the bar
+  float met[kScoreNoted];  // their maxima
+  int kept[kScoreKept];    // those that reach the last bar
+  float bar;
+  int count, notes, keeps;  // of held, noted, kept
   SJ_DEVICE void clear() {
-    bar = 0;
-    count = pieces = 0;
+    bar = -INFINITY;
+    count = notes = keeps = 0;
   }
 };
 
-// The bar: an order that at least `top` of the part's logits reach.  64 groups of threads keep the largest order
-// they have met, of which 16 bits make the bar no higher than it may be; the `top`-th largest of them is one.  It
-// only rises, so one that is out of date still holds.  0 when fewer than `top` groups hold more than forbidden
-// tokens.
+// The bar: a logit that at least `top` of the part's reach.  64 groups of threads keep the largest order that they
+// have met, of which 16 bits make the bar no higher than it may be; the `top`-th largest of them is one.  One that is
+// out of date still holds.  -inf when fewer than `top` groups hold more than forbidden tokens.
 SJ_DEVICE void score_group(ScoreBest& b, uint32_t order) {
   constexpr int OF = kScoreThreads / 64;  // threads of a group
 #pragma unroll
@@ -473,7 +465,7 @@ SJ_DEVICE void score_raise_bar(ScoreBest& b, int top) {
   const uint32_t other = __shfl_sync(0xffffffffu, v, (top - 2 - lane) & 31) >> 16, low = v & 0xffffu;
   const uint32_t mine = lane < top - 1 ? min(low, other) : lane == top - 1 ? max(low, v >> 16) : 0u;
   const uint32_t bar = __reduce_max_sync(0xffffffffu, mine);
-  if (lane == 0 && bar > kForbidden >> 16) atomicMax(&b.bar, bar << 16);
+  if (lane == 0 && bar > kForbidden >> 16) *const_cast<volatile float*>(&b.bar) = score_value(bar << 16);
 }
 
 // The `top` largest keys of held, which all threads see, in order into list; returns how many there are.
@@ -535,10 +527,10 @@ SJ_DEVICE int score_rank_all(ScoreBest& best, const T* x, int base, int end, int
 
 // Persistent CTAs over the parts of rows, 10 KB at a time; the next chunk, be it of the next part, is on its way
 // to shared memory meanwhile (cp.async; a thread reads back only what it copied, so copies need no barrier).  The
-// sums are each thread's own until the part's end.  Pieces of 16 bytes that reach the bar of the alternatives are
-// noted (of 50001 logits at top = 20 about 70); at the end, each is looked at by a thread of its own and what
-// reaches the bar now is ranked.  After the two barriers of a part's first bar the warps go on without any; in
-// turn, they raise the bar at every other chunk (60.2 us; at every one 61.0).
+// sums are each thread's own until the part's end.  Where a thread's share of a chunk reaches the bar of the
+// alternatives is noted (of 50001 logits at top = 20 about 70 places); at the end, the pieces of those that reach the
+// last bar (about 25) are looked at and the logits that do are ranked.  After the two barriers of a part's first bar
+// the warps go on without any; in turn, they raise the bar at every other chunk (55.7 us; at every one 56.8).
 template <typename T>
 __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
     token_scores_wide_kernel(const T* logits, int ld, int splits, int parts, int* counters, float* partial,
@@ -553,19 +545,19 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
   const uint32_t stages = smem_u32(ring) + t * 16;
   int one;  // not a constant that the compiler sees: gathering a warp's additions costs more than they do
   asm volatile("mov.u32 %0, 1;" : "=r"(one));
-  auto next = [&](int* count, int n) {
+  auto next = [&](int* count) {
     int at;
-    asm volatile("atom.shared.add.u32 %0, [%1], %2;" : "=r"(at) : "r"(smem_u32(count)), "r"(n) : "memory");
+    asm volatile("atom.shared.add.u32 %0, [%1], %2;" : "=r"(at) : "r"(smem_u32(count)), "r"(one) : "memory");
     return at;
   };
   // Files the logits of the piece at column j0 that reach the bar.
   auto look = [&](const T* x, int j0) {
-    const float least = best.bar > kForbidden ? score_value(best.bar) : -INFINITY;
+    const float bar = best.bar;
     auto push = [&](float y, int j) {
-      const int at = next(&best.count, one);
+      const int at = next(&best.count);
       if (at < kScoreHeld) best.held[at] = score_key(y, j);
     };
-    if (best.bar > kForbidden && j0 >= 0 && j0 + Chunk::PER <= vocab) {
+    if (bar > -INFINITY && j0 >= 0 && j0 + Chunk::PER <= vocab) {
       const uint4 q = *reinterpret_cast<const uint4*>(x + j0);
       auto value = [&](int e) {
         const uint32_t w = Chunk::word(q, e * static_cast<int>(sizeof(T)) / 4);
@@ -573,14 +565,14 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
       };
       uint32_t hits = 0;
 #pragma unroll
-      for (int e = 0; e < Chunk::PER; ++e) hits |= value(e) >= least ? 1u << e : 0u;
+      for (int e = 0; e < Chunk::PER; ++e) hits |= value(e) >= bar ? 1u << e : 0u;
       for (; hits; hits &= hits - 1) push(value(__ffs(hits) - 1), j0 + __ffs(hits) - 1);
       return;
     }
 #pragma unroll 1
     for (int j = max(j0, 0); j < min(j0 + Chunk::PER, vocab); ++j) {
       const float y = score_load(x + j);
-      if (score_order(y) >= best.bar) push(y, j);
+      if (!(y < bar)) push(y, j);  // a NaN as well: it comes last
     }
   };
   ScoreWalk<T> ahead(logits, ld, vocab, splits, parts);
@@ -601,14 +593,11 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
       ahead.fetch(stages + (stage == 0 ? kScoreStages - 1 : stage - 1) * kScoreStage);
       stage = stage == kScoreStages - 1 ? 0 : stage + 1;
       if (t == 0 && here.c + 1 == here.c1) target.load(x, vocab);
-      float here_m = -INFINITY;
-      uint32_t most[kScorePieces];
-#pragma unroll
-      for (int v = 0; v < kScorePieces; ++v) most[v] = Chunk::NONE;
+      float here_m = -INFINITY, bar = *const_cast<volatile float*>(&best.bar);
       if (first + warp * 32 * Chunk::PER < vocab) {  // not past the row's end
         Chunk now;
         now.read(x, first, vocab, own);
-        here_m = now.largest(most);
+        here_m = now.largest();
         if (__any_sync(0xffffffffu, here_m > m)) {  // as score_raise
           const float raised = fmaxf(m, here_m);
           const float d = m == raised ? 0.f : fmaxf((m - raised) * kLog2e, -150.f), f = exp2_flush(d);
@@ -623,23 +612,24 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
       }
       if (top == 0) continue;
 
-      score_group(best, score_order(m));  // -inf from nothing: no more than kForbidden
+      score_group(best, score_up(m));  // -inf from nothing: no more than kForbidden
       if (first == here.start) {
         __syncthreads();
         if (warp == 0) score_raise_bar(best, top);
         __syncthreads();
+        bar = best.bar;
       } else if (here.c % 2 == 1 && warp == here.c / 2 % kScoreWarps) {
         score_raise_bar(best, top);
       }
-      // the pieces whose maximum reaches the bar are few: they are noted, and looked at once the bar has risen
-      const uint32_t reach = *const_cast<volatile uint32_t*>(&best.bar);
-      const float least = reach > kForbidden ? score_value(reach) : -INFINITY;
-      if (here_m >= least && Chunk::index(first, 0) < vocab) {  // a thread's first element is its lowest
-        uint32_t hot = 0;
-#pragma unroll
-        for (int v = 0; v < kScorePieces; ++v) hot |= Chunk::of(most[v]) >= least ? 1u << v : 0u;
-        for (int at = next(&best.pieces, __popc(hot)); hot && at < kScoreNoted; hot &= hot - 1)
-          best.piece[at++] = Chunk::index(first, (__ffs(hot) - 1) * Chunk::PER);
+      // the threads that meet the bar are few: they are noted, and looked at once the bar has risen
+      bar = *const_cast<volatile float*>(&best.bar);
+      const int column = Chunk::index(first, 0);  // a thread's first element is its lowest
+      if (here_m >= bar && column < vocab) {
+        const int at = next(&best.notes);
+        if (at < kScoreNoted) {
+          best.noted[at] = column;
+          best.met[at] = here_m;
+        }
       }
     }
 
@@ -649,11 +639,18 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
     int n = 0;
     __syncthreads();
     if (top > 0) {
-      const int pieces = best.pieces;
-      if (pieces <= kScoreNoted)
-        for (int i = t; i < pieces; i += kScoreThreads) look(x, best.piece[i]);
+      const int notes = best.notes;
+      for (int i = t; i < min(notes, kScoreNoted); i += kScoreThreads)
+        if (best.met[i] >= best.bar) {
+          const int at = next(&best.keeps);
+          if (at < kScoreKept) best.kept[at] = best.noted[i];
+        }
       __syncthreads();
-      n = pieces > kScoreNoted || best.count > kScoreHeld
+      const int keeps = best.keeps;
+      for (int i = t; i < min(keeps, kScoreKept) * kScorePieces; i += kScoreThreads)
+        look(x, best.kept[i / kScorePieces] + i % kScorePieces * (Chunk::PER * kScoreThreads));
+      __syncthreads();
+      n = notes > kScoreNoted || keeps > kScoreKept || best.count > kScoreHeld
               ? score_rank_all(best, x, here.start, min(vocab, here.origin + here.c1 * Chunk::SIZE), top)
               : score_rank(best, top);
       if (t == 0) best.clear();  // seen by all after the next part's first barrier

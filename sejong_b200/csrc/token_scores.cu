@@ -593,7 +593,7 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
       ahead.fetch(stages + (stage == 0 ? kScoreStages - 1 : stage - 1) * kScoreStage);
       stage = stage == kScoreStages - 1 ? 0 : stage + 1;
       if (t == 0 && here.c + 1 == here.c1) target.load(x, vocab);
-      float here_m = -INFINITY, bar = *const_cast<volatile float*>(&best.bar);
+      float here_m = -INFINITY;
       if (first + warp * 32 * Chunk::PER < vocab) {  // not past the row's end
         Chunk now;
         now.read(x, first, vocab, own);
@@ -617,12 +617,11 @@ __global__ void __launch_bounds__(kScoreThreads, kScoreCtas)
         __syncthreads();
         if (warp == 0) score_raise_bar(best, top);
         __syncthreads();
-        bar = best.bar;
       } else if (here.c % 2 == 1 && warp == here.c / 2 % kScoreWarps) {
         score_raise_bar(best, top);
       }
       // the threads that meet the bar are few: they are noted, and looked at once the bar has risen
-      bar = *const_cast<volatile float*>(&best.bar);
+      const float bar = *const_cast<volatile float*>(&best.bar);
       const int column = Chunk::index(first, 0);  // a thread's first element is its lowest
       if (here_m >= bar && column < vocab) {
         const int at = next(&best.notes);

@@ -24,13 +24,13 @@ namespace sj {
 namespace {
 constexpr int kScoreMaxTop = 32;
 constexpr int kScoreNarrow = 1024;    // rows of at most this many logits are held by one warp
-// CTAs of an SM, of the kernel that holds R logits a lane: 32768 x 257 f32 with 5 alternatives 21.9 us with ten, 22.5
-// with nine, 23.1 with twelve; 32768 x 500 27.9 with nine, 27.3 with ten; 32768 x 1000 42.5 with seven, 40.5 with eight
-// (some spills), 63.9 without a limit on registers.
+// CTAs of an SM, of the kernel that holds R logits a lane: 32768 x 257 f32 with 5 alternatives 20.6 us with nine, 20.2
+// with ten, 19.9 with twelve; 32768 x 500 23.7 with ten, 24.2 with twelve, 28.1 without a limit on registers; 32768 x
+// 1000 32.6 with seven, 31.8 with eight, 32.3 with nine, 42.5 without a limit.
 template <int R>
-constexpr int kScoreNarrowCtas = R <= 16 ? 10 : 8;
-// Alternatives up to which their bar is found one by one, not by a sort: at 32768 x 257 one alternative takes 17.2 us,
-// not 20.1, five 21.9, not 22.9, and ten the same either way.
+constexpr int kScoreNarrowCtas = R <= 9 ? 12 : R <= 16 ? 10 : 8;
+// Alternatives up to which their bar is found one by one, not by a sort: at 32768 x 257 one alternative takes 16.9 us,
+// not 19.7, five 20.2, not 21.0, and ten the same either way.
 constexpr int kScoreRounds = 8;
 constexpr int kScoreThreads = 128, kScoreWarps = kScoreThreads / 32;  // of the kernel for wider rows
 constexpr int kScorePieces = 5;       // 16-byte pieces of a chunk that a thread takes
@@ -260,14 +260,17 @@ __global__ void __launch_bounds__(128, kScoreNarrowCtas<R>)
   }
   int n = 0;
   if (bar > -INFINITY) {
+    uint32_t left = 0;
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const bool hit = v[i] >= bar;
-      const uint32_t hits = __ballot_sync(0xffffffffu, hit);
-      if (hits == 0) continue;
-      const int at = n + __popc(hits & ((1u << lane) - 1));
-      if (hit && at < 64) listed[warp][at] = score_key(v[i], i * 32 + lane);
-      n += __popc(hits);
+    for (int i = 0; i < R; ++i) left |= v[i] >= bar ? 1u << i : 0u;
+    for (uint32_t have; (have = __ballot_sync(0xffffffffu, left != 0)) != 0;) {
+      const int at = n + __popc(have & ((1u << lane) - 1));
+      if (left) {
+        const int j = (__ffs(left) - 1) * 32 + lane;
+        if (at < 64) listed[warp][at] = score_key(score_load(x + j), j);
+        left &= left - 1;
+      }
+      n += __popc(have);
     }
     __syncwarp();
   }

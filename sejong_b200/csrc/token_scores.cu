@@ -23,12 +23,17 @@ namespace sj {
 
 namespace {
 constexpr int kScoreMaxTop = 32;
-constexpr int kScoreNarrow = 1024;    // rows of at most this many logits are held by one warp
+// Rows of at most this many logits are held by one warp: 8000 x 2000 f32 with 20 alternatives 22.2 us, 48.6 by the
+// kernel for wide rows, bf16 25.8 and 52.2; 4000 x 4096 f32 24.4 and 33.1, but bf16, loaded two bytes at a time, 33.0
+// and 27.8.
+template <typename T>
+constexpr int kScoreNarrow = sizeof(T) == 4 ? 4096 : 2048;
 // CTAs of an SM, of the kernel that holds R logits a lane: 32768 x 257 f32 with 5 alternatives 20.6 us with nine, 20.2
 // with ten, 19.9 with twelve; 32768 x 500 23.7 with ten, 24.2 with twelve, 28.1 without a limit on registers; 32768 x
-// 1000 32.6 with seven, 31.8 with eight, 32.3 with nine, 42.5 without a limit.
+// 1000 32.6 with seven, 31.8 with eight, 32.3 with nine, 42.5 without a limit; 16000 x 1100 36.9 with four, 34.5 with
+// five; 4000 x 4096 28.8 with two, 24.3 with three.
 template <int R>
-constexpr int kScoreNarrowCtas = R <= 9 ? 12 : R <= 16 ? 10 : 8;
+constexpr int kScoreNarrowCtas = R <= 9 ? 12 : R <= 16 ? 10 : R <= 32 ? 8 : R <= 64 ? 5 : 3;
 // Alternatives up to which their bar is found one by one, not by a sort: at 32768 x 257 one alternative takes 16.9 us,
 // not 19.7, five 20.2, not 21.0, and ten the same either way.
 constexpr int kScoreRounds = 8;
@@ -37,9 +42,9 @@ constexpr int kScorePieces = 5;       // 16-byte pieces of a chunk that a thread
 constexpr int kScoreStage = kScoreThreads * kScorePieces * 16;
 // CTAs of an SM, stages of a CTA's ring.  Small CTAs and small chunks waste less of a row's last chunk, many pieces a
 // thread spread a chunk's fixed cost: with 128 threads, five pieces and seven CTAs, 2048 x 50001 bf16 with 20
-// alternatives takes 55.7 us and 8000 x 2000 f32 48.4; with 256, four and four, 68.2 and 83.5; 128, four and eight,
-// 62.2 and 43.5; 128, six and six, 59.9 and 58.5; 64, eight and nine, 61.7 and 73.2.  A third stage leaves room for
-// five CTAs: 63.0 and 62.3.
+// alternatives takes 55.7 us and 1024 x 50001 f32 40.0; with 256, four and four, 68.2 and 49.7; 128, four and eight,
+// 62.2 and 43.0; 128, six and six, 59.9 and 51.2; 64, eight and nine, 61.7 and 45.8.  A third stage leaves room for
+// five CTAs: 63.0 and 48.7.
 constexpr int kScoreCtas = 7, kScoreStages = 2;
 constexpr int kScoreMaxSplits = 16;
 // The gradient of rows of at most 1024 pieces of 16 bytes: four rows a warp (32768 x 257 f32 13.0 us with eight CTAs of
@@ -260,17 +265,20 @@ __global__ void __launch_bounds__(128, kScoreNarrowCtas<R>)
   }
   int n = 0;
   if (bar > -INFINITY) {
-    uint32_t left = 0;
 #pragma unroll
-    for (int i = 0; i < R; ++i) left |= v[i] >= bar ? 1u << i : 0u;
-    for (uint32_t have; (have = __ballot_sync(0xffffffffu, left != 0)) != 0;) {
-      const int at = n + __popc(have & ((1u << lane) - 1));
-      if (left) {
-        const int j = (__ffs(left) - 1) * 32 + lane;
-        if (at < 64) listed[warp][at] = score_key(score_load(x + j), j);
-        left &= left - 1;
+    for (int i0 = 0; i0 < R; i0 += 32) {
+      uint32_t left = 0;
+#pragma unroll
+      for (int i = i0; i < R && i < i0 + 32; ++i) left |= v[i] >= bar ? 1u << (i - i0) : 0u;
+      for (uint32_t have; (have = __ballot_sync(0xffffffffu, left != 0)) != 0;) {
+        const int at = n + __popc(have & ((1u << lane) - 1));
+        if (left) {
+          const int j = (i0 + __ffs(left) - 1) * 32 + lane;
+          if (at < 64) listed[warp][at] = score_key(score_load(x + j), j);
+          left &= left - 1;
+        }
+        n += __popc(have);
       }
-      n += __popc(have);
     }
     __syncwarp();
   }
@@ -924,7 +932,7 @@ int score_ctas() { return kScoreCtas * sm_count(); }
 // two, 26.6 in three; 128 x 130000 f32: 32.5 us in two, 24.8 in four, 24.1 in seven).  For the same reason a partly
 // filled last round of whole rows is left as it is.
 int score_splits(int rows, int vocab) {
-  if (vocab <= kScoreNarrow || rows <= 0) return 1;
+  if (rows <= 0) return 1;
   const int fill = (score_ctas() * 2 / 5 + rows - 1) / rows;
   return std::max(1, std::min({fill, (vocab + 4095) / 4096, kScoreMaxSplits}));
 }
@@ -932,12 +940,14 @@ size_t score_counter_bytes(int rows) { return (static_cast<size_t>(rows) * sizeo
 
 template <typename T>
 int scores(const T* logits, int ld, int rows, const ScoreOut& out, void* workspace, cudaStream_t stream) {
-  if (out.vocab <= kScoreNarrow) {
+  if (out.vocab <= kScoreNarrow<T>) {
     const int regs = (out.vocab + 31) / 32, grid = (rows + 3) / 4;
     launch(regs <= 4   ? token_scores_narrow_kernel<T, 4>
            : regs <= 9 ? token_scores_narrow_kernel<T, 9>
            : regs <= 16 ? token_scores_narrow_kernel<T, 16>
-                        : token_scores_narrow_kernel<T, 32>,
+           : regs <= 32 ? token_scores_narrow_kernel<T, 32>
+           : regs <= 64 ? token_scores_narrow_kernel<T, 64>
+                        : token_scores_narrow_kernel<T, kScoreNarrow<T> / 32>,
            grid, 128, 0, stream, logits, ld, rows, out);
   } else {
     const int splits = score_splits(rows, out.vocab), smem = kScoreStages * kScoreStage;

@@ -114,6 +114,22 @@ def test_scores_of_ties_and_orders(vocab, kind):
         check_scores(x, target, vocab, top)
 
 
+@pytest.mark.parametrize("vocab", [512, 513, 1024, 1025, 2047, 2048, 2049, 4095, 4096, 4097])
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+def test_scores_around_the_widths_of_the_kernels(vocab, kind):
+    """Random rows, equal ones, few distinct values, all but a few forbidden, the best at either end."""
+    x, target = logits(9, vocab, vocab + 3, kind, vocab)
+    step = torch.arange(vocab, device=DEV)
+    x[1, :vocab] = 2.0
+    x[2, :vocab] = (step % 5).to(kind)
+    x[3, :vocab] = torch.where(step % 31 == 7, x[3, :vocab], torch.tensor(-float("inf"), dtype=kind, device=DEV))
+    x[4, vocab - 1], x[4, 0] = 30.0, 30.0
+    x[5, :vocab] = torch.where(step >= vocab - 40, 40.0, 0.0).to(kind)
+    target[:6] = vocab - 1
+    for top in (0, 1, 8, 9):
+        check_scores(x, target, vocab, top)
+
+
 @pytest.mark.parametrize("vocab", [5001, 40000])
 @pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
 def test_scores_of_peaks_anywhere(vocab, kind):

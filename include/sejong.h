@@ -418,7 +418,8 @@ int sj_attn_paged(const void* q, int ldq, const void* k_cache, const void* v_cac
  *                        records SJ_DEV_BAD_INDEX.  Logits of -inf are forbidden tokens (log probability -inf);
  *                        a row of nothing else has lse -inf, entropy 0.  workspace:
  *                        sj_token_scores_workspace bytes, zero before its first use (each call leaves it ready for
- *                        the next); one per stream.
+ *                        the next, of any size); one per stream.  Fewer rows may take more bytes, since they are
+ *                        cut into parts: a buffer for several sizes takes the largest of theirs.
  *   sj_token_scores_bwd  d_logits [rows, ldd] (the logits' type; columns vocab..ldd zeroed) = d_logp (1[target] - p)
  *                        - d_entropy p (log p + entropy) with p = e^(logits - lse); d_logp or d_entropy may be null
  *                        (zero), entropy when d_entropy is.  A target of -1 takes no d_logp.  d_logits may be the

@@ -927,16 +927,19 @@ using namespace sj;
 
 namespace {
 int score_ctas() { return kScoreCtas * sm_count(); }
+// Rows are cut into parts where there are fewer than this many of them.
+int score_cut_rows() { return score_ctas() * 2 / 5; }
 // Parts of a row, of at least 4096 logits: the fewest that give two CTAs of five one, since a CTA that has its SM to
 // itself runs faster and a part costs its own ranking and a share of a join (400 x 32000 f32: 19.0 us whole, 20.7 in
 // two, 26.6 in three; 128 x 130000 f32: 32.5 us in two, 24.8 in four, 24.1 in seven).  For the same reason a partly
 // filled last round of whole rows is left as it is.
 int score_splits(int rows, int vocab) {
-  if (rows <= 0) return 1;
-  const int fill = (score_ctas() * 2 / 5 + rows - 1) / rows;
+  if (rows <= 0 || rows >= score_cut_rows()) return 1;
+  const int fill = (score_cut_rows() + rows - 1) / rows;
   return std::max(1, std::min({fill, (vocab + 4095) / 4096, kScoreMaxSplits}));
 }
-size_t score_counter_bytes(int rows) { return (static_cast<size_t>(rows) * sizeof(int) + 255) / 256 * 256; }
+// Counters of a workspace, ahead of the parts: of a fixed size, so that no call's parts lie on another call's counters.
+size_t score_counter_bytes() { return (static_cast<size_t>(score_cut_rows()) * sizeof(int) + 255) / 256 * 256; }
 
 template <typename T>
 int scores(const T* logits, int ld, int rows, const ScoreOut& out, void* workspace, cudaStream_t stream) {
@@ -959,7 +962,7 @@ int scores(const T* logits, int ld, int rows, const ScoreOut& out, void* workspa
     if (rc != SJ_OK) return rc;
     launch(token_scores_wide_kernel<T>, std::min(rows * splits, score_ctas()), kScoreThreads, smem, stream, logits, ld,
            splits, rows * splits, static_cast<int*>(workspace),
-           reinterpret_cast<float*>(static_cast<char*>(workspace) + score_counter_bytes(rows)), out);
+           reinterpret_cast<float*>(static_cast<char*>(workspace) + score_counter_bytes()), out);
   }
   SJ_LAUNCH_CHECK("token_scores");
   return SJ_OK;
@@ -996,7 +999,7 @@ extern "C" size_t sj_token_scores_workspace(int rows, int vocab, int top) {
   if (rows < 0 || vocab <= 0 || top < 0 || top > kScoreMaxTop) return 0;
   const int splits = score_splits(rows, vocab);
   if (splits == 1) return 16;
-  return score_counter_bytes(rows) + static_cast<size_t>(rows) * splits * score_part(top) * sizeof(float);
+  return score_counter_bytes() + static_cast<size_t>(rows) * splits * score_part(top) * sizeof(float);
 }
 
 extern "C" int sj_token_scores(const void* logits, int dtype, int ld, const int32_t* target, int rows, int vocab,

@@ -312,3 +312,22 @@ def test_gradient_against_differences_of_the_forward_kernel():
         quotient = (value[0] - value[1]) / step
         size = 1 + np.abs(a.cpu().numpy()) + np.abs(b.cpu().numpy())
         assert (np.abs(quotient - g[:, j]) <= size * (h * h / 3 + 2.0 ** -17 / h)).all()
+
+
+# ---------------------------------------------------------------- workspaces and parts of rows
+def test_one_workspace_serves_any_sizes_in_turn():
+    """Zeroed once: what a call leaves in it is no count of a later call with more or fewer rows, columns or
+    alternatives.  Each call equals one with a workspace of its own."""
+    from sejong_b200 import _lib
+    sizes = [(8, 50001, 20), (128, 50001, 20), (8, 50001, 20), (1, 9001, 3), (400, 9001, 32), (64, 131072, 0), (413, 5001, 7),
+             (2, 50001, 1)]
+    size = max(_lib.load().sj_token_scores_workspace(*s) for s in sizes)
+    work = torch.zeros(size, dtype=torch.uint8, device=DEV)
+    for i, (rows, vocab, top) in enumerate(sizes):
+        x, target = logits(rows, vocab, vocab, torch.float32, 100 + i)
+        stats = [torch.full((rows,), 9.0, device=DEV) for _ in range(3)]
+        ids, best = torch.full((rows, top), -9, dtype=torch.int32, device=DEV), torch.full((rows, top), 9.0, device=DEV)
+        _lib.call("sj_token_scores", ptr(x), F32, vocab, ptr(target), rows, vocab, top, *[ptr(t) for t in stats], ptr(ids),
+                  ptr(best), ptr(work), size, stream())
+        for got, own in zip((*stats, ids, best), run_scores(x, target, vocab, top)):
+            np.testing.assert_array_equal(got.cpu().numpy(), own, err_msg=str((rows, vocab, top)))

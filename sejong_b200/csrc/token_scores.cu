@@ -415,7 +415,7 @@ struct ScoreWalk {
     x = logits + static_cast<size_t>(r) * ld;
     origin = -static_cast<int>(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
     const int chunks = (vocab - origin + ScoreChunk<T>::SIZE - 1) / ScoreChunk<T>::SIZE;
-    c = splits == 1 ? 0 : chunks * k / splits;  // at most 2^19 chunks, 16 splits
+    c = splits == 1 ? 0 : chunks * k / splits;  // at most 2^20 chunks, 16 splits; a chunk a part at least
     c1 = splits == 1 ? chunks : chunks * (k + 1) / splits;
     start = base();
   }
@@ -929,9 +929,9 @@ namespace {
 int score_ctas() { return kScoreCtas * sm_count(); }
 // Rows are cut into parts where there are fewer than this many of them.
 int score_cut_rows() { return score_ctas() * 2 / 5; }
-// Parts of a row, of at least 4096 logits: the fewest that give two CTAs of five one, since a CTA that has its SM to
-// itself runs faster and a part costs its own ranking and a share of a join (400 x 32000 f32: 19.0 us whole, 20.7 in
-// two, 26.6 in three; 128 x 130000 f32: 32.5 us in two, 24.8 in four, 24.1 in seven).  For the same reason a partly
+// Parts of a row, one for each 4096 logits at most: the fewest that give two CTAs of five one, since a CTA that has its
+// SM to itself runs faster and a part costs its own ranking and a share of a join (400 x 32000 f32: 19.0 us whole, 20.7
+// in two, 26.6 in three; 128 x 130000 f32: 32.5 us in two, 24.8 in four, 24.1 in seven).  For the same reason a partly
 // filled last round of whole rows is left as it is.
 int score_splits(int rows, int vocab) {
   if (rows <= 0 || rows >= score_cut_rows()) return 1;
@@ -953,7 +953,9 @@ int scores(const T* logits, int ld, int rows, const ScoreOut& out, void* workspa
                         : token_scores_narrow_kernel<T, kScoreNarrow<T> / 32>,
            grid, 128, 0, stream, logits, ld, rows, out);
   } else {
-    const int splits = score_splits(rows, out.vocab), smem = kScoreStages * kScoreStage;
+    // No more parts than chunks: the CTA that ends a row writes the target's logit that it read at its part's last chunk.
+    const int chunks = (out.vocab - 1) / ScoreChunk<T>::SIZE + 1, smem = kScoreStages * kScoreStage;
+    const int splits = std::min(score_splits(rows, out.vocab), chunks);
     if (static_cast<int64_t>(rows) * splits > INT_MAX - score_ctas())
       return fail(SJ_ERR_SHAPE, "sj_token_scores: rows=%d vocab=%d", rows, out.vocab);
     static KernelAttrOnce once;

@@ -331,3 +331,22 @@ def test_one_workspace_serves_any_sizes_in_turn():
                   ptr(best), ptr(work), size, stream())
         for got, own in zip((*stats, ids, best), run_scores(x, target, vocab, top)):
             np.testing.assert_array_equal(got.cpu().numpy(), own, err_msg=str((rows, vocab, top)))
+
+
+@pytest.mark.parametrize("rows,vocab", [(64, 5000), (32, 50001), (3, 8193), (100, 16400)])
+@pytest.mark.parametrize("top", [0, 20])
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+def test_no_part_of_a_row_is_empty(rows, vocab, top, kind):
+    """The part that is done last writes the row with the target's logit that it has read; one of no columns would have
+    read none.  It would also leave its maximum, -inf, in the workspace."""
+    from sejong_b200 import _lib
+    x, target = logits(rows, vocab, vocab, kind, rows)
+    target = target.clamp(min=0)
+    check_scores(x, target, vocab, top)
+    out = [torch.empty(rows, device=DEV) for _ in range(3)]
+    ids, best = torch.empty(rows, top, dtype=torch.int32, device=DEV), torch.empty(rows, top, device=DEV)
+    size = _lib.load().sj_token_scores_workspace(rows, vocab, top)
+    work = torch.zeros(size, dtype=torch.uint8, device=DEV)
+    _lib.call("sj_token_scores", ptr(x), F32 if kind == torch.float32 else BF16, vocab, ptr(target), rows, vocab, top,
+              *[ptr(t) for t in out], ptr(ids), ptr(best), ptr(work), size, stream())
+    assert not torch.isneginf(work.view(torch.float32)).any()

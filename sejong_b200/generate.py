@@ -54,11 +54,16 @@ def _uniform(state):
     return np.float32(((x >> 40) + 0.5) / 16777216.0)
 
 
+def check_sampling(options):
+    """What sample_prepared asks of its options (lib.rs:44-78)."""
+    if options.temperature != options.temperature or options.temperature < 0 or not 0 < options.top_p <= 1:
+        raise ValueError("sampling requires temperature >= 0 and top_p in (0, 1]")
+
+
 def sample(logits, options, state):
     """sample_prepared (lib.rs:44-78): rank by logit (stable, descending), argmax at temperature 0,
     else top-k, exp((v - max) / T), the top-p prefix, and a draw of Rng::uniform * total."""
-    if options.temperature != options.temperature or options.temperature < 0 or not 0 < options.top_p <= 1:
-        raise ValueError("sampling requires temperature >= 0 and top_p in (0, 1]")
+    check_sampling(options)
     x = np.asarray(logits, dtype=np.float32)
     if not np.all(np.isfinite(x)):
         raise ValueError("sampling requires finite logits")

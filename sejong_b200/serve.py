@@ -29,7 +29,7 @@ import torch
 from . import _lib
 from ._lib import (EPI_RESIDUAL, EPI_ROPE, EPI_STORE, EPI_SWIGLU, ROPE_BASE, ROPE_LINEAR, ROPE_RAMP, SJ_BF16, SJ_F32,
                    call)
-from .generate import Sampling, _ptr, sample
+from .generate import Sampling, _ptr, check_sampling, sample
 from .model import EOS, HEAD_DIM, VOCAB, VOCAB_PAD, FlatLayout, global_stage, initialize
 
 
@@ -228,6 +228,24 @@ class BatchGenerator:
         self._head(0, B, self.logits)
 
     # ---------------------------------------------------------------- steps
+    def _clear(self):
+        """An empty cache without requests, whatever a call that was broken off has left."""
+        self.slots = [None] * self.batch
+        self.finished.clear()
+        self.reserved = 0
+        for t in (self.cached, self.lengths, self.summary):
+            t.zero_()
+        self.table.fill_(-1)
+        torch.arange(self.pages, out=self.free)
+        self.free_count.fill_(self.pages)
+        self._device_error()
+
+    def _device_error(self):
+        """The device error word, which is cleared."""
+        code = ctypes.c_int(0)
+        call("sj_device_error", ctypes.byref(code), 1, self._stream())
+        return code.value
+
     def _write(self, added, ids):
         """The host's part of a step: tokens added by slot, pages to return, token ids of the rows."""
         B = self.batch
@@ -323,7 +341,16 @@ class BatchGenerator:
                 raise ValueError(f"a request may need {q.reserved} pages of a cache of {self.pages}")
             if q.options.max_bytes < 1:
                 raise ValueError("max_bytes must be positive")
-        results = [None] * len(prompts)
+            check_sampling(q.options)
+        try:
+            return self._run(waiting, top)
+        except BaseException:
+            self._clear()
+            raise
+
+    def _run(self, waiting, top):
+        """The completions of the waiting requests, in the order of their indices."""
+        results = [None] * len(waiting)
 
         def take(done):
             for i, completion in done:
@@ -345,10 +372,9 @@ class BatchGenerator:
             if live:
                 self._step(live)
                 take(self._draw(live, top))
-        code = ctypes.c_int(0)
-        call("sj_device_error", ctypes.byref(code), 1, self._stream())
-        if code.value:
-            raise RuntimeError(f"device error {code.value} during generation")
+        code = self._device_error()
+        if code:
+            raise RuntimeError(f"device error {code} during generation")
         return results
 
     def score(self, text, top=0):

@@ -200,3 +200,55 @@ def test_commands(tmp_path, made):
     cli.score(where, prompts, 1, out=out)
     record = json.loads(out.getvalue())
     assert record["bytes"] == 18 and len(record["logp"]) == 18 and record["bits_per_byte"] > 0
+
+
+# ---------------------------------------------------------------- calls that fail
+def _all_pages_free(gen):
+    gen._write({}, [])
+    gen._commit_and_plan(0)
+    torch.cuda.synchronize()
+    assert gen.free_count.item() == gen.pages and sorted(gen.free.tolist()) == list(range(gen.pages))
+    assert (gen.lengths == 0).all() and gen.reserved == 0 and gen.slots == [None] * gen.batch
+
+
+@pytest.mark.parametrize("bad", [dict(top_p=0.0), dict(top_p=1.5), dict(temperature=-1.0),
+                                 dict(temperature=float("nan"))])
+def test_generate_checks_the_options_before_it_takes_a_request(made, bad):
+    from sejong_b200.generate import Sampling
+    from sejong_b200.serve import BatchGenerator
+    c, params = made
+    gen = BatchGenerator(c, params, device=0, context=64, batch=2, page=16)
+    good = Sampling(max_bytes=5, temperature=0.9, seed=3)
+    want = gen.generate([b"good", b"ones"], good, top=1)
+    with pytest.raises(ValueError, match="temperature"):
+        gen.generate([b"first", b"bad"], [good, Sampling(max_bytes=5, **bad)], top=1)
+    _all_pages_free(gen)
+    assert gen.generate([b"good", b"ones"], good, top=1) == want
+
+
+@pytest.mark.parametrize("at", ["first draw", "later draw", "between the host's write and the step", "step"])
+def test_generate_after_a_call_that_was_broken_off(made, monkeypatch, at):
+    """Whatever a call that raised has left behind, the next one starts from an empty cache."""
+    from sejong_b200.generate import Sampling
+    from sejong_b200.serve import BatchGenerator
+    c, params = made
+    gen = BatchGenerator(c, params, device=0, context=64, batch=2, page=16)
+    good = Sampling(max_bytes=8, temperature=0.9, seed=3)
+    want = gen.generate([b"good", b"ones", b"more"], good, top=1)
+    name, calls = {"first draw": ("_draw", 1), "later draw": ("_draw", 6), "step": ("_step", 2),
+                   "between the host's write and the step": ("_commit_and_plan", 2)}[at]
+    whole, count = getattr(gen, name), [0]
+
+    def broken(*args):
+        count[0] += 1
+        if count[0] == calls:
+            raise KeyboardInterrupt
+        return whole(*args)
+
+    with monkeypatch.context() as m:
+        m.setattr(gen, name, broken)
+        with pytest.raises(KeyboardInterrupt):
+            gen.generate([b"a", b"b", b"c", b"d"], Sampling(max_bytes=30, temperature=1.0), top=0)
+    assert count[0] == calls
+    assert gen.generate([b"good", b"ones", b"more"], good, top=1) == want
+    _all_pages_free(gen)

@@ -250,5 +250,7 @@ def test_generate_after_a_call_that_was_broken_off(made, monkeypatch, at):
         with pytest.raises(KeyboardInterrupt):
             gen.generate([b"a", b"b", b"c", b"d"], Sampling(max_bytes=30, temperature=1.0), top=0)
     assert count[0] == calls
+    # one request: had it the old ones beside it, their completions would go past its results
+    assert gen.generate([b"good"], good, top=1) == want[:1]
     assert gen.generate([b"good", b"ones", b"more"], good, top=1) == want
     _all_pages_free(gen)

@@ -128,6 +128,7 @@ class BatchGenerator:
         self.input = z(2 * B + rows)
         self.added, self.release, self.ids = self.input[:B], self.input[B:2 * B], self.input[2 * B:]
         self.cached, self.lengths, self.summary = z(B), z(B), z(4)
+        self.planned = torch.zeros(4, dtype=torch.int32, pin_memory=True)  # the host's copy of the summary
         self.table = torch.full((B, self.width), -1, dtype=torch.int32, device=self.dev)
         self.free = torch.arange(self.pages, dtype=torch.int32, device=self.dev)
         self.free_count = torch.full((1,), self.pages, dtype=torch.int32, device=self.dev)
@@ -299,7 +300,11 @@ class BatchGenerator:
 
     def _draw(self, slots, top):
         """A byte for each of the slots from its row of logits; finished requests leave.  Returns what finished."""
+        self.planned.copy_(self.summary, non_blocking=True)  # here when the logits are
         logits = self.logits[:len(slots), :VOCAB].cpu().numpy()
+        status = int(self.planned[2])
+        if status:
+            raise RuntimeError(f"a step could not be planned: status {status}")
         tokens = [sample(logits[r], self.slots[b].options, self.slots[b].state) for r, b in enumerate(slots)]
         scores = None if top is None else self._scores(self.logits, tokens, top)
         done = []

@@ -254,3 +254,29 @@ def test_generate_after_a_call_that_was_broken_off(made, monkeypatch, at):
     assert gen.generate([b"good"], good, top=1) == want[:1]
     assert gen.generate([b"good", b"ones", b"more"], good, top=1) == want
     _all_pages_free(gen)
+
+
+def test_generate_reports_a_step_that_could_not_be_planned(made):
+    """A cache whose free pages are gone: an error, not bytes of a step that never ran; the next call is whole again."""
+    from sejong_b200.generate import Sampling
+    from sejong_b200.serve import BatchGenerator
+    c, params = made
+    gen = BatchGenerator(c, params, device=0, context=64, batch=2, page=4)
+    good = Sampling(max_bytes=8, temperature=0.9, seed=3)
+    want = gen.generate([b"good", b"ones"], good)
+    _all_pages_free(gen)  # those of finished requests as well, which the next commit would return
+    gen.free_count.zero_()  # no page for a prompt
+    with pytest.raises(RuntimeError, match="status 2"):
+        gen.generate([b"good", b"ones"], good)
+    assert gen.generate([b"good", b"ones"], good) == want
+    start = gen._start
+
+    def last_pages(*args):  # pages for the prompt, none for the step that needs one more
+        start(*args)
+        gen.free_count.fill_(2)  # what the step's commit takes off for the prompt's two pages
+
+    gen._start = last_pages
+    with pytest.raises(RuntimeError, match="status 2"):
+        gen.generate([b"seven b"], Sampling(max_bytes=8, temperature=0.0))
+    del gen._start
+    assert gen.generate([b"good", b"ones"], good) == want

@@ -362,8 +362,9 @@ int sj_scale_to_bf16(const float* x, int n, float alpha, void* y, void* stream);
  *                    repeated call writes the same.
  *   sj_paged_commit  ends the step: *free_count -= pages taken, cached = lengths; requests with release[b] !=
  *                    0 (release may be null) give their pages back to the stack and get length 0.  `pages` is
- *                    the stack's capacity; a stack that would leave [0, pages] stays as it is and records
- *                    SJ_DEV_BAD_INDEX.  summary's first two entries are zeroed, so a second call does nothing.
+ *                    the stack's capacity; a stack that would leave [0, pages], or a page id outside [0, pages) to
+ *                    give back, records SJ_DEV_BAD_INDEX and the call changes nothing.  Otherwise summary's first
+ *                    two entries are zeroed, so a second call does nothing.
  *   sj_paged_append  qkv bf16 [rows, ld] with the heads [hq q | hk k | hk v]: the first rope_dim (a multiple of
  *                    16, or 0) dims of q and k are rotated by position[r]'s row of rope_table (rope_len rows of
  *                    rope_dim / 2 (cos, sin) pairs: sj_rope_table or sj_rope_table_scaled), pairs (2i, 2i+1),

@@ -163,24 +163,27 @@ __global__ void __launch_bounds__(1024) paged_commit_kernel(int32_t* cached, int
     if (release && release[b]) n = min((max(lengths[b], 0) + page - 1) / page, ld_table);
   });
   const int top = *free_count - summary[1], back = page_start[batch];
-  __syncthreads();
-  const bool fits = top >= 0 && top + back <= pages;
-  for (int i = threadIdx.x; fits && i < back; i += blockDim.x) {
+  bool refused = top < 0 || back > pages - top;
+  auto page_of = [&](int i) {
     const int b = owner_of(page_start, batch, i);
-    const int id = table[static_cast<size_t>(b) * ld_table + i - page_start[b]];
-    if (id < 0 || id >= pages) record_error(SJ_DEV_BAD_INDEX);
-    free_pages[top + i] = id;
+    return table[static_cast<size_t>(b) * ld_table + i - page_start[b]];
+  };
+  for (int i = threadIdx.x; !refused && i < back; i += blockDim.x) {
+    const int id = page_of(i);
+    refused = id < 0 || id >= pages;
   }
+  if (__syncthreads_or(refused)) {  // nothing is written yet
+    if (threadIdx.x == 0) record_error(SJ_DEV_BAD_INDEX);
+    return;
+  }
+  for (int i = threadIdx.x; i < back; i += blockDim.x) free_pages[top + i] = page_of(i);
   for (int b = threadIdx.x; b < batch; b += blockDim.x) {
     const bool gone = release && release[b];
     if (gone) lengths[b] = 0;
     cached[b] = gone ? 0 : lengths[b];
   }
   if (threadIdx.x == 0) {
-    if (fits)
-      *free_count = top + back;
-    else
-      record_error(SJ_DEV_BAD_INDEX);
+    *free_count = top + back;
     summary[0] = summary[1] = 0;
   }
 }

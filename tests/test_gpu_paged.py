@@ -497,3 +497,39 @@ def test_attention_offsets_past_32_bits():
          ptr(o), hk * dim, ptr(k), ptr(v), pages, page, *strides(k), stream())
     assert torch.equal(k[-1, :, 36].reshape(-1), qkv[0, hk * dim:2 * hk * dim])
     assert torch.equal(v[-1, :, 36].reshape(-1), qkv[0, 2 * hk * dim:])
+
+
+@pytest.mark.parametrize("bad", [-1, -7, 60, 1 << 30])
+def test_commit_refuses_as_a_whole_what_a_page_id_out_of_range_would_return(bad):
+    p = Planner([5, 9, 0], [1, 4, 2], 4, 60, 6, 16)
+    p.plan()
+    p.check()
+    state = (p.cached, p.lengths, p.free, p.count, p.table, p.summary)
+    good = p.table[1, 2].item()
+    p.table[1, 2] = bad
+    before = [t.clone() for t in state]
+    gone = ints([1, 1, 0])
+    p.commit(gone)
+    assert device_error() == 110
+    assert all(torch.equal(a, b) for a, b in zip(state, before))
+    p.table[1, 2] = good
+    p.commit(gone)
+    assert p.cached.tolist() == p.lengths.tolist() == [0, 0, 2]
+    held = [p.table[2, 0].item()]
+    assert sorted(held + p.free[:p.count.item()].tolist()) == list(range(60))
+
+
+@pytest.mark.parametrize("count,pages", [(None, 50), (2, 60)])
+def test_commit_refuses_as_a_whole_a_stack_out_of_bounds(count, pages):
+    """More pages than the stack has room for, or fewer on it than the step took."""
+    p = Planner([5, 9, 0], [1, 4, 2], 4, 60, 6, 16)
+    p.plan()
+    if count is not None:
+        p.count.fill_(count)
+        p.summary[1] = count + 1
+    p.pages = pages
+    state = (p.cached, p.lengths, p.free, p.count, p.table, p.summary)
+    before = [t.clone() for t in state]
+    p.commit(ints([1, 1, 0]))
+    assert device_error() == 110
+    assert all(torch.equal(a, b) for a, b in zip(state, before))

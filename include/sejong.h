@@ -359,7 +359,8 @@ int sj_scale_to_bf16(const float* x, int n, float alpha, void* y, void* stream);
  *                    more than `rows` rows; 2: too few free pages; 3: ld_table too small; 4: a negative or
  *                    overflowing count.  With a status other than 0 nothing is planned: lengths = cached,
  *                    every row -1, block_table untouched.  cached, added and the stack are only read, so a
- *                    repeated call writes the same.
+ *                    repeated call writes the same.  A row whose page id is negative, or has slots past 2^31 - 1,
+ *                    gets slot -1 and records SJ_DEV_BAD_INDEX.
  *   sj_paged_commit  ends the step: *free_count -= pages taken, cached = lengths; requests with release[b] !=
  *                    0 (release may be null) give their pages back to the stack and get length 0.  `pages` is
  *                    the stack's capacity; a stack that would leave [0, pages], or a page id outside [0, pages) to

@@ -139,7 +139,10 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const int32_t* cached,
       const int at = pos / page;
       const int id = at < held ? table[static_cast<size_t>(b) * ld_table + at]
                                : free_pages[count - 1 - (page_start[b] + at - held)];
-      s = id < 0 ? -1 : id * page + pos % page;
+      if (id >= 0 && id <= (INT_MAX - page) / page)
+        s = id * page + pos % page;
+      else
+        record_error(SJ_DEV_BAD_INDEX);
     }
     request[r] = b;
     position[r] = pos;

@@ -533,3 +533,27 @@ def test_commit_refuses_as_a_whole_a_stack_out_of_bounds(count, pages):
     p.commit(ints([1, 1, 0]))
     assert device_error() == 110
     assert all(torch.equal(a, b) for a, b in zip(state, before))
+
+
+@pytest.mark.parametrize("bad", [-1, -9, 134217727, 1 << 28, 1 << 30, 2 ** 31 - 1])
+@pytest.mark.parametrize("where", ["table", "stack"])
+def test_plan_reports_page_ids_without_slots(bad, where):
+    """Ids below 0, and those whose slots would not fit 31 bits (id * 16 would wrap to another request's slot)."""
+    p = Planner([5, 16], [2, 2], 16, 40, 4, 6)
+    if where == "table":
+        p.table[0, 0] = bad  # the page that request 0's new tokens go on with
+    else:
+        p.free[p.count.item() - 1] = bad  # the page that request 1 gets
+    p.plan()
+    assert device_error() == 110
+    own = [p.table0[0, 0] * 16 + 5, p.table0[0, 0] * 16 + 6, p.free0[-1] * 16, p.free0[-1] * 16 + 1, -1, -1]
+    own = [-1, -1] + own[2:] if where == "table" else own[:2] + [-1] * 4
+    assert p.maps[2].tolist() == own
+    assert p.summary.tolist() == [4, 1, 0, len(p.free0) - 1]
+
+
+def test_plan_of_the_largest_page_id():
+    p = Planner([5], [2], 16, 40, 4, 2)
+    p.table[0, 0] = 134217726
+    p.plan()
+    assert p.maps[2].tolist() == [134217726 * 16 + 5, 134217726 * 16 + 6]

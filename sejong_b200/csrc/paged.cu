@@ -266,8 +266,8 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) paged_append_kern
   if (r >= rows) return;
   const int c = lane % LANES, h0 = lane / LANES;
   const int s = slot[r], p = position[r];
-  bool live = s >= 0;
-  if (live && (s >= to.pages * to.page || (rot > 0 && (p < 0 || p >= table_len)))) {
+  bool live = s != -1;
+  if (live && (s < 0 || s >= to.pages * to.page || (rot > 0 && (p < 0 || p >= table_len)))) {
     if (lane == 0) record_error(SJ_DEV_BAD_INDEX);
     live = false;
   }

@@ -557,3 +557,8 @@ def test_plan_of_the_largest_page_id():
     p.table[0, 0] = 134217726
     p.plan()
     assert p.maps[2].tolist() == [134217726 * 16 + 5, 134217726 * 16 + 6]
+
+
+@pytest.mark.parametrize("slot", [-2, -128, -2 ** 31])
+def test_append_reports_slots_below_minus_one(slot):
+    test_append_skips_and_reports_what_is_out_of_range(slot, 3)

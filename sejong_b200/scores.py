@@ -21,6 +21,18 @@ def _stream(t):
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+class _Undifferentiable(torch.autograd.Function):
+    """The gradient as it is, a function of `inputs` whose own derivative is an error.  (A backward that is marked as
+    once differentiable leaves out in silence what it depends on through the saved logits.)"""
+    @staticmethod
+    def forward(ctx, gradient, *inputs):
+        return gradient.view_as(gradient)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("the gradient of token_scores has no derivative")
+
+
 class _Scores(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top):
@@ -47,12 +59,14 @@ class _Scores(torch.autograd.Function):
         call("sj_token_scores_bwd", logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), targets.data_ptr(),
              rows, vocab, lse.data_ptr(), entropy.data_ptr(), d_logp.data_ptr(), d_entropy.data_ptr(), out.data_ptr(),
              vocab, _stream(logits))
+        if torch.is_grad_enabled():  # a graph of the gradient is asked for
+            out = _Undifferentiable.apply(out, logits, d_logp, d_entropy)
         return out, None, None
 
 
 def token_scores(logits, targets, top=0):
     """Log probability of targets[r] (int32; -1: none) and entropy under each row of logits (f32 or bf16 [rows, vocab]
-    on the GPU, any row stride), and the `top` best alternatives (0 to 32)."""
+    on the GPU, any row stride), and the `top` best alternatives (0 to 32).  First derivatives only."""
     if logits.dim() != 2 or targets.shape != logits.shape[:1]:
         raise ValueError("logits [rows, vocab] and targets [rows]")
     if logits.dtype not in _DTYPES:

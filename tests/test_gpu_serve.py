@@ -280,3 +280,23 @@ def test_generate_reports_a_step_that_could_not_be_planned(made):
         gen.generate([b"seven b"], Sampling(max_bytes=8, temperature=0.0))
     del gen._start
     assert gen.generate([b"good", b"ones"], good) == want
+
+
+def test_differentiable_scores_refuse_a_second_derivative():
+    """The gradient kernel's result has no derivative of its own: asking for one is an error, not a term left out.  The
+    first derivative can be part of a graph."""
+    from sejong_b200.scores import token_scores
+    x = torch.randn(5, 257, device="cuda", requires_grad=True)
+    target = torch.arange(5, device="cuda")
+    got = token_scores(x, target)
+    plain, = torch.autograd.grad(got.logp.sum() + got.entropy.sum(), x, retain_graph=True)
+    g, = torch.autograd.grad(got.logp.sum() + got.entropy.sum(), x, create_graph=True)
+    assert torch.equal(g, plain)
+    for again in (g, torch.autograd.grad(got.logp.sum() + (x * x).sum(), x, create_graph=True)[0]):
+        with pytest.raises(RuntimeError, match="token_scores has no derivative"):
+            again.sum().backward()
+    # a gradient that comes back with a graph of its own, and logits without one
+    scale, logits = torch.ones((), device="cuda", requires_grad=True), x.detach().requires_grad_()
+    g, = torch.autograd.grad(token_scores(logits, target).logp.sum() * scale, logits, create_graph=True)
+    with pytest.raises(RuntimeError, match="token_scores has no derivative"):
+        torch.autograd.grad(g.sum(), scale)

@@ -17,6 +17,11 @@ class TokenScores(NamedTuple):
     top_logp: torch.Tensor  # f32 [rows, top], not differentiated
 
 
+def _row_stride(logits):
+    """Of rows that token_scores has seen to; one row has any."""
+    return logits.stride(0) if logits.shape[0] > 1 else logits.shape[1]
+
+
 def _stream(t):
     return torch.cuda.current_stream(t.device).cuda_stream
 
@@ -43,7 +48,7 @@ class _Scores(torch.autograd.Function):
         best = torch.empty(rows, top, dtype=torch.float32, device=dev)
         size = max(_lib.load().sj_token_scores_workspace(rows, vocab, top), 1)
         work = torch.zeros(size, dtype=torch.uint8, device=dev)
-        call("sj_token_scores", logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), targets.data_ptr(), rows,
+        call("sj_token_scores", logits.data_ptr(), _DTYPES[logits.dtype], _row_stride(logits), targets.data_ptr(), rows,
              vocab, top, logp.data_ptr(), entropy.data_ptr(), lse.data_ptr(), ids.data_ptr(), best.data_ptr(),
              work.data_ptr(), size, _stream(logits))
         ctx.save_for_backward(logits, targets, lse, entropy)
@@ -56,7 +61,7 @@ class _Scores(torch.autograd.Function):
         rows, vocab = logits.shape
         d_logp, d_entropy = d_logp.float().contiguous(), d_entropy.float().contiguous()
         out = torch.empty(rows, vocab, dtype=logits.dtype, device=logits.device)
-        call("sj_token_scores_bwd", logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), targets.data_ptr(),
+        call("sj_token_scores_bwd", logits.data_ptr(), _DTYPES[logits.dtype], _row_stride(logits), targets.data_ptr(),
              rows, vocab, lse.data_ptr(), entropy.data_ptr(), d_logp.data_ptr(), d_entropy.data_ptr(), out.data_ptr(),
              vocab, _stream(logits))
         if torch.is_grad_enabled():  # a graph of the gradient is asked for
@@ -73,6 +78,6 @@ def token_scores(logits, targets, top=0):
         raise ValueError(f"logits of {logits.dtype}: float32 or bfloat16")
     if not logits.is_cuda or targets.device != logits.device:
         raise ValueError("logits and targets on the same GPU")
-    if logits.stride(1) != 1 or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
+    if logits.stride(1) != 1 or (logits.shape[0] > 1 and not logits.shape[1] <= logits.stride(0) < 1 << 31):
         logits = logits.contiguous()
     return TokenScores(*_Scores.apply(logits, targets.to(torch.int32).contiguous(), top))

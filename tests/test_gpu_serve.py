@@ -300,3 +300,27 @@ def test_differentiable_scores_refuse_a_second_derivative():
     g, = torch.autograd.grad(token_scores(logits, target).logp.sum() * scale, logits, create_graph=True)
     with pytest.raises(RuntimeError, match="token_scores has no derivative"):
         torch.autograd.grad(g.sum(), scale)
+
+
+@pytest.mark.parametrize("strides", [(1, 1), (0, 1), (7, 1), (3, 2), (2 ** 32 + 264, 1), (2 ** 31 + 8, 1)])
+@pytest.mark.parametrize("rows", [1, 3])
+def test_differentiable_scores_of_any_row_stride(rows, strides):
+    """Rows that overlap, one row of any stride, strides past 32 bits: the values of a contiguous copy."""
+    from sejong_b200.scores import token_scores
+    vocab = 257
+    base = torch.empty((rows - 1) * strides[0] + (vocab - 1) * strides[1] + 1, dtype=torch.bfloat16, device="cuda")
+    x = base.as_strided((rows, vocab), strides)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    for r in range(rows):
+        x[r] = torch.randn(vocab, generator=gen, device="cuda").bfloat16()
+    target = torch.arange(rows, device="cuda")
+    want_x = x.clone(memory_format=torch.contiguous_format).view(-1).view(rows, vocab).requires_grad_()
+    x = x.detach().requires_grad_()
+    got, want = token_scores(x, target, top=3), token_scores(want_x, target, top=3)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    g, = torch.autograd.grad(got.logp.sum() + got.entropy.sum(), x)
+    w, = torch.autograd.grad(want.logp.sum() + want.entropy.sum(), want_x)
+    assert torch.equal(g, w)
+    ref = torch.log_softmax(x.detach().double(), 1)
+    torch.testing.assert_close(got.logp.double(), ref.gather(1, target[:, None])[:, 0], rtol=0, atol=2e-5)

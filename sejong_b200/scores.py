@@ -46,11 +46,12 @@ class _Scores(torch.autograd.Function):
         logp, entropy, lse = (torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(3))
         ids = torch.empty(rows, top, dtype=torch.int32, device=dev)
         best = torch.empty(rows, top, dtype=torch.float32, device=dev)
-        size = max(_lib.load().sj_token_scores_workspace(rows, vocab, top), 1)
-        work = torch.zeros(size, dtype=torch.uint8, device=dev)
-        call("sj_token_scores", logits.data_ptr(), _DTYPES[logits.dtype], _row_stride(logits), targets.data_ptr(), rows,
-             vocab, top, logp.data_ptr(), entropy.data_ptr(), lse.data_ptr(), ids.data_ptr(), best.data_ptr(),
-             work.data_ptr(), size, _stream(logits))
+        with torch.cuda.device(dev):  # the library works on the current one
+            size = max(_lib.load().sj_token_scores_workspace(rows, vocab, top), 1)
+            work = torch.zeros(size, dtype=torch.uint8, device=dev)
+            call("sj_token_scores", logits.data_ptr(), _DTYPES[logits.dtype], _row_stride(logits), targets.data_ptr(),
+                 rows, vocab, top, logp.data_ptr(), entropy.data_ptr(), lse.data_ptr(), ids.data_ptr(),
+                 best.data_ptr(), work.data_ptr(), size, _stream(logits))
         ctx.save_for_backward(logits, targets, lse, entropy)
         ctx.mark_non_differentiable(ids, best)
         return logp, entropy, ids, best
@@ -61,9 +62,10 @@ class _Scores(torch.autograd.Function):
         rows, vocab = logits.shape
         d_logp, d_entropy = d_logp.float().contiguous(), d_entropy.float().contiguous()
         out = torch.empty(rows, vocab, dtype=logits.dtype, device=logits.device)
-        call("sj_token_scores_bwd", logits.data_ptr(), _DTYPES[logits.dtype], _row_stride(logits), targets.data_ptr(),
-             rows, vocab, lse.data_ptr(), entropy.data_ptr(), d_logp.data_ptr(), d_entropy.data_ptr(), out.data_ptr(),
-             vocab, _stream(logits))
+        with torch.cuda.device(logits.device):
+            call("sj_token_scores_bwd", logits.data_ptr(), _DTYPES[logits.dtype], _row_stride(logits),
+                 targets.data_ptr(), rows, vocab, lse.data_ptr(), entropy.data_ptr(), d_logp.data_ptr(),
+                 d_entropy.data_ptr(), out.data_ptr(), vocab, _stream(logits))
         if torch.is_grad_enabled():  # a graph of the gradient is asked for
             out = _Undifferentiable.apply(out, logits, d_logp, d_entropy)
         return out, None, None

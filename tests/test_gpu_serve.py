@@ -324,3 +324,25 @@ def test_differentiable_scores_of_any_row_stride(rows, strides):
     assert torch.equal(g, w)
     ref = torch.log_softmax(x.detach().double(), 1)
     torch.testing.assert_close(got.logp.double(), ref.gather(1, target[:, None])[:, 0], rtol=0, atol=2e-5)
+
+
+def test_differentiable_scores_select_the_device_of_the_logits(monkeypatch):
+    """Forward and backward are launched with the logits' GPU current, whichever is outside."""
+    from sejong_b200 import scores
+    inside, seen, device = [], [], torch.cuda.device
+
+    class Recorded(device):
+        def __enter__(self):
+            inside.append(self.idx)
+            return super().__enter__()
+
+        def __exit__(self, *args):
+            inside.pop()
+            return super().__exit__(*args)
+
+    launch = scores.call
+    monkeypatch.setattr(torch.cuda, "device", Recorded)
+    monkeypatch.setattr(scores, "call", lambda name, *args: (seen.append((name, list(inside))), launch(name, *args))[1])
+    x = torch.randn(4, 257, device="cuda:0", requires_grad=True)
+    scores.token_scores(x, torch.arange(4, device="cuda:0")).logp.sum().backward()
+    assert seen == [("sj_token_scores", [0]), ("sj_token_scores_bwd", [0])]

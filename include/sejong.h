@@ -418,7 +418,8 @@ int sj_attn_paged(const void* q, int ldq, const void* k_cache, const void* v_cac
  *                        equal ones, NaN last): top_id int32 and top_logp f32 [rows, top].  Each of logp, entropy
  *                        and lse may be null.  target -1: logp 0.  A target outside [-1, vocab) counts as -1 and
  *                        records SJ_DEV_BAD_INDEX.  Logits of -inf are forbidden tokens (log probability -inf);
- *                        a row of nothing else has lse -inf, entropy 0.  workspace:
+ *                        a row of nothing else has lse -inf, entropy 0.  vocab (and ldd below) is at most
+ *                        2^31 - 1 - 2^14.  workspace:
  *                        sj_token_scores_workspace bytes, zero before its first use (each call leaves it ready for
  *                        the next, of any size); one per stream.  Fewer rows may take more bytes, since they are
  *                        cut into parts: a buffer for several sizes takes the largest of theirs.

@@ -23,6 +23,7 @@ namespace sj {
 
 namespace {
 constexpr int kScoreMaxTop = 32;
+constexpr int kScoreMaxColumns = INT_MAX - (1 << 14);  // 32 bits count to a chunk or a part past the last column
 // Rows of at most this many logits are held by one warp: 8000 x 2000 f32 with 20 alternatives 22.2 us, 48.6 by the
 // kernel for wide rows, bf16 25.8 and 52.2; 4000 x 4096 f32 24.4 and 33.1, but bf16, loaded two bytes at a time, 33.0
 // and 27.8.
@@ -944,7 +945,7 @@ size_t score_counter_bytes() { return (static_cast<size_t>(score_cut_rows()) * s
 template <typename T>
 int scores(const T* logits, int ld, int rows, const ScoreOut& out, void* workspace, cudaStream_t stream) {
   if (out.vocab <= kScoreNarrow<T>) {
-    const int regs = (out.vocab + 31) / 32, grid = (rows + 3) / 4;
+    const int regs = (out.vocab + 31) / 32, grid = (rows - 1) / 4 + 1;
     launch(regs <= 4   ? token_scores_narrow_kernel<T, 4>
            : regs <= 9 ? token_scores_narrow_kernel<T, 9>
            : regs <= 16 ? token_scores_narrow_kernel<T, 16>
@@ -953,7 +954,8 @@ int scores(const T* logits, int ld, int rows, const ScoreOut& out, void* workspa
                         : token_scores_narrow_kernel<T, kScoreNarrow<T> / 32>,
            grid, 128, 0, stream, logits, ld, rows, out);
   } else {
-    // No more parts than chunks: the CTA that ends a row writes the target's logit that it read at its part's last chunk.
+    // No more parts than chunks: the CTA that ends a row writes with the target's logit that it read at its part's last
+    // chunk.
     const int chunks = (out.vocab - 1) / ScoreChunk<T>::SIZE + 1, smem = kScoreStages * kScoreStage;
     const int splits = std::min(score_splits(rows, out.vocab), chunks);
     if (static_cast<int64_t>(rows) * splits > INT_MAX - score_ctas())
@@ -998,7 +1000,7 @@ int scores_bwd(const T* logits, int ld, T* d_logits, int ldd, int rows, const Sc
 }  // namespace
 
 extern "C" size_t sj_token_scores_workspace(int rows, int vocab, int top) {
-  if (rows < 0 || vocab <= 0 || top < 0 || top > kScoreMaxTop) return 0;
+  if (rows < 0 || vocab <= 0 || vocab > kScoreMaxColumns || top < 0 || top > kScoreMaxTop) return 0;
   const int splits = score_splits(rows, vocab);
   if (splits == 1) return 16;
   return score_counter_bytes() + static_cast<size_t>(rows) * splits * score_part(top) * sizeof(float);
@@ -1007,9 +1009,9 @@ extern "C" size_t sj_token_scores_workspace(int rows, int vocab, int top) {
 extern "C" int sj_token_scores(const void* logits, int dtype, int ld, const int32_t* target, int rows, int vocab,
                                int top, float* logp, float* entropy, float* lse, int32_t* top_id, float* top_logp,
                                void* workspace, size_t workspace_bytes, void* stream) {
-  if (rows < 0 || vocab <= 0 || ld < vocab || top < 0 || top > kScoreMaxTop || top > vocab)
-    return fail(SJ_ERR_SHAPE, "sj_token_scores: rows=%d vocab=%d ld=%d top=%d (up to %d)", rows, vocab, ld, top,
-                kScoreMaxTop);
+  if (rows < 0 || vocab <= 0 || vocab > kScoreMaxColumns || ld < vocab || top < 0 || top > kScoreMaxTop || top > vocab)
+    return fail(SJ_ERR_SHAPE, "sj_token_scores: rows=%d vocab=%d (up to %d) ld=%d top=%d (up to %d)", rows, vocab,
+                kScoreMaxColumns, ld, top, kScoreMaxTop);
   if (dtype != SJ_F32 && dtype != SJ_BF16)
     return fail(SJ_ERR_UNSUPPORTED, "sj_token_scores: dtype %d (this build: f32 or bf16)", dtype);
   if (rows == 0) return SJ_OK;
@@ -1027,8 +1029,9 @@ extern "C" int sj_token_scores(const void* logits, int dtype, int ld, const int3
 extern "C" int sj_token_scores_bwd(const void* logits, int dtype, int ld, const int32_t* target, int rows, int vocab,
                                    const float* lse, const float* entropy, const float* d_logp, const float* d_entropy,
                                    void* d_logits, int ldd, void* stream) {
-  if (rows < 0 || vocab <= 0 || ld < vocab || ldd < vocab)
-    return fail(SJ_ERR_SHAPE, "sj_token_scores_bwd: rows=%d vocab=%d ld=%d ldd=%d", rows, vocab, ld, ldd);
+  if (rows < 0 || vocab <= 0 || ld < vocab || ldd < vocab || ldd > kScoreMaxColumns)
+    return fail(SJ_ERR_SHAPE, "sj_token_scores_bwd: rows=%d vocab=%d ld=%d ldd=%d (up to %d)", rows, vocab, ld, ldd,
+                kScoreMaxColumns);
   if (dtype != SJ_F32 && dtype != SJ_BF16)
     return fail(SJ_ERR_UNSUPPORTED, "sj_token_scores_bwd: dtype %d (this build: f32 or bf16)", dtype);
   if (rows == 0) return SJ_OK;

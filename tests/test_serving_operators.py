@@ -202,3 +202,15 @@ def test_token_scores_refuses(lib):
         token_scores(x.half(), t)
     with pytest.raises(ValueError, match="GPU"):
         token_scores(x, t)
+
+
+@pytest.mark.parametrize("vocab", [2 ** 31 - 1, 2 ** 31 - 2000, 2 ** 31 - 16383])
+def test_scores_refuse_columns_that_32_bits_do_not_count(lib, vocab):
+    for dtype in (0, 4):
+        refused("sj_token_scores", change(SCORES, dtype=dtype, ld=vocab, vocab=vocab), SHAPE)
+        refused("sj_token_scores_bwd", change(GRADIENT, dtype=dtype, ld=vocab, vocab=vocab, ldd=vocab), SHAPE)
+        refused("sj_token_scores_bwd", change(GRADIENT, dtype=dtype, ldd=vocab), SHAPE)
+
+
+def test_plan_takes_fewer_than_2_to_the_19_rows(lib):
+    refused("sj_paged_plan", change(PLAN, rows=1 << 19), SHAPE)

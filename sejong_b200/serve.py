@@ -139,6 +139,7 @@ class BatchGenerator:
         self.slots = [None] * B
         self.finished = set()
         self.reserved = 0
+        torch.cuda.current_stream(self.dev).synchronize()  # calls run on whichever stream is current then
 
     # ---------------------------------------------------------------- kernels
     def _stream(self):

@@ -346,3 +346,26 @@ def test_differentiable_scores_select_the_device_of_the_logits(monkeypatch):
     x = torch.randn(4, 257, device="cuda:0", requires_grad=True)
     scores.token_scores(x, torch.arange(4, device="cuda:0")).logp.sum().backward()
     assert seen == [("sj_token_scores", [0]), ("sj_token_scores_bwd", [0])]
+
+
+def test_a_generator_can_be_used_on_another_stream_than_it_was_made_on(made, monkeypatch):
+    """What the constructor has launched is done when it returns: a call on another stream does not wait for it."""
+    from sejong_b200 import serve
+    c, params = made
+    launch = serve.call
+
+    def slow(name, *args):
+        launch(name, *args)
+        if name == "sj_rope_table":
+            torch.cuda._sleep(200_000_000)  # a tenth of a second
+
+    # a new pinned buffer waits for the GPU, one of an earlier generator does not
+    serve.BatchGenerator(c, params, device=0, context=64, batch=2, page=16)
+    monkeypatch.setattr(serve, "call", slow)
+    gen = serve.BatchGenerator(c, params, device=0, context=64, batch=2, page=16)
+    assert torch.cuda.current_stream().query()
+    monkeypatch.setattr(serve, "call", launch)
+    want = gen.score(b"some text")
+    other = torch.cuda.Stream()
+    with torch.cuda.stream(other):
+        assert gen.score(b"some text") == want

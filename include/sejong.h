@@ -391,7 +391,8 @@ int sj_paged_commit(int32_t* cached, int32_t* lengths, const int32_t* release, i
  * rounded once, with f_i = theta^(-2i/rope_dim) and
  *   SJ_ROPE_PLAIN   amplitude 1
  *   SJ_ROPE_LINEAR  f_i / factor (position interpolation)
- *   SJ_ROPE_BASE    theta * factor^(rope_dim / (rope_dim - 2)) for theta (the lowest frequency is divided by factor)
+ *   SJ_ROPE_BASE    theta * factor^(rope_dim / (rope_dim - 2)) for theta (the lowest frequency is divided by factor;
+ *                   the "NTK-aware" rule, as the YaRN paper gives it)
  *   SJ_ROPE_RAMP    by turns T_i = original * f_i / 2 pi over the original context: w f_i + (1 - w) f_i / factor,
  *                   w = clamp((T_i - slow) / (fast - slow), 0, 1), amplitude 0.1 ln(factor) + 1 (the "NTK-by-parts"
  *                   rule of the YaRN paper, arXiv 2309.00071)

@@ -15,7 +15,8 @@ training step (crates/sejong-cli/src/main.rs:20-164 commands, 165-407 dispatch).
   generate     Generate bytes with the KV cache (main.rs:334-390).
   generate-batch  Generate for every line of a file at once on a paged KV cache; one JSON line each, with the
                log probabilities of the bytes and their best alternatives if asked for.
-  score        Log probability, entropy and alternatives of every byte of a text file, as JSON.
+  score        Log probability, entropy and alternatives of every byte of a text file no longer than the model's
+               context, as JSON.
   inspect      Print a model artifact's configuration and provenance (main.rs:391-405).
 
 Every step runs on the GPU through libsejong_b200.so (ByteTrainer); the host loop only draws batches,

@@ -171,8 +171,8 @@ __global__ void __launch_bounds__(1024) paged_commit_kernel(int32_t* cached, int
   });
   const int top = *free_count - summary[1], back = page_start[batch];
   bool refused = top < 0 || back < 0 || back > pages - top;
-  // The pages to return, a run of them for each warp, kCommitIds of a lane at a time: side by side in the table, so that
-  // a request is looked for where a lane leaves the last one's pages only.
+  // The pages to return, a run of them for each warp, kCommitIds of a lane at a time: side by side in the table, so
+  // that a request is looked for where a lane leaves the last one's pages only.
   const int run = (back / static_cast<int>(blockDim.x) + 1) * 32, i0 = (threadIdx.x >> 5) * run;
   const int i1 = refused ? 0 : min(i0 + run, back);
   auto each_page = [&](auto use) {

@@ -25,8 +25,8 @@ namespace {
 constexpr int kScoreMaxTop = 32;
 constexpr int kScoreMaxColumns = INT_MAX - (1 << 14);  // 32 bits count to a chunk or a part past the last column
 // Rows of at most this many logits are held by one warp: 8000 x 2000 f32 with 20 alternatives 22.2 us, 48.6 by the
-// kernel for wide rows, bf16 25.8 and 52.2; 4000 x 4096 f32 24.4 and 33.1, but bf16, loaded two bytes at a time, 33.0
-// and 27.8.
+// kernel for wide rows, bf16 25.8 and 52.2 (33.5 where the rows are not in L2); 4000 x 4096 f32 24.4 and 33.1, but
+// bf16, loaded two bytes at a time, 33.0 and 27.8.
 template <typename T>
 constexpr int kScoreNarrow = sizeof(T) == 4 ? 4096 : 2048;
 // CTAs of an SM, of the kernel that holds R logits a lane: 32768 x 257 f32 with 5 alternatives 20.6 us with nine, 20.2
@@ -497,7 +497,9 @@ SJ_DEVICE int score_rank(ScoreBest& b, int top) {
 
 // The same where more logits reach the bar than the list holds (equal or rising logits): columns [base, end) once
 // more, 2048 at a time, of which those of the `top` threads with the best maxima join the list; it is ranked each
-// time.  Leaves best.list; returns its length.
+// time.  Leaves best.list; returns its length.  2048 x 50001 bf16 with 20 alternatives take 550 us where all are equal,
+// 1590 where they rise along the row, 333 where 100 tokens of a row are allowed and 605 where 11 are, since fewer than
+// `top` groups of threads then hold one and there is no bar (57 us at random, 99 where they fall).
 template <typename T>
 SJ_DEVICE int score_rank_all(ScoreBest& best, const T* x, int base, int end, int top) {
   constexpr int N = 16;  // logits of a thread at a time
@@ -895,7 +897,9 @@ __global__ void __launch_bounds__(256, kGradCtas<T>)
   }
 }
 
-// Any strides and alignments: a CTA for 2048 elements of a row, side by side.
+// Any strides and alignments: a CTA for 2048 elements of a row, side by side.  1024 x 50001 f32 79 us (63 on 16-byte
+// boundaries), 2048 x 65537 bf16 174 (83.5); narrow rows leave most of a CTA idle: 32768 x 257 f32 67 us (12.9), bf16
+// 68 (10.3).
 template <typename T>
 __global__ void __launch_bounds__(256) token_scores_bwd_any_kernel(const T* logits, int ld, T* d_logits, int ldd,
                                                                    int parts, ScoreGrad in) {
@@ -931,9 +935,9 @@ int score_ctas() { return kScoreCtas * sm_count(); }
 // Rows are cut into parts where there are fewer than this many of them.
 int score_cut_rows() { return score_ctas() * 2 / 5; }
 // Parts of a row, one for each 4096 logits at most: the fewest that give two CTAs of five one, since a CTA that has its
-// SM to itself runs faster and a part costs its own ranking and a share of a join (400 x 32000 f32: 19.0 us whole, 20.7
-// in two, 26.6 in three; 128 x 130000 f32: 32.5 us in two, 24.8 in four, 24.1 in seven).  For the same reason a partly
-// filled last round of whole rows is left as it is.
+// SM to itself runs faster and a part costs its own ranking and a share of a join (128 x 130000 f32, which it cuts in
+// four: 29.7 us in two, 23.4 in four, 25.8 in seven; 400 x 32000 f32, at its border: 18.4 us whole, 20.5 in two, 28.7
+// in three).  For the same reason a partly filled last round of whole rows is left as it is.
 int score_splits(int rows, int vocab) {
   if (rows <= 0 || rows >= score_cut_rows()) return 1;
   const int fill = (score_cut_rows() + rows - 1) / rows;

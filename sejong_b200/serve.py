@@ -10,13 +10,15 @@ to `batch` requests in one cache of `pages` pages a layer and steps them togethe
     sj_paged_append files its keys and values;
   * a decode step is one CUDA graph for `batch` rows, whatever number of them is live: the QKV GEMM, the rotary
     append at each row's own position, sj_attn_paged, the rest of the block, the head;
+  * prompts are run one at a time, between decode steps;
   * bytes are sampled on the host as `Generator` does, each request with its own Sampling and Rng, and
     sj_token_scores gives the sampled bytes' log probabilities, the entropies and the best alternatives;
   * requests wait until the pages that they may come to need are free, so a step never runs out of them; a full
-    context restarts from its last `context` tokens, as the reference does.
+    context restarts from its last `context` tokens, as the reference does;
+  * a call that raises leaves an empty cache.
 
-`score` gives the same figures for the bytes of a given text.  `rope_scaling` stretches the rotary positions
-beyond the trained context (sj_rope_table_scaled).
+`score` gives the same figures for the bytes of a given text of at most `context` bytes.  `rope_scaling` stretches the
+rotary positions beyond the trained context (sj_rope_table_scaled).
 """
 import ctypes
 from collections import deque

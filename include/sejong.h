@@ -411,6 +411,71 @@ int sj_attn_paged(const void* q, int ldq, const void* k_cache, const void* v_cac
                   int head_dim, int window, void* o, int ldo, float* lse, void* workspace, size_t workspace_bytes,
                   void* stream);
 
+/* ------------------------------------------------------------------ several continuations of one prompt
+ * No counterpart in the reference.  Requests (beams, samples, rows of one long prompt) share the pages of their common
+ * beginning.  shares (int32 [pages]) counts the requests that hold a page beyond the first, and is 0 for a free page,
+ * so that a page which sj_paged_plan takes needs no entry.  pages <= 2^18 here.
+ *
+ *   sj_paged_fork    the next state of a cache in which request b goes on from what request parent[b] holds (parent
+ *                    [batch], batch <= 4096: its own number to go on, another's to take over a copy, -1 to be empty).
+ *                    Full pages are shared.  A half-filled last page stays with the lowest b of its parent's
+ *                    children; each of the others, in order, takes a page from the top of the free stack, and
+ *                    copies (int32 [batch, 3]) gets {page, fresh page, tokens} for sj_paged_copy, and {-1, -1, 0}
+ *                    past the last.  Pages that nobody holds any more go on top of the stack, the lowest id first.
+ *                    The state (cached, block_table, shares, free_pages, *free_count) is only read, so a repeated
+ *                    call writes the same; the new one goes to buffers of its own (the entries of table_out and
+ *                    free_out that hold pages).  Call it between sj_paged_commit, whose release then is null, and
+ *                    sj_paged_plan.  summary (int32 [4]) = {copies, pages back, status, pages left}.  status 0:
+ *                    done; 2: too few free pages; 3: ld_table too small; 4: a parent, length or stack out of range.
+ *                    With a status other than 0 the new state is the old one.  A page id outside [0, pages), or one
+ *                    given back more often than it was held, records SJ_DEV_BAD_INDEX and is not counted.
+ *   sj_paged_copy    rows 0 .. tokens - 1 of page copies[i][0] to page copies[i][1], keys and values of every head
+ *                    and of `layers` caches that lie layer_stride elements apart in k_cache and v_cache.  An entry
+ *                    whose first value is -1 is passed over; one out of range records SJ_DEV_BAD_INDEX.  A page
+ *                    that one entry writes is none that another reads or writes.
+ *   sj_paged_compact maps the pages in use (those not on the free stack) to the ids 0 .. used - 1: the i-th page in
+ *                    use from `used` on goes to the i-th free page below.  table_out, shares_out and free_out (the
+ *                    lowest id on top) are the new state, in buffers of its own; moves (int32 [most, 3]) gets {from,
+ *                    to, page} for sj_paged_copy, {-1, -1, 0} past the last.  summary = {moves, used, status, pages
+ *                    left}.  status 1: more than `most` moves; 4: a stack with ids out of range or twice; then the
+ *                    new state is the old one.  A length that does not fit ld_table, or a page id that is out of
+ *                    range or free, records SJ_DEV_BAD_INDEX; its row, or entry, is left out, or stays.
+ *   sj_attn_paged_shared  sj_attn_paged, for rows that share keys.  group (int32 [groups, 3]) = {first row, request,
+ *                    tokens}, by first rows in order: the rows from the first one to the next group's (or `rows`) all
+ *                    have the first `tokens` tokens of that request among theirs, at the same positions, so they
+ *                    are read once for all of them.  Each row still sees no more than position[r] + 1 tokens and its
+ *                    window.  A group out of order or out of range records SJ_DEV_BAD_INDEX and has no tokens in
+ *                    common.  Results are those of sj_attn_paged but for the order of the sums. */
+int sj_paged_fork(const int32_t* parent, int batch, int page, const int32_t* cached, const int32_t* block_table,
+                  int ld_table, const int32_t* shares, const int32_t* free_pages, const int32_t* free_count, int pages,
+                  int32_t* cached_out, int32_t* table_out, int32_t* shares_out, int32_t* free_out, int32_t* count_out,
+                  int32_t* copies, int32_t* summary, void* stream);
+int sj_paged_copy(const int32_t* copies, int most, void* k_cache, void* v_cache, int layers, int64_t layer_stride,
+                  int pages, int page, int64_t page_stride, int64_t head_stride, int64_t token_stride, int hk,
+                  int head_dim, void* stream);
+int sj_paged_compact(const int32_t* cached, int batch, int page, const int32_t* block_table, int ld_table,
+                     const int32_t* shares, const int32_t* free_pages, const int32_t* free_count, int pages,
+                     int32_t* table_out, int32_t* shares_out, int32_t* free_out, int32_t* moves, int most,
+                     int32_t* summary, void* stream);
+size_t sj_attn_paged_shared_workspace(int rows, int groups, int hq, int hk, int head_dim);
+int sj_attn_paged_shared(const void* q, int ldq, const void* k_cache, const void* v_cache, int pages, int page,
+                         int64_t page_stride, int64_t head_stride, int64_t token_stride, const int32_t* block_table,
+                         int ld_table, int requests, const int32_t* request, const int32_t* position, int rows,
+                         const int32_t* group, int groups, int hq, int hk, int head_dim, int window, void* o, int ldo,
+                         float* lse, void* workspace, size_t workspace_bytes, void* stream);
+/* The best continuations of each request's beams: of the totals score[r][b] + log softmax(logits[r * beams + b])[t] (logits
+ * f32 or bf16 by dtype, [requests * beams, ld], the first vocab columns; score f32 [requests, beams]) the `keep` largest
+ * in order, the lowest b * vocab + t first among equal ones: parent = b, token = t, new_score = total, each [requests,
+ * keep].  Totals are compared before they are rounded to f32.  A logit of -inf is a forbidden token and a score of -inf
+ * an empty beam; they, and rows with a NaN or +inf, have no candidates.  Past the last candidate parent = token = -1
+ * and new_score = -inf.  requests <= 4096, beams <= 64, keep <= min(64, beams * vocab), vocab <= 2^31 - 1 - 2^16.
+ * workspace: sj_beam_select_workspace bytes (0 for small vocabularies), zero before its first use (each call leaves it
+ * ready for the next, of any size); one per stream.  Fewer rows may take more bytes, since they are cut into parts. */
+size_t sj_beam_select_workspace(int requests, int beams, int vocab, int keep);
+int sj_beam_select(const void* logits, int dtype, int ld, const float* score, int requests, int beams, int vocab,
+                   int keep, int32_t* parent, int32_t* token, float* new_score, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------ token scores
  * No counterpart in the reference, which trains by cross entropy only (kernels.py:176-191).
  *   sj_token_scores      per row of logits (f32 or bf16 by dtype, [rows, ld], the first vocab columns):

@@ -75,6 +75,19 @@ SIGNATURES = {
     "sj_attn_paged": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_i64, c_i64, c_i64, c_void_p,
                               c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int,
                               c_void_p, c_void_p, c_size_t, c_void_p]),
+    "sj_attn_paged_shared_workspace": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "sj_attn_paged_shared": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_i64, c_i64, c_i64, c_void_p,
+                                     c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int,
+                                     c_int, c_void_p, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "sj_paged_fork": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int,
+                              c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "sj_paged_copy": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int, c_i64, c_int, c_int, c_i64, c_i64, c_i64,
+                              c_int, c_int, c_void_p]),
+    "sj_paged_compact": (c_int, [c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int,
+                                 c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    "sj_beam_select_workspace": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "sj_beam_select": (c_int, [c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
+                               c_void_p, c_void_p, c_size_t, c_void_p]),
     "sj_token_scores_workspace": (c_size_t, [c_int, c_int, c_int]),
     "sj_token_scores": (c_int, [c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
                                 c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),

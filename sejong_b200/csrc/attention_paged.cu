@@ -689,3 +689,23 @@ extern "C" int sj_attn_paged(const void* q, int ldq, const void* k_cache, const 
   if (head_dim == 64) return nq == 1 ? attend<64, 1>(a, s) : attend<64, 2>(a, s);
   return nq == 1 ? attend<128, 1>(a, s) : attend<128, 2>(a, s);
 }
+
+// Groups say which keys rows share; this form reads them for each row.
+extern "C" size_t sj_attn_paged_shared_workspace(int rows, int groups, int hq, int hk, int head_dim) {
+  if (groups < 0) return 0;
+  return sj_attn_paged_workspace(rows, hq, hk, head_dim);
+}
+
+extern "C" int sj_attn_paged_shared(const void* q, int ldq, const void* k_cache, const void* v_cache, int pages,
+                                    int page, int64_t page_stride, int64_t head_stride, int64_t token_stride,
+                                    const int32_t* block_table, int ld_table, int requests, const int32_t* request,
+                                    const int32_t* position, int rows, const int32_t* group, int groups, int hq,
+                                    int hk, int head_dim, int window, void* o, int ldo, float* lse, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  if (groups < 0 || (rows > 0 && groups > rows))
+    return fail(SJ_ERR_SHAPE, "sj_attn_paged_shared: groups=%d rows=%d", groups, rows);
+  if (rows > 0 && groups > 0 && !group) return fail(SJ_ERR_ARGUMENT, "sj_attn_paged_shared: null operand");
+  return sj_attn_paged(q, ldq, k_cache, v_cache, pages, page, page_stride, head_stride, token_stride, block_table,
+                       ld_table, requests, request, position, rows, hq, hk, head_dim, window, o, ldo, lse, workspace,
+                       workspace_bytes, stream);
+}

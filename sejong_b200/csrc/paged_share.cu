@@ -1,0 +1,491 @@
+// Pages of a cache that several requests share: a step's reordering of requests, copies of pages, and
+// the pages in use moved to the front of the cache (paged.cu plans and ends the steps themselves).
+//
+//   paged_fork_kernel     block tables, owners and the free stack after each request took over another's pages
+//   paged_copy_kernel     rows of pages to other pages, in every layer
+//   paged_compact_kernel  the pages in use mapped to the lowest ids
+//
+// shares[p] is the number of requests that hold page p beyond the first, 0 for a free page, so that a page that
+// sj_paged_plan takes from the stack needs no entry of its own.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <climits>
+
+#include "common.cuh"
+#include "internal.h"
+
+namespace cg = cooperative_groups;
+
+namespace sj {
+
+namespace {
+constexpr int kShareMaxBatch = 4096, kShareMaxPages = 1 << 18;  // their counters fit a cluster's shared memory
+constexpr int kForkNoPages = 2, kForkTableNarrow = 3, kForkBad = 4;
+constexpr int kCompactMovesOver = 1, kCompactBad = 4;
+constexpr int kForkCluster = 8, kForkThreads = 512, kForkWarps = kForkThreads / 32;
+constexpr int kForkChunk = 128;       // entries of a block table that a warp counts at a time
+constexpr int kCopyThreads = 256, kCopyPieces = 8;  // 16-byte pieces of a thread
+constexpr int kCompactThreads = 1024;
+}  // namespace
+
+// ---------------------------------------------------------------- fork
+struct Fork {
+  const int32_t *parent, *cached, *table, *shares, *stack, *stack_count;
+  int32_t *cached_out, *table_out, *shares_out, *stack_out, *count_out, *copies, *summary;
+  int batch, page, ld_table, pages, per;  // per: pages whose owners a CTA counts
+};
+
+// A slot's pages pass to its children: full ones are shared, a half-filled last page goes to the lowest child and is
+// copied to a fresh page for each of the others.  Every CTA scans the batch for itself.  The first cluster counts: an
+// entry of a slot with c children changes its page's owners by c - 1 (the half-filled page of a slot without children
+// by -1); the counters of a CTA's share of the pages lie in its shared memory, which the others add to.  Integer sums,
+// so their order does not matter.  Then each CTA knows which of its pages nobody holds, and after one exchange of
+// numbers where on the stack they go.  The other clusters (the same one, where there is only one) write tables.
+__global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) {
+  pdl_wait();
+  extern __shared__ int dynamic[];
+  int* children = dynamic;                       // [batch + 1]
+  int* lowest = children + (a.batch + 1);        // [batch + 1]
+  int* rank = lowest + (a.batch + 1);            // [batch + 1] copies of the slots before
+  int* counter = rank + (a.batch + 1);           // [per], in the first cluster
+  __shared__ int s_bad, s_narrow, s_back, s_warp[kForkWarps];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, batch = a.batch, page = a.page;
+  const int cta = cluster.block_rank(), ctas = cluster.num_blocks();
+  const bool counts = blockIdx.x < static_cast<unsigned>(ctas);
+  if (t == 0) s_bad = s_narrow = 0;
+  for (int b = t; b < batch; b += kForkThreads) {
+    children[b] = 0;
+    lowest[b] = INT_MAX;
+  }
+  if (counts)
+    for (int i = t; i < a.per; i += kForkThreads) counter[i] = 0;
+  __syncthreads();
+  auto length = [&](int b) { return a.cached[b]; };
+  for (int b = t; b < batch; b += kForkThreads) {
+    const int p = a.parent[b], n = length(b);
+    if (p < -1 || p >= batch || n < 0 || n > INT_MAX - page) {
+      s_bad = 1;
+      continue;
+    }
+    if ((n + page - 1) / page > a.ld_table) s_narrow = 1;
+    if (p >= 0) {
+      atomicAdd(&children[p], 1);
+      atomicMin(&lowest[p], b);
+    }
+  }
+  const int count = *a.stack_count;
+  if (count < 0 || count > a.pages) s_bad = 1;
+  __syncthreads();
+  int status = s_bad ? kForkBad : s_narrow ? kForkTableNarrow : 0;
+  // copies of the slots before each, 32 slots a warp at a time
+  {
+    int taken = 0;
+    for (int b0 = 0; b0 < batch; b0 += kForkThreads) {
+      const int b = b0 + t, p = b < batch && !status ? a.parent[b] : -1;
+      const bool copied = p >= 0 && lowest[p] != b && length(p) % page != 0;
+      const unsigned have = __ballot_sync(0xffffffffu, copied);
+      if (lane == 0) s_warp[warp] = __popc(have);
+      __syncthreads();
+      int before = taken, all = 0;
+      for (int w = 0; w < kForkWarps; ++w) {
+        if (w < warp) before += s_warp[w];
+        all += s_warp[w];
+      }
+      if (b < batch) rank[b] = copied ? before + __popc(have & ((1u << lane) - 1)) : -1;
+      taken += all;
+      __syncthreads();
+    }
+    if (t == 0) s_back = taken;
+    __syncthreads();
+  }
+  int taken = s_back;
+  if (!status && taken > count) status = kForkNoPages;
+  if (status) taken = 0;
+  // with a status, every slot keeps what it holds
+  auto source = [&](int b) { return status ? b : a.parent[b]; };
+  auto held = [&](int p) {
+    const int n = length(p);
+    return n < 0 || n > INT_MAX - page ? 0 : min((n + page - 1) / page, a.ld_table);
+  };
+  auto fresh = [&](int b) { return a.stack[count - 1 - rank[b]]; };
+
+  // ---- tables, lengths, copies, what stays of the stack
+  const int writers = gridDim.x > static_cast<unsigned>(ctas) ? gridDim.x - ctas : gridDim.x;
+  const int writer = gridDim.x > static_cast<unsigned>(ctas) ? static_cast<int>(blockIdx.x) - ctas : blockIdx.x;
+  if (writer >= 0) {
+    for (int b = writer * kForkWarps + warp; b < batch; b += writers * kForkWarps) {
+      const int p = source(b);
+      const bool copied = !status && rank[b] >= 0;
+      const int n = p < 0 ? 0 : held(p), own = copied ? n - 1 : -1;
+      const int32_t* from = a.table + static_cast<size_t>(max(p, 0)) * a.ld_table;
+      int32_t* to = a.table_out + static_cast<size_t>(b) * a.ld_table;
+      for (int j = lane; j < n; j += 128) {
+        int32_t id[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) id[e] = j + 32 * e < n ? from[j + 32 * e] : 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (j + 32 * e < n && j + 32 * e != own) to[j + 32 * e] = id[e];
+      }
+      if (lane == 0) {
+        a.cached_out[b] = p < 0 ? 0 : length(p);
+        if (copied) {
+          const int dst = fresh(b), at = rank[b], src = from[own];
+          to[own] = dst;
+          const bool fine = dst >= 0 && dst < a.pages && src >= 0 && src < a.pages;
+          if (!fine) record_error(SJ_DEV_BAD_INDEX);
+          a.copies[3 * at] = fine ? src : -1;
+          a.copies[3 * at + 1] = fine ? dst : -1;
+          a.copies[3 * at + 2] = fine ? length(p) % page : 0;
+        }
+      }
+    }
+    const int first = writer * kForkThreads + t, step = writers * kForkThreads;
+    for (int i = taken + first; i < batch; i += step) {
+      a.copies[3 * i] = a.copies[3 * i + 1] = -1;
+      a.copies[3 * i + 2] = 0;
+    }
+    const int stays = min(max(count, 0), a.pages) - taken;
+    for (int i = first; i < stays; i += step) a.stack_out[i] = a.stack[i];
+  }
+  if (!counts) return;
+
+  // ---- owners
+  cluster.sync();  // every counter of the cluster is zero
+  if (!status) {
+    const int chunks = (a.ld_table + kForkChunk - 1) / kForkChunk;
+    for (int u = cta * kForkWarps + warp; u < batch * chunks; u += ctas * kForkWarps) {
+      const int p = u / chunks, j0 = u % chunks * kForkChunk, c = children[p];
+      if (c == 1) continue;
+      const int n = held(p), full = length(p) / page, end = min(j0 + kForkChunk, c == 0 ? n : full);
+      int32_t id[kForkChunk / 32];
+#pragma unroll
+      for (int e = 0; e < kForkChunk / 32; ++e) {
+        const int j = j0 + 32 * e + lane;
+        id[e] = j < end ? a.table[static_cast<size_t>(p) * a.ld_table + j] : 0;
+      }
+#pragma unroll
+      for (int e = 0; e < kForkChunk / 32; ++e) {
+        if (j0 + 32 * e + lane >= end) continue;
+        if (id[e] < 0 || id[e] >= a.pages) {
+          record_error(SJ_DEV_BAD_INDEX);
+          continue;
+        }
+        const int at = id[e] / a.per;
+        atomicAdd(cluster.map_shared_rank(counter, at) + (id[e] - at * a.per), c - 1);
+      }
+    }
+  }
+  cluster.sync();
+  // a warp's run of this CTA's pages, in order
+  const int page0 = cta * a.per, mine = max(0, min(a.per, a.pages - page0));
+  const int run = ((mine + kForkWarps - 1) / kForkWarps + 31) / 32 * 32;
+  const int i0 = min(warp * run, mine), i1 = min(i0 + run, mine);
+  int gone = 0;
+  for (int i = i0 + lane; i - lane < i1; i += 32) {
+    bool is = false;
+    if (i < i1) {
+      const int more = a.shares[page0 + i], left = more + counter[i];
+      is = left == -1 && counter[i] != 0;
+      if (left < 0 && !is && !status) record_error(SJ_DEV_BAD_INDEX);  // given back more often than it was held
+      a.shares_out[page0 + i] = status ? more : max(left, 0);
+      counter[i] = is;
+    }
+    gone += __popc(__ballot_sync(0xffffffffu, is));
+  }
+  if (lane == 0) s_warp[warp] = gone;
+  __syncthreads();
+  if (t == 0) {
+    int sum = 0;
+    for (int w = 0; w < kForkWarps; ++w) sum += s_warp[w];
+    s_back = sum;
+  }
+  cluster.sync();
+  int back = count - taken, all = 0;
+  for (int k = 0; k < ctas; ++k) {
+    const int n = *cluster.map_shared_rank(&s_back, k);
+    if (k < cta) back += n;
+    all += n;
+  }
+  for (int w = 0; w < warp; ++w) back += s_warp[w];
+  for (int i = i0 + lane; i - lane < i1; i += 32) {
+    const bool is = i < i1 && counter[i] != 0;
+    const unsigned have = __ballot_sync(0xffffffffu, is);
+    const int at = back + __popc(have & ((1u << lane) - 1));
+    if (is) {
+      if (at >= 0 && at < a.pages)
+        a.stack_out[at] = page0 + i;
+      else
+        record_error(SJ_DEV_BAD_INDEX);
+    }
+    back += __popc(have);
+  }
+  if (cta == 0 && t == 0) {
+    const int left = min(count - taken + all, a.pages);
+    *a.count_out = status ? count : left;
+    a.summary[0] = taken;
+    a.summary[1] = all;
+    a.summary[2] = status;
+    a.summary[3] = status ? count : left;
+  }
+  cluster.sync();  // nobody's shared memory goes while another reads it
+}
+
+// ---------------------------------------------------------------- copy
+struct PagedCopy {
+  const int32_t* copies;
+  __nv_bfloat16 *k, *v;
+  int64_t layer_stride, page_stride, head_stride, token_stride;
+  int pages, page, hk, parts, tokens_outside;
+};
+
+// A CTA takes kCopyThreads * kCopyPieces pieces of 16 bytes of one copy, of K or of V of one layer; a page's rows and
+// heads go in the order in which they lie in memory.  All loads of a thread are in flight before its first store.
+template <int DIM>
+__global__ void __launch_bounds__(kCopyThreads) paged_copy_kernel(const PagedCopy a) {
+  pdl_wait();
+  const int entry = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+  const int from = a.copies[3 * entry], to = a.copies[3 * entry + 1], rows = a.copies[3 * entry + 2];
+  if (from == -1) return;
+  if (from < 0 || from >= a.pages || to < 0 || to >= a.pages || rows < 0 || rows > a.page) {
+    if (threadIdx.x == 0) record_error(SJ_DEV_BAD_INDEX);
+    return;
+  }
+  constexpr int PER = DIM / 8;  // pieces of a row of a head
+  const int inner = a.tokens_outside ? a.hk : rows, lines = rows * a.hk;
+  __nv_bfloat16* base = (blockIdx.y & 1 ? a.v : a.k) + static_cast<int64_t>(blockIdx.y >> 1) * a.layer_stride;
+  const __nv_bfloat16* src = base + from * a.page_stride;
+  __nv_bfloat16* dst = base + to * a.page_stride;
+  uint4 x[kCopyPieces];
+  int64_t at[kCopyPieces];
+#pragma unroll
+  for (int i = 0; i < kCopyPieces; ++i) {
+    const int piece = (part * kCopyPieces + i) * kCopyThreads + static_cast<int>(threadIdx.x), line = piece / PER;
+    at[i] = -1;
+    if (line < lines) {
+      const int outer = line / inner, in = line - outer * inner;
+      const int64_t head = a.tokens_outside ? in : outer, row = a.tokens_outside ? outer : in;
+      at[i] = head * a.head_stride + row * a.token_stride + piece % PER * 8;
+      x[i] = *reinterpret_cast<const uint4*>(src + at[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kCopyPieces; ++i)
+    if (at[i] >= 0) *reinterpret_cast<uint4*>(dst + at[i]) = x[i];
+}
+
+// ---------------------------------------------------------------- compact
+struct Compact {
+  const int32_t *cached, *table, *shares, *stack, *stack_count;
+  int32_t *table_out, *shares_out, *stack_out, *moves, *summary;
+  int batch, page, ld_table, pages, most;
+};
+
+// Every CTA reads the whole stack into a bit mask of the free pages with the numbers of pages in use before each word,
+// and writes its share of the results: the i-th page in use from `used` on goes to the i-th free page below it.
+__global__ void __launch_bounds__(kCompactThreads) paged_compact_kernel(const Compact a) {
+  pdl_wait();
+  extern __shared__ uint32_t bits[];                          // a bit for each page: free
+  const int words = (a.pages + 31) / 32, t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  int* before = reinterpret_cast<int*>(bits + words);         // [words + 1] pages in use before each word
+  __shared__ int s_warp[32], s_bad;
+  const int count = *a.stack_count;
+  bool bad = count < 0 || count > a.pages;
+  for (int w = t; w < words; w += kCompactThreads) bits[w] = 0;
+  if (t == 0) s_bad = 0;
+  __syncthreads();
+  for (int i = t; i < (bad ? 0 : count); i += kCompactThreads) {
+    const int id = a.stack[i];
+    if (id < 0 || id >= a.pages)
+      s_bad = 1;
+    else if (atomicOr(&bits[id >> 5], 1u << (id & 31)) >> (id & 31) & 1)
+      s_bad = 1;  // twice on the stack
+  }
+  __syncthreads();
+  const int per = (words + kCompactThreads - 1) / kCompactThreads, w0 = min(t * per, words), w1 = min(w0 + per, words);
+  auto in_word = [&](int w) { return min(32, a.pages - w * 32) - __popc(bits[w]); };
+  int mine = 0;
+  for (int w = w0; w < w1; ++w) mine += in_word(w);
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += u;
+  }
+  if (lane == 31) s_warp[warp] = upto;
+  __syncthreads();
+  int base = upto - mine;
+  for (int w = 0; w < warp; ++w) base += s_warp[w];
+  for (int w = w0; w < w1; ++w) {
+    before[w] = base;
+    base += in_word(w);
+  }
+  bad |= s_bad != 0;
+  __syncthreads();
+  const int used = bad ? 0 : a.pages - count;
+  auto is_free = [&](int p) { return (bits[p >> 5] >> (p & 31) & 1) != 0; };
+  auto in_use_before = [&](int p) {  // p < pages
+    return before[p >> 5] + (p & 31) - __popc(bits[p >> 5] & ((1u << (p & 31)) - 1));
+  };
+  const int kept = bad || used == a.pages ? used : in_use_before(used), moved = used - kept;
+  const int status = bad ? kCompactBad : moved > a.most ? kCompactMovesOver : 0;
+  auto target = [&](int p) {
+    if (status || p < used) return p;
+    const int r = in_use_before(p) - kept;  // the r-th hole: the last word with at most r holes before it
+    int lo = 0, hi = (used + 31) / 32;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (mid * 32 - before[mid] <= r)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    return lo * 32 + static_cast<int>(__fns(bits[lo], 0, r - (lo * 32 - before[lo]) + 1));
+  };
+  const int first = blockIdx.x * kCompactThreads + t, step = gridDim.x * kCompactThreads;
+  for (int b = first >> 5; b < a.batch; b += step >> 5) {
+    const int n = a.cached[b];
+    if (n < 0 || n > INT_MAX - a.page || (n + a.page - 1) / a.page > a.ld_table) {
+      if (lane == 0) record_error(SJ_DEV_BAD_INDEX);
+      continue;
+    }
+    const size_t row = static_cast<size_t>(b) * a.ld_table;
+    for (int j = lane; j < (n + a.page - 1) / a.page; j += 32) {
+      const int id = a.table[row + j];
+      const bool fine = id >= 0 && id < a.pages && (bad || !is_free(id));
+      if (!fine) record_error(SJ_DEV_BAD_INDEX);
+      a.table_out[row + j] = fine ? target(id) : id;
+    }
+  }
+  for (int p = first; p < a.pages; p += step) {
+    if (status) {
+      a.shares_out[p] = a.shares[p];
+      continue;
+    }
+    if (!is_free(p)) {
+      const int to = target(p);
+      a.shares_out[to] = a.shares[p];
+      if (to != p) {
+        const int i = in_use_before(p) - kept;
+        a.moves[3 * i] = p;
+        a.moves[3 * i + 1] = to;
+        a.moves[3 * i + 2] = a.page;
+      }
+    }
+    if (p >= used) a.shares_out[p] = 0;
+  }
+  for (int i = (status ? 0 : moved) + first; i < a.most; i += step) {
+    a.moves[3 * i] = a.moves[3 * i + 1] = -1;
+    a.moves[3 * i + 2] = 0;
+  }
+  for (int i = first; i < min(max(count, 0), a.pages); i += step) a.stack_out[i] = status ? a.stack[i] : a.pages - 1 - i;
+  if (first == 0) {
+    a.summary[0] = status ? 0 : moved;
+    a.summary[1] = used;
+    a.summary[2] = status;
+    a.summary[3] = count;
+  }
+}
+
+}  // namespace sj
+
+using namespace sj;
+
+extern "C" int sj_paged_fork(const int32_t* parent, int batch, int page, const int32_t* cached,
+                             const int32_t* block_table, int ld_table, const int32_t* shares,
+                             const int32_t* free_pages, const int32_t* free_count, int pages, int32_t* cached_out,
+                             int32_t* table_out, int32_t* shares_out, int32_t* free_out, int32_t* count_out,
+                             int32_t* copies, int32_t* summary, void* stream) {
+  if (batch <= 0 || batch > kShareMaxBatch || page <= 0 || page > (1 << 20) || ld_table <= 0 || pages <= 0 ||
+      pages > kShareMaxPages)
+    return fail(SJ_ERR_SHAPE, "sj_paged_fork: batch=%d (up to %d) page=%d ld_table=%d pages=%d (up to %d)", batch,
+                kShareMaxBatch, page, ld_table, pages, kShareMaxPages);
+  if (!parent || !cached || !block_table || !shares || !free_pages || !free_count || !cached_out || !table_out ||
+      !shares_out || !free_out || !count_out || !copies || !summary)
+    return fail(SJ_ERR_ARGUMENT, "sj_paged_fork: null operand");
+  if (cached == cached_out || block_table == table_out || shares == shares_out || free_pages == free_out ||
+      free_count == count_out)
+    return fail(SJ_ERR_ARGUMENT, "sj_paged_fork: the new state needs buffers of its own");
+  Fork a{parent, cached, block_table, shares, free_pages, free_count, cached_out, table_out, shares_out,
+         free_out, count_out, copies, summary, batch, page, ld_table, pages, (pages + kForkCluster - 1) / kForkCluster};
+  const int smem = (3 * (batch + 1) + a.per) * static_cast<int>(sizeof(int));
+  static KernelAttrOnce once;
+  constexpr int most = (3 * (kShareMaxBatch + 1) + kShareMaxPages / kForkCluster) * static_cast<int>(sizeof(int));
+  const int rc = ensure_max_smem(once, reinterpret_cast<const void*>(paged_fork_kernel), most,
+                                 "sj_paged_fork: shared memory");
+  if (rc != SJ_OK) return rc;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = kForkCluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  const int writers = std::min((batch + kForkWarps - 1) / kForkWarps, sm_count() / 2);
+  cfg.gridDim = dim3(kForkCluster * (1 + (writers + kForkCluster - 1) / kForkCluster));
+  cfg.blockDim = dim3(kForkThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = as_stream(stream);
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  void* args[] = {&a};
+  cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(paged_fork_kernel), args);
+  SJ_LAUNCH_CHECK("paged_fork");
+  return SJ_OK;
+}
+
+extern "C" int sj_paged_copy(const int32_t* copies, int most, void* k_cache, void* v_cache, int layers,
+                             int64_t layer_stride, int pages, int page, int64_t page_stride, int64_t head_stride,
+                             int64_t token_stride, int hk, int head_dim, void* stream) {
+  if (most < 0 || hk <= 0 || hk > 4096 || layers <= 0 || layers > 4096)
+    return fail(SJ_ERR_SHAPE, "sj_paged_copy: most=%d hk=%d layers=%d (up to 4096)", most, hk, layers);
+  const int rc = check_paged_cache("sj_paged_copy", k_cache, v_cache, pages, page, page_stride, head_stride,
+                                   token_stride, hk, head_dim);
+  if (rc != SJ_OK) return rc;
+  if (layer_stride < 0 || layer_stride % 8 || layer_stride > (int64_t{1} << 62) / layers)
+    return fail(SJ_ERR_ARGUMENT, "sj_paged_copy: a layer stride that is a multiple of 8");
+  if (most == 0) return SJ_OK;
+  if (!copies) return fail(SJ_ERR_ARGUMENT, "sj_paged_copy: null operand");
+  const int64_t pieces = static_cast<int64_t>(page) * hk * (head_dim / 8);
+  constexpr int each = kCopyThreads * kCopyPieces;
+  const int64_t parts = (pieces + each - 1) / each;
+  if (pieces > INT_MAX - each || parts * most > INT_MAX)
+    return fail(SJ_ERR_SHAPE, "sj_paged_copy: most=%d page=%d hk=%d", most, page, hk);
+  PagedCopy a{copies, static_cast<__nv_bfloat16*>(k_cache), static_cast<__nv_bfloat16*>(v_cache), layer_stride,
+              page_stride, head_stride, token_stride, pages, page, hk, static_cast<int>(parts),
+              token_stride > head_stride ? 1 : 0};
+  launch(head_dim == 64 ? paged_copy_kernel<64> : paged_copy_kernel<128>,
+         dim3(static_cast<unsigned>(parts * most), 2 * layers), kCopyThreads, 0, as_stream(stream), a);
+  SJ_LAUNCH_CHECK("paged_copy");
+  return SJ_OK;
+}
+
+extern "C" int sj_paged_compact(const int32_t* cached, int batch, int page, const int32_t* block_table, int ld_table,
+                                const int32_t* shares, const int32_t* free_pages, const int32_t* free_count,
+                                int pages, int32_t* table_out, int32_t* shares_out, int32_t* free_out, int32_t* moves,
+                                int most, int32_t* summary, void* stream) {
+  if (batch <= 0 || batch > kShareMaxBatch || page <= 0 || page > (1 << 20) || ld_table <= 0 || pages <= 0 ||
+      pages > kShareMaxPages || most < 0 || most > INT_MAX / 3)
+    return fail(SJ_ERR_SHAPE, "sj_paged_compact: batch=%d (up to %d) page=%d ld_table=%d pages=%d (up to %d) most=%d",
+                batch, kShareMaxBatch, page, ld_table, pages, kShareMaxPages, most);
+  if (!cached || !block_table || !shares || !free_pages || !free_count || !table_out || !shares_out || !free_out ||
+      !summary || (most > 0 && !moves))
+    return fail(SJ_ERR_ARGUMENT, "sj_paged_compact: null operand");
+  if (block_table == table_out || shares == shares_out || free_pages == free_out)
+    return fail(SJ_ERR_ARGUMENT, "sj_paged_compact: the new state needs buffers of its own");
+  const int words = (pages + 31) / 32;
+  static KernelAttrOnce once;
+  const int rc = ensure_max_smem(once, reinterpret_cast<const void*>(paged_compact_kernel),
+                                 (kShareMaxPages / 32 * 2 + 1) * static_cast<int>(sizeof(int)),
+                                 "sj_paged_compact: shared memory");
+  if (rc != SJ_OK) return rc;
+  const Compact a{cached, block_table, shares, free_pages, free_count, table_out, shares_out, free_out,
+                  moves, summary, batch, page, ld_table, pages, most};
+  const int64_t work = std::max<int64_t>(static_cast<int64_t>(batch) * 32, std::max(pages, most));
+  const int grid = static_cast<int>(std::min<int64_t>((work + kCompactThreads - 1) / kCompactThreads, sm_count()));
+  launch(paged_compact_kernel, grid, kCompactThreads, (2 * words + 1) * sizeof(int), as_stream(stream), a);
+  SJ_LAUNCH_CHECK("paged_compact");
+  return SJ_OK;
+}

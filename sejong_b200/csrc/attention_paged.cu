@@ -31,6 +31,7 @@
 #include <climits>
 #include <cmath>
 
+#include "attention_paged.cuh"
 #include "common.cuh"
 #include "internal.h"
 
@@ -49,17 +50,6 @@ constexpr int kWarps = 4, kCtas = 3, kStages = 2;  // of a CTA, of an SM, of a w
 constexpr int kLastPosition = INT_MAX - 4096;  // key indices step past the end by less than this
 constexpr uint32_t kNoKey = 0xffffffffu;     // past any offset: buffers hold at most 2^32 16-byte chunks
 }  // namespace
-
-struct PagedAttention {
-  const __nv_bfloat16 *q, *k, *v;
-  const int32_t *table, *request, *position;
-  __nv_bfloat16* o;
-  float* lse;
-  int* counters;   // parts written of each first group of a unit, of other groups, groups of a unit: a CTA one of each
-  float* partial;  // two slots per CTA
-  int64_t page_stride, head_stride, token_stride;
-  int ldq, ldo, pages, page, ld_table, requests, rows, hq, hk, window;
-};
 
 // 16 bytes from global to shared memory without passing through registers; zeros when !seen.
 SJ_DEVICE void copy16(uint32_t dst, const __nv_bfloat16* src, bool seen) {
@@ -230,9 +220,102 @@ SJ_DEVICE int arrive(int* counter) {
   return before;
 }
 
-// DIM: head_dim; NQ: query tiles of 8 that a unit holds (a query's columns of S^T; 2 above 8 heads a KV head).
-template <int DIM, int NQ>
-__global__ void __launch_bounds__(kWarps * 32, kCtas) attn_paged_kernel(const PagedAttention a) {
+// A row's own part (of `heads` heads from `head` on: outputs `own` [heads][DIM], maxima and sums) joined with the parts of
+// its keys in common, and written.  The parts of those are taken by `shares` threads a float4 each, in the order of the
+// parts, then one after the other.
+constexpr int kScratch = 1024;  // float4 of `so` that hold a unit's joined outputs
+template <int DIM, int Q, int WARPS>
+__device__ __noinline__ void join_shared(const PagedAttention& a, const SharedSpans& s, const SharedRow& row, int r,
+                                         int head, int q0, int heads, const float* own, const float* own_m,
+                                         const float* own_l, float4* scratch, float (*weight)[Q]) {
+  constexpr int THREADS = WARPS * 32;
+  const int t = threadIdx.x, items = heads * (DIM / 4), fan = a.hq / a.hk;
+  int from = 0, parts = 0, query = 0;
+  if (row.group >= 0) {
+    const SharedGroup g = s.groups[row.group];
+    const int per = kSharedQueries / fan, at = r - g.first, tile = at / per;
+    const bool two = tile / 2 < g.tiles / 2;
+    const SharedCut cut(*s.total, s.ctas);
+    const unsigned long long begin = g.base + (head / fan) * g.head_items() + static_cast<unsigned long long>(tile / 2) * g.keys;
+    from = cut.of(begin);
+    parts = cut.of(begin + (two ? g.keys : g.halves()) - 1) - from + 1;
+    query = (two ? (tile & 1) * kSharedQueries : 0) + at % per * fan + q0;
+  }
+  const int shares = max(1, min(parts, THREADS / items));
+#pragma unroll 1
+  for (int i = t; i < items * shares; i += THREADS) {
+    const int share = i / items, qi = i % items / (DIM / 4), d = i % (DIM / 4) * 4;
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int p0 = share; p0 < parts; p0 += 4 * shares) {
+      float pm[4], pl[4];
+      float4 x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int p = min(p0 + e * shares, parts - 1);
+        if (p == 0) {
+          const size_t at = static_cast<size_t>(r) * a.hq + head + qi;
+          pm[e] = s.m[at];
+          pl[e] = s.l[at];
+          x[e] = *reinterpret_cast<const float4*>(s.o + at * DIM + d);
+        } else {
+          const float* slot = shared_slot<DIM>(s, from + p, query + qi);
+          pm[e] = slot[0];
+          pl[e] = slot[1];
+          x[e] = *reinterpret_cast<const float4*>(slot + 4 + d);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (p0 + e * shares >= parts) continue;
+        const float top = fmaxf(m, pm[e]), base = top == -INFINITY ? 0.f : top;
+        const float f = exp2_fast(m - base), g = exp2_fast(pm[e] - base);
+        l = f * l + g * pl[e];
+        acc.x = f * acc.x + g * x[e].x;
+        acc.y = f * acc.y + g * x[e].y;
+        acc.z = f * acc.z + g * x[e].z;
+        acc.w = f * acc.w + g * x[e].w;
+        m = top;
+      }
+    }
+    scratch[i] = acc;
+    if (d == 0) {
+      weight[2 * share][qi] = m;
+      weight[2 * share + 1][qi] = l;
+    }
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int i = t; i < items; i += THREADS) {
+    const int qi = i / (DIM / 4), d = i % (DIM / 4) * 4;
+    float m = own_m[qi], l = own_l[qi];
+    float4 acc = *reinterpret_cast<const float4*>(own + qi * DIM + d);
+#pragma unroll 1
+    for (int w = 0; w < (parts ? shares : 0); ++w) {
+      const float pm = weight[2 * w][qi], top = fmaxf(m, pm), base = top == -INFINITY ? 0.f : top;
+      const float f = exp2_fast(m - base), g = exp2_fast(pm - base);
+      const float4 x = scratch[w * items + i];
+      l = f * l + g * weight[2 * w + 1][qi];
+      acc.x = f * acc.x + g * x.x;
+      acc.y = f * acc.y + g * x.y;
+      acc.z = f * acc.z + g * x.z;
+      acc.w = f * acc.w + g * x.w;
+      m = top;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    *reinterpret_cast<uint2*>(a.o + static_cast<size_t>(r) * a.ldo + (head + qi) * DIM + d) =
+        make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+    if (d == 0 && a.lse)
+      a.lse[static_cast<size_t>(r) * a.hq + head + qi] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  }
+  __syncthreads();  // the caller goes on with the shared arrays
+}
+
+// DIM: head_dim; NQ: query tiles of 8 that a unit holds (a query's columns of S^T; 2 above 8 heads a KV head).  SHARED:
+// `spans` says which keys of each row attn_shared_kernel has taken; keys are then counted without those.
+template <int DIM, int NQ, bool SHARED>
+__global__ void __launch_bounds__(kWarps * 32, kCtas) attn_paged_kernel(const PagedAttention a, const SharedSpans spans) {
   pdl_wait();
   constexpr int WARPS = kWarps, STAGES = kStages, KT = 128 / DIM;  // KT: 16-key tiles of a warp's step
   constexpr int CC = DIM / 32, CH = DIM / 64, MT = DIM / 16, Q = NQ * 8, KEYS = KT * 16, STEP = WARPS * KEYS;
@@ -245,10 +328,20 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attn_paged_kernel(const Pa
   uint8_t* smem = unaligned + (-smem_u32(unaligned) & 127);
   float* so = reinterpret_cast<float*>(smem);  // [WARPS][Q][LD], once a unit's stages are read
   __shared__ float sm[WARPS][Q], sl[WARPS][Q], weight[kGroupMost][Q];
+  __shared__ __align__(16) float fin[SHARED ? Q * DIM : 4], fm[Q], fl[Q];
   __shared__ unsigned long long scan[WARPS], s_base;
   __shared__ int s_row, s_last;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = lane >> 2, c = lane & 3;
   const int group = a.hq / a.hk, sets = (group + Q - 1) / Q, units = a.hk * sets;
+  auto row_span = [&](int r, int& lo, int& n) {  // [lo, n): of a row's own keys, counted from its first
+    if constexpr (SHARED) {
+      const SharedRow row = spans.rows[r];
+      lo = 0;
+      n = row.n - row.lo - (row.p1 - row.p0);
+    } else {
+      sj::row_span(a, r, lo, n);
+    }
+  };
   const float scale = 1.4426950408889634f * rsqrtf(static_cast<float>(DIM));
   const uint32_t ring = smem_u32(smem) + warp * STAGES * STAGE;
   // shared-memory addresses inside a stage: 128-byte rows (of a half of DIM) whose 16-byte chunks are permuted
@@ -262,7 +355,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attn_paged_kernel(const Pa
   unsigned long long mine = 0;
   for (int r = r0; r < r1; ++r) {
     int lo, n;
-    row_span(a, r, lo, n);
+    row_span(r, lo, n);
     mine += static_cast<unsigned long long>(span_tiles(lo, n)) * units;
   }
   unsigned long long upto = mine;
@@ -288,7 +381,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attn_paged_kernel(const Pa
     unsigned long long base = before;
     for (int r = r0; r < r1; ++r) {
       int lo, n;
-      row_span(a, r, lo, n);
+      row_span(r, lo, n);
       const unsigned long long next = base + static_cast<unsigned long long>(span_tiles(lo, n)) * units;
       if (at < next) {
         s_row = r;
@@ -303,9 +396,11 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attn_paged_kernel(const Pa
 
   for (int r = s_row; at < end; ++r) {
     int lo, n;
-    row_span(a, r, lo, n);
+    row_span(r, lo, n);
     const int tiles = span_tiles(lo, n);
     const int32_t* table = a.table + static_cast<size_t>(n > 0 ? (a.request ? a.request[r] : r) : 0) * a.ld_table;
+    SharedRow whole_row{};
+    if constexpr (SHARED) whole_row = spans.rows[r];
     int unit = static_cast<int>((at - base) / tiles), first = static_cast<int>((at - base) % tiles);
     if (first > 0 && tiles <= kWhole) {  // a short unit stays with the CTA that its first tile falls to
       at += tiles - first;
@@ -323,7 +418,14 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attn_paged_kernel(const Pa
       // then resolves where the key lies (in 16-byte chunks)
       const int steps = k1 > k0 + warp * KEYS ? (k1 - k0 - warp * KEYS + STEP - 1) / STEP : 0;
       int key = k0 + warp * KEYS + lane, found = 0;
-      int pg = key / a.page, off = key % a.page;
+      auto place = [&](int own) {  // a row's keys before and after those in common
+        if constexpr (SHARED) {
+          own += whole_row.lo;
+          if (own >= whole_row.p0) own += whole_row.p1 - whole_row.p0;
+        }
+        return own;
+      };
+      int pg = place(key) / a.page, off = place(key) % a.page;
       const int step_page = STEP / a.page, step_off = STEP % a.page;
       auto look_up = [&]() {
         if (lane < KEYS && key < k1) found = table[pg];
@@ -337,6 +439,11 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attn_paged_kernel(const Pa
             record_error(SJ_DEV_BAD_INDEX);
         }
         key += STEP;
+        if constexpr (SHARED) {
+          pg = place(key) / a.page;
+          off = place(key) - pg * a.page;
+          return where;
+        }
         pg += step_page;
         off += step_off;
         if (off >= a.page) {
@@ -541,7 +648,13 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attn_paged_kernel(const Pa
           out.w += x.w;
           sum += exp2_fast(sm[w][qi] - ref) * sl[w][qi];
         }
-        if (whole) {
+        if (SHARED && whole) {
+          *reinterpret_cast<float4*>(fin + qi * DIM + d) = out;
+          if (d == 0) {
+            fm[qi] = top;
+            fl[qi] = sum;
+          }
+        } else if (whole) {
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
           const int head = h * group + q0 + qi;
           *reinterpret_cast<uint2*>(a.o + static_cast<size_t>(r) * a.ldo + head * DIM + d) =
@@ -556,6 +669,11 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attn_paged_kernel(const Pa
             slot[Q + qi] = sum;
           }
         }
+      }
+      if (SHARED && whole) {
+        __syncthreads();
+        join_shared<DIM, Q, WARPS>(a, spans, whole_row, r, h * group + q0, q0, heads, fin, fm, fl,
+                                   reinterpret_cast<float4*>(so) + kScratch, weight);
       }
       if (!whole) {
         // ---- the unit's parts joined by the CTA that writes the last of them: tile x falls to the last chunk w
@@ -591,7 +709,10 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attn_paged_kernel(const Pa
           joined = last_of(a.counters + 2 * gridDim.x + from, groups);
           if (joined) join_parts<DIM, Q, WARPS>(a.partial, from, from, groups, size, heads, sm[0], sl[0], weight, sums);
         }
-        if (joined) {
+        if (SHARED && joined) {
+          join_shared<DIM, Q, WARPS>(a, spans, whole_row, r, h * group + q0, q0, heads, so, sm[0], sl[0],
+                                     reinterpret_cast<float4*>(so) + kScratch, weight);
+        } else if (joined) {
           for (int i = t; i < heads * (DIM / 4); i += WARPS * 32) {
             const int qi = i / (DIM / 4), d = i % (DIM / 4) * 4, head = h * group + q0 + qi;
             const float sum = sl[0][qi], inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -621,19 +742,30 @@ int query_tiles(int hq, int hk) { return hq / hk > 8 ? 2 : 1; }
 int most_ctas() { return kCtas * sm_count(); }
 size_t counter_bytes() { return (3 * static_cast<size_t>(most_ctas()) * sizeof(int) + 255) / 256 * 256; }
 
-template <int DIM, int NQ>
-int attend(const PagedAttention& a, cudaStream_t stream) {
+template <int DIM, int NQ, bool SHARED>
+int attend(const PagedAttention& a, const SharedSpans& spans, cudaStream_t stream) {
   constexpr int outputs = kWarps * NQ * 8 * (DIM + 8) * 4, rings = kWarps * kStages * 8192;
   constexpr int smem = (outputs > rings ? outputs : rings) + 128;
+  static_assert(2 * kScratch * 16 <= rings && NQ * 8 * DIM / 4 <= kScratch, "joined outputs, and parts beside them");
   static KernelAttrOnce once;
-  const int rc = ensure_max_smem(once, reinterpret_cast<const void*>(attn_paged_kernel<DIM, NQ>), smem,
+  const int rc = ensure_max_smem(once, reinterpret_cast<const void*>(attn_paged_kernel<DIM, NQ, SHARED>), smem,
                                  "sj_attn_paged: shared memory");
   if (rc != SJ_OK) return rc;
-  launch(attn_paged_kernel<DIM, NQ>, most_ctas(), kWarps * 32, smem, stream, a);
+  launch(attn_paged_kernel<DIM, NQ, SHARED>, most_ctas(), kWarps * 32, smem, stream, a, spans);
   SJ_LAUNCH_CHECK("attn_paged");
   return SJ_OK;
 }
+template <bool SHARED>
+int attend(const PagedAttention& a, const SharedSpans& spans, int head_dim, cudaStream_t s) {
+  const int nq = query_tiles(a.hq, a.hk);
+  if (head_dim == 64) return nq == 1 ? attend<64, 1, SHARED>(a, spans, s) : attend<64, 2, SHARED>(a, spans, s);
+  return nq == 1 ? attend<128, 1, SHARED>(a, spans, s) : attend<128, 2, SHARED>(a, spans, s);
+}
 }  // namespace
+
+int sj::attn_paged_rows(const PagedAttention& a, const SharedSpans* spans, int head_dim, cudaStream_t stream) {
+  return spans ? attend<true>(a, *spans, head_dim, stream) : attend<false>(a, SharedSpans{}, head_dim, stream);
+}
 
 extern "C" size_t sj_attn_paged_workspace(int rows, int hq, int hk, int head_dim) {
   if (rows < 0 || hq <= 0 || hk <= 0 || hq % hk || (head_dim != 64 && head_dim != 128)) return 0;
@@ -641,26 +773,26 @@ extern "C" size_t sj_attn_paged_workspace(int rows, int hq, int hk, int head_dim
   return counter_bytes() + static_cast<size_t>(most_ctas()) * 2 * nq * 8 * (head_dim + 2) * sizeof(float);
 }
 
-extern "C" int sj_attn_paged(const void* q, int ldq, const void* k_cache, const void* v_cache, int pages, int page,
-                             int64_t page_stride, int64_t head_stride, int64_t token_stride,
-                             const int32_t* block_table, int ld_table, int requests, const int32_t* request,
-                             const int32_t* position, int rows, int hq, int hk, int head_dim, int window, void* o,
-                             int ldo, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+int sj::paged_attention_args(const char* who, PagedAttention& a, const void* q, int ldq, const void* k_cache,
+                             const void* v_cache, int pages, int page, int64_t page_stride, int64_t head_stride,
+                             int64_t token_stride, const int32_t* block_table, int ld_table, int requests,
+                             const int32_t* request, const int32_t* position, int rows, int hq, int hk, int head_dim,
+                             int window, void* o, int ldo, float* lse, void* workspace, size_t workspace_bytes,
+                             size_t need) {
   if (rows < 0 || requests <= 0 || ld_table <= 0 || hq <= 0 || hk <= 0 || hq % hk || hq > 4096 || window < 0 ||
       (!request && rows > requests))
-    return fail(SJ_ERR_SHAPE, "sj_attn_paged: rows=%d requests=%d ld_table=%d hq=%d hk=%d window=%d", rows, requests,
+    return fail(SJ_ERR_SHAPE, "%s: rows=%d requests=%d ld_table=%d hq=%d hk=%d window=%d", who, rows, requests,
                 ld_table, hq, hk, window);
-  const int rc = check_paged_cache("sj_attn_paged", k_cache, v_cache, pages, page, page_stride, head_stride,
+  const int rc = check_paged_cache(who, k_cache, v_cache, pages, page, page_stride, head_stride,
                                    token_stride, hk, head_dim);
   if (rc != SJ_OK) return rc;
   if (ldq < hq * head_dim || ldo < hq * head_dim)
-    return fail(SJ_ERR_SHAPE, "sj_attn_paged: ldq=%d ldo=%d", ldq, ldo);
+    return fail(SJ_ERR_SHAPE, "%s: ldq=%d ldo=%d", who, ldq, ldo);
   if (rows == 0) return SJ_OK;
   if (!q || !o || !block_table || !position || !aligned16(q) || !aligned16(o) || ldq % 8 || ldo % 8)
-    return fail(SJ_ERR_ARGUMENT, "sj_attn_paged: null or unaligned operand, or a row stride not a multiple of 8");
-  if (!workspace || !aligned16(workspace) || workspace_bytes < sj_attn_paged_workspace(rows, hq, hk, head_dim))
-    return fail(SJ_ERR_CAPACITY, "sj_attn_paged: workspace of %zu bytes", workspace_bytes);
-  PagedAttention a;
+    return fail(SJ_ERR_ARGUMENT, "%s: null or unaligned operand, or a row stride not a multiple of 8", who);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < need)
+    return fail(SJ_ERR_CAPACITY, "%s: workspace of %zu bytes", who, workspace_bytes);
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.k = static_cast<const __nv_bfloat16*>(k_cache);
   a.v = static_cast<const __nv_bfloat16*>(v_cache);
@@ -684,28 +816,19 @@ extern "C" int sj_attn_paged(const void* q, int ldq, const void* k_cache, const 
   a.hq = hq;
   a.hk = hk;
   a.window = window;
-  const int nq = query_tiles(hq, hk);
-  cudaStream_t s = as_stream(stream);
-  if (head_dim == 64) return nq == 1 ? attend<64, 1>(a, s) : attend<64, 2>(a, s);
-  return nq == 1 ? attend<128, 1>(a, s) : attend<128, 2>(a, s);
+  return SJ_OK;
 }
 
-// Groups say which keys rows share; this form reads them for each row.
-extern "C" size_t sj_attn_paged_shared_workspace(int rows, int groups, int hq, int hk, int head_dim) {
-  if (groups < 0) return 0;
-  return sj_attn_paged_workspace(rows, hq, hk, head_dim);
-}
-
-extern "C" int sj_attn_paged_shared(const void* q, int ldq, const void* k_cache, const void* v_cache, int pages,
-                                    int page, int64_t page_stride, int64_t head_stride, int64_t token_stride,
-                                    const int32_t* block_table, int ld_table, int requests, const int32_t* request,
-                                    const int32_t* position, int rows, const int32_t* group, int groups, int hq,
-                                    int hk, int head_dim, int window, void* o, int ldo, float* lse, void* workspace,
-                                    size_t workspace_bytes, void* stream) {
-  if (groups < 0 || (rows > 0 && groups > rows))
-    return fail(SJ_ERR_SHAPE, "sj_attn_paged_shared: groups=%d rows=%d", groups, rows);
-  if (rows > 0 && groups > 0 && !group) return fail(SJ_ERR_ARGUMENT, "sj_attn_paged_shared: null operand");
-  return sj_attn_paged(q, ldq, k_cache, v_cache, pages, page, page_stride, head_stride, token_stride, block_table,
-                       ld_table, requests, request, position, rows, hq, hk, head_dim, window, o, ldo, lse, workspace,
-                       workspace_bytes, stream);
+extern "C" int sj_attn_paged(const void* q, int ldq, const void* k_cache, const void* v_cache, int pages, int page,
+                             int64_t page_stride, int64_t head_stride, int64_t token_stride,
+                             const int32_t* block_table, int ld_table, int requests, const int32_t* request,
+                             const int32_t* position, int rows, int hq, int hk, int head_dim, int window, void* o,
+                             int ldo, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  PagedAttention a;
+  const int rc = paged_attention_args("sj_attn_paged", a, q, ldq, k_cache, v_cache, pages, page, page_stride,
+                                      head_stride, token_stride, block_table, ld_table, requests, request, position,
+                                      rows, hq, hk, head_dim, window, o, ldo, lse, workspace, workspace_bytes,
+                                      sj_attn_paged_workspace(rows, hq, hk, head_dim));
+  if (rc != SJ_OK || rows == 0) return rc;
+  return attn_paged_rows(a, nullptr, head_dim, as_stream(stream));
 }

@@ -1,0 +1,77 @@
+// The arguments of attn_paged_kernel, and what the kernels of sj_attn_paged_shared hand to one another through the
+// workspace.
+#pragma once
+#include "common.cuh"
+
+namespace sj {
+
+struct PagedAttention {
+  const __nv_bfloat16 *q, *k, *v;
+  const int32_t *table, *request, *position;
+  __nv_bfloat16* o;
+  float* lse;
+  int* counters;   // parts written of each first group of a unit, of other groups, groups of a unit: a CTA one of each
+  float* partial;  // two slots per CTA
+  int64_t page_stride, head_stride, token_stride;
+  int ldq, ldo, pages, page, ld_table, requests, rows, hq, hk, window;
+};
+
+constexpr int kSharedKeys = 128;     // keys of a tile
+constexpr int kSharedQueries = 128;  // queries of a tile: whole rows of hq / hk heads that share a KV head
+
+// Ranges of equal length of `total` items, one for a CTA.
+struct SharedCut {
+  unsigned long long total;
+  int count;
+  SJ_DEVICE SharedCut(unsigned long long items, int ctas)
+      : total(items), count(static_cast<int>(min(static_cast<unsigned long long>(ctas), items))) {}
+  SJ_DEVICE unsigned long long begin(int id) const { return total * id / count; }
+  // the last range that begins at or before item x, which holds it
+  SJ_DEVICE int of(unsigned long long x) const {
+    return static_cast<int>(((x + 1) * count + total - 1) / total) - 1;
+  }
+};
+
+// A group: its rows, the keys [p0, p1) that every live one of them sees, and its first item.  The queries of a KV head
+// lie in `tiles` tiles.  A unit is two tiles of queries, whose item is a tile of keys for both, or the one tile that is
+// left, whose item is two tiles of keys: an item is the same work either way.
+struct SharedGroup {
+  unsigned long long base;
+  int first, rows, request, p0, p1, tiles, keys;  // keys: tiles of them
+  SJ_DEVICE int halves() const { return (keys + 1) / 2; }
+  SJ_DEVICE unsigned long long head_items() const {
+    return static_cast<unsigned long long>(tiles / 2) * keys + (tiles & 1) * halves();
+  }
+};
+
+// A row: keys [lo, p0) and [p1, n) are its own, group -1: all of [lo, n).
+struct SharedRow {
+  int lo, n, p0, p1, group;
+};
+
+struct SharedSpans {
+  unsigned long long* total;  // items of all groups
+  SharedGroup* groups;
+  SharedRow* rows;
+  float *m, *l, *o;  // [rows, hq (, dim)]: the part of a row's common keys that begins its unit
+  int ctas;          // of attn_shared_kernel
+  float* slots;      // [ctas][2 * kSharedQueries][dim + 4]: the part that goes on with a unit, of each CTA
+};
+
+template <int DIM>
+SJ_DEVICE float* shared_slot(const SharedSpans& s, int cta, int query) {  // m, l, o
+  return s.slots + (static_cast<size_t>(cta) * (2 * kSharedQueries) + query) * (DIM + 4);
+}
+
+// Checks the arguments of sj_attn_paged, or of a call (`who`) that has the same ones and a workspace of `need` bytes
+// that begins with that of sj_attn_paged.
+int paged_attention_args(const char* who, PagedAttention& a, const void* q, int ldq, const void* k_cache,
+                         const void* v_cache, int pages, int page, int64_t page_stride, int64_t head_stride,
+                         int64_t token_stride, const int32_t* block_table, int ld_table, int requests,
+                         const int32_t* request, const int32_t* position, int rows, int hq, int hk, int head_dim,
+                         int window, void* o, int ldo, float* lse, void* workspace, size_t workspace_bytes,
+                         size_t need);
+// Launches attn_paged_kernel: all of a row's keys, or (spans not null) its own ones, joined with those in common.
+int attn_paged_rows(const PagedAttention& a, const SharedSpans* spans, int head_dim, cudaStream_t stream);
+
+}  // namespace sj

@@ -1,0 +1,721 @@
+// The keys that the rows of a group have in common, read once for all of them (sj_attn_paged_shared).
+//
+//   shared_spans_kernel   each group's keys that all of its rows see, and the work that they are
+//   attn_shared_kernel    the queries of a group against those keys, on the tensor cores
+//
+// attn_paged_kernel (attention_paged.cu) then takes each row's own keys and joins the two.  With M queries a KV head, M
+// multiply-adds are made of each cache element: memory bounds a few of them, the exponentials and the tensor cores
+// many.  A row's keys outside [p0, p1), by its window or its length, are its own, so no tile needs a mask but for the
+// last one's end, and a value that a row does not see reaches no sum of it.
+#include <algorithm>
+#include <climits>
+#include <cmath>
+
+#include "attention_paged.cuh"
+#include "common.cuh"
+#include "internal.h"
+
+namespace sj {
+
+namespace {
+constexpr int kSharedGroups = 1024;
+constexpr int kSoftmaxWarps = 8, kMmaWarp = 8, kLoadWarps = 4;
+constexpr int kSharedThreads = 32 * (kSoftmaxWarps + 1 + kLoadWarps);
+constexpr int kSeen = 8;                   // tiles whose masks of valid keys are kept
+constexpr float kLazy = 8.f;               // a maximum may stand this far (of log2) below the true one
+constexpr uint32_t kColO = 256;            // TMEM columns: S of two streams (their P over it), then O
+constexpr uint32_t kTmemAll = 512;
+constexpr uint32_t kNowhere = 0xffffffffu;
+constexpr int kLastSeen = INT_MAX - 4096;
+}  // namespace
+
+// ---------------------------------------------------------------- spans
+struct SpansArgs {
+  const int32_t *request, *position, *group;
+  int rows, groups, requests, page, ld_table, window, fan, hk, least;
+  SharedSpans out;
+};
+
+// One CTA.  A group's p0 is the highest first key of its live rows, p1 the lowest end.
+__global__ void __launch_bounds__(1024) shared_spans_kernel(const SpansArgs a) {
+  pdl_wait();
+  __shared__ int first[kSharedGroups + 1], p0[kSharedGroups], p1[kSharedGroups], live[kSharedGroups];
+  __shared__ unsigned long long s_scan[32];
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int64_t most = static_cast<int64_t>(a.ld_table) * a.page;
+  if (t < a.groups) {
+    const int at = a.group[3 * t], b = a.group[3 * t + 1], n = a.group[3 * t + 2];
+    const int next = t + 1 < a.groups ? a.group[3 * t + 3] : a.rows;
+    const bool fine = at >= 0 && at < next && next <= a.rows && b >= 0 && b < a.requests && n >= 0 && n <= most;
+    if (!fine) record_error(SJ_DEV_BAD_INDEX);
+    first[t] = at;
+    p0[t] = 0;
+    p1[t] = fine ? n : -1;
+    live[t] = 0;
+  }
+  const bool ordered = __syncthreads_and(t >= a.groups || p1[t] >= 0);
+  auto owner = [&](int r) {
+    if (!ordered || a.groups == 0 || r < first[0]) return -1;
+    int lo = 0, hi = a.groups;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (first[mid] <= r)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    return lo;
+  };
+  for (int r = t; r < a.rows; r += 1024) {
+    const int b = a.request ? a.request[r] : r, pos = a.position[r];
+    int n = b == -1 || pos > kLastSeen ? 0 : pos + 1;
+    if (b < -1 || b >= a.requests || pos < -1 || pos > kLastSeen || n > most) {
+      record_error(SJ_DEV_BAD_INDEX);
+      n = 0;
+    }
+    const int lo = a.window > 0 ? max(0, n - a.window) : 0, g = owner(r);
+    a.out.rows[r] = SharedRow{lo, n, 0, 0, g};
+    if (g >= 0 && n > 0) {
+      atomicMax(&p0[g], lo);
+      atomicMin(&p1[g], n);
+      atomicAdd(&live[g], 1);
+    }
+  }
+  __syncthreads();
+  unsigned long long items = 0;
+  SharedGroup g{};
+  if (t < a.groups) {
+    g.first = first[t];
+    g.rows = (t + 1 < a.groups ? first[t + 1] : a.rows) - first[t];
+    g.request = a.group[3 * t + 1];
+    g.p0 = p0[t];
+    g.p1 = max(p1[t], p0[t]);
+    if (!ordered || live[t] < a.least) g.p1 = g.p0;
+    p1[t] = g.p1;
+    const int per = kSharedQueries / a.fan;  // rows of a tile
+    g.tiles = (g.rows + per - 1) / per;
+    g.keys = (g.p1 - g.p0 + kSharedKeys - 1) / kSharedKeys;
+    items = g.head_items() * a.hk;
+  }
+  unsigned long long upto = items;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned long long u = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += u;
+  }
+  if (lane == 31) s_scan[warp] = upto;
+  __syncthreads();
+  g.base = upto - items;
+  unsigned long long total = 0;
+  for (int w = 0; w < 32; ++w) {
+    if (w == warp) g.base += total;
+    total += s_scan[w];
+  }
+  if (t < a.groups) a.out.groups[t] = g;
+  if (t == 0) *a.out.total = total;
+  for (int r = t; r < a.rows; r += 1024) {
+    SharedRow& row = a.out.rows[r];
+    if (row.group >= 0 && row.n > 0 && p1[row.group] > p0[row.group]) {
+      row.p0 = p0[row.group];
+      row.p1 = p1[row.group];
+    } else {
+      row.group = -1;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- tensor-core pass
+struct SharedArgs {
+  const __nv_bfloat16 *q, *k, *v;
+  const int32_t* table;
+  int64_t page_stride, head_stride, token_stride;
+  int ldq, pages, page, ld_table, groups, hq, hk, fan;
+  float scale;  // log2(e) / sqrt(dim)
+  SharedSpans s;
+};
+
+SJ_DEVICE float shared_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+SJ_DEVICE void shared_copy16(uint32_t dst, const __nv_bfloat16* src, bool is) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(is ? 16 : 0) : "memory");
+}
+template <int LEFT>
+SJ_DEVICE void shared_copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+// 32 lanes x 16 consecutive 32-bit columns, from thread i to lane (base + i).
+SJ_DEVICE void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+SJ_DEVICE void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// D[tmem] (+)= A[tmem] * B[smem desc]: A holds two bf16 of a row in each 32-bit column.
+SJ_DEVICE void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+template <int DIM>
+struct SharedLay {
+  static constexpr int SLOT = kSharedKeys * DIM * 2;  // a tile of K, of V, or of queries
+  static constexpr int HALF = kSharedKeys * 128;      // 64 dims of it: rows of 128 bytes
+  static constexpr int STAGES = DIM == 64 ? 9 : 4;    // of the ring of K and V tiles
+  static constexpr int AHEAD = DIM == 64 ? 5 : 3;     // tiles of a load warp in flight
+  static constexpr int Q = 0, RING = 2 * SLOT, SEEN = RING + STAGES * SLOT, SUMS = SEEN + 2 * kSeen * 16,
+                       BARS = SUMS + 2 * kSharedQueries * 4, SMEM = BARS + 512 + 1024;
+};
+
+// A CTA's share of a unit: items [i0, i1) of one KV head and one or two tiles of queries.
+struct SharedPiece {
+  SharedGroup g;
+  int h, tile, i0, i1;
+  bool two;  // two tiles of queries over the same keys; else one, over alternate tiles of keys
+  int steps[2];
+  SJ_DEVICE int key(int stream, int step) const {
+    return g.p0 + (two ? i0 + step : 2 * (i0 + step) + stream) * kSharedKeys;
+  }
+};
+struct SharedWalk {
+  const SharedArgs& a;
+  unsigned long long at, end;
+  SJ_DEVICE explicit SharedWalk(const SharedArgs& a_) : a(a_), at(0), end(0) {
+    const SharedCut cut(*a.s.total, gridDim.x);
+    if (static_cast<int>(blockIdx.x) >= cut.count) return;
+    at = cut.begin(blockIdx.x);
+    end = cut.begin(blockIdx.x + 1);
+  }
+  SJ_DEVICE bool next(SharedPiece& p) {
+    if (at >= end) return false;
+    int lo = 0, hi = a.groups;
+    while (hi - lo > 1) {  // the last group that begins at or before the item; those without items begin with the next
+      const int mid = (lo + hi) >> 1;
+      if (a.s.groups[mid].base <= at)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    p.g = a.s.groups[lo];
+    const unsigned long long x = at - p.g.base, head = p.g.head_items();
+    p.h = static_cast<int>(x / head);
+    const unsigned long long y = x % head, pairs = static_cast<unsigned long long>(p.g.tiles / 2) * p.g.keys;
+    p.two = y < pairs;
+    p.tile = p.two ? static_cast<int>(y / p.g.keys) * 2 : p.g.tiles - 1;
+    p.i0 = static_cast<int>(p.two ? y % p.g.keys : y - pairs);
+    const int items = p.two ? p.g.keys : p.g.halves();
+    p.i1 = static_cast<int>(min(static_cast<unsigned long long>(items), p.i0 + (end - at)));
+    at += p.i1 - p.i0;
+    p.steps[0] = p.i1 - p.i0;
+    p.steps[1] = p.two ? p.steps[0] : min(p.g.keys - p.i1, p.i1) - p.i0;
+    return true;
+  }
+};
+
+// 13 warps, one CTA an SM.  Two streams share the tensor cores, so that one's products run under the other's softmax:
+//   warps 0-3, 4-7  softmax of streams 0 and 1: a thread for a query.  S is read from TMEM twice, for the maximum and for
+//                   the exponentials, in pieces of 32 columns; P goes over S in bf16, where the product with V reads
+//                   it.  The output is rescaled only where a maximum has grown by more than 2^8: until then the sums
+//                   are taken by the old one.
+//   warp 8          one thread issues S = Q K^T and O += P V of both streams
+//   warps 9-12      pages of K and V into a ring of tiles (cp.async, since a page may have any number of rows; 128-byte
+//                   rows swizzled as the products read them)
+template <int DIM>
+__global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const SharedArgs a) {
+  using L = SharedLay<DIM>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
+  uint64_t* full = bars;                    // STAGES
+  uint64_t* empty = full + L::STAGES;       // STAGES
+  uint64_t* q_full = empty + L::STAGES;     // 2
+  uint64_t* s_full = q_full + 2;            // 2
+  uint64_t* p_full = s_full + 2;            // 2
+  uint64_t* o_full = p_full + 2;            // 2
+  uint64_t* sums_full = o_full + 2;         // 1
+  uint64_t* drain = sums_full + 1;          // 1
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint32_t* seen = reinterpret_cast<uint32_t*>(smem + L::SEEN);  // [2][kSeen][4]
+  float* sums = reinterpret_cast<float*>(smem + L::SUMS);        // m and l of stream 1
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::STAGES; ++i) {
+      mbar_init(&full[i], kLoadWarps);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 4);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+    }
+    mbar_init(sums_full, 4);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbarrier_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(tmem_slot, kTmemAll);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_wait();
+  const uint32_t tmem = *tmem_slot;
+  SharedWalk walk(a);
+  SharedPiece p;
+
+  if (warp < kSoftmaxWarps) {
+    const int stream = warp >> 2, row = (warp & 3) * 32 + lane, per = kSharedQueries / a.fan;
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t col_s = tmem + lane_off + stream * kSharedKeys, col_o = tmem + lane_off + kColO + stream * DIM;
+    int step_at = 0, piece_at = 0, sums_at = 0;
+    bool ok = true;
+    while (ok && walk.next(p)) {
+      const int steps = p.steps[stream];
+      const int at = (p.tile + (p.two ? stream : 0)) * per + row / a.fan;  // the query's row in its group
+      const int r = p.g.first + at, head = p.h * a.fan + row % a.fan;
+      const bool is = row < per * a.fan && at < p.g.rows;
+      if (stream == 0 || p.two) {  // this stream's queries
+        uint8_t* dst = smem + L::Q + stream * L::SLOT + row * 128;
+        const uint4* src = reinterpret_cast<const uint4*>(a.q + static_cast<size_t>(is ? r : 0) * a.ldq + head * DIM);
+#pragma unroll
+        for (int c = 0; c < DIM / 8; ++c) {
+          const uint4 x = is ? src[c] : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(dst + (c >> 3) * L::HALF + (((c & 7) ^ (row & 7)) << 4)) = x;
+        }
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[stream]);
+      }
+      const bool idle = !__any_sync(0xffffffffu, is);  // a warp without queries leaves S as it is
+      float m = -INFINITY, l = 0.f;
+      for (int step = 0; step < steps; ++step, ++step_at) {
+        if (!mbar_wait(&s_full[stream], step_at & 1, abort_flag, SJ_DEV_ATTN_WAIT)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (idle) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[stream]);
+          continue;
+        }
+        const uint4 valid = *reinterpret_cast<const uint4*>(seen + (stream * kSeen + (step_at & (kSeen - 1))) * 4);
+        const bool all = (valid.x & valid.y & valid.z & valid.w) == 0xffffffffu;
+        auto load = [&](int c, uint32_t (&x)[32]) {
+          tmem_ld_32x32b_x32(col_s + c * 32, x);
+          tmem_wait_ld();
+          if (!all) {
+            const uint32_t word = c == 0 ? valid.x : c == 1 ? valid.y : c == 2 ? valid.z : valid.w;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!(word >> i & 1)) x[i] = 0xff800000u;
+          }
+        };
+        float top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t x[32];
+          load(c, x);
+          float u[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < 32; ++i) u[i & 3] = fmaxf(u[i & 3], __uint_as_float(x[i]));
+          top = fmaxf(top, fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])));
+        }
+        top *= a.scale;
+        const bool grown = step == 0 || !(top <= m + kLazy);
+        if (__any_sync(0xffffffffu, grown && top > m)) {
+          const float next = fmaxf(m, top), f = m == next ? 1.f : shared_exp2(m - next);
+          l *= f;
+          m = next;
+          if (step > 0) {
+#pragma unroll
+            for (int c = 0; c < DIM / 16; ++c) {
+              uint32_t x[16];
+              tmem_ld_32x32b_x16(col_o + c * 16, x);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(f * __uint_as_float(x[i]));
+              tmem_st_32x32b_x16(col_o + c * 16, x);
+            }
+          }
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t x[32], y[16];
+          load(c, x);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float e = shared_exp2(fmaf(__uint_as_float(x[i]), a.scale, -base));
+            part[i & 3] += e;
+            x[i] = __float_as_uint(e);
+          }
+          // rounded to bf16, the product's operand; the sums take it unrounded
+#pragma unroll
+          for (int i = 0; i < 16; ++i) y[i] = pack_bf16x2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+          tmem_st_32x32b_x16(col_s + c * 16, y);
+        }
+        l += (part[0] + part[1]) + (part[2] + part[3]);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[stream]);
+      }
+      if (!ok) break;
+      if (steps > 0) {
+        if (!mbar_wait(&o_full[stream], piece_at & 1, abort_flag, SJ_DEV_ATTN_WAIT)) break;
+        ++piece_at;
+        tc_fence_after();
+      }
+      if (!p.two && stream == 1) {  // stream 0 has the same queries, and joins the two
+        if (steps > 0) {
+          sums[row] = m;
+          sums[kSharedQueries + row] = l;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sums_full);
+        }
+        continue;
+      }
+      const bool joined = !p.two && p.steps[1] > 0;
+      float f = 1.f, g = 0.f;
+      if (joined) {
+        if (!mbar_wait(sums_full, sums_at & 1, abort_flag, SJ_DEV_ATTN_WAIT)) break;
+        ++sums_at;
+        tc_fence_after();
+        const float m2 = sums[row], top = fmaxf(m, m2), base = top == -INFINITY ? 0.f : top;
+        f = shared_exp2(m - base);
+        g = shared_exp2(m2 - base);
+        l = f * l + g * sums[kSharedQueries + row];
+        m = top;
+      }
+      float *to_o, *to_m, *to_l;
+      if (p.i0 == 0) {
+        const size_t query = static_cast<size_t>(is ? r : 0) * a.hq + head;
+        to_m = a.s.m + query;
+        to_l = a.s.l + query;
+        to_o = a.s.o + query * DIM;
+      } else {
+        to_m = shared_slot<DIM>(a.s, blockIdx.x, (p.two ? stream * kSharedQueries : 0) + row);
+        to_l = to_m + 1;
+        to_o = to_m + 4;
+      }
+#pragma unroll
+      for (int c = 0; c < DIM / 16; ++c) {
+        uint32_t x[16], y[16];
+        tmem_ld_32x32b_x16(col_o + c * 16, x);
+        if (joined) tmem_ld_32x32b_x16(col_o + DIM + c * 16, y);
+        tmem_wait_ld();
+        if (joined) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float u = f == 0.f ? 0.f : f * __uint_as_float(x[i]), w = g == 0.f ? 0.f : g * __uint_as_float(y[i]);
+            x[i] = __float_as_uint(u + w);
+          }
+        }
+        if (is) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<uint4*>(to_o + c * 16 + i) = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+        }
+      }
+      if (is) {
+        *to_m = m;
+        *to_l = l;
+      }
+      tc_fence_before();
+    }
+  } else if (warp == kMmaWarp) {
+    if (lane == 0) {
+      constexpr uint32_t kIdescS = umma_idesc_bf16(kSharedQueries, kSharedKeys, 0, 0);
+      constexpr uint32_t kIdescO = umma_idesc_bf16(kSharedQueries, DIM, 0, 1);
+      int tile_at = 0, q_at[2] = {0, 0}, p_at[2] = {0, 0};
+      bool ok = true;
+      auto slot_of = [&](int n) { return n % L::STAGES; };
+      auto wait_tile = [&](int n) {
+        ok = ok && mbar_wait(&full[slot_of(n)], (n / L::STAGES) & 1, abort_flag, SJ_DEV_ATTN_WAIT);
+        tc_fence_after();
+      };
+      auto scores = [&](int stream, int queries, int n) {  // S = Q K^T
+        if (!ok) return;
+        const uint32_t q_addr = smem_u32(smem + L::Q + queries * L::SLOT);
+        const uint32_t k_addr = smem_u32(smem + L::RING + slot_of(n) * L::SLOT);
+#pragma unroll
+        for (int kk = 0; kk < DIM / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * L::HALF + (kk & 3) * 32;
+          umma_f16(tmem + stream * kSharedKeys, umma_desc(q_addr + off, 16, 1024), umma_desc(k_addr + off, 16, 1024),
+                   kIdescS, kk > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[stream]);
+      };
+      auto wait_p = [&](int stream) {
+        ok = ok && mbar_wait(&p_full[stream], p_at[stream] & 1, abort_flag, SJ_DEV_ATTN_WAIT);
+        ++p_at[stream];
+        tc_fence_after();
+      };
+      auto outputs = [&](int stream, int n, bool first) {  // O += P V
+        if (!ok) return;
+        const uint32_t v_addr = smem_u32(smem + L::RING + slot_of(n) * L::SLOT);
+#pragma unroll
+        for (int kk = 0; kk < kSharedKeys / 16; ++kk)
+          umma_f16_ts(tmem + kColO + stream * DIM, tmem + stream * kSharedKeys + kk * 8,
+                      umma_desc(v_addr + kk * 2048, L::HALF, 1024), kIdescO, !first || kk > 0 ? 1u : 0u);
+      };
+      auto release = [&](int n) {
+        if (ok) umma_commit(&empty[slot_of(n)]);
+      };
+      auto finished = [&](int stream) {
+        if (ok) umma_commit(&o_full[stream]);
+      };
+      auto wait_q = [&](int stream) {
+        ok = ok && mbar_wait(&q_full[stream], q_at[stream] & 1, abort_flag, SJ_DEV_ATTN_WAIT);
+        ++q_at[stream];
+        tc_fence_after();
+      };
+      while (ok && walk.next(p)) {
+        const int n0 = p.steps[0], n1 = p.steps[1];
+        wait_q(0);
+        wait_tile(tile_at);
+        scores(0, 0, tile_at);
+        if (p.two) {
+          wait_q(1);
+          scores(1, 1, tile_at);
+          release(tile_at++);
+          for (int i = 0; i < n0 && ok; ++i) {
+            const int v = tile_at, k = tile_at + 1;
+            const bool more = i + 1 < n0;
+            wait_p(0);
+            wait_tile(v);
+            outputs(0, v, i == 0);
+            if (more) {
+              wait_tile(k);
+              scores(0, 0, k);
+            } else {
+              finished(0);
+            }
+            wait_p(1);
+            outputs(1, v, i == 0);
+            release(v);
+            if (more) {
+              scores(1, 1, k);
+              release(k);
+            } else {
+              finished(1);
+            }
+            tile_at += more ? 2 : 1;
+          }
+        } else {
+          release(tile_at++);
+          if (n1 > 0) {
+            wait_tile(tile_at);
+            scores(1, 0, tile_at);
+            release(tile_at++);
+          }
+          for (int i = 0; i < n0 && ok; ++i) {
+#pragma unroll
+            for (int stream = 0; stream < 2; ++stream) {
+              const int steps = stream == 0 ? n0 : n1;
+              if (i >= steps) continue;
+              wait_p(stream);
+              wait_tile(tile_at);
+              outputs(stream, tile_at, i == 0);
+              release(tile_at++);
+              if (i + 1 < steps) {
+                wait_tile(tile_at);
+                scores(stream, 0, tile_at);
+                release(tile_at++);
+              } else {
+                finished(stream);
+              }
+            }
+          }
+        }
+      }
+      umma_commit(drain);
+      mbar_wait(drain, 0, nullptr, SJ_DEV_ATTN_WAIT);
+    }
+  } else {
+    const int w = warp - kMmaWarp - 1;
+    int issued = 0, passed = 0, seen_at[2] = {0, 0};  // tiles on their way, tiles handed over
+    bool ok = true;
+    auto hand_over = [&]() {  // this thread's copies of the oldest tile are in
+      fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[passed % L::STAGES]);
+      ++passed;
+    };
+    auto look_up = [&](int key) {
+      key += w * 32 + lane;
+      return key < p.g.p1 ? a.table[static_cast<size_t>(p.g.request) * a.ld_table + key / a.page] : -1;
+    };
+    // where this lane's key lies, in 16-byte pieces
+    auto resolve = [&](int key, int found) {
+      key += w * 32 + lane;
+      if (key >= p.g.p1) return kNowhere;
+      if (found < 0 || found >= a.pages) {
+        record_error(SJ_DEV_BAD_INDEX);
+        return kNowhere;
+      }
+      return static_cast<uint32_t>((found * a.page_stride + p.h * a.head_stride + key % a.page * a.token_stride) >> 3);
+    };
+    auto mark = [&](int stream, uint32_t where) {
+      const uint32_t have = __ballot_sync(0xffffffffu, where != kNowhere);
+      if (lane == 0) seen[(stream * kSeen + (seen_at[stream] & (kSeen - 1))) * 4 + w] = have;
+      ++seen_at[stream];
+    };
+    auto fetch = [&](const __nv_bfloat16* from, uint32_t where) {
+      const int slot = issued % L::STAGES;
+      const uint32_t parity = ((issued / L::STAGES) & 1) ^ 1;
+      if (!__all_sync(0xffffffffu, mbar_test_wait(&empty[slot], parity))) {
+        // what is on its way is handed over before this warp waits, for what it waits for may need it
+        shared_copies_wait<0>();
+        while (passed < issued) hand_over();
+        if (!mbar_wait(&empty[slot], parity, abort_flag, SJ_DEV_ATTN_WAIT)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
+      }
+      __syncwarp();
+      constexpr int LANES = DIM / 8, ROWS = 32 / LANES;  // of a row, in one instruction
+      const uint32_t dst = smem_u32(smem + L::RING + slot * L::SLOT) + ((lane % LANES) >> 3) * L::HALF;
+#pragma unroll
+      for (int i = 0; i < 32 / ROWS; ++i) {
+        const int key = i * ROWS + lane / LANES;
+        const uint32_t at = __shfl_sync(0xffffffffu, where, key);
+        shared_copy16(dst + (w * 32 + key) * 128 + (((lane & 7) ^ (key & 7)) << 4),
+                      from + (at == kNowhere ? 0 : static_cast<size_t>(at) * 8 + (lane % LANES) * 8), at != kNowhere);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      ++issued;
+      if (issued - passed >= L::AHEAD) {
+        shared_copies_wait<L::AHEAD - 1>();
+        hand_over();
+      }
+    };
+    while (ok && walk.next(p)) {
+      const int n0 = p.steps[0], n1 = p.two ? 0 : p.steps[1];
+      uint32_t now[2] = {kNowhere, kNowhere};
+      int found[2];
+      found[0] = look_up(p.key(0, 0));
+      found[1] = n1 > 0 ? look_up(p.key(1, 0)) : -1;
+      auto keys = [&](int stream, int step, int steps) {  // a tile of K; the next one's pages are looked up
+        now[stream] = resolve(p.key(stream, step), found[stream]);
+        if (step + 1 < steps) found[stream] = look_up(p.key(stream, step + 1));
+        mark(stream, now[stream]);
+        if (p.two) mark(1, now[stream]);
+        fetch(a.k, now[stream]);
+      };
+      keys(0, 0, n0);
+      if (ok && n1 > 0) keys(1, 0, n1);
+      for (int i = 0; i < n0 && ok; ++i) {
+        fetch(a.v, now[0]);
+        if (ok && i + 1 < n0) keys(0, i + 1, n0);
+        if (ok && i < n1) fetch(a.v, now[1]);
+        if (ok && i + 1 < n1) keys(1, i + 1, n1);
+      }
+    }
+    shared_copies_wait<0>();
+    while (passed < issued) hand_over();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemAll);
+  }
+}
+
+namespace {
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+// Where the parts of the workspace lie, from its own start.
+size_t shared_layout(SharedSpans* s, char* at, int rows, int groups, int hq, int head_dim) {
+  size_t n = 0;
+  auto take = [&](size_t bytes) {
+    const size_t was = n;
+    n += up256(bytes);
+    return at + was;
+  };
+  char* total = take(sizeof(unsigned long long));
+  char* group = take(sizeof(SharedGroup) * groups);
+  char* row = take(sizeof(SharedRow) * rows);
+  const size_t queries = static_cast<size_t>(rows) * hq;
+  char* m = take(queries * sizeof(float));
+  char* l = take(queries * sizeof(float));
+  char* o = take(queries * head_dim * sizeof(float));
+  char* slots = take(static_cast<size_t>(sm_count()) * 2 * kSharedQueries * (head_dim + 4) * sizeof(float));
+  if (s)
+    *s = SharedSpans{reinterpret_cast<unsigned long long*>(total), reinterpret_cast<SharedGroup*>(group),
+                     reinterpret_cast<SharedRow*>(row), reinterpret_cast<float*>(m), reinterpret_cast<float*>(l),
+                     reinterpret_cast<float*>(o), sm_count(), reinterpret_cast<float*>(slots)};
+  return n;
+}
+
+template <int DIM>
+int shared_pass(const SharedArgs& a, cudaStream_t stream) {
+  static KernelAttrOnce once;
+  const int rc = ensure_max_smem(once, reinterpret_cast<const void*>(attn_shared_kernel<DIM>), SharedLay<DIM>::SMEM,
+                                 "sj_attn_paged_shared: shared memory");
+  if (rc != SJ_OK) return rc;
+  launch(attn_shared_kernel<DIM>, a.s.ctas, kSharedThreads, SharedLay<DIM>::SMEM, stream, a);
+  SJ_LAUNCH_CHECK("attn_shared");
+  return SJ_OK;
+}
+}  // namespace
+}  // namespace sj
+
+using namespace sj;
+
+namespace {
+// Groups that the tensor-core pass takes: tiles hold whole rows, and one CTA knows all groups.
+bool shares(int groups, int hq, int hk) { return groups > 0 && groups <= kSharedGroups && hq / hk <= kSharedQueries; }
+}  // namespace
+
+extern "C" size_t sj_attn_paged_shared_workspace(int rows, int groups, int hq, int hk, int head_dim) {
+  const size_t own = sj_attn_paged_workspace(rows, hq, hk, head_dim);
+  if (own == 0 || groups < 0) return 0;
+  return up256(own) + shared_layout(nullptr, nullptr, rows, std::min(groups, kSharedGroups), hq, head_dim);
+}
+
+extern "C" int sj_attn_paged_shared(const void* q, int ldq, const void* k_cache, const void* v_cache, int pages,
+                                    int page, int64_t page_stride, int64_t head_stride, int64_t token_stride,
+                                    const int32_t* block_table, int ld_table, int requests, const int32_t* request,
+                                    const int32_t* position, int rows, const int32_t* group, int groups, int hq,
+                                    int hk, int head_dim, int window, void* o, int ldo, float* lse, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  constexpr const char* who = "sj_attn_paged_shared";
+  if (groups < 0 || (rows > 0 && groups > rows)) return fail(SJ_ERR_SHAPE, "%s: groups=%d rows=%d", who, groups, rows);
+  PagedAttention a;
+  int rc = paged_attention_args(who, a, q, ldq, k_cache, v_cache, pages, page, page_stride, head_stride, token_stride,
+                                block_table, ld_table, requests, request, position, rows, hq, hk, head_dim, window, o,
+                                ldo, lse, workspace, workspace_bytes,
+                                sj_attn_paged_shared_workspace(rows, groups, hq, hk, head_dim));
+  if (rc != SJ_OK || rows == 0) return rc;
+  if (groups > 0 && !group) return fail(SJ_ERR_ARGUMENT, "%s: null operand", who);
+  cudaStream_t s = as_stream(stream);
+  if (!shares(groups, hq, hk)) return attn_paged_rows(a, nullptr, head_dim, s);
+  SharedSpans spans;
+  shared_layout(&spans, static_cast<char*>(workspace) + up256(sj_attn_paged_workspace(rows, hq, hk, head_dim)), rows,
+                groups, hq, head_dim);
+  const SpansArgs sa{request, position, group, rows, groups, requests, page, ld_table, window, hq / hk, hk, 2, spans};
+  launch(shared_spans_kernel, 1, 1024, 0, s, sa);
+  SJ_LAUNCH_CHECK("shared_spans");
+  const SharedArgs ta{a.q, a.k, a.v, block_table, page_stride, head_stride, token_stride, ldq, pages, page, ld_table,
+                      groups, hq, hk, hq / hk, 1.4426950408889634f / sqrtf(static_cast<float>(head_dim)), spans};
+  rc = head_dim == 64 ? shared_pass<64>(ta, s) : shared_pass<128>(ta, s);
+  if (rc != SJ_OK) return rc;
+  return attn_paged_rows(a, &spans, head_dim, s);
+}

@@ -19,11 +19,11 @@ namespace sj {
 
 namespace {
 constexpr int kSharedGroups = 1024;
-constexpr int kSoftmaxWarps = 8, kMmaWarp = 8, kLoadWarps = 4;
-constexpr int kSharedThreads = 32 * (kSoftmaxWarps + 1 + kLoadWarps);
-constexpr int kSeen = 8;                   // tiles whose masks of valid keys are kept
+constexpr int kSoftmaxWarps = 8, kMmaWarp = 8, kFenceWarp = 9, kLoadWarp = 10, kLoadWarps = 2;
+constexpr int kSharedThreads = 32 * (kLoadWarp + kLoadWarps);
+constexpr int kSeen = 16;                  // tiles whose masks of valid keys are kept
 constexpr float kLazy = 8.f;               // a maximum may stand this far (of log2) below the true one
-constexpr uint32_t kColO = 256;            // TMEM columns: S of two streams (their P over it), then O
+constexpr uint32_t kColO = 256;            // TMEM columns: two S of each of two streams (their P over them), then O
 constexpr uint32_t kTmemAll = 512;
 constexpr uint32_t kNowhere = 0xffffffffu;
 constexpr int kLastSeen = INT_MAX - 4096;
@@ -139,12 +139,33 @@ SJ_DEVICE float shared_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+SJ_DEVICE float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// Two f32 at a time: sm_100 adds and fuses a register pair in one instruction.
+SJ_DEVICE uint64_t pair2(float a, float b) {
+  return static_cast<uint64_t>(__float_as_uint(b)) << 32 | __float_as_uint(a);
+}
+SJ_DEVICE float low2(uint64_t p) { return __uint_as_float(static_cast<uint32_t>(p)); }
+SJ_DEVICE float high2(uint64_t p) { return __uint_as_float(static_cast<uint32_t>(p >> 32)); }
+SJ_DEVICE uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t y;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+  return y;
+}
+SJ_DEVICE uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t y;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
+  return y;
+}
+// 16 bytes from global to shared memory; zeros when !is.
+SJ_DEVICE void shared_copy16(uint32_t dst, const __nv_bfloat16* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 SJ_DEVICE void shared_copy16(uint32_t dst, const __nv_bfloat16* src, bool is) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(is ? 16 : 0) : "memory");
-}
-template <int LEFT>
-SJ_DEVICE void shared_copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
 }
 // 32 lanes x 16 consecutive 32-bit columns, from thread i to lane (base + i).
 SJ_DEVICE void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -155,24 +176,51 @@ SJ_DEVICE void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
       : "memory");
 }
 SJ_DEVICE void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// D[tmem] (+)= A[tmem] * B[smem desc]: A holds two bf16 of a row in each 32-bit column.
-SJ_DEVICE void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+// One lane of a warp.
+SJ_DEVICE uint32_t elect_one() {
+  uint32_t is;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(is));
+  return is;
+}
+// The instructions of the thread that issues products, as a whole warp executes them, by the lane that `is`: the
+// operands are then uniform, where a branch of one lane would move each of them to uniform registers before every product
+// (80 to 95 cycles a product).
+//   D[tmem] (+)= A B: A from shared memory, or from TMEM with two bf16 of a row in each 32-bit column; B from shared memory
+SJ_DEVICE void product_ss(uint32_t is, uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(add), "r"(is)
+      : "memory");
+}
+SJ_DEVICE void product_ts(uint32_t is, uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t add) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(add), "r"(is)
+      : "memory");
+}
+SJ_DEVICE void commit_products(uint32_t is, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(is)
       : "memory");
 }
 
 template <int DIM>
 struct SharedLay {
-  static constexpr int SLOT = kSharedKeys * DIM * 2;  // a tile of K, of V, or of queries
+  static constexpr int SLOT = kSharedKeys * DIM * 2;  // a tile of K or of V
   static constexpr int HALF = kSharedKeys * 128;      // 64 dims of it: rows of 128 bytes
-  static constexpr int STAGES = DIM == 64 ? 9 : 4;    // of the ring of K and V tiles
-  static constexpr int AHEAD = DIM == 64 ? 5 : 3;     // tiles of a load warp in flight
-  static constexpr int Q = 0, RING = 2 * SLOT, SEEN = RING + STAGES * SLOT, SUMS = SEEN + 2 * kSeen * 16,
-                       BARS = SUMS + 2 * kSharedQueries * 4, SMEM = BARS + 512 + 1024;
+  static constexpr int QUERIES = kSharedQueries * DIM * 2, QUERIES_HALF = kSharedQueries * 128;
+  static constexpr int STAGES = DIM == 64 ? 18 : 10;   // of the ring of K and V tiles
+  static constexpr int Q = 0, RING = 2 * QUERIES, SEEN = RING + STAGES * SLOT, SUMS = SEEN + 2 * kSeen * 8,
+                       BARS = SUMS + 2 * kSharedQueries * 4, SMEM = BARS + 768 + 1024;
 };
 
 // A CTA's share of a unit: items [i0, i1) of one KV head and one or two tiles of queries.
@@ -180,7 +228,7 @@ struct SharedPiece {
   SharedGroup g;
   int h, tile, i0, i1;
   bool two;  // two tiles of queries over the same keys; else one, over alternate tiles of keys
-  int steps[2];
+  int steps0, steps1;  // of the streams
   SJ_DEVICE int key(int stream, int step) const {
     return g.p0 + (two ? i0 + step : 2 * (i0 + step) + stream) * kSharedKeys;
   }
@@ -214,50 +262,54 @@ struct SharedWalk {
     const int items = p.two ? p.g.keys : p.g.halves();
     p.i1 = static_cast<int>(min(static_cast<unsigned long long>(items), p.i0 + (end - at)));
     at += p.i1 - p.i0;
-    p.steps[0] = p.i1 - p.i0;
-    p.steps[1] = p.two ? p.steps[0] : min(p.g.keys - p.i1, p.i1) - p.i0;
+    p.steps0 = p.i1 - p.i0;
+    p.steps1 = p.two ? p.steps0 : min(p.g.keys - p.i1, p.i1) - p.i0;
     return true;
   }
 };
 
-// 13 warps, one CTA an SM.  Two streams share the tensor cores, so that one's products run under the other's softmax:
-//   warps 0-3, 4-7  softmax of streams 0 and 1: a thread for a query.  S is read from TMEM twice, for the maximum and for
-//                   the exponentials, in pieces of 32 columns; P goes over S in bf16, where the product with V reads
-//                   it.  The output is rescaled only where a maximum has grown by more than 2^8: until then the sums
-//                   are taken by the old one.
+// 12 warps, one CTA an SM.  Two streams of tiles, each with two S in TMEM, so that a tile's scores are there when the
+// softmax of the one before ends, and the products of one stream run under the other's softmax:
+//   warps 0-3, 4-7  softmax of streams 0 and 1: a thread for a query, which has its 64 scores in registers.  P goes over
+//                   S in bf16, where the product with V reads it.  The output is rescaled only where a maximum has
+//                   grown by more than 2^8: until then the sums are taken by the old one.
 //   warp 8          one thread issues S = Q K^T and O += P V of both streams
-//   warps 9-12      pages of K and V into a ring of tiles (cp.async, since a page may have any number of rows; 128-byte
-//                   rows swizzled as the products read them)
+//   warp 9          one thread hands tiles that have come over to the asynchronous proxy, since a fence takes the thread
+//                   that issues the products 250 cycles
+//   warps 10-11     pages of K and V into a ring of tiles (cp.async, since a page may have any number of rows; 128-byte
+//                   rows swizzled as the products read them), which arrive by themselves
 template <int DIM>
 __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const SharedArgs a) {
   using L = SharedLay<DIM>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
-  uint64_t* full = bars;                    // STAGES
-  uint64_t* empty = full + L::STAGES;       // STAGES
+  uint64_t* full = bars;                    // STAGES: copies are in
+  uint64_t* ready = full + L::STAGES;       // STAGES: and seen by the products
+  uint64_t* empty = ready + L::STAGES;      // STAGES
   uint64_t* q_full = empty + L::STAGES;     // 2
-  uint64_t* s_full = q_full + 2;            // 2
-  uint64_t* p_full = s_full + 2;            // 2
-  uint64_t* o_full = p_full + 2;            // 2
-  uint64_t* sums_full = o_full + 2;         // 1
+  uint64_t* s_full = q_full + 2;            // 2 of each stream
+  uint64_t* p_full = s_full + 4;            // 2 of each stream
+  uint64_t* o_done = p_full + 4;            // 2 of each stream, in turn: a tile's product with V
+  uint64_t* sums_full = o_done + 4;         // 1
   uint64_t* drain = sums_full + 1;          // 1
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  uint32_t* seen = reinterpret_cast<uint32_t*>(smem + L::SEEN);  // [2][kSeen][4]
+  uint32_t* seen = reinterpret_cast<uint32_t*>(smem + L::SEEN);  // [2][kSeen][2]
   float* sums = reinterpret_cast<float*>(smem + L::SUMS);        // m and l of stream 1
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::STAGES; ++i) {
-      mbar_init(&full[i], kLoadWarps);
+      mbar_init(&full[i], kLoadWarps * 32);
+      mbar_init(&ready[i], 1);
       mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 4);
+    for (int i = 0; i < 2; ++i) mbar_init(&q_full[i], 4);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&o_done[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
-      mbar_init(&o_full[i], 1);
     }
     mbar_init(sums_full, 4);
     mbar_init(drain, 1);
@@ -272,28 +324,32 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
   __syncthreads();
   tc_fence_after();
   pdl_wait();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   SharedWalk walk(a);
   SharedPiece p;
 
   if (warp < kSoftmaxWarps) {
     const int stream = warp >> 2, row = (warp & 3) * 32 + lane, per = kSharedQueries / a.fan;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t col_s = tmem + lane_off + stream * kSharedKeys, col_o = tmem + lane_off + kColO + stream * DIM;
-    int step_at = 0, piece_at = 0, sums_at = 0;
+    const uint32_t col_s2 = tmem + lane_off + stream * 2 * kSharedKeys, col_o = tmem + lane_off + kColO + stream * DIM;
+    int step_at = 0, sums_at = 0;
+    // the product of the stream's n-th tile; that of the one two before is known to be done
+    auto wait_output = [&](int n) {
+      return mbar_wait(&o_done[stream * 2 + (n & 1)], (n >> 1) & 1, abort_flag, SJ_DEV_ATTN_WAIT);
+    };
     bool ok = true;
     while (ok && walk.next(p)) {
-      const int steps = p.steps[stream];
+      const int steps = stream == 0 ? p.steps0 : p.steps1;
       const int at = (p.tile + (p.two ? stream : 0)) * per + row / a.fan;  // the query's row in its group
       const int r = p.g.first + at, head = p.h * a.fan + row % a.fan;
       const bool is = row < per * a.fan && at < p.g.rows;
       if (stream == 0 || p.two) {  // this stream's queries
-        uint8_t* dst = smem + L::Q + stream * L::SLOT + row * 128;
+        uint8_t* dst = smem + L::Q + stream * L::QUERIES + row * 128;
         const uint4* src = reinterpret_cast<const uint4*>(a.q + static_cast<size_t>(is ? r : 0) * a.ldq + head * DIM);
 #pragma unroll
         for (int c = 0; c < DIM / 8; ++c) {
           const uint4 x = is ? src[c] : make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(dst + (c >> 3) * L::HALF + (((c & 7) ^ (row & 7)) << 4)) = x;
+          *reinterpret_cast<uint4*>(dst + (c >> 3) * L::QUERIES_HALF + (((c & 7) ^ (row & 7)) << 4)) = x;
         }
         fence_proxy_async_shared();
         __syncwarp();
@@ -302,7 +358,9 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
       const bool idle = !__any_sync(0xffffffffu, is);  // a warp without queries leaves S as it is
       float m = -INFINITY, l = 0.f;
       for (int step = 0; step < steps; ++step, ++step_at) {
-        if (!mbar_wait(&s_full[stream], step_at & 1, abort_flag, SJ_DEV_ATTN_WAIT)) {
+        const int buffer = step_at & 1;
+        const uint32_t col_s = col_s2 + buffer * kSharedKeys;
+        if (!mbar_wait(&s_full[stream * 2 + buffer], (step_at >> 1) & 1, abort_flag, SJ_DEV_ATTN_WAIT)) {
           ok = false;
           break;
         }
@@ -310,76 +368,74 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
         if (idle) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[stream]);
+          if (lane == 0) mbar_arrive(&p_full[stream * 2 + buffer]);
           continue;
         }
-        const uint4 valid = *reinterpret_cast<const uint4*>(seen + (stream * kSeen + (step_at & (kSeen - 1))) * 4);
-        const bool all = (valid.x & valid.y & valid.z & valid.w) == 0xffffffffu;
-        auto load = [&](int c, uint32_t (&x)[32]) {
-          tmem_ld_32x32b_x32(col_s + c * 32, x);
-          tmem_wait_ld();
-          if (!all) {
-            const uint32_t word = c == 0 ? valid.x : c == 1 ? valid.y : c == 2 ? valid.z : valid.w;
+        uint32_t x[kSharedKeys];
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!(word >> i & 1)) x[i] = 0xff800000u;
-          }
-        };
-        float top = -INFINITY;
+        for (int c = 0; c < kSharedKeys / 32; ++c)
+          tmem_ld_32x32b_x32(col_s + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&x[c * 32]));
+        const uint2 valid = *reinterpret_cast<const uint2*>(seen + (stream * kSeen + (step_at & (kSeen - 1))) * 2);
+        tmem_wait_ld();
+        if ((valid.x & valid.y) != 0xffffffffu) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t x[32];
-          load(c, x);
-          float u[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int i = 0; i < 32; ++i) u[i & 3] = fmaxf(u[i & 3], __uint_as_float(x[i]));
-          top = fmaxf(top, fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])));
+          for (int i = 0; i < kSharedKeys; ++i)
+            if (!((i < 32 ? valid.x : valid.y) >> (i & 31) & 1)) x[i] = 0xff800000u;
         }
-        top *= a.scale;
+        float u[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < kSharedKeys; i += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            u[e] = max3(u[e], __uint_as_float(x[i + 2 * e]), __uint_as_float(x[i + 2 * e + 1]));
+        const float top = fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])) * a.scale;
         const bool grown = step == 0 || !(top <= m + kLazy);
         if (__any_sync(0xffffffffu, grown && top > m)) {
           const float next = fmaxf(m, top), f = m == next ? 1.f : shared_exp2(m - next);
           l *= f;
           m = next;
-          if (step > 0) {
+          if (step > 0) {  // the product of the tile before has to be in the output
+            if (!wait_output(step_at - 1)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
 #pragma unroll
             for (int c = 0; c < DIM / 16; ++c) {
-              uint32_t x[16];
-              tmem_ld_32x32b_x16(col_o + c * 16, x);
+              uint32_t y[16];
+              tmem_ld_32x32b_x16(col_o + c * 16, y);
               tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(f * __uint_as_float(x[i]));
-              tmem_st_32x32b_x16(col_o + c * 16, x);
+              for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(f * __uint_as_float(y[i]));
+              tmem_st_32x32b_x16(col_o + c * 16, y);
             }
           }
         }
         const float base = m == -INFINITY ? 0.f : m;
-        float part[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t scale2 = pair2(a.scale, a.scale), base2 = pair2(-base, -base);
+        uint64_t part[2] = {0, 0};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t x[32], y[16];
-          load(c, x);
+        for (int c = 0; c < kSharedKeys / 32; ++c) {
+          uint32_t y[16];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float e = shared_exp2(fmaf(__uint_as_float(x[i]), a.scale, -base));
-            part[i & 3] += e;
-            x[i] = __float_as_uint(e);
+          for (int i = 0; i < 16; ++i) {
+            const int at = c * 32 + 2 * i;
+            const uint64_t d = fma2(pair2(__uint_as_float(x[at]), __uint_as_float(x[at + 1])), scale2, base2);
+            const float e0 = shared_exp2(low2(d)), e1 = shared_exp2(high2(d));
+            part[i & 1] = add2(part[i & 1], pair2(e0, e1));
+            y[i] = pack_bf16x2(e0, e1);  // the product's operand; the sums take it unrounded
           }
-          // rounded to bf16, the product's operand; the sums take it unrounded
-#pragma unroll
-          for (int i = 0; i < 16; ++i) y[i] = pack_bf16x2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
           tmem_st_32x32b_x16(col_s + c * 16, y);
         }
-        l += (part[0] + part[1]) + (part[2] + part[3]);
+        l += (low2(part[0]) + high2(part[0])) + (low2(part[1]) + high2(part[1]));
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[stream]);
+        if (lane == 0) mbar_arrive(&p_full[stream * 2 + buffer]);
       }
       if (!ok) break;
       if (steps > 0) {
-        if (!mbar_wait(&o_full[stream], piece_at & 1, abort_flag, SJ_DEV_ATTN_WAIT)) break;
-        ++piece_at;
+        if (!wait_output(step_at - 1)) break;
         tc_fence_after();
       }
       if (!p.two && stream == 1) {  // stream 0 has the same queries, and joins the two
@@ -391,7 +447,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
         }
         continue;
       }
-      const bool joined = !p.two && p.steps[1] > 0;
+      const bool joined = !p.two && p.steps1 > 0;
       float f = 1.f, g = 0.f;
       if (joined) {
         if (!mbar_wait(sums_full, sums_at & 1, abort_flag, SJ_DEV_ATTN_WAIT)) break;
@@ -440,195 +496,239 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
       tc_fence_before();
     }
   } else if (warp == kMmaWarp) {
-    if (lane == 0) {
+    {
+      const uint32_t is = elect_one();
       constexpr uint32_t kIdescS = umma_idesc_bf16(kSharedQueries, kSharedKeys, 0, 0);
       constexpr uint32_t kIdescO = umma_idesc_bf16(kSharedQueries, DIM, 0, 1);
-      int tile_at = 0, q_at[2] = {0, 0}, p_at[2] = {0, 0};
-      bool ok = true;
-      auto slot_of = [&](int n) { return n % L::STAGES; };
-      auto wait_tile = [&](int n) {
-        ok = ok && mbar_wait(&full[slot_of(n)], (n / L::STAGES) & 1, abort_flag, SJ_DEV_ATTN_WAIT);
+      // descriptors differ in their addresses only, which are in the low words
+      auto desc = [](uint32_t low, uint32_t off) {
+        constexpr uint32_t high = (1024 >> 4) | 1u << 14 | 2u << 29;
+        return static_cast<uint64_t>(high) << 32 | (low + (off >> 4));
+      };
+      auto low = [](const uint8_t* at, uint32_t lead) { return ((smem_u32(at) >> 4) & 0x3fffu) | (lead >> 4) << 16; };
+      const uint32_t q_low = low(smem + L::Q, 16), k_low = low(smem + L::RING, 16), v_low = low(smem + L::RING, L::HALF);
+      int slot = 0, turn = 0, q_at[2] = {0, 0}, s_at[2] = {0, 0}, p_at[2] = {0, 0};
+      // After a wait that gave up the piece's products are of no use, but harmless, and its other waits give up at once.
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        mbar_wait(bar, parity, abort_flag, SJ_DEV_ATTN_WAIT);
         tc_fence_after();
       };
-      auto scores = [&](int stream, int queries, int n) {  // S = Q K^T
-        if (!ok) return;
-        const uint32_t q_addr = smem_u32(smem + L::Q + queries * L::SLOT);
-        const uint32_t k_addr = smem_u32(smem + L::RING + slot_of(n) * L::SLOT);
-#pragma unroll
-        for (int kk = 0; kk < DIM / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * L::HALF + (kk & 3) * 32;
-          umma_f16(tmem + stream * kSharedKeys, umma_desc(q_addr + off, 16, 1024), umma_desc(k_addr + off, 16, 1024),
-                   kIdescS, kk > 0 ? 1u : 0u);
+      auto wait_tile = [&]() { wait(&ready[slot], turn); };
+      auto release = [&]() {  // the tile at hand is done with when the products so far are
+        commit_products(is, &empty[slot]);
+        if (++slot == L::STAGES) {
+          slot = 0;
+          turn ^= 1;
         }
-        umma_commit(&s_full[stream]);
       };
-      auto wait_p = [&](int stream) {
-        ok = ok && mbar_wait(&p_full[stream], p_at[stream] & 1, abort_flag, SJ_DEV_ATTN_WAIT);
-        ++p_at[stream];
-        tc_fence_after();
+      auto scores = [&](int stream, int queries) {  // S = Q K^T
+        const uint32_t q = q_low + queries * (L::QUERIES >> 4), k = k_low + slot * (L::SLOT >> 4);
+        const uint32_t to = tmem + (stream * 2 + (s_at[stream] & 1)) * kSharedKeys;
+#pragma unroll
+        for (int kk = 0; kk < DIM / 16; ++kk)
+          product_ss(is, to, desc(q, (kk >> 2) * L::QUERIES_HALF + (kk & 3) * 32), desc(k, (kk >> 2) * L::HALF + (kk & 3) * 32),
+                   kIdescS, kk > 0 ? 1u : 0u);
+        commit_products(is, &s_full[stream * 2 + (s_at[stream] & 1)]);
+        ++s_at[stream];
       };
-      auto outputs = [&](int stream, int n, bool first) {  // O += P V
-        if (!ok) return;
-        const uint32_t v_addr = smem_u32(smem + L::RING + slot_of(n) * L::SLOT);
+      auto wait_p = [&](int stream) { wait(&p_full[stream * 2 + (p_at[stream] & 1)], (p_at[stream] >> 1) & 1); };
+      auto outputs = [&](int stream, bool first) {  // O += P V
+        const uint32_t v = v_low + slot * (L::SLOT >> 4);
+        const uint32_t from = tmem + (stream * 2 + (p_at[stream] & 1)) * kSharedKeys;
 #pragma unroll
         for (int kk = 0; kk < kSharedKeys / 16; ++kk)
-          umma_f16_ts(tmem + kColO + stream * DIM, tmem + stream * kSharedKeys + kk * 8,
-                      umma_desc(v_addr + kk * 2048, L::HALF, 1024), kIdescO, !first || kk > 0 ? 1u : 0u);
-      };
-      auto release = [&](int n) {
-        if (ok) umma_commit(&empty[slot_of(n)]);
-      };
-      auto finished = [&](int stream) {
-        if (ok) umma_commit(&o_full[stream]);
+          product_ts(is, tmem + kColO + stream * DIM, from + kk * 8, desc(v, kk * 2048), kIdescO, !first || kk > 0 ? 1u : 0u);
+        commit_products(is, &o_done[stream * 2 + (p_at[stream] & 1)]);
+        ++p_at[stream];
       };
       auto wait_q = [&](int stream) {
-        ok = ok && mbar_wait(&q_full[stream], q_at[stream] & 1, abort_flag, SJ_DEV_ATTN_WAIT);
+        wait(&q_full[stream], q_at[stream] & 1);
         ++q_at[stream];
-        tc_fence_after();
       };
-      while (ok && walk.next(p)) {
-        const int n0 = p.steps[0], n1 = p.steps[1];
+      while (__shfl_sync(0xffffffffu, *abort_flag == 0 && walk.next(p) ? 1 : 0, 0)) {
+        const int n0 = __shfl_sync(0xffffffffu, p.steps0, 0), n1 = __shfl_sync(0xffffffffu, p.steps1, 0);
         wait_q(0);
-        wait_tile(tile_at);
-        scores(0, 0, tile_at);
-        if (p.two) {
+        if (__shfl_sync(0xffffffffu, p.two ? 1 : 0, 0)) {
           wait_q(1);
-          scores(1, 1, tile_at);
-          release(tile_at++);
-          for (int i = 0; i < n0 && ok; ++i) {
-            const int v = tile_at, k = tile_at + 1;
-            const bool more = i + 1 < n0;
+          for (int i = 0; i < min(2, n0); ++i) {
+            wait_tile();
+            scores(0, 0);
+            scores(1, 1);
+            release();
+          }
+          for (int i = 0; i < n0; ++i) {
+            // V of this tile, K of the one after the next, for both streams
+            const bool more = i + 2 < n0;
+            const int v_slot = slot, v_turn = turn, next = slot + 1 == L::STAGES ? 0 : slot + 1;
+            auto at_key = [&]() {
+              slot = next;
+              turn = next == 0 ? v_turn ^ 1 : v_turn;
+            };
+            auto at_value = [&]() {
+              slot = v_slot;
+              turn = v_turn;
+            };
             wait_p(0);
-            wait_tile(v);
-            outputs(0, v, i == 0);
+            wait_tile();
+            outputs(0, i == 0);
             if (more) {
-              wait_tile(k);
-              scores(0, 0, k);
-            } else {
-              finished(0);
+              at_key();
+              wait_tile();
+              scores(0, 0);
+              at_value();
             }
             wait_p(1);
-            outputs(1, v, i == 0);
-            release(v);
+            outputs(1, i == 0);
+            release();
             if (more) {
-              scores(1, 1, k);
-              release(k);
-            } else {
-              finished(1);
+              scores(1, 1);
+              release();
             }
-            tile_at += more ? 2 : 1;
           }
         } else {
-          release(tile_at++);
-          if (n1 > 0) {
-            wait_tile(tile_at);
-            scores(1, 0, tile_at);
-            release(tile_at++);
+          for (int i = 0; i < min(2, n0); ++i) {
+            wait_tile();
+            scores(0, 0);
+            release();
+            if (i >= n1) continue;
+            wait_tile();
+            scores(1, 0);
+            release();
           }
-          for (int i = 0; i < n0 && ok; ++i) {
+          for (int i = 0; i < n0; ++i) {
 #pragma unroll
             for (int stream = 0; stream < 2; ++stream) {
               const int steps = stream == 0 ? n0 : n1;
               if (i >= steps) continue;
               wait_p(stream);
-              wait_tile(tile_at);
-              outputs(stream, tile_at, i == 0);
-              release(tile_at++);
-              if (i + 1 < steps) {
-                wait_tile(tile_at);
-                scores(stream, 0, tile_at);
-                release(tile_at++);
-              } else {
-                finished(stream);
+              wait_tile();
+              outputs(stream, i == 0);
+              release();
+              if (i + 2 < steps) {
+                wait_tile();
+                scores(stream, 0);
+                release();
               }
             }
           }
         }
       }
-      umma_commit(drain);
+      commit_products(is, drain);
       mbar_wait(drain, 0, nullptr, SJ_DEV_ATTN_WAIT);
     }
+  } else if (warp == kFenceWarp) {
+    if (lane == 0) {
+      int slot = 0, turn = 0;
+      bool ok = true;
+      while (ok && walk.next(p)) {
+        const int tiles = 2 * (p.two ? p.steps0 : p.steps0 + p.steps1);
+        for (int i = 0; i < tiles && ok; ++i) {
+          ok = mbar_wait(&full[slot], turn, abort_flag, SJ_DEV_ATTN_WAIT);
+          fence_proxy_async_shared();  // cp.async wrote by the generic proxy
+          if (ok) mbar_arrive(&ready[slot]);
+          if (++slot == L::STAGES) {
+            slot = 0;
+            turn ^= 1;
+          }
+        }
+      }
+    }
   } else {
-    const int w = warp - kMmaWarp - 1;
-    int issued = 0, passed = 0, seen_at[2] = {0, 0};  // tiles on their way, tiles handed over
+    const int w = warp - kLoadWarp;
+    int slot = 0, turn = 0, seen_at[2] = {0, 0};
     bool ok = true;
-    auto hand_over = [&]() {  // this thread's copies of the oldest tile are in
-      fence_proxy_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&full[passed % L::STAGES]);
-      ++passed;
+    struct At {  // this lane's key of a tile, its page in the block table and its row there, and the page
+      int key, index, row, page;
     };
-    auto look_up = [&](int key) {
-      key += w * 32 + lane;
-      return key < p.g.p1 ? a.table[static_cast<size_t>(p.g.request) * a.ld_table + key / a.page] : -1;
+    auto look_up = [&](At& x) {
+      x.page = x.key < p.g.p1 ? a.table[static_cast<size_t>(p.g.request) * a.ld_table + x.index] : 0;
     };
-    // where this lane's key lies, in 16-byte pieces
-    auto resolve = [&](int key, int found) {
-      key += w * 32 + lane;
-      if (key >= p.g.p1) return kNowhere;
-      if (found < 0 || found >= a.pages) {
+    auto place = [&](const At& x) {  // where it lies, in 16-byte pieces
+      if (x.key >= p.g.p1) return kNowhere;
+      if (x.page < 0 || x.page >= a.pages) {
         record_error(SJ_DEV_BAD_INDEX);
         return kNowhere;
       }
-      return static_cast<uint32_t>((found * a.page_stride + p.h * a.head_stride + key % a.page * a.token_stride) >> 3);
+      return static_cast<uint32_t>((x.page * a.page_stride + p.h * a.head_stride + x.row * a.token_stride) >> 3);
     };
     auto mark = [&](int stream, uint32_t where) {
       const uint32_t have = __ballot_sync(0xffffffffu, where != kNowhere);
-      if (lane == 0) seen[(stream * kSeen + (seen_at[stream] & (kSeen - 1))) * 4 + w] = have;
+      if (lane == 0) seen[(stream * kSeen + (seen_at[stream] & (kSeen - 1))) * 2 + w] = have;
       ++seen_at[stream];
     };
+    constexpr int LANES = DIM / 8, ROWS = 32 / LANES;  // of a row, in one instruction
+    const uint32_t ring = smem_u32(smem + L::RING) + ((lane % LANES) >> 3) * L::HALF + (w * 32 + lane / LANES) * 128;
     auto fetch = [&](const __nv_bfloat16* from, uint32_t where) {
-      const int slot = issued % L::STAGES;
-      const uint32_t parity = ((issued / L::STAGES) & 1) ^ 1;
-      if (!__all_sync(0xffffffffu, mbar_test_wait(&empty[slot], parity))) {
-        // what is on its way is handed over before this warp waits, for what it waits for may need it
-        shared_copies_wait<0>();
-        while (passed < issued) hand_over();
-        if (!mbar_wait(&empty[slot], parity, abort_flag, SJ_DEV_ATTN_WAIT)) ok = false;
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) return;
-      }
-      __syncwarp();
-      constexpr int LANES = DIM / 8, ROWS = 32 / LANES;  // of a row, in one instruction
-      const uint32_t dst = smem_u32(smem + L::RING + slot * L::SLOT) + ((lane % LANES) >> 3) * L::HALF;
+      if (!mbar_wait(&empty[slot], turn ^ 1, abort_flag, SJ_DEV_ATTN_WAIT)) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      const uint32_t dst = ring + slot * L::SLOT;
+      const __nv_bfloat16* src = from + (lane % LANES) * 8;
+      const bool all = __all_sync(0xffffffffu, where != kNowhere);
+      uint32_t at[32 / ROWS];
+#pragma unroll
+      for (int i = 0; i < 32 / ROWS; ++i) at[i] = __shfl_sync(0xffffffffu, where, i * ROWS + lane / LANES);
 #pragma unroll
       for (int i = 0; i < 32 / ROWS; ++i) {
-        const int key = i * ROWS + lane / LANES;
-        const uint32_t at = __shfl_sync(0xffffffffu, where, key);
-        shared_copy16(dst + (w * 32 + key) * 128 + (((lane & 7) ^ (key & 7)) << 4),
-                      from + (at == kNowhere ? 0 : static_cast<size_t>(at) * 8 + (lane % LANES) * 8), at != kNowhere);
+        const uint32_t to = dst + i * ROWS * 128 + (((lane & 7) ^ ((i * ROWS + lane / LANES) & 7)) << 4);
+        if (all)
+          shared_copy16(to, src + static_cast<size_t>(at[i]) * 8);
+        else
+          shared_copy16(to, at[i] == kNowhere ? from : src + static_cast<size_t>(at[i]) * 8, at[i] != kNowhere);
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      ++issued;
-      if (issued - passed >= L::AHEAD) {
-        shared_copies_wait<L::AHEAD - 1>();
-        hand_over();
+      // this thread's arrival, once its copies are in
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[slot])) : "memory");
+      if (++slot == L::STAGES) {
+        slot = 0;
+        turn ^= 1;
       }
     };
     while (ok && walk.next(p)) {
-      const int n0 = p.steps[0], n1 = p.two ? 0 : p.steps[1];
-      uint32_t now[2] = {kNowhere, kNowhere};
-      int found[2];
-      found[0] = look_up(p.key(0, 0));
-      found[1] = n1 > 0 ? look_up(p.key(1, 0)) : -1;
-      auto keys = [&](int stream, int step, int steps) {  // a tile of K; the next one's pages are looked up
-        now[stream] = resolve(p.key(stream, step), found[stream]);
-        if (step + 1 < steps) found[stream] = look_up(p.key(stream, step + 1));
-        mark(stream, now[stream]);
-        if (p.two) mark(1, now[stream]);
-        fetch(a.k, now[stream]);
+      const int n0 = p.steps0, n1 = p.two ? 0 : p.steps1;
+      // of each stream: where the keys of the tile whose V comes next, and of the one after it, lie
+      uint32_t now[2] = {kNowhere, kNowhere}, after[2] = {kNowhere, kNowhere};
+      At next[2];
+      const int ahead = p.two ? kSharedKeys : 2 * kSharedKeys, ahead_pages = ahead / a.page, ahead_rows = ahead % a.page;
+#pragma unroll
+      for (int stream = 0; stream < 2; ++stream) {
+        At& x = next[stream];
+        x.key = p.key(stream, 0) + w * 32 + lane;
+        x.index = x.key / a.page;
+        x.row = x.key - x.index * a.page;
+        look_up(x);
+      }
+      auto keys = [&](int stream) {  // a tile of K; the next one's pages are looked up
+        At& x = next[stream];
+        const uint32_t where = place(x);
+        x.key += ahead;
+        x.index += ahead_pages;
+        x.row += ahead_rows;
+        if (x.row >= a.page) {
+          x.row -= a.page;
+          ++x.index;
+        }
+        look_up(x);
+        mark(stream, where);
+        if (p.two) mark(1, where);
+        fetch(a.k, where);
+        return where;
       };
-      keys(0, 0, n0);
-      if (ok && n1 > 0) keys(1, 0, n1);
+      now[0] = keys(0);
+      if (ok && n1 > 0) now[1] = keys(1);
+      if (ok && n0 > 1) after[0] = keys(0);
+      if (ok && n1 > 1) after[1] = keys(1);
       for (int i = 0; i < n0 && ok; ++i) {
-        fetch(a.v, now[0]);
-        if (ok && i + 1 < n0) keys(0, i + 1, n0);
-        if (ok && i < n1) fetch(a.v, now[1]);
-        if (ok && i + 1 < n1) keys(1, i + 1, n1);
+#pragma unroll
+        for (int stream = 0; stream < 2; ++stream) {
+          const int steps = stream == 0 ? n0 : n1;
+          if (i >= steps || !ok) continue;
+          fetch(a.v, now[stream]);
+          now[stream] = after[stream];
+          if (ok && i + 2 < steps) after[stream] = keys(stream);
+        }
       }
     }
-    shared_copies_wait<0>();
-    while (passed < issued) hand_over();
+    asm volatile("cp.async.wait_all;" ::: "memory");  // nothing lands after the CTA has gone
   }
   tc_fence_before();
   __syncthreads();

@@ -220,98 +220,6 @@ SJ_DEVICE int arrive(int* counter) {
   return before;
 }
 
-// A row's own part (of `heads` heads from `head` on: outputs `own` [heads][DIM], maxima and sums) joined with the parts of
-// its keys in common, and written.  The parts of those are taken by `shares` threads a float4 each, in the order of the
-// parts, then one after the other.
-constexpr int kScratch = 1024;  // float4 of `so` that hold a unit's joined outputs
-template <int DIM, int Q, int WARPS>
-__device__ __noinline__ void join_shared(const PagedAttention& a, const SharedSpans& s, const SharedRow& row, int r,
-                                         int head, int q0, int heads, const float* own, const float* own_m,
-                                         const float* own_l, float4* scratch, float (*weight)[Q]) {
-  constexpr int THREADS = WARPS * 32;
-  const int t = threadIdx.x, items = heads * (DIM / 4), fan = a.hq / a.hk;
-  int from = 0, parts = 0, query = 0;
-  if (row.group >= 0) {
-    const SharedGroup g = s.groups[row.group];
-    const int per = kSharedQueries / fan, at = r - g.first, tile = at / per;
-    const bool two = tile / 2 < g.tiles / 2;
-    const SharedCut cut(*s.total, s.ctas);
-    const unsigned long long begin = g.base + (head / fan) * g.head_items() + static_cast<unsigned long long>(tile / 2) * g.keys;
-    from = cut.of(begin);
-    parts = cut.of(begin + (two ? g.keys : g.halves()) - 1) - from + 1;
-    query = (two ? (tile & 1) * kSharedQueries : 0) + at % per * fan + q0;
-  }
-  const int shares = max(1, min(parts, THREADS / items));
-#pragma unroll 1
-  for (int i = t; i < items * shares; i += THREADS) {
-    const int share = i / items, qi = i % items / (DIM / 4), d = i % (DIM / 4) * 4;
-    float m = -INFINITY, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-    for (int p0 = share; p0 < parts; p0 += 4 * shares) {
-      float pm[4], pl[4];
-      float4 x[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int p = min(p0 + e * shares, parts - 1);
-        if (p == 0) {
-          const size_t at = static_cast<size_t>(r) * a.hq + head + qi;
-          pm[e] = s.m[at];
-          pl[e] = s.l[at];
-          x[e] = *reinterpret_cast<const float4*>(s.o + at * DIM + d);
-        } else {
-          const float* slot = shared_slot<DIM>(s, from + p, query + qi);
-          pm[e] = slot[0];
-          pl[e] = slot[1];
-          x[e] = *reinterpret_cast<const float4*>(slot + 4 + d);
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (p0 + e * shares >= parts) continue;
-        const float top = fmaxf(m, pm[e]), base = top == -INFINITY ? 0.f : top;
-        const float f = exp2_fast(m - base), g = exp2_fast(pm[e] - base);
-        l = f * l + g * pl[e];
-        acc.x = f * acc.x + g * x[e].x;
-        acc.y = f * acc.y + g * x[e].y;
-        acc.z = f * acc.z + g * x[e].z;
-        acc.w = f * acc.w + g * x[e].w;
-        m = top;
-      }
-    }
-    scratch[i] = acc;
-    if (d == 0) {
-      weight[2 * share][qi] = m;
-      weight[2 * share + 1][qi] = l;
-    }
-  }
-  __syncthreads();
-#pragma unroll 1
-  for (int i = t; i < items; i += THREADS) {
-    const int qi = i / (DIM / 4), d = i % (DIM / 4) * 4;
-    float m = own_m[qi], l = own_l[qi];
-    float4 acc = *reinterpret_cast<const float4*>(own + qi * DIM + d);
-#pragma unroll 1
-    for (int w = 0; w < (parts ? shares : 0); ++w) {
-      const float pm = weight[2 * w][qi], top = fmaxf(m, pm), base = top == -INFINITY ? 0.f : top;
-      const float f = exp2_fast(m - base), g = exp2_fast(pm - base);
-      const float4 x = scratch[w * items + i];
-      l = f * l + g * weight[2 * w + 1][qi];
-      acc.x = f * acc.x + g * x.x;
-      acc.y = f * acc.y + g * x.y;
-      acc.z = f * acc.z + g * x.z;
-      acc.w = f * acc.w + g * x.w;
-      m = top;
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    *reinterpret_cast<uint2*>(a.o + static_cast<size_t>(r) * a.ldo + (head + qi) * DIM + d) =
-        make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-    if (d == 0 && a.lse)
-      a.lse[static_cast<size_t>(r) * a.hq + head + qi] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-  }
-  __syncthreads();  // the caller goes on with the shared arrays
-}
-
 // DIM: head_dim; NQ: query tiles of 8 that a unit holds (a query's columns of S^T; 2 above 8 heads a KV head).  SHARED:
 // `spans` says which keys of each row attn_shared_kernel has taken; keys are then counted without those.
 template <int DIM, int NQ, bool SHARED>
@@ -328,7 +236,6 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attn_paged_kernel(const Pa
   uint8_t* smem = unaligned + (-smem_u32(unaligned) & 127);
   float* so = reinterpret_cast<float*>(smem);  // [WARPS][Q][LD], once a unit's stages are read
   __shared__ float sm[WARPS][Q], sl[WARPS][Q], weight[kGroupMost][Q];
-  __shared__ __align__(16) float fin[SHARED ? Q * DIM : 4], fm[Q], fl[Q];
   __shared__ unsigned long long scan[WARPS], s_base;
   __shared__ int s_row, s_last;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = lane >> 2, c = lane & 3;
@@ -649,10 +556,11 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attn_paged_kernel(const Pa
           sum += exp2_fast(sm[w][qi] - ref) * sl[w][qi];
         }
         if (SHARED && whole) {
-          *reinterpret_cast<float4*>(fin + qi * DIM + d) = out;
+          const size_t query = static_cast<size_t>(r) * a.hq + h * group + q0 + qi;
+          *reinterpret_cast<float4*>(spans.own.o + query * DIM + d) = out;
           if (d == 0) {
-            fm[qi] = top;
-            fl[qi] = sum;
+            spans.own.m[query] = top;
+            spans.own.l[query] = sum;
           }
         } else if (whole) {
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -669,11 +577,6 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attn_paged_kernel(const Pa
             slot[Q + qi] = sum;
           }
         }
-      }
-      if (SHARED && whole) {
-        __syncthreads();
-        join_shared<DIM, Q, WARPS>(a, spans, whole_row, r, h * group + q0, q0, heads, fin, fm, fl,
-                                   reinterpret_cast<float4*>(so) + kScratch, weight);
       }
       if (!whole) {
         // ---- the unit's parts joined by the CTA that writes the last of them: tile x falls to the last chunk w
@@ -710,8 +613,15 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attn_paged_kernel(const Pa
           if (joined) join_parts<DIM, Q, WARPS>(a.partial, from, from, groups, size, heads, sm[0], sl[0], weight, sums);
         }
         if (SHARED && joined) {
-          join_shared<DIM, Q, WARPS>(a, spans, whole_row, r, h * group + q0, q0, heads, so, sm[0], sl[0],
-                                     reinterpret_cast<float4*>(so) + kScratch, weight);
+          for (int i = t; i < heads * (DIM / 4); i += WARPS * 32) {
+            const int qi = i / (DIM / 4), d = i % (DIM / 4) * 4;
+            const size_t query = static_cast<size_t>(r) * a.hq + h * group + q0 + qi;
+            *reinterpret_cast<float4*>(spans.own.o + query * DIM + d) = sums[i];
+            if (d == 0) {
+              spans.own.m[query] = sm[0][qi];
+              spans.own.l[query] = sl[0][qi];
+            }
+          }
         } else if (joined) {
           for (int i = t; i < heads * (DIM / 4); i += WARPS * 32) {
             const int qi = i / (DIM / 4), d = i % (DIM / 4) * 4, head = h * group + q0 + qi;
@@ -746,7 +656,6 @@ template <int DIM, int NQ, bool SHARED>
 int attend(const PagedAttention& a, const SharedSpans& spans, cudaStream_t stream) {
   constexpr int outputs = kWarps * NQ * 8 * (DIM + 8) * 4, rings = kWarps * kStages * 8192;
   constexpr int smem = (outputs > rings ? outputs : rings) + 128;
-  static_assert(2 * kScratch * 16 <= rings && NQ * 8 * DIM / 4 <= kScratch, "joined outputs, and parts beside them");
   static KernelAttrOnce once;
   const int rc = ensure_max_smem(once, reinterpret_cast<const void*>(attn_paged_kernel<DIM, NQ, SHARED>), smem,
                                  "sj_attn_paged: shared memory");

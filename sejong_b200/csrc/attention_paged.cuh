@@ -33,15 +33,18 @@ struct SharedCut {
 };
 
 // A group: its rows, the keys [p0, p1) that every live one of them sees, and its first item.  The queries of a KV head
-// lie in `tiles` tiles.  A unit is two tiles of queries, whose item is a tile of keys for both, or the one tile that is
-// left, whose item is two tiles of keys: an item is the same work either way.
+// lie in `tiles` tiles.  An item is a tile of keys for two tiles of queries, or two tiles of keys for the one tile that
+// may be left: the same work either way.  A head's items are those of its pairs of tiles, a chunk of the keys at a time,
+// so that CTAs which run side by side read the same keys, then those of the tile that is left.
 struct SharedGroup {
   unsigned long long base;
-  int first, rows, request, p0, p1, tiles, keys;  // keys: tiles of them
+  size_t main;  // the first query of the group's parts that begin a block (chunk and pair): [chunks][rows][hq]
+  int first, rows, request, p0, p1, tiles, keys, chunks;  // keys: tiles of them
   SJ_DEVICE int halves() const { return (keys + 1) / 2; }
   SJ_DEVICE unsigned long long head_items() const {
     return static_cast<unsigned long long>(tiles / 2) * keys + (tiles & 1) * halves();
   }
+  SJ_DEVICE int chunk(int c) const { return static_cast<int>(static_cast<long long>(keys) * c / chunks); }  // its first tile
 };
 
 // A row: keys [lo, p0) and [p1, n) are its own, group -1: all of [lo, n).
@@ -49,19 +52,21 @@ struct SharedRow {
   int lo, n, p0, p1, group;
 };
 
+// A softmax's part: maximum (of log2), sum and outputs of each query.
+struct SharedParts {
+  float *m, *l, *o;  // o: [queries][dim]
+};
+
 struct SharedSpans {
   unsigned long long* total;  // items of all groups
   SharedGroup* groups;
   SharedRow* rows;
-  float *m, *l, *o;  // [rows, hq (, dim)]: the part of a row's common keys that begins its unit
-  int ctas;          // of attn_shared_kernel
-  float* slots;      // [ctas][2 * kSharedQueries][dim + 4]: the part that goes on with a unit, of each CTA
+  SharedParts own;    // [rows, hq]: a row's own keys
+  SharedParts main;   // the parts that begin a block
+  SharedParts slots;  // [ctas][2 * kSharedQueries]: the part that goes on with a block, of each CTA
+  size_t main_queries;
+  int ctas;  // of attn_shared_kernel
 };
-
-template <int DIM>
-SJ_DEVICE float* shared_slot(const SharedSpans& s, int cta, int query) {  // m, l, o
-  return s.slots + (static_cast<size_t>(cta) * (2 * kSharedQueries) + query) * (DIM + 4);
-}
 
 // Checks the arguments of sj_attn_paged, or of a call (`who`) that has the same ones and a workspace of `need` bytes
 // that begins with that of sj_attn_paged.
@@ -71,7 +76,7 @@ int paged_attention_args(const char* who, PagedAttention& a, const void* q, int 
                          const int32_t* request, const int32_t* position, int rows, int hq, int hk, int head_dim,
                          int window, void* o, int ldo, float* lse, void* workspace, size_t workspace_bytes,
                          size_t need);
-// Launches attn_paged_kernel: all of a row's keys, or (spans not null) its own ones, joined with those in common.
+// Launches attn_paged_kernel: all of a row's keys, or (spans not null) its own ones, as a part.
 int attn_paged_rows(const PagedAttention& a, const SharedSpans* spans, int head_dim, cudaStream_t stream);
 
 }  // namespace sj

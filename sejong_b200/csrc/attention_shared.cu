@@ -2,8 +2,10 @@
 //
 //   shared_spans_kernel   each group's keys that all of its rows see, and the work that they are
 //   attn_shared_kernel    the queries of a group against those keys, on the tensor cores
+//   attn_paged_kernel     (attention_paged.cu) each row against its own keys
+//   shared_join_kernel    the parts of each row and head joined
 //
-// attn_paged_kernel (attention_paged.cu) then takes each row's own keys and joins the two.  With M queries a KV head, M
+//  With M queries a KV head, M
 // multiply-adds are made of each cache element: memory bounds a few of them, the exponentials and the tensor cores
 // many.  A row's keys outside [p0, p1), by its window or its length, are its own, so no tile needs a mask but for the
 // last one's end, and a value that a row does not see reaches no sum of it.
@@ -19,8 +21,9 @@ namespace sj {
 
 namespace {
 constexpr int kSharedGroups = 1024;
-constexpr int kSoftmaxWarps = 8, kMmaWarp = 8, kFenceWarp = 9, kLoadWarp = 10, kLoadWarps = 2;
-constexpr int kSharedThreads = 32 * (kLoadWarp + kLoadWarps);
+constexpr int kSoftmaxWarps = 8, kMmaWarp = 8, kFenceWarp = 9, kLoadWarp = 10;
+constexpr int kLoadWarps = 2;                // of K, and as many of V
+constexpr int kSharedThreads = 32 * (kLoadWarp + 2 * kLoadWarps);
 constexpr int kSeen = 16;                  // tiles whose masks of valid keys are kept
 constexpr float kLazy = 8.f;               // a maximum may stand this far (of log2) below the true one
 constexpr uint32_t kColO = 256;            // TMEM columns: two S of each of two streams (their P over them), then O
@@ -32,7 +35,7 @@ constexpr int kLastSeen = INT_MAX - 4096;
 // ---------------------------------------------------------------- spans
 struct SpansArgs {
   const int32_t *request, *position, *group;
-  int rows, groups, requests, page, ld_table, window, fan, hk, least;
+  int rows, groups, requests, page, ld_table, window, hq, fan, hk, least;
   SharedSpans out;
 };
 
@@ -97,22 +100,39 @@ __global__ void __launch_bounds__(1024) shared_spans_kernel(const SpansArgs a) {
     g.keys = (g.p1 - g.p0 + kSharedKeys - 1) / kSharedKeys;
     items = g.head_items() * a.hk;
   }
-  unsigned long long upto = items;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const unsigned long long u = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += u;
-  }
-  if (lane == 31) s_scan[warp] = upto;
-  __syncthreads();
-  g.base = upto - items;
   unsigned long long total = 0;
-  for (int w = 0; w < 32; ++w) {
-    if (w == warp) g.base += total;
-    total += s_scan[w];
+  auto before = [&](unsigned long long mine) {  // the sum of the threads' before this one; total: of all
+    unsigned long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long u = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += u;
+    }
+    __syncthreads();
+    if (lane == 31) s_scan[warp] = upto;
+    __syncthreads();
+    unsigned long long base = upto - mine;
+    total = 0;
+    for (int w = 0; w < 32; ++w) {
+      if (w == warp) base += total;
+      total += s_scan[w];
+    }
+    return base;
+  };
+  g.base = before(items);
+  const unsigned long long all = total;
+  if (t == 0) *a.out.total = all;
+  // about a CTA's items a chunk, so that a block is about a CTA's
+  const unsigned long long ctas = min(static_cast<unsigned long long>(a.out.ctas), all);
+  const unsigned long long chunks = all > 0 && g.tiles > 1 ? g.keys * ctas / all : 1;  // at most g.keys
+  g.chunks = static_cast<int>(max(chunks, 1ull));
+  const unsigned long long queries = static_cast<unsigned long long>(g.rows) * a.hq;
+  g.main = before(t < a.groups ? queries * g.chunks : 0);
+  if (total > a.out.main_queries) {  // not reached: a head's blocks are about as many as the CTAs
+    g.chunks = 1;
+    g.main = before(t < a.groups ? queries : 0);
   }
   if (t < a.groups) a.out.groups[t] = g;
-  if (t == 0) *a.out.total = total;
   for (int r = t; r < a.rows; r += 1024) {
     SharedRow& row = a.out.rows[r];
     if (row.group >= 0 && row.n > 0 && p1[row.group] > p0[row.group]) {
@@ -226,7 +246,8 @@ struct SharedLay {
 // A CTA's share of a unit: items [i0, i1) of one KV head and one or two tiles of queries.
 struct SharedPiece {
   SharedGroup g;
-  int h, tile, i0, i1;
+  int h, tile, chunk, i0, i1;
+  bool begins;  // a block
   bool two;  // two tiles of queries over the same keys; else one, over alternate tiles of keys
   int steps0, steps1;  // of the streams
   SJ_DEVICE int key(int stream, int step) const {
@@ -255,11 +276,26 @@ struct SharedWalk {
     p.g = a.s.groups[lo];
     const unsigned long long x = at - p.g.base, head = p.g.head_items();
     p.h = static_cast<int>(x / head);
-    const unsigned long long y = x % head, pairs = static_cast<unsigned long long>(p.g.tiles / 2) * p.g.keys;
-    p.two = y < pairs;
-    p.tile = p.two ? static_cast<int>(y / p.g.keys) * 2 : p.g.tiles - 1;
-    p.i0 = static_cast<int>(p.two ? y % p.g.keys : y - pairs);
-    const int items = p.two ? p.g.keys : p.g.halves();
+    const unsigned long long y = x % head;
+    const int pairs = p.g.tiles / 2;
+    p.two = y < static_cast<unsigned long long>(pairs) * p.g.keys;
+    int items;
+    if (p.two) {
+      const int column = static_cast<int>(y / pairs);  // the chunk that holds this tile of keys holds the item
+      p.chunk = static_cast<int>((static_cast<long long>(column + 1) * p.g.chunks - 1) / p.g.keys);
+      const int k0 = p.g.chunk(p.chunk), len = p.g.chunk(p.chunk + 1) - k0;
+      const unsigned long long z = y - static_cast<unsigned long long>(pairs) * k0;
+      p.tile = static_cast<int>(z / len) * 2;
+      p.i0 = k0 + static_cast<int>(z % len);
+      p.begins = p.i0 == k0;
+      items = k0 + len;
+    } else {
+      p.chunk = 0;
+      p.tile = p.g.tiles - 1;
+      p.i0 = static_cast<int>(y - static_cast<unsigned long long>(pairs) * p.g.keys);
+      p.begins = p.i0 == 0;
+      items = p.g.halves();
+    }
     p.i1 = static_cast<int>(min(static_cast<unsigned long long>(items), p.i0 + (end - at)));
     at += p.i1 - p.i0;
     p.steps0 = p.i1 - p.i0;
@@ -268,7 +304,7 @@ struct SharedWalk {
   }
 };
 
-// 12 warps, one CTA an SM.  Two streams of tiles, each with two S in TMEM, so that a tile's scores are there when the
+// 14 warps, one CTA an SM.  Two streams of tiles, each with two S in TMEM, so that a tile's scores are there when the
 // softmax of the one before ends, and the products of one stream run under the other's softmax:
 //   warps 0-3, 4-7  softmax of streams 0 and 1: a thread for a query, which has its 64 scores in registers.  P goes over
 //                   S in bf16, where the product with V reads it.  The output is rescaled only where a maximum has
@@ -276,7 +312,7 @@ struct SharedWalk {
 //   warp 8          one thread issues S = Q K^T and O += P V of both streams
 //   warp 9          one thread hands tiles that have come over to the asynchronous proxy, since a fence takes the thread
 //                   that issues the products 250 cycles
-//   warps 10-11     pages of K and V into a ring of tiles (cp.async, since a page may have any number of rows; 128-byte
+//   warps 10-13     pages of K and of V into a ring of tiles (cp.async, since a page may have any number of rows; 128-byte
 //                   rows swizzled as the products read them), which arrive by themselves
 template <int DIM>
 __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const SharedArgs a) {
@@ -459,17 +495,11 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
         l = f * l + g * sums[kSharedQueries + row];
         m = top;
       }
-      float *to_o, *to_m, *to_l;
-      if (p.i0 == 0) {
-        const size_t query = static_cast<size_t>(is ? r : 0) * a.hq + head;
-        to_m = a.s.m + query;
-        to_l = a.s.l + query;
-        to_o = a.s.o + query * DIM;
-      } else {
-        to_m = shared_slot<DIM>(a.s, blockIdx.x, (p.two ? stream * kSharedQueries : 0) + row);
-        to_l = to_m + 1;
-        to_o = to_m + 4;
-      }
+      const SharedParts& to = p.begins ? a.s.main : a.s.slots;
+      const size_t query = p.begins ? p.g.main + (static_cast<size_t>(p.chunk) * p.g.rows + (is ? at : 0)) * a.hq + head
+                                    : static_cast<size_t>(blockIdx.x) * (2 * kSharedQueries) +
+                                          (p.two ? stream * kSharedQueries : 0) + row;
+      float* to_o = to.o + query * DIM;
 #pragma unroll
       for (int c = 0; c < DIM / 16; ++c) {
         uint32_t x[16], y[16];
@@ -490,8 +520,8 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
         }
       }
       if (is) {
-        *to_m = m;
-        *to_l = l;
+        to.m[query] = m;
+        to.l[query] = l;
       }
       tc_fence_before();
     }
@@ -634,7 +664,9 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
       }
     }
   } else {
-    const int w = warp - kLoadWarp;
+    const int w = (warp - kLoadWarp) % kLoadWarps;
+    const bool of_k = warp < kLoadWarp + kLoadWarps;
+    const __nv_bfloat16* from = of_k ? a.k : a.v;
     int slot = 0, turn = 0, seen_at[2] = {0, 0};
     bool ok = true;
     struct At {  // this lane's key of a tile, its page in the block table and its row there, and the page
@@ -658,7 +690,13 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
     };
     constexpr int LANES = DIM / 8, ROWS = 32 / LANES;  // of a row, in one instruction
     const uint32_t ring = smem_u32(smem + L::RING) + ((lane % LANES) >> 3) * L::HALF + (w * 32 + lane / LANES) * 128;
-    auto fetch = [&](const __nv_bfloat16* from, uint32_t where) {
+    auto pass = [&]() {
+      if (++slot == L::STAGES) {
+        slot = 0;
+        turn ^= 1;
+      }
+    };
+    auto fetch = [&](uint32_t where) {
       if (!mbar_wait(&empty[slot], turn ^ 1, abort_flag, SJ_DEV_ATTN_WAIT)) ok = false;
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
@@ -678,10 +716,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
       }
       // this thread's arrival, once its copies are in
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[slot])) : "memory");
-      if (++slot == L::STAGES) {
-        slot = 0;
-        turn ^= 1;
-      }
+      pass();
     };
     while (ok && walk.next(p)) {
       const int n0 = p.steps0, n1 = p.two ? 0 : p.steps1;
@@ -708,9 +743,13 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
           ++x.index;
         }
         look_up(x);
-        mark(stream, where);
-        if (p.two) mark(1, where);
-        fetch(a.k, where);
+        if (of_k) {
+          mark(stream, where);
+          if (p.two) mark(1, where);
+          fetch(where);
+        } else {
+          pass();
+        }
         return where;
       };
       now[0] = keys(0);
@@ -722,7 +761,10 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
         for (int stream = 0; stream < 2; ++stream) {
           const int steps = stream == 0 ? n0 : n1;
           if (i >= steps || !ok) continue;
-          fetch(a.v, now[stream]);
+          if (of_k)
+            pass();
+          else
+            fetch(now[stream]);
           now[stream] = after[stream];
           if (ok && i + 2 < steps) after[stream] = keys(stream);
         }
@@ -736,6 +778,82 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
     tc_fence_after();
     tmem_dealloc(tmem, kTmemAll);
   }
+}
+
+// ---------------------------------------------------------------- join
+// A warp for a row and head: its own part, then the parts of its keys in common, 32 at a time in the order of chunks and
+// CTAs; the lanes take the weights, then each its dims of all parts.
+template <int DIM>
+__global__ void __launch_bounds__(256) shared_join_kernel(const SharedSpans s, int rows, int hq, int fan, __nv_bfloat16* o,
+                                                          int ldo, float* lse) {
+  pdl_wait();
+  constexpr int PER = DIM / 32;
+  const int lane = threadIdx.x & 31, at = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (at >= rows * hq) return;
+  const int r = at / hq, head = at - r * hq;
+  float m = s.own.m[at], l = s.own.l[at], acc[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) acc[e] = s.own.o[static_cast<size_t>(at) * DIM + lane * PER + e];
+  const SharedRow row = s.rows[r];
+  if (row.group >= 0) {
+    const SharedGroup g = s.groups[row.group];
+    const SharedCut cut(*s.total, s.ctas);
+    const int per = kSharedQueries / fan, in = r - g.first, tile = in / per, pairs = g.tiles / 2;
+    const bool two = tile / 2 < pairs;
+    const int chunks = two ? g.chunks : 1;
+    const int slot = (two ? (tile & 1) * kSharedQueries : 0) + in % per * fan + head % fan;
+    const unsigned long long base = g.base + (head / fan) * g.head_items();
+    for (int c0 = 0; c0 < chunks; c0 += 32) {
+      const int c = c0 + (chunks > 1 ? lane : 0);
+      int from = 0, to = -1;
+      if (c < chunks) {
+        const int k0 = two ? g.chunk(c) : 0, len = two ? g.chunk(c + 1) - k0 : g.halves();
+        const unsigned long long begin =
+            base + (two ? static_cast<unsigned long long>(pairs) * k0 + static_cast<unsigned long long>(tile / 2) * len
+                        : static_cast<unsigned long long>(pairs) * g.keys);
+        from = cut.of(begin);
+        to = cut.of(begin + len - 1);
+      }
+      const int first = chunks > 1 ? 0 : lane, step = chunks > 1 ? 1 : 32;
+      for (int k = first; __any_sync(0xffffffffu, from + k <= to); k += step) {
+        const bool is = from + k <= to;
+        const SharedParts& part = k == 0 ? s.main : s.slots;
+        const size_t query = !is ? 0
+                             : k == 0 ? g.main + (static_cast<size_t>(c) * g.rows + in) * hq + head
+                                      : static_cast<size_t>(from + k) * (2 * kSharedQueries) + slot;
+        const float pm = is ? part.m[query] : -INFINITY, pl = is ? part.l[query] : 0.f;
+        const float* from_o = part.o + query * DIM;
+        const float top = fmaxf(m, warp_max(pm)), ref = top == -INFINITY ? 0.f : top;
+        const float f = shared_exp2(m - ref), w = shared_exp2(pm - ref);
+        l = f * l + warp_sum(w * pl);
+        m = top;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) acc[e] *= f;
+        const uint32_t have = __ballot_sync(0xffffffffu, is);
+        const int most = 32 - __clz(have);
+        for (int j0 = 0; j0 < most; j0 += 8) {
+          float x[8][PER], weight[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            weight[j] = __shfl_sync(0xffffffffu, w, j0 + j);
+            const float* src = reinterpret_cast<const float*>(
+                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(from_o), j0 + j));
+#pragma unroll
+            for (int e = 0; e < PER; ++e) x[j][e] = have >> (j0 + j) & 1 ? src[lane * PER + e] : 0.f;
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int e = 0; e < PER; ++e) acc[e] += weight[j] * x[j][e];
+        }
+      }
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint32_t* dst = reinterpret_cast<uint32_t*>(o + static_cast<size_t>(r) * ldo + head * DIM + lane * PER);
+#pragma unroll
+  for (int e = 0; e < PER; e += 2) dst[e / 2] = pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
+  if (lane == 0 && lse) lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
 namespace {
@@ -752,15 +870,18 @@ size_t shared_layout(SharedSpans* s, char* at, int rows, int groups, int hq, int
   char* total = take(sizeof(unsigned long long));
   char* group = take(sizeof(SharedGroup) * groups);
   char* row = take(sizeof(SharedRow) * rows);
-  const size_t queries = static_cast<size_t>(rows) * hq;
-  char* m = take(queries * sizeof(float));
-  char* l = take(queries * sizeof(float));
-  char* o = take(queries * head_dim * sizeof(float));
-  char* slots = take(static_cast<size_t>(sm_count()) * 2 * kSharedQueries * (head_dim + 4) * sizeof(float));
-  if (s)
-    *s = SharedSpans{reinterpret_cast<unsigned long long*>(total), reinterpret_cast<SharedGroup*>(group),
-                     reinterpret_cast<SharedRow*>(row), reinterpret_cast<float*>(m), reinterpret_cast<float*>(l),
-                     reinterpret_cast<float*>(o), sm_count(), reinterpret_cast<float*>(slots)};
+  auto parts = [&](size_t queries) {
+    float* m = reinterpret_cast<float*>(take(queries * sizeof(float)));
+    float* l = reinterpret_cast<float*>(take(queries * sizeof(float)));
+    return SharedParts{m, l, reinterpret_cast<float*>(take(queries * head_dim * sizeof(float)))};
+  };
+  // chunks * pairs * hk of a group is at most its share of the CTAs, and a pair brings a third tile at most
+  const size_t own = static_cast<size_t>(rows) * hq, ctas = static_cast<size_t>(sm_count());
+  const size_t main_queries = own + ctas * 3 * kSharedQueries;
+  const SharedSpans all{reinterpret_cast<unsigned long long*>(total), reinterpret_cast<SharedGroup*>(group),
+                        reinterpret_cast<SharedRow*>(row), parts(own), parts(main_queries),
+                        parts(ctas * 2 * kSharedQueries), main_queries, static_cast<int>(ctas)};
+  if (s) *s = all;
   return n;
 }
 
@@ -787,7 +908,8 @@ bool shares(int groups, int hq, int hk) { return groups > 0 && groups <= kShared
 extern "C" size_t sj_attn_paged_shared_workspace(int rows, int groups, int hq, int hk, int head_dim) {
   const size_t own = sj_attn_paged_workspace(rows, hq, hk, head_dim);
   if (own == 0 || groups < 0) return 0;
-  return up256(own) + shared_layout(nullptr, nullptr, rows, std::min(groups, kSharedGroups), hq, head_dim);
+  if (!shares(groups, hq, hk)) return own;
+  return up256(own) + shared_layout(nullptr, nullptr, rows, groups, hq, head_dim);
 }
 
 extern "C" int sj_attn_paged_shared(const void* q, int ldq, const void* k_cache, const void* v_cache, int pages,
@@ -797,7 +919,8 @@ extern "C" int sj_attn_paged_shared(const void* q, int ldq, const void* k_cache,
                                     int hk, int head_dim, int window, void* o, int ldo, float* lse, void* workspace,
                                     size_t workspace_bytes, void* stream) {
   constexpr const char* who = "sj_attn_paged_shared";
-  if (groups < 0 || (rows > 0 && groups > rows)) return fail(SJ_ERR_SHAPE, "%s: groups=%d rows=%d", who, groups, rows);
+  if (groups < 0 || (rows > 0 && groups > rows) || (hq > 0 && rows > INT_MAX / hq))
+    return fail(SJ_ERR_SHAPE, "%s: groups=%d rows=%d", who, groups, rows);
   PagedAttention a;
   int rc = paged_attention_args(who, a, q, ldq, k_cache, v_cache, pages, page, page_stride, head_stride, token_stride,
                                 block_table, ld_table, requests, request, position, rows, hq, hk, head_dim, window, o,
@@ -810,12 +933,17 @@ extern "C" int sj_attn_paged_shared(const void* q, int ldq, const void* k_cache,
   SharedSpans spans;
   shared_layout(&spans, static_cast<char*>(workspace) + up256(sj_attn_paged_workspace(rows, hq, hk, head_dim)), rows,
                 groups, hq, head_dim);
-  const SpansArgs sa{request, position, group, rows, groups, requests, page, ld_table, window, hq / hk, hk, 2, spans};
+  const SpansArgs sa{request, position, group, rows, groups, requests, page, ld_table, window, hq, hq / hk, hk, 2, spans};
   launch(shared_spans_kernel, 1, 1024, 0, s, sa);
   SJ_LAUNCH_CHECK("shared_spans");
   const SharedArgs ta{a.q, a.k, a.v, block_table, page_stride, head_stride, token_stride, ldq, pages, page, ld_table,
                       groups, hq, hk, hq / hk, 1.4426950408889634f / sqrtf(static_cast<float>(head_dim)), spans};
   rc = head_dim == 64 ? shared_pass<64>(ta, s) : shared_pass<128>(ta, s);
+  if (rc == SJ_OK) rc = attn_paged_rows(a, &spans, head_dim, s);
   if (rc != SJ_OK) return rc;
-  return attn_paged_rows(a, &spans, head_dim, s);
+  const int64_t queries = static_cast<int64_t>(rows) * hq;
+  launch(head_dim == 64 ? shared_join_kernel<64> : shared_join_kernel<128>, static_cast<unsigned>((queries + 7) / 8), 256, 0,
+         s, spans, rows, hq, hq / hk, a.o, ldo, lse);
+  SJ_LAUNCH_CHECK("shared_join");
+  return SJ_OK;
 }

@@ -16,7 +16,7 @@ struct PagedAttention {
   int ldq, ldo, pages, page, ld_table, requests, rows, hq, hk, window;
 };
 
-constexpr int kSharedKeys = 64;      // keys of a tile
+constexpr int kSharedKeys = 128;     // keys of a tile
 constexpr int kSharedQueries = 128;  // queries of a tile: whole rows of hq / hk heads that share a KV head
 
 // Ranges of equal length of `total` items, one for a CTA.

@@ -23,10 +23,12 @@ namespace {
 constexpr int kSharedGroups = 1024;
 constexpr int kSoftmaxWarps = 8, kMmaWarp = 8, kFenceWarp = 9, kLoadWarp = 10;
 constexpr int kLoadWarps = 2;                // of K, and as many of V
+constexpr int kHalf = kSharedKeys / 2;       // keys of which a softmax thread has the scores at a time
 constexpr int kSharedThreads = 32 * (kLoadWarp + 2 * kLoadWarps);
-constexpr int kSeen = 16;                  // tiles whose masks of valid keys are kept
+constexpr int kSeen = 8;                   // tiles whose masks of valid keys are kept
+constexpr int kByHand = 0;                 // of 8 pairs of exponentials, those taken by the other pipes
 constexpr float kLazy = 8.f;               // a maximum may stand this far (of log2) below the true one
-constexpr uint32_t kColO = 256;            // TMEM columns: two S of each of two streams (their P over them), then O
+constexpr uint32_t kColO = 256;            // TMEM columns: S of two streams (their P over them), then O
 constexpr uint32_t kTmemAll = 512;
 constexpr uint32_t kNowhere = 0xffffffffu;
 constexpr int kLastSeen = INT_MAX - 4096;
@@ -180,6 +182,30 @@ SJ_DEVICE uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
   return y;
 }
+SJ_DEVICE uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t y;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+  return y;
+}
+// 2^d of two d <= 8 or so, without the unit for exponentials: d = n + f with n the nearest whole number, 2^f by the
+// polynomial of degree 5 that is off by the least share over |f| <= 1/2 (fitted: 7.5e-8, 2^-22 with its roundings), 2^n
+// by its bits.  0 below 2^-126; a NaN stays one.
+SJ_DEVICE uint64_t exp2_by_hand(uint64_t d) {
+  float x0, x1;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x0) : "f"(low2(d)), "f"(-127.f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x1) : "f"(high2(d)), "f"(-127.f));
+  const uint64_t x = pair2(x0, x1), round = pair2(12582912.f, 12582912.f);  // 1.5 * 2^23: sums have no fraction bits
+  const uint64_t t = add2(x, round), n = add2(t, pair2(-12582912.f, -12582912.f));
+  const uint64_t f = fma2(n, pair2(-1.f, -1.f), x);
+  uint64_t y = pair2(0.001327647129073739f, 0.001327647129073739f);
+  y = fma2(y, f, pair2(0.009675540961325169f, 0.009675540961325169f));
+  y = fma2(y, f, pair2(0.05550713092088699f, 0.05550713092088699f));
+  y = fma2(y, f, pair2(0.24022120237350464f, 0.24022120237350464f));
+  y = fma2(y, f, pair2(0.6931469440460205f, 0.6931469440460205f));
+  y = fma2(y, f, pair2(1.0000001192092896f, 1.0000001192092896f));
+  const uint32_t n0 = static_cast<uint32_t>(t), n1 = static_cast<uint32_t>(t >> 32);
+  return mul2(y, pair2(__uint_as_float((n0 << 23) + 0x3f800000u), __uint_as_float((n1 << 23) + 0x3f800000u)));
+}
 // 16 bytes from global to shared memory; zeros when !is.
 SJ_DEVICE void shared_copy16(uint32_t dst, const __nv_bfloat16* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -238,9 +264,9 @@ struct SharedLay {
   static constexpr int SLOT = kSharedKeys * DIM * 2;  // a tile of K or of V
   static constexpr int HALF = kSharedKeys * 128;      // 64 dims of it: rows of 128 bytes
   static constexpr int QUERIES = kSharedQueries * DIM * 2, QUERIES_HALF = kSharedQueries * 128;
-  static constexpr int STAGES = DIM == 64 ? 18 : 10;   // of the ring of K and V tiles
-  static constexpr int Q = 0, RING = 2 * QUERIES, SEEN = RING + STAGES * SLOT, SUMS = SEEN + 2 * kSeen * 8,
-                       BARS = SUMS + 2 * kSharedQueries * 4, SMEM = BARS + 768 + 1024;
+  static constexpr int STAGES = DIM == 64 ? 10 : 5;    // of the ring of K and V tiles
+  static constexpr int Q = 0, RING = 2 * QUERIES, SEEN = RING + STAGES * SLOT, SUMS = SEEN + 2 * kSeen * 16,
+                       BARS = SUMS + 2 * kSharedQueries * 4, SMEM = BARS + 512 + 1024;
 };
 
 // A CTA's share of a unit: items [i0, i1) of one KV head and one or two tiles of queries.
@@ -304,12 +330,13 @@ struct SharedWalk {
   }
 };
 
-// 14 warps, one CTA an SM.  Two streams of tiles, each with two S in TMEM, so that a tile's scores are there when the
-// softmax of the one before ends, and the products of one stream run under the other's softmax:
-//   warps 0-3, 4-7  softmax of streams 0 and 1: a thread for a query, which has its 64 scores in registers.  P goes over
-//                   S in bf16, where the product with V reads it.  The output is rescaled only where a maximum has
-//                   grown by more than 2^8: until then the sums are taken by the old one.
-//   warp 8          one thread issues S = Q K^T and O += P V of both streams
+// 14 warps, one CTA an SM.  Two streams of tiles, so that the products of one run under the softmax of the other:
+//   warps 0-3, 4-7  softmax of streams 0 and 1: a thread for a query, which has the scores of half a tile in registers.  P
+//                   goes over S in bf16, where the product with V reads it, half a tile at a time.  The output is
+//                   rescaled only where a maximum has grown by more than 2^8: until then the sums are taken by the
+//                   old one.
+//   warp 8          issues S = Q K^T and O += P V of both streams.  S is 128 keys wide, since the tensor cores read Q
+//                   from shared memory for every product: one of 64 keys takes 48 cycles, one of 128 64.
 //   warp 9          one thread hands tiles that have come over to the asynchronous proxy, since a fence takes the thread
 //                   that issues the products 250 cycles
 //   warps 10-13     pages of K and of V into a ring of tiles (cp.async, since a page may have any number of rows; 128-byte
@@ -324,14 +351,15 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
   uint64_t* ready = full + L::STAGES;       // STAGES: and seen by the products
   uint64_t* empty = ready + L::STAGES;      // STAGES
   uint64_t* q_full = empty + L::STAGES;     // 2
-  uint64_t* s_full = q_full + 2;            // 2 of each stream
-  uint64_t* p_full = s_full + 4;            // 2 of each stream
-  uint64_t* o_done = p_full + 4;            // 2 of each stream, in turn: a tile's product with V
-  uint64_t* sums_full = o_done + 4;         // 1
+  uint64_t* s_full = q_full + 2;            // 2
+  uint64_t* p_full = s_full + 2;            // 2 halves of each stream
+  uint64_t* o_half = p_full + 4;            // 2: the product of a tile's first half with V
+  uint64_t* o_full = o_half + 2;            // 2: all products of a piece
+  uint64_t* sums_full = o_full + 2;         // 1
   uint64_t* drain = sums_full + 1;          // 1
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  uint32_t* seen = reinterpret_cast<uint32_t*>(smem + L::SEEN);  // [2][kSeen][2]
+  uint32_t* seen = reinterpret_cast<uint32_t*>(smem + L::SEEN);  // [2][kSeen][4]
   float* sums = reinterpret_cast<float*>(smem + L::SUMS);        // m and l of stream 1
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
@@ -341,12 +369,13 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
       mbar_init(&ready[i], 1);
       mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) mbar_init(&q_full[i], 4);
-    for (int i = 0; i < 4; ++i) {
-      mbar_init(&o_done[i], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 4);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&o_half[i], 1);
+      mbar_init(&o_full[i], 1);
     }
+    for (int i = 0; i < 4; ++i) mbar_init(&p_full[i], 4);
     mbar_init(sums_full, 4);
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -367,25 +396,34 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
   if (warp < kSoftmaxWarps) {
     const int stream = warp >> 2, row = (warp & 3) * 32 + lane, per = kSharedQueries / a.fan;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t col_s2 = tmem + lane_off + stream * 2 * kSharedKeys, col_o = tmem + lane_off + kColO + stream * DIM;
-    int step_at = 0, sums_at = 0;
-    // the product of the stream's n-th tile; that of the one two before is known to be done
-    auto wait_output = [&](int n) {
-      return mbar_wait(&o_done[stream * 2 + (n & 1)], (n >> 1) & 1, abort_flag, SJ_DEV_ATTN_WAIT);
-    };
+    const uint32_t col_s = tmem + lane_off + stream * kSharedKeys, col_o = tmem + lane_off + kColO + stream * DIM;
+    int tile_at = 0, piece_at = 0, sums_at = 0;
     bool ok = true;
+    // 16 bytes of a row of the stream's queries, which later serve to bring outputs into the order of memory
+    auto cell = [&](int of_row, int c) {
+      return reinterpret_cast<uint4*>(smem + L::Q + stream * L::QUERIES + (c >> 3) * L::QUERIES_HALF + of_row * 128 +
+                                      (((c & 7) ^ (of_row & 7)) << 4));
+    };
+    const int row0 = (warp & 3) * 32;
     while (ok && walk.next(p)) {
       const int steps = stream == 0 ? p.steps0 : p.steps1;
       const int at = (p.tile + (p.two ? stream : 0)) * per + row / a.fan;  // the query's row in its group
       const int r = p.g.first + at, head = p.h * a.fan + row % a.fan;
       const bool is = row < per * a.fan && at < p.g.rows;
-      if (stream == 0 || p.two) {  // this stream's queries
-        uint8_t* dst = smem + L::Q + stream * L::QUERIES + row * 128;
-        const uint4* src = reinterpret_cast<const uint4*>(a.q + static_cast<size_t>(is ? r : 0) * a.ldq + head * DIM);
+      if (stream == 0 || p.two) {  // this stream's queries, whole rows of a head at a time
+        constexpr int LANES = DIM / 8, ROWS = 32 / LANES;
+        const unsigned long long src = is ? static_cast<unsigned long long>(r) * a.ldq + head * DIM : ~0ull;
 #pragma unroll
-        for (int c = 0; c < DIM / 8; ++c) {
-          const uint4 x = is ? src[c] : make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(dst + (c >> 3) * L::QUERIES_HALF + (((c & 7) ^ (row & 7)) << 4)) = x;
+        for (int i0 = 0; i0 < 32 / ROWS; i0 += 8) {
+          uint4 x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const unsigned long long from = __shfl_sync(0xffffffffu, src, (i0 + i) * ROWS + lane / LANES);
+            x[i] = make_uint4(0, 0, 0, 0);
+            if (from != ~0ull) x[i] = *reinterpret_cast<const uint4*>(a.q + from + lane % LANES * 8);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) *cell(row0 + (i0 + i) * ROWS + lane / LANES, lane % LANES) = x[i];
         }
         fence_proxy_async_shared();
         __syncwarp();
@@ -393,85 +431,85 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
       }
       const bool idle = !__any_sync(0xffffffffu, is);  // a warp without queries leaves S as it is
       float m = -INFINITY, l = 0.f;
-      for (int step = 0; step < steps; ++step, ++step_at) {
-        const int buffer = step_at & 1;
-        const uint32_t col_s = col_s2 + buffer * kSharedKeys;
-        if (!mbar_wait(&s_full[stream * 2 + buffer], (step_at >> 1) & 1, abort_flag, SJ_DEV_ATTN_WAIT)) {
+      for (int step = 0; ok && step < steps; ++step, ++tile_at) {
+        if (!mbar_wait(&s_full[stream], tile_at & 1, abort_flag, SJ_DEV_ATTN_WAIT)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        if (idle) {
+        const uint2* masks = reinterpret_cast<const uint2*>(seen + (stream * kSeen + (tile_at & (kSeen - 1))) * 4);
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          if (!idle) {
+            const uint32_t col = col_s + half * kHalf;
+            uint32_t x[kHalf];
+#pragma unroll
+            for (int c = 0; c < kHalf / 32; ++c)
+              tmem_ld_32x32b_x32(col + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&x[c * 32]));
+            const uint2 valid = masks[half];
+            tmem_wait_ld();
+            if ((valid.x & valid.y) != 0xffffffffu) {
+#pragma unroll
+              for (int i = 0; i < kHalf; ++i)
+                if (!((i < 32 ? valid.x : valid.y) >> (i & 31) & 1)) x[i] = 0xff800000u;
+            }
+            float u[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < kHalf; i += 8)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                u[e] = max3(u[e], __uint_as_float(x[i + 2 * e]), __uint_as_float(x[i + 2 * e + 1]));
+            const float top = fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])) * a.scale;
+            const bool first = step == 0 && half == 0, grown = first || !(top <= m + kLazy);
+            if (__any_sync(0xffffffffu, grown && top > m)) {
+              const float next = fmaxf(m, top), f = m == next ? 1.f : shared_exp2(m - next);
+              l *= f;
+              m = next;
+              if (!first) {  // the output has the products of all tiles before, since S came after them, but maybe not this one's
+                if (half == 1 && !mbar_wait(&o_half[stream], tile_at & 1, abort_flag, SJ_DEV_ATTN_WAIT)) {
+                  ok = false;
+                  break;
+                }
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < DIM / 16; ++c) {
+                  uint32_t y[16];
+                  tmem_ld_32x32b_x16(col_o + c * 16, y);
+                  tmem_wait_ld();
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(f * __uint_as_float(y[i]));
+                  tmem_st_32x32b_x16(col_o + c * 16, y);
+                }
+              }
+            }
+            const float base = m == -INFINITY ? 0.f : m;
+            const uint64_t scale2 = pair2(a.scale, a.scale), base2 = pair2(-base, -base);
+            uint64_t part[2] = {0, 0};
+#pragma unroll
+            for (int c = 0; c < kHalf / 32; ++c) {
+              uint32_t y[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const int j = c * 32 + 2 * i;
+                const uint64_t d = fma2(pair2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), scale2, base2);
+                const uint64_t e = i % 8 < kByHand ? exp2_by_hand(d) : pair2(shared_exp2(low2(d)), shared_exp2(high2(d)));
+                part[i & 1] = add2(part[i & 1], e);
+                y[i] = pack_bf16x2(low2(e), high2(e));  // the product's operand; the sums take it unrounded
+              }
+              tmem_st_32x32b_x16(col + c * 16, y);
+            }
+            l += (low2(part[0]) + high2(part[0])) + (low2(part[1]) + high2(part[1]));
+            tmem_wait_st();
+          }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[stream * 2 + buffer]);
-          continue;
+          if (lane == 0) mbar_arrive(&p_full[stream * 2 + half]);
         }
-        uint32_t x[kSharedKeys];
-#pragma unroll
-        for (int c = 0; c < kSharedKeys / 32; ++c)
-          tmem_ld_32x32b_x32(col_s + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&x[c * 32]));
-        const uint2 valid = *reinterpret_cast<const uint2*>(seen + (stream * kSeen + (step_at & (kSeen - 1))) * 2);
-        tmem_wait_ld();
-        if ((valid.x & valid.y) != 0xffffffffu) {
-#pragma unroll
-          for (int i = 0; i < kSharedKeys; ++i)
-            if (!((i < 32 ? valid.x : valid.y) >> (i & 31) & 1)) x[i] = 0xff800000u;
-        }
-        float u[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int i = 0; i < kSharedKeys; i += 8)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            u[e] = max3(u[e], __uint_as_float(x[i + 2 * e]), __uint_as_float(x[i + 2 * e + 1]));
-        const float top = fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])) * a.scale;
-        const bool grown = step == 0 || !(top <= m + kLazy);
-        if (__any_sync(0xffffffffu, grown && top > m)) {
-          const float next = fmaxf(m, top), f = m == next ? 1.f : shared_exp2(m - next);
-          l *= f;
-          m = next;
-          if (step > 0) {  // the product of the tile before has to be in the output
-            if (!wait_output(step_at - 1)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < DIM / 16; ++c) {
-              uint32_t y[16];
-              tmem_ld_32x32b_x16(col_o + c * 16, y);
-              tmem_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(f * __uint_as_float(y[i]));
-              tmem_st_32x32b_x16(col_o + c * 16, y);
-            }
-          }
-        }
-        const float base = m == -INFINITY ? 0.f : m;
-        const uint64_t scale2 = pair2(a.scale, a.scale), base2 = pair2(-base, -base);
-        uint64_t part[2] = {0, 0};
-#pragma unroll
-        for (int c = 0; c < kSharedKeys / 32; ++c) {
-          uint32_t y[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int at = c * 32 + 2 * i;
-            const uint64_t d = fma2(pair2(__uint_as_float(x[at]), __uint_as_float(x[at + 1])), scale2, base2);
-            const float e0 = shared_exp2(low2(d)), e1 = shared_exp2(high2(d));
-            part[i & 1] = add2(part[i & 1], pair2(e0, e1));
-            y[i] = pack_bf16x2(e0, e1);  // the product's operand; the sums take it unrounded
-          }
-          tmem_st_32x32b_x16(col_s + c * 16, y);
-        }
-        l += (low2(part[0]) + high2(part[0])) + (low2(part[1]) + high2(part[1]));
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[stream * 2 + buffer]);
       }
       if (!ok) break;
       if (steps > 0) {
-        if (!wait_output(step_at - 1)) break;
+        if (!mbar_wait(&o_full[stream], piece_at & 1, abort_flag, SJ_DEV_ATTN_WAIT)) break;
+        ++piece_at;
         tc_fence_after();
       }
       if (!p.two && stream == 1) {  // stream 0 has the same queries, and joins the two
@@ -495,29 +533,42 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
         l = f * l + g * sums[kSharedQueries + row];
         m = top;
       }
+      if (idle) continue;
       const SharedParts& to = p.begins ? a.s.main : a.s.slots;
       const size_t query = p.begins ? p.g.main + (static_cast<size_t>(p.chunk) * p.g.rows + (is ? at : 0)) * a.hq + head
                                     : static_cast<size_t>(blockIdx.x) * (2 * kSharedQueries) +
                                           (p.two ? stream * kSharedQueries : 0) + row;
-      float* to_o = to.o + query * DIM;
+      const unsigned long long dst = is ? query * DIM : ~0ull;
+      // half of the dims at a time through the cells of this warp's rows, so that stores are of whole lines
 #pragma unroll
-      for (int c = 0; c < DIM / 16; ++c) {
-        uint32_t x[16], y[16];
-        tmem_ld_32x32b_x16(col_o + c * 16, x);
-        if (joined) tmem_ld_32x32b_x16(col_o + DIM + c * 16, y);
-        tmem_wait_ld();
-        if (joined) {
+      for (int c0 = 0; c0 < DIM; c0 += DIM / 2) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float u = f == 0.f ? 0.f : f * __uint_as_float(x[i]), w = g == 0.f ? 0.f : g * __uint_as_float(y[i]);
-            x[i] = __float_as_uint(u + w);
+        for (int c = 0; c < DIM / 32; ++c) {
+          uint32_t x[16], y[16];
+          tmem_ld_32x32b_x16(col_o + c0 + c * 16, x);
+          if (joined) tmem_ld_32x32b_x16(col_o + DIM + c0 + c * 16, y);
+          tmem_wait_ld();
+          if (joined) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float v = f == 0.f ? 0.f : f * __uint_as_float(x[i]), w = g == 0.f ? 0.f : g * __uint_as_float(y[i]);
+              x[i] = __float_as_uint(v + w);
+            }
           }
-        }
-        if (is) {
 #pragma unroll
-          for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<uint4*>(to_o + c * 16 + i) = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+          for (int i = 0; i < 4; ++i)
+            *cell(row, c * 4 + i) = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
         }
+        __syncwarp();
+        constexpr int LANES = DIM / 8, ROWS = 32 / LANES;
+#pragma unroll
+        for (int i = 0; i < 32 / ROWS; ++i) {
+          const int rr = i * ROWS + lane / LANES;
+          const unsigned long long there = __shfl_sync(0xffffffffu, dst, rr);
+          const uint4 x = *cell(row0 + rr, lane % LANES);
+          if (there != ~0ull) *reinterpret_cast<uint4*>(to.o + there + c0 + lane % LANES * 4) = x;
+        }
+        __syncwarp();
       }
       if (is) {
         to.m[query] = m;
@@ -537,10 +588,16 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
       };
       auto low = [](const uint8_t* at, uint32_t lead) { return ((smem_u32(at) >> 4) & 0x3fffu) | (lead >> 4) << 16; };
       const uint32_t q_low = low(smem + L::Q, 16), k_low = low(smem + L::RING, 16), v_low = low(smem + L::RING, L::HALF);
-      int slot = 0, turn = 0, q_at[2] = {0, 0}, s_at[2] = {0, 0}, p_at[2] = {0, 0};
+      int slot = 0, turn = 0, q_at[2] = {0, 0}, tile_at[2] = {0, 0};
       // After a wait that gave up the piece's products are of no use, but harmless, and its other waits give up at once.
       auto wait = [&](uint64_t* bar, uint32_t parity) {
         mbar_wait(bar, parity, abort_flag, SJ_DEV_ATTN_WAIT);
+        tc_fence_after();
+      };
+      // A look at a barrier whose answer is needed after the next products only, so that its latency is hidden.
+      auto peek = [&](uint64_t* bar, uint32_t parity) { return mbar_test_wait(bar, parity); };
+      auto settle = [&](bool done, uint64_t* bar, uint32_t parity) {
+        if (!done) mbar_wait(bar, parity, abort_flag, SJ_DEV_ATTN_WAIT);
         tc_fence_after();
       };
       auto wait_tile = [&]() { wait(&ready[slot], turn); };
@@ -551,95 +608,71 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
           turn ^= 1;
         }
       };
-      auto scores = [&](int stream, int queries) {  // S = Q K^T
-        const uint32_t q = q_low + queries * (L::QUERIES >> 4), k = k_low + slot * (L::SLOT >> 4);
-        const uint32_t to = tmem + (stream * 2 + (s_at[stream] & 1)) * kSharedKeys;
+      auto scores = [&](int stream, int queries, int of) {  // S = Q K^T
+        const uint32_t q = q_low + queries * (L::QUERIES >> 4), k = k_low + of * (L::SLOT >> 4);
 #pragma unroll
         for (int kk = 0; kk < DIM / 16; ++kk)
-          product_ss(is, to, desc(q, (kk >> 2) * L::QUERIES_HALF + (kk & 3) * 32), desc(k, (kk >> 2) * L::HALF + (kk & 3) * 32),
-                   kIdescS, kk > 0 ? 1u : 0u);
-        commit_products(is, &s_full[stream * 2 + (s_at[stream] & 1)]);
-        ++s_at[stream];
+          product_ss(is, tmem + stream * kSharedKeys, desc(q, (kk >> 2) * L::QUERIES_HALF + (kk & 3) * 32),
+                     desc(k, (kk >> 2) * L::HALF + (kk & 3) * 32), kIdescS, kk > 0 ? 1u : 0u);
+        commit_products(is, &s_full[stream]);
       };
-      auto wait_p = [&](int stream) { wait(&p_full[stream * 2 + (p_at[stream] & 1)], (p_at[stream] >> 1) & 1); };
-      auto outputs = [&](int stream, bool first) {  // O += P V
-        const uint32_t v = v_low + slot * (L::SLOT >> 4);
-        const uint32_t from = tmem + (stream * 2 + (p_at[stream] & 1)) * kSharedKeys;
+      auto outputs = [&](int stream, int half, int of, bool first) {  // O += P V
+        const uint32_t v = v_low + of * (L::SLOT >> 4) + half * (kHalf * 128 >> 4);
 #pragma unroll
-        for (int kk = 0; kk < kSharedKeys / 16; ++kk)
-          product_ts(is, tmem + kColO + stream * DIM, from + kk * 8, desc(v, kk * 2048), kIdescO, !first || kk > 0 ? 1u : 0u);
-        commit_products(is, &o_done[stream * 2 + (p_at[stream] & 1)]);
-        ++p_at[stream];
+        for (int kk = 0; kk < kHalf / 16; ++kk)
+          product_ts(is, tmem + kColO + stream * DIM, tmem + stream * kSharedKeys + half * kHalf + kk * 8,
+                     desc(v, kk * 2048), kIdescO, !first || kk > 0 ? 1u : 0u);
       };
       auto wait_q = [&](int stream) {
         wait(&q_full[stream], q_at[stream] & 1);
         ++q_at[stream];
       };
+      // A tile of a stream: both halves of P with the V at hand, then S of the next tile, whose K lies behind it.
+      auto tile = [&](int stream, int queries, bool first, bool more, bool last_user) {
+        const int v = slot, next = slot + 1 == L::STAGES ? 0 : slot + 1, next_turn = next == 0 ? turn ^ 1 : turn;
+        const uint32_t parity = tile_at[stream] & 1;
+        const bool value = peek(&ready[v], turn);
+        wait(&p_full[stream * 2], parity);
+        settle(value, &ready[v], turn);
+        outputs(stream, 0, v, first);
+        commit_products(is, &o_half[stream]);
+        const bool key = peek(&ready[next], next_turn);
+        wait(&p_full[stream * 2 + 1], parity);
+        outputs(stream, 1, v, false);
+        ++tile_at[stream];
+        if (last_user) release();
+        if (more) {
+          settle(key, &ready[next], next_turn);
+          scores(stream, queries, next);
+          if (last_user) release();
+        } else {
+          commit_products(is, &o_full[stream]);
+        }
+      };
       while (__shfl_sync(0xffffffffu, *abort_flag == 0 && walk.next(p) ? 1 : 0, 0)) {
         const int n0 = __shfl_sync(0xffffffffu, p.steps0, 0), n1 = __shfl_sync(0xffffffffu, p.steps1, 0);
+        const bool two = __shfl_sync(0xffffffffu, p.two ? 1 : 0, 0) != 0;
         wait_q(0);
-        if (__shfl_sync(0xffffffffu, p.two ? 1 : 0, 0)) {
+        wait_tile();
+        scores(0, 0, slot);
+        if (two) {
           wait_q(1);
-          for (int i = 0; i < min(2, n0); ++i) {
-            wait_tile();
-            scores(0, 0);
-            scores(1, 1);
-            release();
-          }
+          scores(1, 1, slot);
+          release();
           for (int i = 0; i < n0; ++i) {
-            // V of this tile, K of the one after the next, for both streams
-            const bool more = i + 2 < n0;
-            const int v_slot = slot, v_turn = turn, next = slot + 1 == L::STAGES ? 0 : slot + 1;
-            auto at_key = [&]() {
-              slot = next;
-              turn = next == 0 ? v_turn ^ 1 : v_turn;
-            };
-            auto at_value = [&]() {
-              slot = v_slot;
-              turn = v_turn;
-            };
-            wait_p(0);
-            wait_tile();
-            outputs(0, i == 0);
-            if (more) {
-              at_key();
-              wait_tile();
-              scores(0, 0);
-              at_value();
-            }
-            wait_p(1);
-            outputs(1, i == 0);
-            release();
-            if (more) {
-              scores(1, 1);
-              release();
-            }
+            tile(0, 0, i == 0, i + 1 < n0, false);
+            tile(1, 1, i == 0, i + 1 < n0, true);
           }
         } else {
-          for (int i = 0; i < min(2, n0); ++i) {
+          release();
+          if (n1 > 0) {
             wait_tile();
-            scores(0, 0);
-            release();
-            if (i >= n1) continue;
-            wait_tile();
-            scores(1, 0);
+            scores(1, 0, slot);
             release();
           }
           for (int i = 0; i < n0; ++i) {
-#pragma unroll
-            for (int stream = 0; stream < 2; ++stream) {
-              const int steps = stream == 0 ? n0 : n1;
-              if (i >= steps) continue;
-              wait_p(stream);
-              wait_tile();
-              outputs(stream, i == 0);
-              release();
-              if (i + 2 < steps) {
-                wait_tile();
-                scores(stream, 0);
-                release();
-              }
-            }
+            tile(0, 0, i == 0, i + 1 < n0, true);
+            if (i < n1) tile(1, 0, i == 0, i + 1 < n1, true);
           }
         }
       }
@@ -669,13 +702,16 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
     const __nv_bfloat16* from = of_k ? a.k : a.v;
     int slot = 0, turn = 0, seen_at[2] = {0, 0};
     bool ok = true;
-    struct At {  // this lane's key of a tile, its page in the block table and its row there, and the page
+    struct At {  // a key of a tile, its page in the block table and its row there, and the page
       int key, index, row, page;
+    };
+    struct Where {  // of this lane's two keys, in 16-byte pieces
+      uint32_t x, y;
     };
     auto look_up = [&](At& x) {
       x.page = x.key < p.g.p1 ? a.table[static_cast<size_t>(p.g.request) * a.ld_table + x.index] : 0;
     };
-    auto place = [&](const At& x) {  // where it lies, in 16-byte pieces
+    auto place = [&](const At& x) {
       if (x.key >= p.g.p1) return kNowhere;
       if (x.page < 0 || x.page >= a.pages) {
         record_error(SJ_DEV_BAD_INDEX);
@@ -683,36 +719,41 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
       }
       return static_cast<uint32_t>((x.page * a.page_stride + p.h * a.head_stride + x.row * a.token_stride) >> 3);
     };
-    auto mark = [&](int stream, uint32_t where) {
-      const uint32_t have = __ballot_sync(0xffffffffu, where != kNowhere);
-      if (lane == 0) seen[(stream * kSeen + (seen_at[stream] & (kSeen - 1))) * 2 + w] = have;
+    auto mark = [&](int stream, const Where& where) {
+      const uint32_t x = __ballot_sync(0xffffffffu, where.x != kNowhere), y = __ballot_sync(0xffffffffu, where.y != kNowhere);
+      if (lane == 0)
+        *reinterpret_cast<uint2*>(seen + (stream * kSeen + (seen_at[stream] & (kSeen - 1))) * 4 + 2 * w) = make_uint2(x, y);
       ++seen_at[stream];
     };
     constexpr int LANES = DIM / 8, ROWS = 32 / LANES;  // of a row, in one instruction
-    const uint32_t ring = smem_u32(smem + L::RING) + ((lane % LANES) >> 3) * L::HALF + (w * 32 + lane / LANES) * 128;
+    const uint32_t ring = smem_u32(smem + L::RING) + ((lane % LANES) >> 3) * L::HALF + (w * kHalf + lane / LANES) * 128;
     auto pass = [&]() {
       if (++slot == L::STAGES) {
         slot = 0;
         turn ^= 1;
       }
     };
-    auto fetch = [&](uint32_t where) {
+    auto fetch = [&](const Where& where) {
       if (!mbar_wait(&empty[slot], turn ^ 1, abort_flag, SJ_DEV_ATTN_WAIT)) ok = false;
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
       const uint32_t dst = ring + slot * L::SLOT;
       const __nv_bfloat16* src = from + (lane % LANES) * 8;
-      const bool all = __all_sync(0xffffffffu, where != kNowhere);
-      uint32_t at[32 / ROWS];
+      const bool all = __all_sync(0xffffffffu, where.x != kNowhere && where.y != kNowhere);
 #pragma unroll
-      for (int i = 0; i < 32 / ROWS; ++i) at[i] = __shfl_sync(0xffffffffu, where, i * ROWS + lane / LANES);
+      for (int i0 = 0; i0 < kHalf; i0 += 32) {
+        uint32_t at[32 / ROWS];
 #pragma unroll
-      for (int i = 0; i < 32 / ROWS; ++i) {
-        const uint32_t to = dst + i * ROWS * 128 + (((lane & 7) ^ ((i * ROWS + lane / LANES) & 7)) << 4);
-        if (all)
-          shared_copy16(to, src + static_cast<size_t>(at[i]) * 8);
-        else
-          shared_copy16(to, at[i] == kNowhere ? from : src + static_cast<size_t>(at[i]) * 8, at[i] != kNowhere);
+        for (int i = 0; i < 32 / ROWS; ++i)
+          at[i] = __shfl_sync(0xffffffffu, i0 == 0 ? where.x : where.y, i * ROWS + lane / LANES);
+#pragma unroll
+        for (int i = 0; i < 32 / ROWS; ++i) {
+          const uint32_t to = dst + (i0 + i * ROWS) * 128 + (((lane & 7) ^ ((i * ROWS + lane / LANES) & 7)) << 4);
+          if (all)
+            shared_copy16(to, src + static_cast<size_t>(at[i]) * 8);
+          else
+            shared_copy16(to, at[i] == kNowhere ? from : src + static_cast<size_t>(at[i]) * 8, at[i] != kNowhere);
+        }
       }
       // this thread's arrival, once its copies are in
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[slot])) : "memory");
@@ -720,29 +761,31 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
     };
     while (ok && walk.next(p)) {
       const int n0 = p.steps0, n1 = p.two ? 0 : p.steps1;
-      // of each stream: where the keys of the tile whose V comes next, and of the one after it, lie
-      uint32_t now[2] = {kNowhere, kNowhere}, after[2] = {kNowhere, kNowhere};
-      At next[2];
+      Where now[2];  // where the keys of the tile whose V comes next lie, of each stream
+      At next[2][2];
       const int ahead = p.two ? kSharedKeys : 2 * kSharedKeys, ahead_pages = ahead / a.page, ahead_rows = ahead % a.page;
 #pragma unroll
-      for (int stream = 0; stream < 2; ++stream) {
-        At& x = next[stream];
-        x.key = p.key(stream, 0) + w * 32 + lane;
+      for (int k = 0; k < 4; ++k) {
+        At& x = next[k / 2][k % 2];
+        x.key = p.key(k / 2, 0) + w * kHalf + k % 2 * 32 + lane;
         x.index = x.key / a.page;
         x.row = x.key - x.index * a.page;
         look_up(x);
       }
       auto keys = [&](int stream) {  // a tile of K; the next one's pages are looked up
-        At& x = next[stream];
-        const uint32_t where = place(x);
-        x.key += ahead;
-        x.index += ahead_pages;
-        x.row += ahead_rows;
-        if (x.row >= a.page) {
-          x.row -= a.page;
-          ++x.index;
+        const Where where{place(next[stream][0]), place(next[stream][1])};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          At& x = next[stream][k];
+          x.key += ahead;
+          x.index += ahead_pages;
+          x.row += ahead_rows;
+          if (x.row >= a.page) {
+            x.row -= a.page;
+            ++x.index;
+          }
+          look_up(x);
         }
-        look_up(x);
         if (of_k) {
           mark(stream, where);
           if (p.two) mark(1, where);
@@ -754,8 +797,6 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
       };
       now[0] = keys(0);
       if (ok && n1 > 0) now[1] = keys(1);
-      if (ok && n0 > 1) after[0] = keys(0);
-      if (ok && n1 > 1) after[1] = keys(1);
       for (int i = 0; i < n0 && ok; ++i) {
 #pragma unroll
         for (int stream = 0; stream < 2; ++stream) {
@@ -765,8 +806,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
             pass();
           else
             fetch(now[stream]);
-          now[stream] = after[stream];
-          if (ok && i + 2 < steps) after[stream] = keys(stream);
+          if (ok && i + 1 < steps) now[stream] = keys(stream);
         }
       }
     }

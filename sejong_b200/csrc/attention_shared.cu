@@ -12,6 +12,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <numeric>
 
 #include "attention_paged.cuh"
 #include "common.cuh"
@@ -21,12 +22,10 @@ namespace sj {
 
 namespace {
 constexpr int kSharedGroups = 1024;
-constexpr int kSoftmaxWarps = 8, kMmaWarp = 8, kFenceWarp = 9, kLoadWarp = 10;
-constexpr int kLoadWarps = 2;                // of K, and as many of V
-constexpr int kHalf = kSharedKeys / 2;       // keys of which a softmax thread has the scores at a time
-constexpr int kSharedThreads = 32 * (kLoadWarp + 2 * kLoadWarps);
+constexpr int kSoftmaxWarps = 8, kMmaWarp = 8, kLoadWarp = 9;  // two load warps: K and V
+constexpr int kHalf = kSharedKeys / 2;     // keys whose P is handed over at a time
+constexpr int kSharedThreads = 32 * (kLoadWarp + 2);
 constexpr int kSeen = 8;                   // tiles whose masks of valid keys are kept
-constexpr int kByHand = 0;                 // of 8 pairs of exponentials, those taken by the other pipes
 constexpr float kLazy = 8.f;               // a maximum may stand this far (of log2) below the true one
 constexpr uint32_t kColO = 256;            // TMEM columns: S of two streams (their P over them), then O
 constexpr uint32_t kTmemAll = 512;
@@ -152,10 +151,19 @@ struct SharedArgs {
   const int32_t* table;
   int64_t page_stride, head_stride, token_stride;
   int ldq, pages, page, ld_table, groups, hq, hk, fan;
+  int box;      // rows of a page that a tensor copy takes: page's and the tile's common divisor; 0: copies of 16 bytes only
   float scale;  // log2(e) / sqrt(dim)
   SharedSpans s;
 };
 
+// A box of a cache: 64 dims from x, rows from y, of head z and page w.
+SJ_DEVICE void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
 SJ_DEVICE float shared_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -181,30 +189,6 @@ SJ_DEVICE uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t y;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
   return y;
-}
-SJ_DEVICE uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t y;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
-  return y;
-}
-// 2^d of two d <= 8 or so, without the unit for exponentials: d = n + f with n the nearest whole number, 2^f by the
-// polynomial of degree 5 that is off by the least share over |f| <= 1/2 (fitted: 7.5e-8, 2^-22 with its roundings), 2^n
-// by its bits.  0 below 2^-126; a NaN stays one.
-SJ_DEVICE uint64_t exp2_by_hand(uint64_t d) {
-  float x0, x1;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x0) : "f"(low2(d)), "f"(-127.f));
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x1) : "f"(high2(d)), "f"(-127.f));
-  const uint64_t x = pair2(x0, x1), round = pair2(12582912.f, 12582912.f);  // 1.5 * 2^23: sums have no fraction bits
-  const uint64_t t = add2(x, round), n = add2(t, pair2(-12582912.f, -12582912.f));
-  const uint64_t f = fma2(n, pair2(-1.f, -1.f), x);
-  uint64_t y = pair2(0.001327647129073739f, 0.001327647129073739f);
-  y = fma2(y, f, pair2(0.009675540961325169f, 0.009675540961325169f));
-  y = fma2(y, f, pair2(0.05550713092088699f, 0.05550713092088699f));
-  y = fma2(y, f, pair2(0.24022120237350464f, 0.24022120237350464f));
-  y = fma2(y, f, pair2(0.6931469440460205f, 0.6931469440460205f));
-  y = fma2(y, f, pair2(1.0000001192092896f, 1.0000001192092896f));
-  const uint32_t n0 = static_cast<uint32_t>(t), n1 = static_cast<uint32_t>(t >> 32);
-  return mul2(y, pair2(__uint_as_float((n0 << 23) + 0x3f800000u), __uint_as_float((n1 << 23) + 0x3f800000u)));
 }
 // 16 bytes from global to shared memory; zeros when !is.
 SJ_DEVICE void shared_copy16(uint32_t dst, const __nv_bfloat16* src) {
@@ -330,31 +314,31 @@ struct SharedWalk {
   }
 };
 
-// 14 warps, one CTA an SM.  Two streams of tiles, so that the products of one run under the softmax of the other:
-//   warps 0-3, 4-7  softmax of streams 0 and 1: a thread for a query, which has the scores of half a tile in registers.  P
-//                   goes over S in bf16, where the product with V reads it, half a tile at a time.  The output is
+// 11 warps, one CTA an SM.  Two streams of tiles, so that the products of one run under the softmax of the other:
+//   warps 0-3, 4-7  softmax of streams 0 and 1: a thread for a query, which has a tile's scores in registers.  P goes
+//                   over S in bf16, where the product with V reads it, half a tile at a time.  The output is
 //                   rescaled only where a maximum has grown by more than 2^8: until then the sums are taken by the
 //                   old one.
 //   warp 8          issues S = Q K^T and O += P V of both streams.  S is 128 keys wide, since the tensor cores read Q
 //                   from shared memory for every product: one of 64 keys takes 48 cycles, one of 128 64.
-//   warp 9          one thread hands tiles that have come over to the asynchronous proxy, since a fence takes the thread
-//                   that issues the products 250 cycles
-//   warps 10-13     pages of K and of V into a ring of tiles (cp.async, since a page may have any number of rows; 128-byte
-//                   rows swizzled as the products read them), which arrive by themselves
+//   warps 9-10      pages of K and of V into a ring of tiles: tensor copies of the rows that a page and a tile have in
+//                   common, a lane for each; where those are fewer than the 8 of a swizzled group, in the last tile of a
+//                   group (rows past its end are zeros, whatever the cache holds there) and from a first key that is no
+//                   multiple of them, copies of 16 bytes
 template <int DIM>
-__global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const SharedArgs a) {
+__global__ void __launch_bounds__(kSharedThreads, 1)
+    attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                       const SharedArgs a) {
   using L = SharedLay<DIM>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
-  uint64_t* full = bars;                    // STAGES: copies are in
-  uint64_t* ready = full + L::STAGES;       // STAGES: and seen by the products
-  uint64_t* empty = ready + L::STAGES;      // STAGES
+  uint64_t* full = bars;                    // STAGES
+  uint64_t* empty = full + L::STAGES;       // STAGES
   uint64_t* q_full = empty + L::STAGES;     // 2
   uint64_t* s_full = q_full + 2;            // 2
   uint64_t* p_full = s_full + 2;            // 2 halves of each stream
-  uint64_t* o_half = p_full + 4;            // 2: the product of a tile's first half with V
-  uint64_t* o_full = o_half + 2;            // 2: all products of a piece
+  uint64_t* o_full = p_full + 4;            // 2: all products of a piece
   uint64_t* sums_full = o_full + 2;         // 1
   uint64_t* drain = sums_full + 1;          // 1
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
@@ -365,14 +349,12 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::STAGES; ++i) {
-      mbar_init(&full[i], kLoadWarps * 32);
-      mbar_init(&ready[i], 1);
+      mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 4);
       mbar_init(&s_full[i], 1);
-      mbar_init(&o_half[i], 1);
       mbar_init(&o_full[i], 1);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&p_full[i], 4);
@@ -380,6 +362,10 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbarrier_init();
+    if (a.box > 0) {
+      tma_prefetch_map(&map_k);
+      tma_prefetch_map(&map_v);
+    }
   }
   if (warp == kMmaWarp) {
     tmem_alloc(tmem_slot, kTmemAll);
@@ -437,73 +423,71 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
           break;
         }
         tc_fence_after();
-        const uint2* masks = reinterpret_cast<const uint2*>(seen + (stream * kSeen + (tile_at & (kSeen - 1))) * 4);
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-          if (!idle) {
-            const uint32_t col = col_s + half * kHalf;
-            uint32_t x[kHalf];
+        if (!idle) {
+          uint32_t x[kSharedKeys];
 #pragma unroll
-            for (int c = 0; c < kHalf / 32; ++c)
-              tmem_ld_32x32b_x32(col + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&x[c * 32]));
-            const uint2 valid = masks[half];
-            tmem_wait_ld();
-            if ((valid.x & valid.y) != 0xffffffffu) {
+          for (int c = 0; c < kSharedKeys / 32; ++c)
+            tmem_ld_32x32b_x32(col_s + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&x[c * 32]));
+          const uint4 valid = *reinterpret_cast<const uint4*>(seen + (stream * kSeen + (tile_at & (kSeen - 1))) * 4);
+          tmem_wait_ld();
+          if ((valid.x & valid.y & valid.z & valid.w) != 0xffffffffu) {
 #pragma unroll
-              for (int i = 0; i < kHalf; ++i)
-                if (!((i < 32 ? valid.x : valid.y) >> (i & 31) & 1)) x[i] = 0xff800000u;
+            for (int i = 0; i < kSharedKeys; ++i) {
+              const uint32_t word = i < 32 ? valid.x : i < 64 ? valid.y : i < 96 ? valid.z : valid.w;
+              if (!(word >> (i & 31) & 1)) x[i] = 0xff800000u;
             }
-            float u[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int i = 0; i < kHalf; i += 8)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                u[e] = max3(u[e], __uint_as_float(x[i + 2 * e]), __uint_as_float(x[i + 2 * e + 1]));
-            const float top = fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])) * a.scale;
-            const bool first = step == 0 && half == 0, grown = first || !(top <= m + kLazy);
-            if (__any_sync(0xffffffffu, grown && top > m)) {
-              const float next = fmaxf(m, top), f = m == next ? 1.f : shared_exp2(m - next);
-              l *= f;
-              m = next;
-              if (!first) {  // the output has the products of all tiles before, since S came after them, but maybe not this one's
-                if (half == 1 && !mbar_wait(&o_half[stream], tile_at & 1, abort_flag, SJ_DEV_ATTN_WAIT)) {
-                  ok = false;
-                  break;
-                }
-                tc_fence_after();
-#pragma unroll
-                for (int c = 0; c < DIM / 16; ++c) {
-                  uint32_t y[16];
-                  tmem_ld_32x32b_x16(col_o + c * 16, y);
-                  tmem_wait_ld();
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(f * __uint_as_float(y[i]));
-                  tmem_st_32x32b_x16(col_o + c * 16, y);
-                }
-              }
-            }
-            const float base = m == -INFINITY ? 0.f : m;
-            const uint64_t scale2 = pair2(a.scale, a.scale), base2 = pair2(-base, -base);
-            uint64_t part[2] = {0, 0};
-#pragma unroll
-            for (int c = 0; c < kHalf / 32; ++c) {
-              uint32_t y[16];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const int j = c * 32 + 2 * i;
-                const uint64_t d = fma2(pair2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), scale2, base2);
-                const uint64_t e = i % 8 < kByHand ? exp2_by_hand(d) : pair2(shared_exp2(low2(d)), shared_exp2(high2(d)));
-                part[i & 1] = add2(part[i & 1], e);
-                y[i] = pack_bf16x2(low2(e), high2(e));  // the product's operand; the sums take it unrounded
-              }
-              tmem_st_32x32b_x16(col + c * 16, y);
-            }
-            l += (low2(part[0]) + high2(part[0])) + (low2(part[1]) + high2(part[1]));
-            tmem_wait_st();
           }
+          float u[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < kSharedKeys; i += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              u[e] = max3(u[e], __uint_as_float(x[i + 2 * e]), __uint_as_float(x[i + 2 * e + 1]));
+          const float top = fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])) * a.scale;
+          const bool grown = step == 0 || !(top <= m + kLazy);
+          if (__any_sync(0xffffffffu, grown && top > m)) {
+            const float next = fmaxf(m, top), f = m == next ? 1.f : shared_exp2(m - next);
+            l *= f;
+            m = next;
+            if (step > 0) {  // the output has the products of all tiles before, since S came after them
+#pragma unroll 1
+              for (int c = 0; c < DIM / 16; ++c) {
+                uint32_t y[16];
+                tmem_ld_32x32b_x16(col_o + c * 16, y);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(f * __uint_as_float(y[i]));
+                tmem_st_32x32b_x16(col_o + c * 16, y);
+              }
+            }
+          }
+          const float base = m == -INFINITY ? 0.f : m;
+          const uint64_t scale2 = pair2(a.scale, a.scale), base2 = pair2(-base, -base);
+          uint64_t part[2] = {0, 0};
+#pragma unroll
+          for (int c = 0; c < kSharedKeys / 32; ++c) {
+            uint32_t y[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int j = c * 32 + 2 * i;
+              const uint64_t d = fma2(pair2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), scale2, base2);
+              const float e0 = shared_exp2(low2(d)), e1 = shared_exp2(high2(d));
+              part[i & 1] = add2(part[i & 1], pair2(e0, e1));
+              y[i] = pack_bf16x2(e0, e1);  // the product's operand; the sums take it unrounded
+            }
+            tmem_st_32x32b_x16(col_s + c * 16, y);
+            if (c == kSharedKeys / 64 - 1 || c == kSharedKeys / 32 - 1) {  // half of P is there
+              tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&p_full[stream * 2 + (c == kSharedKeys / 32 - 1 ? 1 : 0)]);
+            }
+          }
+          l += (low2(part[0]) + high2(part[0])) + (low2(part[1]) + high2(part[1]));
+        } else {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[stream * 2 + half]);
+          if (lane < 2) mbar_arrive(&p_full[stream * 2 + lane]);
         }
       }
       if (!ok) break;
@@ -600,7 +584,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
         if (!done) mbar_wait(bar, parity, abort_flag, SJ_DEV_ATTN_WAIT);
         tc_fence_after();
       };
-      auto wait_tile = [&]() { wait(&ready[slot], turn); };
+      auto wait_tile = [&]() { wait(&full[slot], turn); };
       auto release = [&]() {  // the tile at hand is done with when the products so far are
         commit_products(is, &empty[slot]);
         if (++slot == L::STAGES) {
@@ -620,7 +604,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
         const uint32_t v = v_low + of * (L::SLOT >> 4) + half * (kHalf * 128 >> 4);
 #pragma unroll
         for (int kk = 0; kk < kHalf / 16; ++kk)
-          product_ts(is, tmem + kColO + stream * DIM, tmem + stream * kSharedKeys + half * kHalf + kk * 8,
+          product_ts(is, tmem + kColO + stream * DIM, tmem + stream * kSharedKeys + half * (kHalf / 2) + kk * 8,
                      desc(v, kk * 2048), kIdescO, !first || kk > 0 ? 1u : 0u);
       };
       auto wait_q = [&](int stream) {
@@ -631,18 +615,17 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
       auto tile = [&](int stream, int queries, bool first, bool more, bool last_user) {
         const int v = slot, next = slot + 1 == L::STAGES ? 0 : slot + 1, next_turn = next == 0 ? turn ^ 1 : turn;
         const uint32_t parity = tile_at[stream] & 1;
-        const bool value = peek(&ready[v], turn);
+        const bool value = peek(&full[v], turn);
         wait(&p_full[stream * 2], parity);
-        settle(value, &ready[v], turn);
+        settle(value, &full[v], turn);
         outputs(stream, 0, v, first);
-        commit_products(is, &o_half[stream]);
-        const bool key = peek(&ready[next], next_turn);
+        const bool key = peek(&full[next], next_turn);
         wait(&p_full[stream * 2 + 1], parity);
         outputs(stream, 1, v, false);
         ++tile_at[stream];
         if (last_user) release();
         if (more) {
-          settle(key, &ready[next], next_turn);
+          settle(key, &full[next], next_turn);
           scores(stream, queries, next);
           if (last_user) release();
         } else {
@@ -679,138 +662,125 @@ __global__ void __launch_bounds__(kSharedThreads, 1) attn_shared_kernel(const Sh
       commit_products(is, drain);
       mbar_wait(drain, 0, nullptr, SJ_DEV_ATTN_WAIT);
     }
-  } else if (warp == kFenceWarp) {
-    if (lane == 0) {
-      int slot = 0, turn = 0;
-      bool ok = true;
-      while (ok && walk.next(p)) {
-        const int tiles = 2 * (p.two ? p.steps0 : p.steps0 + p.steps1);
-        for (int i = 0; i < tiles && ok; ++i) {
-          ok = mbar_wait(&full[slot], turn, abort_flag, SJ_DEV_ATTN_WAIT);
-          fence_proxy_async_shared();  // cp.async wrote by the generic proxy
-          if (ok) mbar_arrive(&ready[slot]);
-          if (++slot == L::STAGES) {
-            slot = 0;
-            turn ^= 1;
-          }
-        }
-      }
-    }
   } else {
-    const int w = (warp - kLoadWarp) % kLoadWarps;
-    const bool of_k = warp < kLoadWarp + kLoadWarps;
+    // both warps follow the order of all tiles; one fetches those of K, the other those of V
+    const bool of_k = warp == kLoadWarp;
     const __nv_bfloat16* from = of_k ? a.k : a.v;
+    const CUtensorMap* map = of_k ? &map_k : &map_v;
     int slot = 0, turn = 0, seen_at[2] = {0, 0};
     bool ok = true;
-    struct At {  // a key of a tile, its page in the block table and its row there, and the page
-      int key, index, row, page;
-    };
-    struct Where {  // of this lane's two keys, in 16-byte pieces
-      uint32_t x, y;
-    };
-    auto look_up = [&](At& x) {
-      x.page = x.key < p.g.p1 ? a.table[static_cast<size_t>(p.g.request) * a.ld_table + x.index] : 0;
-    };
-    auto place = [&](const At& x) {
-      if (x.key >= p.g.p1) return kNowhere;
-      if (x.page < 0 || x.page >= a.pages) {
-        record_error(SJ_DEV_BAD_INDEX);
-        return kNowhere;
-      }
-      return static_cast<uint32_t>((x.page * a.page_stride + p.h * a.head_stride + x.row * a.token_stride) >> 3);
-    };
-    auto mark = [&](int stream, const Where& where) {
-      const uint32_t x = __ballot_sync(0xffffffffu, where.x != kNowhere), y = __ballot_sync(0xffffffffu, where.y != kNowhere);
-      if (lane == 0)
-        *reinterpret_cast<uint2*>(seen + (stream * kSeen + (seen_at[stream] & (kSeen - 1))) * 4 + 2 * w) = make_uint2(x, y);
-      ++seen_at[stream];
-    };
-    constexpr int LANES = DIM / 8, ROWS = 32 / LANES;  // of a row, in one instruction
-    const uint32_t ring = smem_u32(smem + L::RING) + ((lane % LANES) >> 3) * L::HALF + (w * kHalf + lane / LANES) * 128;
-    auto pass = [&]() {
+    uint32_t fetched = 0;  // of the last tiles, those that this warp has asked for
+    auto pass = [&](uint32_t mine) {
+      fetched = fetched << 1 | mine;
       if (++slot == L::STAGES) {
         slot = 0;
         turn ^= 1;
       }
     };
-    auto fetch = [&](const Where& where) {
+    auto place = [&](int key) {  // where a key lies, in 16-byte pieces
+      if (key >= p.g.p1) return kNowhere;
+      const int index = key / a.page, page = a.table[static_cast<size_t>(p.g.request) * a.ld_table + index];
+      if (page < 0 || page >= a.pages) {
+        record_error(SJ_DEV_BAD_INDEX);
+        return kNowhere;
+      }
+      return static_cast<uint32_t>(
+          (page * a.page_stride + p.h * a.head_stride + (key - index * a.page) * a.token_stride) >> 3);
+    };
+    struct Box {  // this lane's of a tile: its page and the first row there
+      int page, row;
+    };
+    const int boxes = a.box > 0 ? kSharedKeys / a.box : 0;
+    auto look_up = [&](int key) {
+      Box x{0, 0};
+      key += lane * a.box;
+      if (lane < boxes && key < p.g.p1) {
+        const int index = key / a.page;
+        x.page = a.table[static_cast<size_t>(p.g.request) * a.ld_table + index];
+        x.row = key - index * a.page;
+      }
+      return x;
+    };
+    auto mark = [&](int stream, int word, uint32_t have) {
+      if (lane == 0) seen[(stream * kSeen + (seen_at[stream] & (kSeen - 1))) * 4 + word] = have;
+    };
+    auto fetch = [&](int stream, int key, const Box& x) {
       if (!mbar_wait(&empty[slot], turn ^ 1, abort_flag, SJ_DEV_ATTN_WAIT)) ok = false;
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
-      const uint32_t dst = ring + slot * L::SLOT;
-      const __nv_bfloat16* src = from + (lane % LANES) * 8;
-      const bool all = __all_sync(0xffffffffu, where.x != kNowhere && where.y != kNowhere);
+      const uint32_t dst = smem_u32(smem + L::RING + slot * L::SLOT);
+      const bool boxed = boxes > 0 && key % a.box == 0 && key + kSharedKeys <= p.g.p1;
+      if (boxed && __all_sync(0xffffffffu, lane >= boxes || (x.page >= 0 && x.page < a.pages))) {
+        if (of_k) {
 #pragma unroll
-      for (int i0 = 0; i0 < kHalf; i0 += 32) {
-        uint32_t at[32 / ROWS];
-#pragma unroll
-        for (int i = 0; i < 32 / ROWS; ++i)
-          at[i] = __shfl_sync(0xffffffffu, i0 == 0 ? where.x : where.y, i * ROWS + lane / LANES);
-#pragma unroll
-        for (int i = 0; i < 32 / ROWS; ++i) {
-          const uint32_t to = dst + (i0 + i * ROWS) * 128 + (((lane & 7) ^ ((i * ROWS + lane / LANES) & 7)) << 4);
-          if (all)
-            shared_copy16(to, src + static_cast<size_t>(at[i]) * 8);
-          else
-            shared_copy16(to, at[i] == kNowhere ? from : src + static_cast<size_t>(at[i]) * 8, at[i] != kNowhere);
+          for (int i = 0; i < 4; ++i) {
+            mark(stream, i, 0xffffffffu);
+            if (p.two) mark(1, i, 0xffffffffu);
+          }
         }
+        if (lane == 0) mbar_arrive_expect_tx(&full[slot], L::SLOT);
+        __syncwarp();
+        if (lane < boxes) {
+#pragma unroll
+          for (int i = 0; i < DIM / 64; ++i)
+            tma_load_4d(dst + i * L::HALF + lane * a.box * 128, map, &full[slot], i * 64, x.row, p.h, x.page);
+        }
+      } else {
+        constexpr int LANES = DIM / 8, ROWS = 32 / LANES;  // of a row, in one instruction
+#pragma unroll 1
+        for (int i0 = 0; i0 < kSharedKeys; i0 += 32) {
+          const uint32_t where = place(key + i0 + lane), have = __ballot_sync(0xffffffffu, where != kNowhere);
+          if (of_k) {
+            mark(stream, i0 >> 5, have);
+            if (p.two) mark(1, i0 >> 5, have);
+          }
+#pragma unroll
+          for (int i = 0; i < 32; i += ROWS) {
+            const int row = i + lane / LANES;
+            const uint32_t at = __shfl_sync(0xffffffffu, where, row);
+            shared_copy16(dst + ((lane % LANES) >> 3) * L::HALF + (i0 + row) * 128 + (((lane & 7) ^ (row & 7)) << 4),
+                          from + (at == kNowhere ? 0 : static_cast<size_t>(at) * 8 + lane % LANES * 8), at != kNowhere);
+          }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[slot]);
       }
-      // this thread's arrival, once its copies are in
-      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[slot])) : "memory");
-      pass();
+      ++seen_at[stream];
+      if (p.two) ++seen_at[1];
+      pass(1);
     };
     while (ok && walk.next(p)) {
       const int n0 = p.steps0, n1 = p.two ? 0 : p.steps1;
-      Where now[2];  // where the keys of the tile whose V comes next lie, of each stream
-      At next[2][2];
-      const int ahead = p.two ? kSharedKeys : 2 * kSharedKeys, ahead_pages = ahead / a.page, ahead_rows = ahead % a.page;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        At& x = next[k / 2][k % 2];
-        x.key = p.key(k / 2, 0) + w * kHalf + k % 2 * 32 + lane;
-        x.index = x.key / a.page;
-        x.row = x.key - x.index * a.page;
-        look_up(x);
-      }
-      auto keys = [&](int stream) {  // a tile of K; the next one's pages are looked up
-        const Where where{place(next[stream][0]), place(next[stream][1])};
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          At& x = next[stream][k];
-          x.key += ahead;
-          x.index += ahead_pages;
-          x.row += ahead_rows;
-          if (x.row >= a.page) {
-            x.row -= a.page;
-            ++x.index;
-          }
-          look_up(x);
+      Box next[2];  // of the next tile of each stream that this warp fetches
+      next[0] = look_up(p.key(0, 0));
+      if (n1 > 0) next[1] = look_up(p.key(1, 0));
+      auto tile = [&](int stream, int step, bool mine) {
+        if (!mine) {
+          pass(0);
+          return;
         }
-        if (of_k) {
-          mark(stream, where);
-          if (p.two) mark(1, where);
-          fetch(where);
-        } else {
-          pass();
-        }
-        return where;
+        const Box x = next[stream];
+        next[stream] = look_up(p.key(stream, step + 1));  // past the piece's end as well, where it is not used
+        fetch(stream, p.key(stream, step), x);
       };
-      now[0] = keys(0);
-      if (ok && n1 > 0) now[1] = keys(1);
+      tile(0, 0, of_k);
+      if (ok && n1 > 0) tile(1, 0, of_k);
       for (int i = 0; i < n0 && ok; ++i) {
-#pragma unroll
-        for (int stream = 0; stream < 2; ++stream) {
-          const int steps = stream == 0 ? n0 : n1;
-          if (i >= steps || !ok) continue;
-          if (of_k)
-            pass();
-          else
-            fetch(now[stream]);
-          if (ok && i + 1 < steps) now[stream] = keys(stream);
-        }
+        tile(0, i, !of_k);
+        if (ok && i + 1 < n0) tile(0, i + 1, of_k);
+        if (ok && i < n1) tile(1, i, !of_k);
+        if (ok && i + 1 < n1) tile(1, i + 1, of_k);
       }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");  // nothing lands after the CTA has gone
+    // nothing lands after the CTA has gone: every tile that was asked for has been waited for by the products, unless a
+    // wait gave up
+    for (int i = 0; *abort_flag != 0 && i < L::STAGES; ++i, fetched >>= 1) {
+      turn ^= slot == 0 ? 1 : 0;
+      slot = slot == 0 ? L::STAGES - 1 : slot - 1;
+      if (fetched & 1) mbar_wait(&full[slot], turn, nullptr, SJ_DEV_ATTN_WAIT);
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -926,12 +896,25 @@ size_t shared_layout(SharedSpans* s, char* at, int rows, int groups, int hq, int
 }
 
 template <int DIM>
-int shared_pass(const SharedArgs& a, cudaStream_t stream) {
+int shared_pass(SharedArgs a, cudaStream_t stream) {
   static KernelAttrOnce once;
   const int rc = ensure_max_smem(once, reinterpret_cast<const void*>(attn_shared_kernel<DIM>), SharedLay<DIM>::SMEM,
                                  "sj_attn_paged_shared: shared memory");
   if (rc != SJ_OK) return rc;
-  launch(attn_shared_kernel<DIM>, a.s.ctas, kSharedThreads, SharedLay<DIM>::SMEM, stream, a);
+  CUtensorMap maps[2] = {};
+  if (a.box > 0) {
+    const uint64_t dims[4] = {DIM, static_cast<uint64_t>(a.page), static_cast<uint64_t>(a.hk),
+                              static_cast<uint64_t>(a.pages)};
+    const uint64_t strides[3] = {static_cast<uint64_t>(a.token_stride) * 2, static_cast<uint64_t>(a.head_stride) * 2,
+                                 static_cast<uint64_t>(a.page_stride) * 2};
+    const uint32_t box[4] = {64, static_cast<uint32_t>(a.box), 1, 1};
+    for (int i = 0; i < 2; ++i) {
+      const int map_rc = tensor_map(&maps[i], i == 0 ? a.k : a.v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, dims, strides, box,
+                                    CU_TENSOR_MAP_SWIZZLE_128B);
+      if (map_rc != SJ_OK) a.box = 0;  // copies of 16 bytes take any strides
+    }
+  }
+  launch(attn_shared_kernel<DIM>, a.s.ctas, kSharedThreads, SharedLay<DIM>::SMEM, stream, maps[0], maps[1], a);
   SJ_LAUNCH_CHECK("attn_shared");
   return SJ_OK;
 }
@@ -976,8 +959,13 @@ extern "C" int sj_attn_paged_shared(const void* q, int ldq, const void* k_cache,
   const SpansArgs sa{request, position, group, rows, groups, requests, page, ld_table, window, hq, hq / hk, hk, 2, spans};
   launch(shared_spans_kernel, 1, 1024, 0, s, sa);
   SJ_LAUNCH_CHECK("shared_spans");
+  // Tensor copies of boxes that pages and tiles have in common, of whole swizzled groups of 8 rows; strides that a map
+  // takes (not 0, below 2^40 bytes: a head or page that no index reaches may have any).
+  const int divisor = std::gcd(page, kSharedKeys);
+  auto fits = [](int64_t stride) { return stride > 0 && stride < int64_t{1} << 39; };
+  const int box = divisor % 8 == 0 && fits(page_stride) && fits(head_stride) && fits(token_stride) ? divisor : 0;
   const SharedArgs ta{a.q, a.k, a.v, block_table, page_stride, head_stride, token_stride, ldq, pages, page, ld_table,
-                      groups, hq, hk, hq / hk, 1.4426950408889634f / sqrtf(static_cast<float>(head_dim)), spans};
+                      groups, hq, hk, hq / hk, box, 1.4426950408889634f / sqrtf(static_cast<float>(head_dim)), spans};
   rc = head_dim == 64 ? shared_pass<64>(ta, s) : shared_pass<128>(ta, s);
   if (rc == SJ_OK) rc = attn_paged_rows(a, &spans, head_dim, s);
   if (rc != SJ_OK) return rc;

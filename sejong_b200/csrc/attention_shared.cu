@@ -315,8 +315,8 @@ struct SharedWalk {
 };
 
 // 11 warps, one CTA an SM.  Two streams of tiles, so that the products of one run under the softmax of the other:
-//   warps 0-3, 4-7  softmax of streams 0 and 1: a thread for a query, which has a tile's scores in registers.  P goes
-//                   over S in bf16, where the product with V reads it, half a tile at a time.  The output is
+//   warps 0-3, 4-7  softmax of streams 0 and 1: a thread for a query, which has the scores of half a tile in registers.  P
+//                   goes over S in bf16, where the product with V reads it.  The output is
 //                   rescaled only where a maximum has grown by more than 2^8: until then the sums are taken by the
 //                   old one.
 //   warp 8          issues S = Q K^T and O += P V of both streams.  S is 128 keys wide, since the tensor cores read Q
@@ -338,7 +338,8 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
   uint64_t* q_full = empty + L::STAGES;     // 2
   uint64_t* s_full = q_full + 2;            // 2
   uint64_t* p_full = s_full + 2;            // 2 halves of each stream
-  uint64_t* o_full = p_full + 4;            // 2: all products of a piece
+  uint64_t* o_half = p_full + 4;            // 2: the product of a tile's first half with V
+  uint64_t* o_full = o_half + 2;            // 2: all products of a piece
   uint64_t* sums_full = o_full + 2;         // 1
   uint64_t* drain = sums_full + 1;          // 1
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
@@ -355,6 +356,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 4);
       mbar_init(&s_full[i], 1);
+      mbar_init(&o_half[i], 1);
       mbar_init(&o_full[i], 1);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&p_full[i], 4);
@@ -423,72 +425,77 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
           break;
         }
         tc_fence_after();
-        if (!idle) {
-          uint32_t x[kSharedKeys];
-#pragma unroll
-          for (int c = 0; c < kSharedKeys / 32; ++c)
-            tmem_ld_32x32b_x32(col_s + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&x[c * 32]));
-          const uint4 valid = *reinterpret_cast<const uint4*>(seen + (stream * kSeen + (tile_at & (kSeen - 1))) * 4);
-          tmem_wait_ld();
-          if ((valid.x & valid.y & valid.z & valid.w) != 0xffffffffu) {
-#pragma unroll
-            for (int i = 0; i < kSharedKeys; ++i) {
-              const uint32_t word = i < 32 ? valid.x : i < 64 ? valid.y : i < 96 ? valid.z : valid.w;
-              if (!(word >> (i & 31) & 1)) x[i] = 0xff800000u;
-            }
-          }
-          float u[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int i = 0; i < kSharedKeys; i += 8)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              u[e] = max3(u[e], __uint_as_float(x[i + 2 * e]), __uint_as_float(x[i + 2 * e + 1]));
-          const float top = fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])) * a.scale;
-          const bool grown = step == 0 || !(top <= m + kLazy);
-          if (__any_sync(0xffffffffu, grown && top > m)) {
-            const float next = fmaxf(m, top), f = m == next ? 1.f : shared_exp2(m - next);
-            l *= f;
-            m = next;
-            if (step > 0) {  // the output has the products of all tiles before, since S came after them
+        const uint2* masks = reinterpret_cast<const uint2*>(seen + (stream * kSeen + (tile_at & (kSeen - 1))) * 4);
 #pragma unroll 1
-              for (int c = 0; c < DIM / 16; ++c) {
-                uint32_t y[16];
-                tmem_ld_32x32b_x16(col_o + c * 16, y);
-                tmem_wait_ld();
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t col = col_s + half * kHalf;
+          const uint2 valid = masks[half];
+          // The exponentials are taken by the maximum so far while the new one is looked for; where that stands too far
+          // above it, which is rare after the first tile, they are taken again.
+          bool first = step == 0 && half == 0;
+          while (!idle) {
+            uint32_t x[kHalf], y[kHalf / 2];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(f * __uint_as_float(y[i]));
-                tmem_st_32x32b_x16(col_o + c * 16, y);
-              }
+            for (int c = 0; c < kHalf / 32; ++c)
+              tmem_ld_32x32b_x32(col + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&x[c * 32]));
+            const float base = m == -INFINITY ? 0.f : m;
+            const uint64_t scale2 = pair2(a.scale, a.scale), base2 = pair2(-base, -base);
+            uint64_t part[2] = {0, 0};
+            float u[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            tmem_wait_ld();
+            if ((valid.x & valid.y) != 0xffffffffu) {
+#pragma unroll
+              for (int i = 0; i < kHalf; ++i)
+                if (!((i < 32 ? valid.x : valid.y) >> (i & 31) & 1)) x[i] = 0xff800000u;
             }
-          }
-          const float base = m == -INFINITY ? 0.f : m;
-          const uint64_t scale2 = pair2(a.scale, a.scale), base2 = pair2(-base, -base);
-          uint64_t part[2] = {0, 0};
 #pragma unroll
-          for (int c = 0; c < kSharedKeys / 32; ++c) {
-            uint32_t y[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int j = c * 32 + 2 * i;
-              const uint64_t d = fma2(pair2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), scale2, base2);
+            for (int i = 0; i < kHalf / 2; ++i) {
+              const float x0 = __uint_as_float(x[2 * i]), x1 = __uint_as_float(x[2 * i + 1]);
+              const uint64_t d = fma2(pair2(x0, x1), scale2, base2);
               const float e0 = shared_exp2(low2(d)), e1 = shared_exp2(high2(d));
+              u[i & 3] = max3(u[i & 3], x0, x1);
               part[i & 1] = add2(part[i & 1], pair2(e0, e1));
               y[i] = pack_bf16x2(e0, e1);  // the product's operand; the sums take it unrounded
             }
-            tmem_st_32x32b_x16(col_s + c * 16, y);
-            if (c == kSharedKeys / 64 - 1 || c == kSharedKeys / 32 - 1) {  // half of P is there
+            const float top = fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])) * a.scale;
+            const bool grown = first || !(top <= m + kLazy);
+            if (!__any_sync(0xffffffffu, grown && top > m)) {
+              l += (low2(part[0]) + high2(part[0])) + (low2(part[1]) + high2(part[1]));
+#pragma unroll
+              for (int c = 0; c < kHalf / 32; ++c)
+                tmem_st_32x32b_x16(col + c * 16, *reinterpret_cast<uint32_t(*)[16]>(&y[c * 16]));
               tmem_wait_st();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&p_full[stream * 2 + (c == kSharedKeys / 32 - 1 ? 1 : 0)]);
+              break;
             }
+            const float next = fmaxf(m, top), f = m == next ? 1.f : shared_exp2(m - next);
+            l *= f;
+            m = next;
+            if (step > 0 || half > 0) {
+              // the output has the products of all tiles before, since S came after them, but maybe not this one's
+              if (half == 1 && !mbar_wait(&o_half[stream], tile_at & 1, abort_flag, SJ_DEV_ATTN_WAIT)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+#pragma unroll 1
+              for (int c = 0; c < DIM / 16; ++c) {
+                uint32_t z[16];
+                tmem_ld_32x32b_x16(col_o + c * 16, z);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) z[i] = __float_as_uint(f * __uint_as_float(z[i]));
+                tmem_st_32x32b_x16(col_o + c * 16, z);
+              }
+              tmem_wait_st();
+            }
+            first = false;
           }
-          l += (low2(part[0]) + high2(part[0])) + (low2(part[1]) + high2(part[1]));
-        } else {
+          if (!ok) break;
           tc_fence_before();
           __syncwarp();
-          if (lane < 2) mbar_arrive(&p_full[stream * 2 + lane]);
+          if (lane == 0) mbar_arrive(&p_full[stream * 2 + half]);
         }
+        if (!ok) break;
       }
       if (!ok) break;
       if (steps > 0) {
@@ -604,7 +611,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
         const uint32_t v = v_low + of * (L::SLOT >> 4) + half * (kHalf * 128 >> 4);
 #pragma unroll
         for (int kk = 0; kk < kHalf / 16; ++kk)
-          product_ts(is, tmem + kColO + stream * DIM, tmem + stream * kSharedKeys + half * (kHalf / 2) + kk * 8,
+          product_ts(is, tmem + kColO + stream * DIM, tmem + stream * kSharedKeys + half * kHalf + kk * 8,
                      desc(v, kk * 2048), kIdescO, !first || kk > 0 ? 1u : 0u);
       };
       auto wait_q = [&](int stream) {
@@ -619,6 +626,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
         wait(&p_full[stream * 2], parity);
         settle(value, &full[v], turn);
         outputs(stream, 0, v, first);
+        commit_products(is, &o_half[stream]);
         const bool key = peek(&full[next], next_turn);
         wait(&p_full[stream * 2 + 1], parity);
         outputs(stream, 1, v, false);

@@ -19,19 +19,6 @@ struct PagedAttention {
 constexpr int kSharedKeys = 128;     // keys of a tile
 constexpr int kSharedQueries = 128;  // queries of a tile: whole rows of hq / hk heads that share a KV head
 
-// Ranges of equal length of `total` items, one for a CTA.
-struct SharedCut {
-  unsigned long long total;
-  int count;
-  SJ_DEVICE SharedCut(unsigned long long items, int ctas)
-      : total(items), count(static_cast<int>(min(static_cast<unsigned long long>(ctas), items))) {}
-  SJ_DEVICE unsigned long long begin(int id) const { return total * id / count; }
-  // the last range that begins at or before item x, which holds it
-  SJ_DEVICE int of(unsigned long long x) const {
-    return static_cast<int>(((x + 1) * count + total - 1) / total) - 1;
-  }
-};
-
 // A group: its rows, the keys [p0, p1) that every live one of them sees, and its first item.  The queries of a KV head
 // lie in `tiles` tiles.  An item is a tile of keys for two tiles of queries, or two tiles of keys for the one tile that
 // may be left: the same work either way.  A head's items are those of its pairs of tiles, a chunk of the keys at a time,
@@ -39,6 +26,7 @@ struct SharedCut {
 struct SharedGroup {
   unsigned long long base;
   size_t main;  // the first query of the group's parts that begin a block (chunk and pair): [chunks][rows][hq]
+  int blocks;   // its first block: [kv head][chunk][unit], a unit being a pair of tiles or the tile that is left
   int first, rows, request, p0, p1, tiles, keys, chunks;  // keys: tiles of them
   SJ_DEVICE int halves() const { return (keys + 1) / 2; }
   SJ_DEVICE unsigned long long head_items() const {
@@ -61,6 +49,7 @@ struct SharedSpans {
   unsigned long long* total;  // items of all groups
   SharedGroup* groups;
   SharedRow* rows;
+  int2* blocks;       // the first and the last CTA of each block
   SharedParts own;    // [rows, hq]: a row's own keys
   SharedParts main;   // the parts that begin a block
   SharedParts slots;  // [ctas][2 * kSharedQueries]: the part that goes on with a block, of each CTA

@@ -13,6 +13,7 @@
 #include <climits>
 #include <cmath>
 #include <numeric>
+#include <type_traits>
 
 #include "attention_paged.cuh"
 #include "common.cuh"
@@ -70,7 +71,7 @@ __global__ void __launch_bounds__(1024) shared_spans_kernel(const SpansArgs a) {
     }
     return lo;
   };
-  for (int r = t; r < a.rows; r += 1024) {
+  for (int r = t; r < a.rows; r += static_cast<int>(blockDim.x)) {
     const int b = a.request ? a.request[r] : r, pos = a.position[r];
     int n = b == -1 || pos > kLastSeen ? 0 : pos + 1;
     if (b < -1 || b >= a.requests || pos < -1 || pos > kLastSeen || n > most) {
@@ -114,7 +115,7 @@ __global__ void __launch_bounds__(1024) shared_spans_kernel(const SpansArgs a) {
     __syncthreads();
     unsigned long long base = upto - mine;
     total = 0;
-    for (int w = 0; w < 32; ++w) {
+    for (int w = 0; w < static_cast<int>(blockDim.x) / 32; ++w) {
       if (w == warp) base += total;
       total += s_scan[w];
     }
@@ -133,8 +134,9 @@ __global__ void __launch_bounds__(1024) shared_spans_kernel(const SpansArgs a) {
     g.chunks = 1;
     g.main = before(t < a.groups ? queries : 0);
   }
+  g.blocks = static_cast<int>(before(t < a.groups ? static_cast<unsigned long long>(a.hk) * g.chunks * ((g.tiles + 1) / 2) : 0));
   if (t < a.groups) a.out.groups[t] = g;
-  for (int r = t; r < a.rows; r += 1024) {
+  for (int r = t; r < a.rows; r += static_cast<int>(blockDim.x)) {
     SharedRow& row = a.out.rows[r];
     if (row.group >= 0 && row.n > 0 && p1[row.group] > p0[row.group]) {
       row.p0 = p0[row.group];
@@ -257,9 +259,10 @@ struct SharedLay {
 struct SharedPiece {
   SharedGroup g;
   int h, tile, chunk, i0, i1;
-  bool begins;  // a block
+  bool begins, ends;  // a block
   bool two;  // two tiles of queries over the same keys; else one, over alternate tiles of keys
   int steps0, steps1;  // of the streams
+  SJ_DEVICE int block() const { return g.blocks + (h * g.chunks + chunk) * ((g.tiles + 1) / 2) + tile / 2; }
   SJ_DEVICE int key(int stream, int step) const {
     return g.p0 + (two ? i0 + step : 2 * (i0 + step) + stream) * kSharedKeys;
   }
@@ -268,10 +271,11 @@ struct SharedWalk {
   const SharedArgs& a;
   unsigned long long at, end;
   SJ_DEVICE explicit SharedWalk(const SharedArgs& a_) : a(a_), at(0), end(0) {
-    const SharedCut cut(*a.s.total, gridDim.x);
-    if (static_cast<int>(blockIdx.x) >= cut.count) return;
-    at = cut.begin(blockIdx.x);
-    end = cut.begin(blockIdx.x + 1);
+    // the items in ranges of equal length, one for a CTA
+    const unsigned long long total = *a.s.total, count = min(static_cast<unsigned long long>(gridDim.x), total);
+    if (blockIdx.x >= count) return;
+    at = total * blockIdx.x / count;
+    end = total * (blockIdx.x + 1) / count;
   }
   SJ_DEVICE bool next(SharedPiece& p) {
     if (at >= end) return false;
@@ -307,6 +311,7 @@ struct SharedWalk {
       items = p.g.halves();
     }
     p.i1 = static_cast<int>(min(static_cast<unsigned long long>(items), p.i0 + (end - at)));
+    p.ends = p.i1 == items;
     at += p.i1 - p.i0;
     p.steps0 = p.i1 - p.i0;
     p.steps1 = p.two ? p.steps0 : min(p.g.keys - p.i1, p.i1) - p.i0;
@@ -394,6 +399,11 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
     };
     const int row0 = (warp & 3) * 32;
     while (ok && walk.next(p)) {
+      if (threadIdx.x == 0) {
+        int2* block = a.s.blocks + p.block();
+        if (p.begins) block->x = blockIdx.x;
+        if (p.ends) block->y = blockIdx.x;
+      }
       const int steps = stream == 0 ? p.steps0 : p.steps1;
       const int at = (p.tile + (p.two ? stream : 0)) * per + row / a.fan;  // the query's row in its group
       const int r = p.g.first + at, head = p.h * a.fan + row % a.fan;
@@ -799,68 +809,65 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
 }
 
 // ---------------------------------------------------------------- join
-// A warp for a row and head: its own part, then the parts of its keys in common, 32 at a time in the order of chunks and
-// CTAs; the lanes take the weights, then each its dims of all parts.
+// A warp for a row and head: its own part, then the parts of its keys in common, 32 at a time: of 16 chunks two CTAs
+// each, or of one chunk 32 CTAs.  The lanes take the weights, then each its dims of all parts, in order.
 template <int DIM>
 __global__ void __launch_bounds__(256) shared_join_kernel(const SharedSpans s, int rows, int hq, int fan, __nv_bfloat16* o,
                                                           int ldo, float* lse) {
   pdl_wait();
-  constexpr int PER = DIM / 32;
+  constexpr int PER = DIM / 32, AT_ONCE = 4;
+  using Dims = typename std::conditional<PER == 4, float4, float2>::type;
   const int lane = threadIdx.x & 31, at = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (at >= rows * hq) return;
   const int r = at / hq, head = at - r * hq;
-  float m = s.own.m[at], l = s.own.l[at], acc[PER];
-#pragma unroll
-  for (int e = 0; e < PER; ++e) acc[e] = s.own.o[static_cast<size_t>(at) * DIM + lane * PER + e];
   const SharedRow row = s.rows[r];
+  float m = s.own.m[at], l = s.own.l[at], acc[PER];
+  auto take = [&](float (&to)[PER], const float* from) {
+    const Dims x = *reinterpret_cast<const Dims*>(from + lane * PER);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) to[e] = reinterpret_cast<const float*>(&x)[e];
+  };
+  take(acc, s.own.o + static_cast<size_t>(at) * DIM);
   if (row.group >= 0) {
     const SharedGroup g = s.groups[row.group];
-    const SharedCut cut(*s.total, s.ctas);
-    const int per = kSharedQueries / fan, in = r - g.first, tile = in / per, pairs = g.tiles / 2;
-    const bool two = tile / 2 < pairs;
+    const int per = kSharedQueries / fan, in = r - g.first, tile = in / per;
+    const bool two = tile / 2 < g.tiles / 2;
     const int chunks = two ? g.chunks : 1;
     const int slot = (two ? (tile & 1) * kSharedQueries : 0) + in % per * fan + head % fan;
-    const unsigned long long base = g.base + (head / fan) * g.head_items();
-    for (int c0 = 0; c0 < chunks; c0 += 32) {
-      const int c = c0 + (chunks > 1 ? lane : 0);
-      int from = 0, to = -1;
-      if (c < chunks) {
-        const int k0 = two ? g.chunk(c) : 0, len = two ? g.chunk(c + 1) - k0 : g.halves();
-        const unsigned long long begin =
-            base + (two ? static_cast<unsigned long long>(pairs) * k0 + static_cast<unsigned long long>(tile / 2) * len
-                        : static_cast<unsigned long long>(pairs) * g.keys);
-        from = cut.of(begin);
-        to = cut.of(begin + len - 1);
-      }
-      const int first = chunks > 1 ? 0 : lane, step = chunks > 1 ? 1 : 32;
-      for (int k = first; __any_sync(0xffffffffu, from + k <= to); k += step) {
-        const bool is = from + k <= to;
+    const int2* blocks = s.blocks + g.blocks + (head / fan) * g.chunks * ((g.tiles + 1) / 2) + tile / 2;
+    const int side = chunks > 1 ? 2 : 32;  // CTAs of a chunk at a time
+    for (int c0 = 0; c0 < chunks; c0 += 32 / side) {
+      const int c = c0 + lane / side;
+      const int2 span = c < chunks ? blocks[c * ((g.tiles + 1) / 2)] : make_int2(0, -1);
+      for (int k = lane % side; __any_sync(0xffffffffu, span.x + k <= span.y); k += side) {
+        const bool is = span.x + k <= span.y;
         const SharedParts& part = k == 0 ? s.main : s.slots;
         const size_t query = !is ? 0
                              : k == 0 ? g.main + (static_cast<size_t>(c) * g.rows + in) * hq + head
-                                      : static_cast<size_t>(from + k) * (2 * kSharedQueries) + slot;
+                                      : static_cast<size_t>(span.x + k) * (2 * kSharedQueries) + slot;
         const float pm = is ? part.m[query] : -INFINITY, pl = is ? part.l[query] : 0.f;
-        const float* from_o = part.o + query * DIM;
+        const unsigned long long from = reinterpret_cast<unsigned long long>(part.o + query * DIM);
         const float top = fmaxf(m, warp_max(pm)), ref = top == -INFINITY ? 0.f : top;
         const float f = shared_exp2(m - ref), w = shared_exp2(pm - ref);
         l = f * l + warp_sum(w * pl);
         m = top;
 #pragma unroll
         for (int e = 0; e < PER; ++e) acc[e] *= f;
-        const uint32_t have = __ballot_sync(0xffffffffu, is);
-        const int most = 32 - __clz(have);
-        for (int j0 = 0; j0 < most; j0 += 8) {
-          float x[8][PER], weight[8];
+        uint32_t left = __ballot_sync(0xffffffffu, is);
+        while (left) {
+          float x[AT_ONCE][PER], weight[AT_ONCE];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            weight[j] = __shfl_sync(0xffffffffu, w, j0 + j);
-            const float* src = reinterpret_cast<const float*>(
-                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(from_o), j0 + j));
+          for (int j = 0; j < AT_ONCE; ++j) {
+            const int of = left ? __ffs(left) - 1 : -1;
+            left &= left - 1;
+            weight[j] = of < 0 ? 0.f : __shfl_sync(0xffffffffu, w, of);
+            const unsigned long long src = __shfl_sync(0xffffffffu, from, max(of, 0));
 #pragma unroll
-            for (int e = 0; e < PER; ++e) x[j][e] = have >> (j0 + j) & 1 ? src[lane * PER + e] : 0.f;
+            for (int e = 0; e < PER; ++e) x[j][e] = 0.f;
+            if (of >= 0) take(x[j], reinterpret_cast<const float*>(src));
           }
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
+          for (int j = 0; j < AT_ONCE; ++j)
 #pragma unroll
             for (int e = 0; e < PER; ++e) acc[e] += weight[j] * x[j][e];
         }
@@ -878,7 +885,7 @@ namespace {
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Where the parts of the workspace lie, from its own start.
-size_t shared_layout(SharedSpans* s, char* at, int rows, int groups, int hq, int head_dim) {
+size_t shared_layout(SharedSpans* s, char* at, int rows, int groups, int hq, int hk, int head_dim) {
   size_t n = 0;
   auto take = [&](size_t bytes) {
     const size_t was = n;
@@ -888,6 +895,8 @@ size_t shared_layout(SharedSpans* s, char* at, int rows, int groups, int hq, int
   char* total = take(sizeof(unsigned long long));
   char* group = take(sizeof(SharedGroup) * groups);
   char* row = take(sizeof(SharedRow) * rows);
+  // of a group with pairs of tiles twice its chunks * pairs * hk at most, else a unit a KV head
+  char* block = take(sizeof(int2) * (2 * static_cast<size_t>(sm_count()) + static_cast<size_t>(hk) * (2 * rows + groups)));
   auto parts = [&](size_t queries) {
     float* m = reinterpret_cast<float*>(take(queries * sizeof(float)));
     float* l = reinterpret_cast<float*>(take(queries * sizeof(float)));
@@ -897,7 +906,7 @@ size_t shared_layout(SharedSpans* s, char* at, int rows, int groups, int hq, int
   const size_t own = static_cast<size_t>(rows) * hq, ctas = static_cast<size_t>(sm_count());
   const size_t main_queries = own + ctas * 3 * kSharedQueries;
   const SharedSpans all{reinterpret_cast<unsigned long long*>(total), reinterpret_cast<SharedGroup*>(group),
-                        reinterpret_cast<SharedRow*>(row), parts(own), parts(main_queries),
+                        reinterpret_cast<SharedRow*>(row), reinterpret_cast<int2*>(block), parts(own), parts(main_queries),
                         parts(ctas * 2 * kSharedQueries), main_queries, static_cast<int>(ctas)};
   if (s) *s = all;
   return n;
@@ -940,7 +949,7 @@ extern "C" size_t sj_attn_paged_shared_workspace(int rows, int groups, int hq, i
   const size_t own = sj_attn_paged_workspace(rows, hq, hk, head_dim);
   if (own == 0 || groups < 0) return 0;
   if (!shares(groups, hq, hk)) return own;
-  return up256(own) + shared_layout(nullptr, nullptr, rows, groups, hq, head_dim);
+  return up256(own) + shared_layout(nullptr, nullptr, rows, groups, hq, hk, head_dim);
 }
 
 extern "C" int sj_attn_paged_shared(const void* q, int ldq, const void* k_cache, const void* v_cache, int pages,
@@ -963,9 +972,9 @@ extern "C" int sj_attn_paged_shared(const void* q, int ldq, const void* k_cache,
   if (!shares(groups, hq, hk)) return attn_paged_rows(a, nullptr, head_dim, s);
   SharedSpans spans;
   shared_layout(&spans, static_cast<char*>(workspace) + up256(sj_attn_paged_workspace(rows, hq, hk, head_dim)), rows,
-                groups, hq, head_dim);
+                groups, hq, hk, head_dim);
   const SpansArgs sa{request, position, group, rows, groups, requests, page, ld_table, window, hq, hq / hk, hk, 2, spans};
-  launch(shared_spans_kernel, 1, 1024, 0, s, sa);
+  launch(shared_spans_kernel, 1, groups <= 256 && rows <= 1024 ? 256 : 1024, 0, s, sa);
   SJ_LAUNCH_CHECK("shared_spans");
   // Tensor copies of boxes that pages and tiles have in common, of whole swizzled groups of 8 rows; strides that a map
   // takes (not 0, below 2^40 bytes: a head or page that no index reaches may have any).

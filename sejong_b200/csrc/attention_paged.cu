@@ -221,7 +221,8 @@ SJ_DEVICE int arrive(int* counter) {
 }
 
 // DIM: head_dim; NQ: query tiles of 8 that a unit holds (a query's columns of S^T; 2 above 8 heads a KV head).  SHARED:
-// `spans` says which keys of each row attn_shared_kernel has taken; keys are then counted without those.
+// `spans` says which keys of each row attn_shared_kernel has taken; keys are then counted without those, and such rows
+// are written as parts.
 template <int DIM, int NQ, bool SHARED>
 __global__ void __launch_bounds__(kWarps * 32, kCtas) attn_paged_kernel(const PagedAttention a, const SharedSpans spans) {
   pdl_wait();
@@ -555,7 +556,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attn_paged_kernel(const Pa
           out.w += x.w;
           sum += exp2_fast(sm[w][qi] - ref) * sl[w][qi];
         }
-        if (SHARED && whole) {
+        if (SHARED && whole && whole_row.group >= 0) {
           const size_t query = static_cast<size_t>(r) * a.hq + h * group + q0 + qi;
           *reinterpret_cast<float4*>(spans.own.o + query * DIM + d) = out;
           if (d == 0) {
@@ -612,7 +613,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attn_paged_kernel(const Pa
           joined = last_of(a.counters + 2 * gridDim.x + from, groups);
           if (joined) join_parts<DIM, Q, WARPS>(a.partial, from, from, groups, size, heads, sm[0], sl[0], weight, sums);
         }
-        if (SHARED && joined) {
+        if (SHARED && joined && whole_row.group >= 0) {
           for (int i = t; i < heads * (DIM / 4); i += WARPS * 32) {
             const int qi = i / (DIM / 4), d = i % (DIM / 4) * 4;
             const size_t query = static_cast<size_t>(r) * a.hq + h * group + q0 + qi;

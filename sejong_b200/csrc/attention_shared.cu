@@ -12,6 +12,8 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <cstdlib>
+#include <cstring>
 #include <numeric>
 #include <type_traits>
 
@@ -32,12 +34,19 @@ constexpr uint32_t kColO = 256;            // TMEM columns: S of two streams (th
 constexpr uint32_t kTmemAll = 512;
 constexpr uint32_t kNowhere = 0xffffffffu;
 constexpr int kLastSeen = INT_MAX - 4096;
+// When sharing pays: rows that each read the keys in common get them out of L2 at about 9 TB/s (134 MB in 16 us besides
+// the kernel's own 5, 268 in 25), where the tensor-core pass costs 15 us to start and to join, and 1.6 (2.2 for wide
+// heads) an item on each CTA.  Measured, rows apart against sharing: 8 rows of 16384 keys, 12 / 4 heads of 64 20.7 and
+// 29.3 us; 32 rows of 2048 keys, 16 / 4 heads of 128 20.6 and 25.2, 64 rows 30.3 and 27.7; 16 x 16 rows of 2048 to 16384
+// keys, 12 / 4 heads of 64 164 and 79.
+constexpr double kSharedRate = 9e6, kSharedStart = 15.0;  // bytes a microsecond, microseconds
+__host__ __device__ constexpr double shared_item_us(int head_dim) { return head_dim == 64 ? 1.6 : 2.2; }
 }  // namespace
 
 // ---------------------------------------------------------------- spans
 struct SpansArgs {
   const int32_t *request, *position, *group;
-  int rows, groups, requests, page, ld_table, window, hq, fan, hk, least;
+  int rows, groups, requests, page, ld_table, window, hq, hk, head_dim, always;
   SharedSpans out;
 };
 
@@ -95,9 +104,8 @@ __global__ void __launch_bounds__(1024) shared_spans_kernel(const SpansArgs a) {
     g.request = a.group[3 * t + 1];
     g.p0 = p0[t];
     g.p1 = max(p1[t], p0[t]);
-    if (!ordered || live[t] < a.least) g.p1 = g.p0;
-    p1[t] = g.p1;
-    const int per = kSharedQueries / a.fan;  // rows of a tile
+    if (!ordered || live[t] < 2) g.p1 = g.p0;
+    const int per = kSharedQueries / (a.hq / a.hk);  // rows of a tile
     g.tiles = (g.rows + per - 1) / per;
     g.keys = (g.p1 - g.p0 + kSharedKeys - 1) / kSharedKeys;
     items = g.head_items() * a.hk;
@@ -122,7 +130,16 @@ __global__ void __launch_bounds__(1024) shared_spans_kernel(const SpansArgs a) {
     return base;
   };
   g.base = before(items);
-  const unsigned long long all = total;
+  unsigned long long all = total;
+  // bytes that the rows would read of the keys in common if each read them for itself
+  before(static_cast<unsigned long long>(g.p1 - g.p0) * (t < a.groups ? live[t] : 0) * a.hk * a.head_dim * 4);
+  if (!a.always && total < kSharedRate * (kSharedStart + all * shared_item_us(a.head_dim) / a.out.ctas)) {
+    all = 0;
+    g.p1 = g.p0;
+    g.keys = 0;
+    g.base = 0;
+  }
+  if (t < a.groups) p1[t] = g.p1;
   if (t == 0) *a.out.total = all;
   // about a CTA's items a chunk, so that a block is about a CTA's
   const unsigned long long ctas = min(static_cast<unsigned long long>(a.out.ctas), all);
@@ -821,6 +838,7 @@ __global__ void __launch_bounds__(256) shared_join_kernel(const SharedSpans s, i
   if (at >= rows * hq) return;
   const int r = at / hq, head = at - r * hq;
   const SharedRow row = s.rows[r];
+  if (row.group < 0) return;  // written already
   float m = s.own.m[at], l = s.own.l[at], acc[PER];
   auto take = [&](float (&to)[PER], const float* from) {
     const Dims x = *reinterpret_cast<const Dims*>(from + lane * PER);
@@ -828,7 +846,7 @@ __global__ void __launch_bounds__(256) shared_join_kernel(const SharedSpans s, i
     for (int e = 0; e < PER; ++e) to[e] = reinterpret_cast<const float*>(&x)[e];
   };
   take(acc, s.own.o + static_cast<size_t>(at) * DIM);
-  if (row.group >= 0) {
+  {
     const SharedGroup g = s.groups[row.group];
     const int per = kSharedQueries / fan, in = r - g.first, tile = in / per;
     const bool two = tile / 2 < g.tiles / 2;
@@ -969,11 +987,14 @@ extern "C" int sj_attn_paged_shared(const void* q, int ldq, const void* k_cache,
   if (rc != SJ_OK || rows == 0) return rc;
   if (groups > 0 && !group) return fail(SJ_ERR_ARGUMENT, "%s: null operand", who);
   cudaStream_t s = as_stream(stream);
-  if (!shares(groups, hq, hk)) return attn_paged_rows(a, nullptr, head_dim, s);
+  const double most = static_cast<double>(rows) * hk * head_dim * 4 * ld_table * page;  // bytes that rows apart read
+  const char* wish = std::getenv("SJ_ATTN_SHARE");
+  const bool always = wish && std::strcmp(wish, "always") == 0;
+  if (!shares(groups, hq, hk) || (!always && most < kSharedRate * kSharedStart)) return attn_paged_rows(a, nullptr, head_dim, s);
   SharedSpans spans;
   shared_layout(&spans, static_cast<char*>(workspace) + up256(sj_attn_paged_workspace(rows, hq, hk, head_dim)), rows,
                 groups, hq, hk, head_dim);
-  const SpansArgs sa{request, position, group, rows, groups, requests, page, ld_table, window, hq, hq / hk, hk, 2, spans};
+  const SpansArgs sa{request, position, group, rows, groups, requests, page, ld_table, window, hq, hk, head_dim, always ? 1 : 0, spans};
   launch(shared_spans_kernel, 1, groups <= 256 && rows <= 1024 ? 256 : 1024, 0, s, sa);
   SJ_LAUNCH_CHECK("shared_spans");
   // Tensor copies of boxes that pages and tiles have in common, of whole swizzled groups of 8 rows; strides that a map

@@ -30,6 +30,12 @@ def lib():
 
 
 @pytest.fixture(autouse=True)
+def share_always(monkeypatch):
+    """Small cases go the way of large ones."""
+    monkeypatch.setenv("SJ_ATTN_SHARE", "always")
+
+
+@pytest.fixture(autouse=True)
 def no_device_error(lib):
     yield
     assert device_error() == 0
@@ -530,6 +536,19 @@ def test_shared_without_groups():
     shared_case([], 4, 2, 64, 16, loose=4)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_shared_where_it_does_not_pay(monkeypatch, dim):
+    """The same by the rule: too little to share for the host to see, and for the GPU (wide block tables)."""
+    monkeypatch.delenv("SJ_ATTN_SHARE")
+    shared_case([(160, [161, 200, 0, 170]), (300, [301, None])], 4, 2, dim, 16, loose=1, seed=dim)
+    shared_case([(160, [161, 200, 0, 170] * 20), (300, [300, None]), (200, [30000])], 8, 8, dim, 128, loose=1, seed=dim)
+
+
+def test_shared_where_it_pays(monkeypatch):
+    monkeypatch.delenv("SJ_ATTN_SHARE")
+    shared_case([(2500, [2501 + i % 40 for i in range(80)])], 8, 4, 128, 64, seed=9)
+
+
 @pytest.mark.parametrize("group", [[(0, 9, 32)], [(0, -1, 32)], [(-1, 0, 32)], [(5, 0, 32)], [(0, 0, -3)], [(0, 0, 1000)],
                                    [(2, 0, 32), (1, 0, 32)], [(1, 0, 32), (1, 0, 32)]])
 def test_shared_reports_groups_out_of_range(group):
@@ -549,7 +568,7 @@ def test_shared_reports_groups_out_of_range(group):
         call(name, ptr(q), 256, ptr(k), ptr(v), 8, 16, *k.stride()[:3], ptr(table), 3, 4, 0, ptr(pos), 4, *extra, 4, 2, 64, 0,
              ptr(o), 256, ptr(lse), ptr(work), size, stream())
         out.append((o, lse))
-    assert device_error() in (BAD_INDEX, 0)
+    assert device_error() == BAD_INDEX
     assert (out[0][0].float() - out[1][0].float()).abs().max() < 0.02
     assert (out[0][1] - out[1][1]).abs().max() < 1e-4
 

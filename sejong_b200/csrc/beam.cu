@@ -374,10 +374,16 @@ __global__ void __launch_bounds__(kBeamThreads, 4)
   uint64_t s = 0;
   if (t == 0) s_count = 0;
   if (score > -INFINITY) {
+    uint4 ahead[kBeamPieces];  // on their way while the last ones are added up
+#pragma unroll
+    for (int i = 0; i < kBeamPieces; ++i) ahead[i] = row.load(first + t + i * kBeamThreads, last);
     for (int p = first + t; p - t < last; p += STEP) {
       uint4 q[kBeamPieces];
 #pragma unroll
-      for (int i = 0; i < kBeamPieces; ++i) q[i] = row.load(p + i * kBeamThreads, last);
+      for (int i = 0; i < kBeamPieces; ++i) {
+        q[i] = ahead[i];
+        ahead[i] = row.load(p + STEP + i * kBeamThreads, last);
+      }
       float here = -INFINITY;
 #pragma unroll
       for (int i = 0; i < kBeamPieces; ++i) here = fmaxf(here, BeamRow<T>::largest(q[i]));
@@ -406,8 +412,10 @@ __global__ void __launch_bounds__(kBeamThreads, 4)
   __syncthreads();
   float bar = s_bar[0];
   for (int k = 1; k < kBeamWarps; ++k) bar = fminf(bar, s_bar[k]);
-  if (m >= bar && m > -INFINITY) {  // this thread's logits once more
-    for (int p = first + t; p < last; p += kBeamThreads) {
+  // the logits of the threads that hold candidates once more, a thread's by its whole warp
+  for (uint32_t who = __ballot_sync(0xffffffffu, m >= bar && m > -INFINITY); who; who &= who - 1) {
+    const int of = warp * 32 + __ffs(who) - 1;
+    for (int p = first + of + lane * kBeamThreads; p < last; p += 32 * kBeamThreads) {
       const uint4 q = row.load(p, last);
       if (!(BeamRow<T>::largest(q) >= bar)) continue;
 #pragma unroll

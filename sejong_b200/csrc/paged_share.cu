@@ -20,13 +20,17 @@ namespace cg = cooperative_groups;
 namespace sj {
 
 namespace {
-constexpr int kShareMaxBatch = 4096, kShareMaxPages = 1 << 18;  // their counters fit a cluster's shared memory
+constexpr int kShareMaxBatch = 4096, kShareMaxPages = 1 << 18;  // masks of them fit shared memory
 constexpr int kForkNoPages = 2, kForkTableNarrow = 3, kForkBad = 4;
 constexpr int kCompactMovesOver = 1, kCompactBad = 4;
 constexpr int kForkCluster = 8, kForkThreads = 512, kForkWarps = kForkThreads / 32;
-constexpr int kForkChunk = 128;       // entries of a block table that a warp counts at a time
+constexpr int kForkOne = 2048;        // pages up to which one CTA counts them: five exchanges fewer
+constexpr int kForkChunk = 128;       // entries of a block table that a warp takes at a time
+constexpr int kForkRun = 8;           // slots whose entries it counts together
+constexpr int kForkUnits = 4;         // owners that a thread asks for at a time
+constexpr int kNoEntry = INT_MIN;
 constexpr int kCopyThreads = 256, kCopyPieces = 8;  // 16-byte pieces of a thread
-constexpr int kCompactThreads = 1024;
+constexpr int kCompactThreads = 1024, kCompactIds = 8;  // of the stack, that a thread asks for at a time
 }  // namespace
 
 // ---------------------------------------------------------------- fork
@@ -39,16 +43,18 @@ struct Fork {
 // A slot's pages pass to its children: full ones are shared, a half-filled last page goes to the lowest child and is
 // copied to a fresh page for each of the others.  Every CTA scans the batch for itself.  The first cluster counts: an
 // entry of a slot with c children changes its page's owners by c - 1 (the half-filled page of a slot without children
-// by -1); the counters of a CTA's share of the pages lie in its shared memory, which the others add to.  Integer sums,
-// so their order does not matter.  Then each CTA knows which of its pages nobody holds, and after one exchange of
-// numbers where on the stack they go.  The other clusters (the same one, where there is only one) write tables.
+// by -1), by integer additions to shares_out, whose order does not matter.  Then each CTA knows which of its pages
+// nobody holds, and after one exchange of numbers where on the stack they go.  The other clusters (the same one, where
+// there is only one) write tables.
 __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) {
   pdl_wait();
   extern __shared__ int dynamic[];
   int* children = dynamic;                       // [batch + 1]
   int* lowest = children + (a.batch + 1);        // [batch + 1]
-  int* rank = lowest + (a.batch + 1);            // [batch + 1] copies of the slots before
-  int* counter = rank + (a.batch + 1);           // [per], in the first cluster
+  int* rank = lowest + (a.batch + 1);            // [batch + 1] copies of the slots before, -1: no copy
+  int* parents = rank + (a.batch + 1);           // [batch + 1]
+  int* lengths = parents + (a.batch + 1);        // [batch + 1]
+  uint32_t* gone_bits = reinterpret_cast<uint32_t*>(lengths + (a.batch + 1));  // of the CTA's pages
   __shared__ int s_bad, s_narrow, s_back, s_warp[kForkWarps];
   cg::cluster_group cluster = cg::this_cluster();
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, batch = a.batch, page = a.page;
@@ -58,13 +64,26 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) 
   for (int b = t; b < batch; b += kForkThreads) {
     children[b] = 0;
     lowest[b] = INT_MAX;
+    parents[b] = a.parent[b];
+    lengths[b] = a.cached[b];
   }
-  if (counts)
-    for (int i = t; i < a.per; i += kForkThreads) counter[i] = 0;
+  // this CTA's share of the pages
+  const int page0 = min(cta * a.per, a.pages), mine = counts ? min(a.per, a.pages - page0) : 0;
+  for (int i = t; i < mine; i += kForkThreads * kForkUnits) {
+    int more[kForkUnits];
+#pragma unroll
+    for (int e = 0; e < kForkUnits; ++e)
+      more[e] = i + e * kForkThreads < mine ? a.shares[page0 + i + e * kForkThreads] : 0;
+#pragma unroll
+    for (int e = 0; e < kForkUnits; ++e) {
+      if (more[e] < 0) record_error(SJ_DEV_BAD_INDEX);
+      if (i + e * kForkThreads < mine) a.shares_out[page0 + i + e * kForkThreads] = max(more[e], 0);
+    }
+  }
   __syncthreads();
-  auto length = [&](int b) { return a.cached[b]; };
+  auto length = [&](int b) { return lengths[b]; };
   for (int b = t; b < batch; b += kForkThreads) {
-    const int p = a.parent[b], n = length(b);
+    const int p = parents[b], n = length(b);
     if (p < -1 || p >= batch || n < 0 || n > INT_MAX - page) {
       s_bad = 1;
       continue;
@@ -83,7 +102,7 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) 
   {
     int taken = 0;
     for (int b0 = 0; b0 < batch; b0 += kForkThreads) {
-      const int b = b0 + t, p = b < batch && !status ? a.parent[b] : -1;
+      const int b = b0 + t, p = b < batch && !status ? parents[b] : -1;
       const bool copied = p >= 0 && lowest[p] != b && length(p) % page != 0;
       const unsigned have = __ballot_sync(0xffffffffu, copied);
       if (lane == 0) s_warp[warp] = __popc(have);
@@ -104,7 +123,7 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) 
   if (!status && taken > count) status = kForkNoPages;
   if (status) taken = 0;
   // with a status, every slot keeps what it holds
-  auto source = [&](int b) { return status ? b : a.parent[b]; };
+  auto source = [&](int b) { return status ? b : parents[b]; };
   auto held = [&](int p) {
     const int n = length(p);
     return n < 0 || n > INT_MAX - page ? 0 : min((n + page - 1) / page, a.ld_table);
@@ -115,21 +134,20 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) 
   const int writers = gridDim.x > static_cast<unsigned>(ctas) ? gridDim.x - ctas : gridDim.x;
   const int writer = gridDim.x > static_cast<unsigned>(ctas) ? static_cast<int>(blockIdx.x) - ctas : blockIdx.x;
   if (writer >= 0) {
-    for (int b = writer * kForkWarps + warp; b < batch; b += writers * kForkWarps) {
-      const int p = source(b);
+    const int chunks = (a.ld_table + kForkChunk - 1) / kForkChunk;
+    for (int u = writer * kForkWarps + warp; u < batch * chunks; u += writers * kForkWarps) {
+      const int b = u % batch, j0 = u / batch * kForkChunk, p = source(b);
       const bool copied = !status && rank[b] >= 0;
-      const int n = p < 0 ? 0 : held(p), own = copied ? n - 1 : -1;
+      const int n = p < 0 ? 0 : held(p), own = copied ? n - 1 : -1, end = min(n, j0 + kForkChunk);
       const int32_t* from = a.table + static_cast<size_t>(max(p, 0)) * a.ld_table;
       int32_t* to = a.table_out + static_cast<size_t>(b) * a.ld_table;
-      for (int j = lane; j < n; j += 128) {
-        int32_t id[4];
+      int32_t id[kForkChunk / 32];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) id[e] = j + 32 * e < n ? from[j + 32 * e] : 0;
+      for (int e = 0; e < kForkChunk / 32; ++e) id[e] = j0 + 32 * e + lane < end ? from[j0 + 32 * e + lane] : 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (j + 32 * e < n && j + 32 * e != own) to[j + 32 * e] = id[e];
-      }
-      if (lane == 0) {
+      for (int e = 0; e < kForkChunk / 32; ++e)
+        if (j0 + 32 * e + lane < end && j0 + 32 * e + lane != own) to[j0 + 32 * e + lane] = id[e];
+      if (lane == 0 && j0 == 0) {
         a.cached_out[b] = p < 0 ? 0 : length(p);
         if (copied) {
           const int dst = fresh(b), at = rank[b], src = from[own];
@@ -153,47 +171,71 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) 
   if (!counts) return;
 
   // ---- owners
-  cluster.sync();  // every counter of the cluster is zero
+  __threadfence();
+  cluster.sync();  // shares_out holds the owners so far
   if (!status) {
-    const int chunks = (a.ld_table + kForkChunk - 1) / kForkChunk;
-    for (int u = cta * kForkWarps + warp; u < batch * chunks; u += ctas * kForkWarps) {
-      const int p = u / chunks, j0 = u % chunks * kForkChunk, c = children[p];
-      if (c == 1) continue;
-      const int n = held(p), full = length(p) / page, end = min(j0 + kForkChunk, c == 0 ? n : full);
-      int32_t id[kForkChunk / 32];
+    // A warp takes a chunk of the tables of kForkRun slots side by side.  Slots that came from one share their first pages,
+    // and what their children take and leave there mostly adds up to nothing: it is added up here, as long as the page
+    // is the same, before it goes to memory.
+    const int chunks = (a.ld_table + kForkChunk - 1) / kForkChunk, runs = (batch + kForkRun - 1) / kForkRun;
+    constexpr int PER = kForkChunk / 32;
+    for (int u = cta * kForkWarps + warp; u < runs * chunks; u += ctas * kForkWarps) {
+      const int p0 = u % runs * kForkRun, j0 = u / runs * kForkChunk + lane;
+      int32_t id[kForkRun][PER];
 #pragma unroll
-      for (int e = 0; e < kForkChunk / 32; ++e) {
-        const int j = j0 + 32 * e + lane;
-        id[e] = j < end ? a.table[static_cast<size_t>(p) * a.ld_table + j] : 0;
+      for (int k = 0; k < kForkRun; ++k) {
+        const int p = min(p0 + k, batch - 1), change = p0 + k < batch ? children[p] - 1 : 0;
+        const int end = change == 0 ? 0 : change < 0 ? held(p) : length(p) / page;
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+          id[k][e] = j0 + 32 * e < end ? a.table[static_cast<size_t>(p) * a.ld_table + j0 + 32 * e] : kNoEntry;
       }
 #pragma unroll
-      for (int e = 0; e < kForkChunk / 32; ++e) {
-        if (j0 + 32 * e + lane >= end) continue;
-        if (id[e] < 0 || id[e] >= a.pages) {
-          record_error(SJ_DEV_BAD_INDEX);
-          continue;
+      for (int e = 0; e < PER; ++e) {
+        int32_t now = kNoEntry;
+        int sum = 0;
+        auto add = [&]() {
+          if (now == kNoEntry || sum == 0) return;
+          if (now < 0 || now >= a.pages)
+            record_error(SJ_DEV_BAD_INDEX);
+          else
+            atomicAdd(&a.shares_out[now], sum);
+        };
+#pragma unroll
+        for (int k = 0; k < kForkRun; ++k) {
+          if (id[k][e] == kNoEntry) continue;
+          if (id[k][e] != now) {
+            add();
+            now = id[k][e];
+            sum = 0;
+          }
+          sum += children[min(p0 + k, batch - 1)] - 1;
         }
-        const int at = id[e] / a.per;
-        atomicAdd(cluster.map_shared_rank(counter, at) + (id[e] - at * a.per), c - 1);
+        add();
       }
     }
   }
+  __threadfence();
   cluster.sync();
   // a warp's run of this CTA's pages, in order
-  const int page0 = cta * a.per, mine = max(0, min(a.per, a.pages - page0));
   const int run = ((mine + kForkWarps - 1) / kForkWarps + 31) / 32 * 32;
   const int i0 = min(warp * run, mine), i1 = min(i0 + run, mine);
   int gone = 0;
-  for (int i = i0 + lane; i - lane < i1; i += 32) {
-    bool is = false;
-    if (i < i1) {
-      const int more = a.shares[page0 + i], left = more + counter[i];
-      is = left == -1 && counter[i] != 0;
-      if (left < 0 && !is && !status) record_error(SJ_DEV_BAD_INDEX);  // given back more often than it was held
-      a.shares_out[page0 + i] = status ? more : max(left, 0);
-      counter[i] = is;
+  for (int i = i0 + lane; i - lane < i1; i += 32 * kForkUnits) {
+    int left[kForkUnits];
+#pragma unroll
+    for (int e = 0; e < kForkUnits; ++e) left[e] = i + 32 * e < i1 ? __ldcg(a.shares_out + page0 + i + 32 * e) : 0;
+#pragma unroll
+    for (int e = 0; e < kForkUnits; ++e) {
+      const bool is = left[e] == -1 && !status;
+      if (left[e] < 0 && !status) {
+        if (left[e] < -1) record_error(SJ_DEV_BAD_INDEX);  // given back more often than it was held
+        a.shares_out[page0 + i + 32 * e] = 0;
+      }
+      const unsigned have = __ballot_sync(0xffffffffu, is);
+      if (lane == 0 && i + 32 * e < i1) gone_bits[(i + 32 * e) >> 5] = have;
+      gone += __popc(have);
     }
-    gone += __popc(__ballot_sync(0xffffffffu, is));
   }
   if (lane == 0) s_warp[warp] = gone;
   __syncthreads();
@@ -211,8 +253,8 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) 
   }
   for (int w = 0; w < warp; ++w) back += s_warp[w];
   for (int i = i0 + lane; i - lane < i1; i += 32) {
-    const bool is = i < i1 && counter[i] != 0;
-    const unsigned have = __ballot_sync(0xffffffffu, is);
+    const unsigned have = gone_bits[i >> 5];
+    const bool is = have >> lane & 1;
     const int at = back + __popc(have & ((1u << lane) - 1));
     if (is) {
       if (at >= 0 && at < a.pages)
@@ -296,12 +338,18 @@ __global__ void __launch_bounds__(kCompactThreads) paged_compact_kernel(const Co
   for (int w = t; w < words; w += kCompactThreads) bits[w] = 0;
   if (t == 0) s_bad = 0;
   __syncthreads();
-  for (int i = t; i < (bad ? 0 : count); i += kCompactThreads) {
-    const int id = a.stack[i];
-    if (id < 0 || id >= a.pages)
-      s_bad = 1;
-    else if (atomicOr(&bits[id >> 5], 1u << (id & 31)) >> (id & 31) & 1)
-      s_bad = 1;  // twice on the stack
+  for (int i = t; i < (bad ? 0 : count); i += kCompactThreads * kCompactIds) {
+    int id[kCompactIds];
+#pragma unroll
+    for (int e = 0; e < kCompactIds; ++e) id[e] = i + e * kCompactThreads < count ? a.stack[i + e * kCompactThreads] : 0;
+#pragma unroll
+    for (int e = 0; e < kCompactIds; ++e) {
+      if (i + e * kCompactThreads >= count) break;
+      if (id[e] < 0 || id[e] >= a.pages)
+        s_bad = 1;
+      else if (atomicOr(&bits[id[e] >> 5], 1u << (id[e] & 31)) >> (id[e] & 31) & 1)
+        s_bad = 1;  // twice on the stack
+    }
   }
   __syncthreads();
   const int per = (words + kCompactThreads - 1) / kCompactThreads, w0 = min(t * per, words), w1 = min(w0 + per, words);
@@ -342,21 +390,38 @@ __global__ void __launch_bounds__(kCompactThreads) paged_compact_kernel(const Co
       else
         hi = mid;
     }
-    return lo * 32 + static_cast<int>(__fns(bits[lo], 0, r - (lo * 32 - before[lo]) + 1));
+    uint32_t holes = bits[lo];
+    int skip = r - (lo * 32 - before[lo]), at = 0;  // the skip-th set bit: by halves of what is left of the word
+#pragma unroll
+    for (int half = 16; half > 0; half >>= 1) {
+      const int below = __popc(holes & ((1u << half) - 1));
+      if (skip >= below) {
+        skip -= below;
+        at += half;
+        holes >>= half;
+      }
+    }
+    return lo * 32 + at;
   };
   const int first = blockIdx.x * kCompactThreads + t, step = gridDim.x * kCompactThreads;
-  for (int b = first >> 5; b < a.batch; b += step >> 5) {
-    const int n = a.cached[b];
+  const int chunks = (a.ld_table + kForkChunk - 1) / kForkChunk;
+  for (int u = first >> 5; u < a.batch * chunks; u += step >> 5) {
+    const int b = u % a.batch, j0 = u / a.batch * kForkChunk, n = a.cached[b];
     if (n < 0 || n > INT_MAX - a.page || (n + a.page - 1) / a.page > a.ld_table) {
       if (lane == 0) record_error(SJ_DEV_BAD_INDEX);
       continue;
     }
     const size_t row = static_cast<size_t>(b) * a.ld_table;
-    for (int j = lane; j < (n + a.page - 1) / a.page; j += 32) {
-      const int id = a.table[row + j];
-      const bool fine = id >= 0 && id < a.pages && (bad || !is_free(id));
+    const int end = min((n + a.page - 1) / a.page, j0 + kForkChunk);
+    int id[kForkChunk / 32];
+#pragma unroll
+    for (int e = 0; e < kForkChunk / 32; ++e) id[e] = j0 + 32 * e + lane < end ? a.table[row + j0 + 32 * e + lane] : 0;
+#pragma unroll
+    for (int e = 0; e < kForkChunk / 32; ++e) {
+      if (j0 + 32 * e + lane >= end) continue;
+      const bool fine = id[e] >= 0 && id[e] < a.pages && (bad || !is_free(id[e]));
       if (!fine) record_error(SJ_DEV_BAD_INDEX);
-      a.table_out[row + j] = fine ? target(id) : id;
+      a.table_out[row + j0 + 32 * e + lane] = fine ? target(id[e]) : id[e];
     }
   }
   for (int p = first; p < a.pages; p += step) {
@@ -398,8 +463,8 @@ extern "C" int sj_paged_fork(const int32_t* parent, int batch, int page, const i
                              const int32_t* free_pages, const int32_t* free_count, int pages, int32_t* cached_out,
                              int32_t* table_out, int32_t* shares_out, int32_t* free_out, int32_t* count_out,
                              int32_t* copies, int32_t* summary, void* stream) {
-  if (batch <= 0 || batch > kShareMaxBatch || page <= 0 || page > (1 << 20) || ld_table <= 0 || pages <= 0 ||
-      pages > kShareMaxPages)
+  if (batch <= 0 || batch > kShareMaxBatch || page <= 0 || page > (1 << 20) || ld_table <= 0 ||
+      ld_table > INT_MAX / kShareMaxBatch * kForkChunk - kForkChunk || pages <= 0 || pages > kShareMaxPages)
     return fail(SJ_ERR_SHAPE, "sj_paged_fork: batch=%d (up to %d) page=%d ld_table=%d pages=%d (up to %d)", batch,
                 kShareMaxBatch, page, ld_table, pages, kShareMaxPages);
   if (!parent || !cached || !block_table || !shares || !free_pages || !free_count || !cached_out || !table_out ||
@@ -409,10 +474,12 @@ extern "C" int sj_paged_fork(const int32_t* parent, int batch, int page, const i
       free_count == count_out)
     return fail(SJ_ERR_ARGUMENT, "sj_paged_fork: the new state needs buffers of its own");
   Fork a{parent, cached, block_table, shares, free_pages, free_count, cached_out, table_out, shares_out,
-         free_out, count_out, copies, summary, batch, page, ld_table, pages, (pages + kForkCluster - 1) / kForkCluster};
-  const int smem = (3 * (batch + 1) + a.per) * static_cast<int>(sizeof(int));
+         free_out, count_out, copies, summary, batch, page, ld_table, pages, 0};
+  const int ctas = pages <= kForkOne ? 1 : kForkCluster;
+  a.per = (pages + ctas - 1) / ctas;
+  const int smem = (5 * (batch + 1) + a.per / 32 + 1) * static_cast<int>(sizeof(int));
   static KernelAttrOnce once;
-  constexpr int most = (3 * (kShareMaxBatch + 1) + kShareMaxPages / kForkCluster) * static_cast<int>(sizeof(int));
+  constexpr int most = (5 * (kShareMaxBatch + 1) + kShareMaxPages / 32 + 1) * static_cast<int>(sizeof(int));
   const int rc = ensure_max_smem(once, reinterpret_cast<const void*>(paged_fork_kernel), most,
                                  "sj_paged_fork: shared memory");
   if (rc != SJ_OK) return rc;
@@ -420,11 +487,13 @@ extern "C" int sj_paged_fork(const int32_t* parent, int batch, int page, const i
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = kForkCluster;
+  attr[1].val.clusterDim.x = ctas;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  const int writers = std::min((batch + kForkWarps - 1) / kForkWarps, sm_count() / 2);
-  cfg.gridDim = dim3(kForkCluster * (1 + (writers + kForkCluster - 1) / kForkCluster));
+  // tables of more chunks than the counting CTAs have warps are written by CTAs of their own
+  const int64_t units = static_cast<int64_t>(batch) * ((ld_table + kForkChunk - 1) / kForkChunk);
+  const int64_t writers = units <= ctas * kForkWarps ? 0 : std::min<int64_t>((units - 1) / kForkWarps + 1, sm_count() / 2);
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas * (1 + (writers + ctas - 1) / ctas)));
   cfg.blockDim = dim3(kForkThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = as_stream(stream);
@@ -466,8 +535,8 @@ extern "C" int sj_paged_compact(const int32_t* cached, int batch, int page, cons
                                 const int32_t* shares, const int32_t* free_pages, const int32_t* free_count,
                                 int pages, int32_t* table_out, int32_t* shares_out, int32_t* free_out, int32_t* moves,
                                 int most, int32_t* summary, void* stream) {
-  if (batch <= 0 || batch > kShareMaxBatch || page <= 0 || page > (1 << 20) || ld_table <= 0 || pages <= 0 ||
-      pages > kShareMaxPages || most < 0 || most > INT_MAX / 3)
+  if (batch <= 0 || batch > kShareMaxBatch || page <= 0 || page > (1 << 20) || ld_table <= 0 ||
+      ld_table > INT_MAX / kShareMaxBatch * kForkChunk - kForkChunk || pages <= 0 || pages > kShareMaxPages || most < 0 || most > INT_MAX / 3)
     return fail(SJ_ERR_SHAPE, "sj_paged_compact: batch=%d (up to %d) page=%d ld_table=%d pages=%d (up to %d) most=%d",
                 batch, kShareMaxBatch, page, ld_table, pages, kShareMaxPages, most);
   if (!cached || !block_table || !shares || !free_pages || !free_count || !table_out || !shares_out || !free_out ||
@@ -483,7 +552,8 @@ extern "C" int sj_paged_compact(const int32_t* cached, int batch, int page, cons
   if (rc != SJ_OK) return rc;
   const Compact a{cached, block_table, shares, free_pages, free_count, table_out, shares_out, free_out,
                   moves, summary, batch, page, ld_table, pages, most};
-  const int64_t work = std::max<int64_t>(static_cast<int64_t>(batch) * 32, std::max(pages, most));
+  const int64_t units = static_cast<int64_t>(batch) * ((ld_table + kForkChunk - 1) / kForkChunk);
+  const int64_t work = std::max<int64_t>(units * 32, std::max(pages, most));
   const int grid = static_cast<int>(std::min<int64_t>((work + kCompactThreads - 1) / kCompactThreads, sm_count()));
   launch(paged_compact_kernel, grid, kCompactThreads, (2 * words + 1) * sizeof(int), as_stream(stream), a);
   SJ_LAUNCH_CHECK("paged_compact");

@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4)
     BeamList list;
   } u;
   __shared__ BeamOffset offset[kBeamMaxBeams];
-  __shared__ float s_bar[kBeamWarps];
+  __shared__ float s_bar[32];
   __shared__ BeamSum s_sum[kBeamWarps];
   __shared__ int s_count, s_last;
   __shared__ unsigned long long s_bars;
@@ -404,26 +404,54 @@ __global__ void __launch_bounds__(kBeamThreads, 4)
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
     w = beam_join(w, BeamSum{__shfl_xor_sync(0xffffffffu, w.m, o), __shfl_xor_sync(0xffffffffu, w.s, o)});
-  const float nth = beam_warp_nth(m, (keep + kBeamWarps - 1) / kBeamWarps);
-  if (lane == 0) {
-    s_bar[warp] = nth;
-    s_sum[warp] = w;
-  }
-  __syncthreads();
-  float bar = s_bar[0];
-  for (int k = 1; k < kBeamWarps; ++k) bar = fminf(bar, s_bar[k]);
-  // the logits of the threads that hold candidates once more, a thread's by its whole warp
-  for (uint32_t who = __ballot_sync(0xffffffffu, m >= bar && m > -INFINITY); who; who &= who - 1) {
-    const int of = warp * 32 + __ffs(who) - 1;
-    for (int p = first + of + lane * kBeamThreads; p < last; p += 32 * kBeamThreads) {
-      const uint4 q = row.load(p, last);
-      if (!(BeamRow<T>::largest(q) >= bar)) continue;
+  // `keep` <= 32: the keep-th largest of the four best maxima of each warp; more: the lowest of the warps' shares of them
+  constexpr int BEST = 32 / kBeamWarps;
+  const bool few = keep <= 32;
+  if (few) {
+    float left = m;
 #pragma unroll
-      for (int e = 0; e < PER; ++e) {
-        const float v = BeamRow<T>::at(q, e);
-        if (!(v >= bar) || v == -INFINITY) continue;
-        const int at = atomicAdd(&s_count, 1);
-        if (at < kBeamHeld) u.held[at] = beam_key(v, row.origin + p * PER + e);
+    for (int k = 0; k < BEST; ++k) {
+      const float best = beam_warp_largest(left);
+      const uint32_t is = __ballot_sync(0xffffffffu, left == best);
+      if (lane == 0) s_bar[warp * BEST + k] = best;
+      if (lane == __ffs(is) - 1) left = -INFINITY;
+    }
+  } else {
+    const float nth = beam_warp_nth(m, (keep + kBeamWarps - 1) / kBeamWarps);
+    if (lane < BEST) s_bar[warp * BEST + lane] = nth;
+  }
+  if (lane == 0) s_sum[warp] = w;
+  __syncthreads();
+  float bar = s_bar[lane];
+  if (few) {
+    int above = 0;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) above += s_bar[k] > bar ? 1 : 0;
+    if (above >= keep) bar = INFINITY;
+  }
+  bar = -beam_warp_largest(-bar);
+  // the logits of the threads that hold candidates once more, a thread's by its whole warp, four threads' at a time
+  for (uint32_t who = __ballot_sync(0xffffffffu, m >= bar && m > -INFINITY); who;) {
+    int of[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      of[k] = who ? first + warp * 32 + __ffs(who) - 1 : last;
+      who &= who - 1;
+    }
+    for (int p = lane * kBeamThreads; first + p < last; p += 32 * kBeamThreads) {
+      uint4 q[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) q[k] = row.load(of[k] + p, last);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (!(BeamRow<T>::largest(q[k]) >= bar)) continue;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+          const float v = BeamRow<T>::at(q[k], e);
+          if (!(v >= bar) || v == -INFINITY) continue;
+          const int at = atomicAdd(&s_count, 1);
+          if (at < kBeamHeld) u.held[at] = beam_key(v, row.origin + (of[k] + p) * PER + e);
+        }
       }
     }
   }

@@ -23,8 +23,7 @@ namespace {
 constexpr int kShareMaxBatch = 4096, kShareMaxPages = 1 << 18;  // masks of them fit shared memory
 constexpr int kForkNoPages = 2, kForkTableNarrow = 3, kForkBad = 4;
 constexpr int kCompactMovesOver = 1, kCompactBad = 4;
-constexpr int kForkCluster = 8, kForkThreads = 512, kForkWarps = kForkThreads / 32;
-constexpr int kForkOne = 2048;        // pages up to which one CTA counts them: five exchanges fewer
+constexpr int kForkCluster = 8, kForkThreads = 1024;
 constexpr int kForkChunk = 128;       // entries of a block table that a warp takes at a time
 constexpr int kForkRun = 8;           // slots whose entries it counts together
 constexpr int kForkUnits = 4;         // owners that a thread asks for at a time
@@ -55,13 +54,14 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) 
   int* parents = rank + (a.batch + 1);           // [batch + 1]
   int* lengths = parents + (a.batch + 1);        // [batch + 1]
   uint32_t* gone_bits = reinterpret_cast<uint32_t*>(lengths + (a.batch + 1));  // of the CTA's pages
-  __shared__ int s_bad, s_narrow, s_back, s_warp[kForkWarps];
+  __shared__ int s_bad, s_narrow, s_back, s_warp[kForkThreads / 32];
   cg::cluster_group cluster = cg::this_cluster();
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, batch = a.batch, page = a.page;
+  const int threads = blockDim.x, warps = threads >> 5;
   const int cta = cluster.block_rank(), ctas = cluster.num_blocks();
   const bool counts = blockIdx.x < static_cast<unsigned>(ctas);
   if (t == 0) s_bad = s_narrow = 0;
-  for (int b = t; b < batch; b += kForkThreads) {
+  for (int b = t; b < batch; b += threads) {
     children[b] = 0;
     lowest[b] = INT_MAX;
     parents[b] = a.parent[b];
@@ -69,20 +69,20 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) 
   }
   // this CTA's share of the pages
   const int page0 = min(cta * a.per, a.pages), mine = counts ? min(a.per, a.pages - page0) : 0;
-  for (int i = t; i < mine; i += kForkThreads * kForkUnits) {
+  for (int i = t; i < mine; i += threads * kForkUnits) {
     int more[kForkUnits];
 #pragma unroll
     for (int e = 0; e < kForkUnits; ++e)
-      more[e] = i + e * kForkThreads < mine ? a.shares[page0 + i + e * kForkThreads] : 0;
+      more[e] = i + e * threads < mine ? a.shares[page0 + i + e * threads] : 0;
 #pragma unroll
     for (int e = 0; e < kForkUnits; ++e) {
       if (more[e] < 0) record_error(SJ_DEV_BAD_INDEX);
-      if (i + e * kForkThreads < mine) a.shares_out[page0 + i + e * kForkThreads] = max(more[e], 0);
+      if (i + e * threads < mine) a.shares_out[page0 + i + e * threads] = max(more[e], 0);
     }
   }
   __syncthreads();
   auto length = [&](int b) { return lengths[b]; };
-  for (int b = t; b < batch; b += kForkThreads) {
+  for (int b = t; b < batch; b += threads) {
     const int p = parents[b], n = length(b);
     if (p < -1 || p >= batch || n < 0 || n > INT_MAX - page) {
       s_bad = 1;
@@ -101,14 +101,14 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) 
   // copies of the slots before each, 32 slots a warp at a time
   {
     int taken = 0;
-    for (int b0 = 0; b0 < batch; b0 += kForkThreads) {
+    for (int b0 = 0; b0 < batch; b0 += threads) {
       const int b = b0 + t, p = b < batch && !status ? parents[b] : -1;
       const bool copied = p >= 0 && lowest[p] != b && length(p) % page != 0;
       const unsigned have = __ballot_sync(0xffffffffu, copied);
       if (lane == 0) s_warp[warp] = __popc(have);
       __syncthreads();
       int before = taken, all = 0;
-      for (int w = 0; w < kForkWarps; ++w) {
+      for (int w = 0; w < warps; ++w) {
         if (w < warp) before += s_warp[w];
         all += s_warp[w];
       }
@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) 
   const int writer = gridDim.x > static_cast<unsigned>(ctas) ? static_cast<int>(blockIdx.x) - ctas : blockIdx.x;
   if (writer >= 0) {
     const int chunks = (a.ld_table + kForkChunk - 1) / kForkChunk;
-    for (int u = writer * kForkWarps + warp; u < batch * chunks; u += writers * kForkWarps) {
+    for (int u = writer * warps + warp; u < batch * chunks; u += writers * warps) {
       const int b = u % batch, j0 = u / batch * kForkChunk, p = source(b);
       const bool copied = !status && rank[b] >= 0;
       const int n = p < 0 ? 0 : held(p), own = copied ? n - 1 : -1, end = min(n, j0 + kForkChunk);
@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) 
         }
       }
     }
-    const int first = writer * kForkThreads + t, step = writers * kForkThreads;
+    const int first = writer * threads + t, step = writers * threads;
     for (int i = taken + first; i < batch; i += step) {
       a.copies[3 * i] = a.copies[3 * i + 1] = -1;
       a.copies[3 * i + 2] = 0;
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) 
     // is the same, before it goes to memory.
     const int chunks = (a.ld_table + kForkChunk - 1) / kForkChunk, runs = (batch + kForkRun - 1) / kForkRun;
     constexpr int PER = kForkChunk / 32;
-    for (int u = cta * kForkWarps + warp; u < runs * chunks; u += ctas * kForkWarps) {
+    for (int u = cta * warps + warp; u < runs * chunks; u += ctas * warps) {
       const int p0 = u % runs * kForkRun, j0 = u / runs * kForkChunk + lane;
       int32_t id[kForkRun][PER];
 #pragma unroll
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) 
   __threadfence();
   cluster.sync();
   // a warp's run of this CTA's pages, in order
-  const int run = ((mine + kForkWarps - 1) / kForkWarps + 31) / 32 * 32;
+  const int run = ((mine + warps - 1) / warps + 31) / 32 * 32;
   const int i0 = min(warp * run, mine), i1 = min(i0 + run, mine);
   int gone = 0;
   for (int i = i0 + lane; i - lane < i1; i += 32 * kForkUnits) {
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) 
   __syncthreads();
   if (t == 0) {
     int sum = 0;
-    for (int w = 0; w < kForkWarps; ++w) sum += s_warp[w];
+    for (int w = 0; w < warps; ++w) sum += s_warp[w];
     s_back = sum;
   }
   cluster.sync();
@@ -475,7 +475,7 @@ extern "C" int sj_paged_fork(const int32_t* parent, int batch, int page, const i
     return fail(SJ_ERR_ARGUMENT, "sj_paged_fork: the new state needs buffers of its own");
   Fork a{parent, cached, block_table, shares, free_pages, free_count, cached_out, table_out, shares_out,
          free_out, count_out, copies, summary, batch, page, ld_table, pages, 0};
-  const int ctas = pages <= kForkOne ? 1 : kForkCluster;
+  constexpr int ctas = kForkCluster;
   a.per = (pages + ctas - 1) / ctas;
   const int smem = (5 * (batch + 1) + a.per / 32 + 1) * static_cast<int>(sizeof(int));
   static KernelAttrOnce once;
@@ -490,11 +490,11 @@ extern "C" int sj_paged_fork(const int32_t* parent, int batch, int page, const i
   attr[1].val.clusterDim.x = ctas;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  // tables of more chunks than the counting CTAs have warps are written by CTAs of their own
   const int64_t units = static_cast<int64_t>(batch) * ((ld_table + kForkChunk - 1) / kForkChunk);
-  const int64_t writers = units <= ctas * kForkWarps ? 0 : std::min<int64_t>((units - 1) / kForkWarps + 1, sm_count() / 2);
+  const int threads = units <= 512 ? 256 : kForkThreads;
+  const int64_t writers = std::min<int64_t>((units * 32 - 1) / threads + 1, sm_count() / 2);
   cfg.gridDim = dim3(static_cast<unsigned>(ctas * (1 + (writers + ctas - 1) / ctas)));
-  cfg.blockDim = dim3(kForkThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = as_stream(stream);
   cfg.attrs = attr;

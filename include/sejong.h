@@ -446,8 +446,9 @@ int sj_attn_paged(const void* q, int ldq, const void* k_cache, const void* v_cac
  *                    are read once for all of them, where that is faster (decided on the GPU by the sizes; with
  *                    SJ_ATTN_SHARE=always in the environment, wherever two rows share keys).  Each row still sees no
  *                    more than position[r] + 1 tokens and its window.  groups <= rows; more than 1024 of them, or
- *                    more than 128 query heads a KV head, share nothing.  A group out of order or out of range
- *                    records SJ_DEV_BAD_INDEX, and then no rows share.  Results are those of sj_attn_paged but for
+ *                    more than 128 query heads a KV head, share nothing.  Groups at the end whose first row is
+ *                    `rows` are empty.  A group out of order or out of range records SJ_DEV_BAD_INDEX, and then no
+ *                    rows share.  Results are those of sj_attn_paged but for
  *                    the order of the sums.  workspace: sj_attn_paged_shared_workspace bytes, zero before its first
  *                    use (each call leaves it ready for the next, of any size); one per stream. */
 int sj_paged_fork(const int32_t* parent, int batch, int page, const int32_t* cached, const int32_t* block_table,

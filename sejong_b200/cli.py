@@ -14,7 +14,8 @@ training step (crates/sejong-cli/src/main.rs:20-164 commands, 165-407 dispatch).
   init         Initialise a model and save its weights (main.rs:306-318).
   generate     Generate bytes with the KV cache (main.rs:334-390).
   generate-batch  Generate for every line of a file at once on a paged KV cache; one JSON line each, with the
-               log probabilities of the bytes and their best alternatives if asked for.
+               log probabilities of the bytes and their best alternatives if asked for.  Several samples of each
+               line, or the best of a beam search, share the line's pages.
   score        Log probability, entropy and alternatives of every byte of a text file no longer than the model's
                context, as JSON.
   inspect      Print a model artifact's configuration and provenance (main.rs:391-405).
@@ -741,8 +742,9 @@ def _score_record(scores):
 
 
 def generate_batch(model, prompts, max_bytes, temperature, top_k, top_p, seed, batch, page, pages, top, device=0,
-                   out=None):
-    """Generate for each line of the file `prompts` together; the i-th prompt draws with seed + i."""
+                   out=None, samples=1, beams=0):
+    """Generate for each line of the file `prompts` together; the i-th prompt draws with seed + i * samples.  `beams` > 0: a
+    beam search instead."""
     from . import checkpoint
     from .generate import Sampling
     from .serve import BatchGenerator
@@ -750,14 +752,27 @@ def generate_batch(model, prompts, max_bytes, temperature, top_k, top_p, seed, b
     with open(prompts, "rb") as fh:
         lines = fh.read().splitlines()
     gen = BatchGenerator(config, params=params, device=device, batch=batch, page=page, pages=pages)
-    options = [Sampling(temperature=temperature, top_k=top_k, top_p=top_p, seed=seed + i, max_bytes=max_bytes)
+    options = [Sampling(temperature=temperature, top_k=top_k, top_p=top_p, seed=seed + i * samples, max_bytes=max_bytes)
                for i in range(len(lines))]
-    for line, done in zip(lines, gen.generate(lines, options, top=top)):
-        record = {"prompt": line.decode(errors="replace"), "text": done.text.decode(errors="replace"),
-                  "ended": done.ended}
-        if done.scores is not None:
-            record["scores"] = _score_record(done.scores)
-        print(json.dumps(record), file=out or sys.stdout)
+
+    def record(done):
+        r = {"text": done.text.decode(errors="replace"), "ended": done.ended}
+        if getattr(done, "scores", None) is not None:
+            r["scores"] = _score_record(done.scores)
+        if beams:
+            r["score"] = done.score
+        return r
+
+    if beams:
+        found = gen.beam_search(lines, beams=beams, max_bytes=max_bytes)
+    else:
+        found = gen.generate(lines, options, top=top, samples=samples)
+    for line, done in zip(lines, found):
+        prompt = {"prompt": line.decode(errors="replace")}
+        if beams or samples > 1:
+            print(json.dumps({**prompt, "beams" if beams else "samples": [record(d) for d in done]}), file=out or sys.stdout)
+        else:
+            print(json.dumps({**prompt, **record(done)}), file=out or sys.stdout)
 
 
 def score(model, data, top, device=0, out=None):
@@ -821,6 +836,8 @@ def main(argv=None):
     p.add_argument("--page", type=int, default=16)
     p.add_argument("--pages", type=int, default=None)
     p.add_argument("--alternatives", type=int, default=None, help="score the drawn bytes, with this many alternatives")
+    p.add_argument("--samples", type=int, default=1, help="continuations of each prompt")
+    p.add_argument("--beams", type=int, default=0, help="the best continuations of a beam search instead")
     p = sub.add_parser("score", help="log probabilities of the bytes of a text file")
     p.add_argument("--model", required=True)
     p.add_argument("--data", required=True)
@@ -848,7 +865,7 @@ def main(argv=None):
         generate(a.model, a.prompt, a.max_bytes, a.temperature, a.top_k, a.top_p, a.seed, a.raw)
     elif a.command == "generate-batch":
         generate_batch(a.model, a.prompts, a.max_bytes, a.temperature, a.top_k, a.top_p, a.seed, a.batch, a.page,
-                       a.pages, a.alternatives)
+                       a.pages, a.alternatives, samples=a.samples, beams=a.beams)
     elif a.command == "score":
         score(a.model, a.data, a.alternatives)
     return 0

@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(1024) shared_spans_kernel(const SpansArgs a) {
   if (t < a.groups) {
     const int at = a.group[3 * t], b = a.group[3 * t + 1], n = a.group[3 * t + 2];
     const int next = t + 1 < a.groups ? a.group[3 * t + 3] : a.rows;
-    const bool fine = at >= 0 && at < next && next <= a.rows && b >= 0 && b < a.requests && n >= 0 && n <= most;
+    const bool fine = at >= 0 && (at < next || at == a.rows) && next <= a.rows && b >= 0 && b < a.requests && n >= 0 && n <= most;
     if (!fine) record_error(SJ_DEV_BAD_INDEX);
     first[t] = at;
     p0[t] = 0;

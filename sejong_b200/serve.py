@@ -17,6 +17,11 @@ to `batch` requests in one cache of `pages` pages a layer and steps them togethe
     context restarts from its last `context` tokens, as the reference does;
   * a call that raises leaves an empty cache.
 
+`generate` with `samples`, and `beam_search`, keep several continuations of each prompt.  The prompt runs once, and its
+requests share its pages: a step begins with a sj_paged_fork of the requests (which counts the owners of pages, and takes
+back those that nobody holds), a sj_paged_copy of half-filled pages, and its attention is sj_attn_paged_shared;
+sj_beam_select finds the best continuations of a request's beams.
+
 `score` gives the same figures for the bytes of a given text of at most `context` bytes.  `rope_scaling` stretches the
 rotary positions beyond the trained context (sj_rope_table_scaled).
 """
@@ -69,6 +74,24 @@ class Completion:
 
 
 @dataclass
+class Hypothesis:
+    """A beam search's result: `score` is the sum of the bytes' log probabilities, `ranked` what they are ordered by."""
+    text: bytes
+    ended: bool
+    score: float
+    ranked: float
+
+
+@dataclass
+class _Beams:
+    index: int
+    tokens: list
+    reserved: int
+    live: list = field(default_factory=list)     # (drawn bytes, score) of each beam
+    ended: list = field(default_factory=list)    # hypotheses
+
+
+@dataclass
 class _Request:
     index: int
     tokens: list
@@ -110,9 +133,8 @@ class BatchGenerator:
         e = lambda *shape, dt=torch.bfloat16: torch.empty(*shape, dtype=dt, device=self.dev)  # noqa: E731
         z = lambda *shape, dt=torch.int32: torch.zeros(*shape, dtype=dt, device=self.dev)  # noqa: E731
         # caches: heads outermost inside a page, so a page of a head is one run of memory
-        self.k = [e(self.pages, s.kv_heads, P, HEAD_DIM) for _ in range(s.layers)]
-        self.v = [e(self.pages, s.kv_heads, P, HEAD_DIM) for _ in range(s.layers)]
-        self.strides = self.k[0].stride()[:3]
+        self.k, self.v = (e(s.layers, self.pages, s.kv_heads, P, HEAD_DIM) for _ in range(2))
+        self.strides = self.k.stride()[1:4]
         self.rope = e(L * HEAD_DIM, dt=f32)
         if rope_scaling is None:
             call("sj_rope_table", _ptr(self.rope), L, HEAD_DIM, 0, float(c.rope_theta), self._stream())
@@ -129,11 +151,16 @@ class BatchGenerator:
         self.host = torch.zeros(2 * B + rows, dtype=torch.int32, pin_memory=True)
         self.input = z(2 * B + rows)
         self.added, self.release, self.ids = self.input[:B], self.input[B:2 * B], self.input[2 * B:]
-        self.cached, self.lengths, self.summary = z(B), z(B), z(4)
+        self.lengths, self.summary = z(B), z(4)
         self.planned = torch.zeros(4, dtype=torch.int32, pin_memory=True)  # the host's copy of the summary
-        self.table = torch.full((B, self.width), -1, dtype=torch.int32, device=self.dev)
-        self.free = torch.arange(self.pages, dtype=torch.int32, device=self.dev)
-        self.free_count = torch.full((1,), self.pages, dtype=torch.int32, device=self.dev)
+        # the cache's books in one buffer, so that they are replaced as a whole
+        self.state = z(B + B * self.width + 2 * self.pages + 1)
+        self.cached, self.table, self.shares, self.free, self.free_count = self._books(self.state)
+        self.table.fill_(-1)
+        torch.arange(self.pages, out=self.free)
+        self.free_count.fill_(self.pages)
+        self.spare = None  # what sharing needs, made when it is first used
+        self.shared_graph = None
         self.request, self.position, self.slot = z(rows), z(rows), z(rows)
         self.work = z(self.lib.sj_attn_paged_workspace(B, s.heads, s.kv_heads, HEAD_DIM), dt=torch.uint8)
         self.score_work = z(self.lib.sj_token_scores_workspace(rows, VOCAB, 32), dt=torch.uint8)
@@ -142,6 +169,11 @@ class BatchGenerator:
         self.finished = set()
         self.reserved = 0
         torch.cuda.current_stream(self.dev).synchronize()  # calls run on whichever stream is current then
+
+    def _books(self, state):
+        B, W, N = self.batch, self.width, self.pages
+        parts = torch.split(state, [B, B * W, N, N, 1])
+        return parts[0], parts[1].view(B, W), *parts[2:]
 
     # ---------------------------------------------------------------- kernels
     def _stream(self):
@@ -237,7 +269,7 @@ class BatchGenerator:
         self.slots = [None] * self.batch
         self.finished.clear()
         self.reserved = 0
-        for t in (self.cached, self.lengths, self.summary):
+        for t in (self.cached, self.lengths, self.summary, self.shares):
             t.zero_()
         self.table.fill_(-1)
         torch.arange(self.pages, out=self.free)
@@ -328,21 +360,327 @@ class BatchGenerator:
                 self.reserved -= q.reserved
         return done
 
+    # ---------------------------------------------------------------- requests that share pages
+    def _share(self):
+        """Buffers of steps whose requests share pages."""
+        if self.spare is not None:
+            return
+        B, s = self.batch, self.s
+        z = lambda *shape, dt=torch.int32: torch.zeros(*shape, dtype=dt, device=self.dev)  # noqa: E731
+        spare = torch.full_like(self.state, -1)
+        self.spare_books = self._books(spare)
+        # what the host writes for a step: tokens added, token ids, parents, groups (first row, request, tokens)
+        self.shared_host = torch.zeros(6 * B, dtype=torch.int32, pin_memory=True)
+        self.shared_input = z(6 * B)
+        self.shared_added, self.shared_ids, self.parent, self.group = torch.split(self.shared_input, [B, B, B, 3 * B])
+        self.copies, self.forked = z(B, 3), z(4)
+        self.shared_planned = torch.zeros(8, dtype=torch.int32, pin_memory=True)
+        self.shared_work = z(self.lib.sj_attn_paged_shared_workspace(B, B, s.heads, s.kv_heads, HEAD_DIM), dt=torch.uint8)
+        self.spare = spare
+
+    def _fork_and_plan(self, rows):
+        B, P, W = self.batch, self.page, self.width
+        call("sj_paged_commit", _ptr(self.cached), _ptr(self.lengths), 0, B, P, _ptr(self.table), W, _ptr(self.free),
+             _ptr(self.free_count), self.pages, _ptr(self.summary), self._stream())
+        cached, table, shares, free, count = self.spare_books
+        call("sj_paged_fork", _ptr(self.parent), B, P, _ptr(self.cached), _ptr(self.table), W, _ptr(self.shares),
+             _ptr(self.free), _ptr(self.free_count), self.pages, _ptr(cached), _ptr(table), _ptr(shares), _ptr(free),
+             _ptr(count), _ptr(self.copies), _ptr(self.forked), self._stream())
+        self.state.copy_(self.spare)
+        call("sj_paged_copy", _ptr(self.copies), B, _ptr(self.k), _ptr(self.v), self.s.layers, self.k.stride(0), self.pages,
+             P, *self.strides, self.s.kv_heads, HEAD_DIM, self._stream())
+        call("sj_paged_plan", _ptr(self.cached), _ptr(self.shared_added), B, P, _ptr(self.free), _ptr(self.free_count),
+             _ptr(self.table), W, _ptr(self.lengths), _ptr(self.request), _ptr(self.position), _ptr(self.slot), rows,
+             _ptr(self.summary), self._stream())
+
+    def _decode_shared(self):
+        """As _decode, after a fork of the requests, for rows that share keys."""
+        s, B = self.s, self.batch
+        d, cq = s.width, s.qkv_width
+
+        def attend(i, p):
+            self._gemm(_ptr(self.z), d, self._wb(f"{p}.qkv"), cq, _ptr(self.qkv), cq, SJ_BF16, B, cq, d)
+            self._append(i, _ptr(self.qkv), B, s.heads, HEAD_DIM, _ptr(self.qkv))
+            call("sj_attn_paged_shared", _ptr(self.qkv), cq, _ptr(self.k[i]), _ptr(self.v[i]), self.pages, self.page,
+                 *self.strides, _ptr(self.table), self.width, B, _ptr(self.request), _ptr(self.position), B,
+                 _ptr(self.group), B, s.heads, s.kv_heads, HEAD_DIM, s.window, _ptr(self.o), d, 0, _ptr(self.shared_work),
+                 self.shared_work.numel(), self._stream())
+
+        self._fork_and_plan(B)
+        call("sj_embedding_fwd", self._wb("embedding"), _ptr(self.shared_ids), _ptr(self.x), SJ_F32, B, s.width, VOCAB,
+             self._stream())
+        self._blocks(B, attend)
+        self._head(0, B, self.logits)
+
+    def _write_shared(self, parents, added, ids=(), groups=()):
+        """The host's part of a step.  `added`: tokens by slot; `groups`: (first row, slot, tokens in common)."""
+        B = self.batch
+        torch.cuda.current_stream(self.dev).synchronize()  # the last step's copy has been read
+        host = self.shared_host.numpy()
+        host[:2 * B] = 0
+        for b, n in added.items():
+            host[b] = n
+        host[B:B + len(ids)] = ids
+        host[2 * B:3 * B] = parents
+        rows = host[3 * B:].reshape(B, 3)
+        rows[:] = (B, 0, 0)  # an empty group
+        rows[:len(groups)] = np.asarray(groups, dtype=np.int32).reshape(-1, 3)
+        self.shared_input.copy_(self.shared_host, non_blocking=True)
+
+    def _start_shared(self, slot, tokens, pending):
+        """A prompt into a slot that is empty or has finished; its last row's logits are row 0.  `pending`: the next step's
+        parents, whose pages stay until then."""
+        gone = self.finished - {p for b, p in enumerate(pending) if p != b}
+        self.finished -= gone
+        self._write_shared([-1 if b in gone else b for b in range(self.batch)], {slot: len(tokens)})
+        self.ids[:len(tokens)].copy_(torch.tensor(tokens, dtype=torch.int32))
+        self._fork_and_plan(len(tokens))
+        self._prompt(len(tokens), True)
+        self._head(len(tokens) - 1, 1, self.logits)
+
+    def _step_shared(self, parents, live, ids, common):
+        """One step of the live slots, slot b going on from what parents[b] holds; common[b]: (block, tokens) that its
+        neighbours of the same block share."""
+        groups, last = [], None
+        for r, b in enumerate(live):
+            if common[b] is None or common[b] != last:
+                groups.append((r, b, 0 if common[b] is None else common[b][1]))
+            last = common[b]
+        for b in self.finished:
+            parents[b] = -1
+        self.finished.clear()
+        self._write_shared(parents, {b: 1 for b in live}, ids, groups)
+        if self.shared_graph is None:
+            self._decode_shared()  # what a first call sets up is not captured
+            torch.cuda.current_stream(self.dev).synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                self._decode_shared()
+            self.shared_graph = graph
+        else:
+            self.shared_graph.replay()
+
+    def _check_shared(self):
+        """After the step's results have been waited for."""
+        self.shared_planned[:4].copy_(self.summary)
+        self.shared_planned[4:].copy_(self.forked)
+        status, forked = int(self.shared_planned[2]), int(self.shared_planned[6])
+        if status or forked:
+            raise RuntimeError(f"a step could not be planned: status {status}, of the fork {forked}")
+
+    def _reserve(self, tokens, most_bytes, count):
+        """Pages that `count` continuations of a prompt may come to need: its full pages once, the rest and a page that a
+        fork takes before it returns others for each; all of them for each where a full context may start again."""
+        most = -(-min(self.context, len(tokens) + most_bytes) // self.page)
+        shared = len(tokens) // self.page if len(tokens) + most_bytes <= self.context else 0
+        pages = shared + count * (most - shared + 1)
+        if pages > self.pages:
+            raise ValueError(f"{count} continuations of a prompt may need {pages} pages of a cache of {self.pages}")
+        return pages
+
+    def _run_samples(self, waiting, count, top):
+        """`count` continuations of each prompt: (tokens, options, reserved) in, lists of completions out."""
+        results = [[None] * count for _ in waiting]
+        blocks = [None] * (self.batch // count)  # slots b * count .. of a prompt
+        todo = deque(enumerate(waiting))
+        parents, ids, common = list(range(self.batch)), {}, [None] * self.batch
+        left = {}  # pages and continuations of a block
+
+        def draw(slots, rows):
+            """A byte for each slot from a row of logits; finished ones leave."""
+            logits = self.logits[:max(rows) + 1, :VOCAB].cpu().numpy()
+            self._check_shared()
+            tokens = [sample(logits[r], self.slots[b].options, self.slots[b].state) for b, r in zip(slots, rows)]
+            scores = None
+            if top is not None:
+                scores = self._scores(self.logits[torch.tensor(rows, device=self.dev)], tokens, top)
+            for i, (b, token) in enumerate(zip(slots, tokens)):
+                q = self.slots[b]
+                if scores is not None:
+                    q.scores.logp.append(scores.logp[i])
+                    q.scores.entropy.append(scores.entropy[i])
+                    q.scores.alternatives.append(scores.alternatives[i])
+                if token != EOS:
+                    q.out.append(token)
+                    q.tokens.append(token)
+                if token == EOS or len(q.out) >= q.options.max_bytes:
+                    results[q.index][b % count] = Completion(bytes(q.out), token == EOS, q.scores)
+                    self.slots[b], parents[b] = None, b
+                    self.finished.add(b)
+                    left[b // count][1] -= 1
+                    if left[b // count][1] == 0:
+                        self.reserved -= left.pop(b // count)[0]
+                        blocks[b // count] = None
+                else:
+                    ids[b] = token
+
+        while todo or left:
+            for n, block in enumerate(blocks):
+                if block is None and todo and self.reserved + todo[0][1][2] <= self.pages:
+                    index, (tokens, options, reserved) = todo.popleft()
+                    blocks[n], left[n] = index, [reserved, count]
+                    self.reserved += reserved
+                    first = n * count
+                    self._start_shared(first, tokens, parents)
+                    for b in range(first, first + count):
+                        state = ctypes.c_uint64((int(options.seed) + b - first) & (2**64 - 1))
+                        self.slots[b] = _Request(index, list(tokens), options, state, 0, len(tokens),
+                                                 scores=None if top is None else Scores())
+                        parents[b], common[b] = first, (n, len(tokens))
+                    draw(list(range(first, first + count)), [0] * count)
+            for b, q in enumerate(self.slots):
+                if q is not None and q.length == self.context:  # a full context starts again from its tail, by itself
+                    self.finished.add(b)
+                    tail = q.tokens[-self.context:]
+                    self._start_shared(b, tail, parents)
+                    q.length, common[b] = len(tail), None
+                    draw([b], [0])
+            live = [b for b, q in enumerate(self.slots) if q is not None and q.length < self.context]
+            if live:
+                self._step_shared(parents, live, [ids[b] for b in live], common)
+                parents[:] = range(self.batch)
+                for b in live:
+                    self.slots[b].length += 1
+                draw(live, list(range(len(live))))
+        return results
+
+    def _select(self, rows, scores, beams, keep):
+        """(parent, token, score) [requests, keep] of the first rows of logits and the beams' scores."""
+        requests = rows // beams
+        score = torch.tensor(scores, dtype=torch.float32).to(self.dev)
+        ids = torch.empty(2, requests, keep, dtype=torch.int32, device=self.dev)
+        best = torch.empty(requests, keep, dtype=torch.float32, device=self.dev)
+        size = self.lib.sj_beam_select_workspace(requests, beams, VOCAB, keep)
+        work = torch.zeros(max(size, 1), dtype=torch.uint8, device=self.dev)
+        call("sj_beam_select", _ptr(self.logits), SJ_F32, VOCAB_PAD, _ptr(score), requests, beams, VOCAB, keep, _ptr(ids[0]),
+             _ptr(ids[1]), _ptr(best), _ptr(work), work.numel(), self._stream())
+        parent, token = ids.cpu().tolist()
+        self._check_shared()
+        return parent, token, best.cpu().tolist()
+
+    def _run_beams(self, waiting, beams, most_bytes, penalty):
+        results = [None] * len(waiting)
+        blocks = [None] * (self.batch // beams)
+        todo = deque(waiting)
+        parents, ids = list(range(self.batch)), {}
+
+        def rank(score, length):
+            return score / max(length, 1) ** penalty
+
+        def advance(n, parent, token, score):
+            """The best continuations of a block's beams: those that end are kept aside, the others go on."""
+            q, first, live = blocks[n], n * beams, []
+            for at, (p, t, total) in enumerate(zip(parent, token, score)):
+                if p < 0 or len(live) == beams:
+                    break
+                drawn = q.live[p][0]
+                if t == EOS:
+                    if at < beams:
+                        q.ended.append(Hypothesis(bytes(drawn), True, total, rank(total, len(drawn) + 1)))
+                    continue
+                parents[first + len(live)], ids[first + len(live)] = first + p, t
+                live.append((drawn + [t], total))
+            q.ended.sort(key=lambda h: -h.ranked)
+            del q.ended[beams:]
+            q.live = live
+            length = len(live[0][0]) if live else 0
+            # what goes on may still be worth more than the worst that has ended
+            hope = max((rank(s, length) for _, s in live), default=-float("inf"))
+            done = not live or length >= most_bytes or (len(q.ended) == beams and q.ended[-1].ranked >= hope)
+            if done:
+                rest = [Hypothesis(bytes(d), False, s, rank(s, len(d))) for d, s in live]
+                results[q.index] = sorted(q.ended + rest, key=lambda h: -h.ranked)[:beams]
+                blocks[n] = None
+                self.reserved -= q.reserved
+                parents[first:first + beams] = range(first, first + beams)
+                self.finished.update(range(first, first + beams))
+            else:
+                for b in range(first + len(live), first + beams):  # fewer tokens are allowed than there are beams
+                    parents[b], ids[b] = first, live[0][0][-1]
+                q.live += [(live[0][0], -float("inf"))] * (beams - len(live))
+
+        while todo or any(q is not None for q in blocks):
+            for n in range(len(blocks)):
+                if blocks[n] is None and todo and self.reserved + todo[0].reserved <= self.pages:
+                    blocks[n] = q = todo.popleft()
+                    self.reserved += q.reserved
+                    self._start_shared(n * beams, q.tokens, parents)
+                    q.live = [([], 0.0)]
+                    found = self._select(1, [0.0], 1, min(2 * beams, VOCAB))
+                    advance(n, *(f[0] for f in found))
+            running = [n for n, q in enumerate(blocks) if q is not None]
+            if not running:
+                continue
+            live = [n * beams + i for n in running for i in range(beams)]
+            common = [None] * self.batch
+            for b in live:
+                common[b] = (b // beams, len(blocks[b // beams].tokens))
+            self._step_shared(parents, live, [ids[b] for b in live], common)
+            parents[:] = range(self.batch)
+            scores = [s for n in running for _, s in blocks[n].live]
+            found = self._select(len(live), scores, beams, 2 * beams)
+            for i, n in enumerate(running):
+                advance(n, *(f[i] for f in found))
+        return results
+
+    def _guard(self, run, *args):
+        """run(*args), which leaves no requests behind, whether it ends or raises."""
+        try:
+            self._share()
+            results = run(*args)
+            code = self._device_error()
+            if code:
+                raise RuntimeError(f"device error {code} during generation")
+        except BaseException:
+            self._clear()
+            raise
+        self._clear()  # pages that were shared are counted anew
+        return results
+
+    def beam_search(self, prompts, beams=4, max_bytes=64, length_penalty=1.0):
+        """For each prompt the `beams` best continuations found (Hypothesis, the best first): those that end, or have
+        `max_bytes` bytes, ordered by their log probability over length ** length_penalty."""
+        if not 1 <= beams <= min(self.batch, 32):
+            raise ValueError("beams must be 1 to 32, and at most the batch")
+        if max_bytes < 1:
+            raise ValueError("max_bytes must be positive")
+        waiting = []
+        for i, prompt in enumerate(prompts):
+            tokens = [EOS] + list(bytes(prompt))
+            if len(tokens) + max_bytes > self.context:
+                raise ValueError("a prompt and its continuations have to fit the context")
+            waiting.append(_Beams(i, tokens, self._reserve(tokens, max_bytes, beams)))
+        return self._guard(self._run_beams, waiting, beams, max_bytes, float(length_penalty))
+
     def _admit(self, index, prompt, options, top):
         tokens = ([EOS] + list(bytes(prompt)))[-self.context:]
         most = min(self.context, len(tokens) + options.max_bytes)
         return _Request(index, tokens, options, ctypes.c_uint64(int(options.seed) & (2**64 - 1)), -(-most // self.page),
                         scores=None if top is None else Scores())
 
-    def generate(self, prompts, options=None, top=None):
+    def generate(self, prompts, options=None, top=None, samples=1):
         """Completions of the prompts (bytes), in their order.  `options`: one Sampling for all, or one each.
-        `top`: None for no scores, else how many alternatives (0 to 32) beside each drawn token's."""
+        `top`: None for no scores, else how many alternatives (0 to 32) beside each drawn token's.  `samples` > 1: a
+        list of that many completions for each prompt, drawn with its seed, its seed + 1, ...; they share its pages."""
         if options is None or isinstance(options, Sampling):
             options = [options or Sampling()] * len(prompts)
         if len(options) != len(prompts):
             raise ValueError("one Sampling for all prompts, or one for each")
         if top is not None and not 0 <= top <= 32:
             raise ValueError("top must be 0 to 32")
+        if not 1 <= samples <= self.batch:
+            raise ValueError("samples must be 1 to the batch")
+        if samples > 1:
+            shared = []
+            for prompt, o in zip(prompts, options):
+                if o.max_bytes < 1:
+                    raise ValueError("max_bytes must be positive")
+                check_sampling(o)
+                tokens = ([EOS] + list(bytes(prompt)))[-self.context:]
+                if len(tokens) == self.context:
+                    raise ValueError("a prompt that fills the context cannot be shared")
+                shared.append((tokens, o, self._reserve(tokens, o.max_bytes, samples)))
+            return self._guard(self._run_samples, shared, samples, top)
         waiting = deque(self._admit(i, p, o, top) for i, (p, o) in enumerate(zip(prompts, options)))
         for q in waiting:
             if q.reserved > self.pages:

@@ -645,18 +645,20 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
         wait(&q_full[stream], q_at[stream] & 1);
         ++q_at[stream];
       };
-      // A tile of a stream: both halves of P with the V at hand, then S of the next tile, whose K lies behind it.
-      auto tile = [&](int stream, int queries, bool first, bool more, bool last_user) {
-        const int v = slot, next = slot + 1 == L::STAGES ? 0 : slot + 1, next_turn = next == 0 ? turn ^ 1 : turn;
-        const uint32_t parity = tile_at[stream] & 1;
-        const bool value = peek(&full[v], turn);
-        wait(&p_full[stream * 2], parity);
-        settle(value, &full[v], turn);
-        outputs(stream, 0, v, first);
+      // A tile of a stream, in two steps: the product of the first half of P with the V at hand; that of the second, and
+      // S of the stream's next tile, whose K lies in the slot behind.
+      auto first_half = [&](int stream, bool first) {
+        const bool value = peek(&full[slot], turn);
+        wait(&p_full[stream * 2], tile_at[stream] & 1);
+        settle(value, &full[slot], turn);
+        outputs(stream, 0, slot, first);
         commit_products(is, &o_half[stream]);
+      };
+      auto second_half = [&](int stream, int queries, bool more, bool last_user) {
+        const int next = slot + 1 == L::STAGES ? 0 : slot + 1, next_turn = next == 0 ? turn ^ 1 : turn;
         const bool key = peek(&full[next], next_turn);
-        wait(&p_full[stream * 2 + 1], parity);
-        outputs(stream, 1, v, false);
+        wait(&p_full[stream * 2 + 1], tile_at[stream] & 1);
+        outputs(stream, 1, slot, false);
         ++tile_at[stream];
         if (last_user) release();
         if (more) {
@@ -678,8 +680,10 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
           scores(1, 1, slot);
           release();
           for (int i = 0; i < n0; ++i) {
-            tile(0, 0, i == 0, i + 1 < n0, false);
-            tile(1, 1, i == 0, i + 1 < n0, true);
+            first_half(0, i == 0);
+            first_half(1, i == 0);
+            second_half(0, 0, i + 1 < n0, false);
+            second_half(1, 1, i + 1 < n0, true);
           }
         } else {
           release();
@@ -689,8 +693,11 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
             release();
           }
           for (int i = 0; i < n0; ++i) {
-            tile(0, 0, i == 0, i + 1 < n0, true);
-            if (i < n1) tile(1, 0, i == 0, i + 1 < n1, true);
+            first_half(0, i == 0);
+            second_half(0, 0, i + 1 < n0, true);
+            if (i >= n1) continue;
+            first_half(1, i == 0);
+            second_half(1, 0, i + 1 < n1, true);
           }
         }
       }

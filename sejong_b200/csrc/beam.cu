@@ -24,8 +24,12 @@ namespace {
 constexpr int kBeamMaxBeams = 64, kBeamMaxKeep = 64, kBeamMaxRequests = 4096;
 constexpr int kBeamMaxColumns = INT_MAX - (1 << 16);  // 32 bits count to a chunk past the last column
 constexpr int kBeamNarrow = 1024;                       // logits of a row that a warp holds
-constexpr int kBeamThreads = 256, kBeamWarps = kBeamThreads / 32;
-constexpr int kBeamPieces = 4;                          // 16-byte pieces of a thread at a time
+// Small CTAs, since a part's end is a chain of waits (its sums, bar, candidates, their ranks, the arrival: about 7 us)
+// that the others have to cover: 1024 x 50001 bf16 41.9 us with eight CTAs of 128 threads an SM, 48.3 with ten (fewer
+// registers), 45.4 with four of 256; rows cut in two 62.
+constexpr int kBeamThreads = 128, kBeamWarps = kBeamThreads / 32, kBeamCtas = 8;
+constexpr int kBeamPieces = 3;                          // 16-byte pieces of a thread at a time (four: 2 us more)
+constexpr int kBeamLook = 4;                            // threads whose logits a warp looks at again at a time
 constexpr int kBeamMaxSplits = 32;
 constexpr int kBeamHeld = 512;                          // candidates of a part, or of a request
 constexpr size_t kBeamCounterBytes = kBeamMaxRequests * sizeof(int);  // of any call, so that calls of all sizes share a workspace
@@ -292,24 +296,47 @@ __global__ void __launch_bounds__(1024) beam_narrow_kernel(const T* logits, int 
 }
 
 // ---------------------------------------------------------------- wide rows
-// A part of a row in pieces of 16 bytes, counted from the 16-byte boundary at or before the row.
-template <typename T>
+// A row in pieces of 16 bytes from its first column on, so that equal rows have equal sums wherever they lie: beams that
+// are alike tie.  A row that does not begin at a multiple of 16 bytes takes a piece from two aligned ones.
+template <typename T, bool ALIGNED>
 struct BeamRow {
   static constexpr int PER = 16 / sizeof(T);
   static constexpr uint32_t NONE = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;  // -inf
   const T* x;
-  int vocab, origin;
+  int vocab, shift;  // bytes from the boundary before the row
   SJ_DEVICE BeamRow(const T* row, int vocab_)
-      : x(row), vocab(vocab_), origin(-static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T))) {}
-  SJ_DEVICE int pieces() const { return (vocab - origin + PER - 1) / PER; }
+      : x(row), vocab(vocab_), shift(ALIGNED ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16)) {}
+  SJ_DEVICE int pieces() const { return (vocab + PER - 1) / PER; }
   SJ_DEVICE uint4 load(int piece, int end) const {  // -inf outside the row, or from piece `end` on
-    const int j = origin + piece * PER;
+    const int j = piece * PER;
     if (piece >= end) return make_uint4(NONE, NONE, NONE, NONE);
-    if (j >= 0 && j + PER <= vocab) return *reinterpret_cast<const uint4*>(x + j);
+    if (shift == 0 && j + PER <= vocab) return *reinterpret_cast<const uint4*>(x + j);
+    if (!ALIGNED && shift != 0 && piece > 0 && j + 2 * PER - shift / static_cast<int>(sizeof(T)) <= vocab) {
+      const uint4* from = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(x + j) - shift);
+      const uint4 lo = from[0], hi = from[1];
+      uint32_t w[6] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y};
+      if (shift & 8) {
+        w[0] = lo.z;
+        w[1] = lo.w;
+        w[2] = hi.x;
+        w[3] = hi.y;
+        w[4] = hi.z;
+        w[5] = hi.w;
+      }
+      if (shift & 4) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+      }
+      if (shift & 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+      }
+      return make_uint4(w[0], w[1], w[2], w[3]);
+    }
     uint32_t w[4] = {NONE, NONE, NONE, NONE};
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-      if (j + e < 0 || j + e >= vocab) continue;
+      if (j + e >= vocab) continue;
       const uint32_t bits = __float_as_uint(beam_load(x + j + e));
       if (sizeof(T) == 4)
         w[e % 4] = bits;
@@ -337,20 +364,22 @@ struct BeamRow {
 __host__ __device__ constexpr size_t beam_part_bytes(int keep) { return 8 * (1 + static_cast<size_t>(keep)); }
 
 // Keys of [first, last) pieces that the CTA's threads own: f(key).
-template <typename T, typename F>
-SJ_DEVICE void beam_each_key(const BeamRow<T>& row, int first, int last, F f) {
+template <typename Row, typename F>
+SJ_DEVICE void beam_each_key(const Row& row, int first, int last, F f) {
   for (int p = first + static_cast<int>(threadIdx.x); p < last; p += kBeamThreads) {
     const uint4 q = row.load(p, last);
 #pragma unroll
-    for (int e = 0; e < BeamRow<T>::PER; ++e) f(beam_key(BeamRow<T>::at(q, e), row.origin + p * BeamRow<T>::PER + e));
+    for (int e = 0; e < Row::PER; ++e) f(beam_key(Row::at(q, e), p * Row::PER + e));
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kBeamThreads, 4)
+// ALIGNED: every row begins at a multiple of 16 bytes (the other form takes 1.3 times as long).
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(kBeamThreads, kBeamCtas)
     beam_wide_kernel(const T* logits, int ld, int splits, int* counters, uint64_t* parts, BeamOut out) {
   pdl_wait();
-  constexpr int PER = BeamRow<T>::PER, STEP = kBeamThreads * kBeamPieces;
+  using Row = BeamRow<T, ALIGNED>;
+  constexpr int PER = Row::PER, STEP = kBeamThreads * kBeamPieces;
   __shared__ union {
     uint64_t held[kBeamHeld];
     BeamList list;
@@ -359,24 +388,24 @@ __global__ void __launch_bounds__(kBeamThreads, 4)
   __shared__ float s_bar[32];
   __shared__ BeamSum s_sum[kBeamWarps];
   __shared__ int s_count, s_last;
-  __shared__ unsigned long long s_bars;
+  __shared__ unsigned long long s_bars, s_shares;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, keep = out.keep;
   const int row_at = blockIdx.x / splits, split = blockIdx.x % splits;
   const int request = row_at / out.beams;
   const size_t slot = beam_part_bytes(keep) / 8;
   uint64_t* mine = parts + static_cast<size_t>(blockIdx.x) * slot;
   const float score = out.score[row_at];
-  const BeamRow<T> row(logits + static_cast<size_t>(row_at) * ld, out.vocab);
+  const Row row(logits + static_cast<size_t>(row_at) * ld, out.vocab);
   const int pieces = row.pieces();
   const int first = static_cast<int>(static_cast<int64_t>(pieces) * split / splits);
   const int last = static_cast<int>(static_cast<int64_t>(pieces) * (split + 1) / splits);
   float m = -INFINITY;
   uint64_t s = 0;
   if (t == 0) s_count = 0;
-  if (score > -INFINITY) {
-    uint4 ahead[kBeamPieces];  // on their way while the last ones are added up
+  uint4 ahead[kBeamPieces];  // on their way while the last ones are added up, the first ones while the score is
 #pragma unroll
-    for (int i = 0; i < kBeamPieces; ++i) ahead[i] = row.load(first + t + i * kBeamThreads, last);
+  for (int i = 0; i < kBeamPieces; ++i) ahead[i] = row.load(first + t + i * kBeamThreads, last);
+  if (score > -INFINITY) {
     for (int p = first + t; p - t < last; p += STEP) {
       uint4 q[kBeamPieces];
 #pragma unroll
@@ -386,7 +415,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4)
       }
       float here = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < kBeamPieces; ++i) here = fmaxf(here, BeamRow<T>::largest(q[i]));
+      for (int i = 0; i < kBeamPieces; ++i) here = fmaxf(here, Row::largest(q[i]));
       if (here > m) {
         const float f = beam_exp2((m - here) * kLog2e);
         s = beam_mul2(s, beam_pair(f, f));
@@ -396,7 +425,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4)
 #pragma unroll
       for (int i = 0; i < kBeamPieces; ++i)
 #pragma unroll
-        for (int e = 0; e < PER; e += 2) s = beam_sum2(s, BeamRow<T>::at(q[i], e), BeamRow<T>::at(q[i], e + 1), base);
+        for (int e = 0; e < PER; e += 2) s = beam_sum2(s, Row::at(q[i], e), Row::at(q[i], e + 1), base);
     }
   }
   // ---- the part's sums, and a bar that at least `keep` of its logits reach: each warp brings its share of them
@@ -430,27 +459,27 @@ __global__ void __launch_bounds__(kBeamThreads, 4)
     if (above >= keep) bar = INFINITY;
   }
   bar = -beam_warp_largest(-bar);
-  // the logits of the threads that hold candidates once more, a thread's by its whole warp, four threads' at a time
+  // the logits of the threads that hold candidates once more, a thread's by its whole warp, several threads' at a time
   for (uint32_t who = __ballot_sync(0xffffffffu, m >= bar && m > -INFINITY); who;) {
-    int of[4];
+    int of[kBeamLook];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < kBeamLook; ++k) {
       of[k] = who ? first + warp * 32 + __ffs(who) - 1 : last;
       who &= who - 1;
     }
     for (int p = lane * kBeamThreads; first + p < last; p += 32 * kBeamThreads) {
-      uint4 q[4];
+      uint4 q[kBeamLook];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) q[k] = row.load(of[k] + p, last);
+      for (int k = 0; k < kBeamLook; ++k) q[k] = row.load(of[k] + p, last);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (!(BeamRow<T>::largest(q[k]) >= bar)) continue;
+      for (int k = 0; k < kBeamLook; ++k) {
+        if (!(Row::largest(q[k]) >= bar)) continue;
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
-          const float v = BeamRow<T>::at(q[k], e);
+          const float v = Row::at(q[k], e);
           if (!(v >= bar) || v == -INFINITY) continue;
           const int at = atomicAdd(&s_count, 1);
-          if (at < kBeamHeld) u.held[at] = beam_key(v, row.origin + (of[k] + p) * PER + e);
+          if (at < kBeamHeld) u.held[at] = beam_key(v, (of[k] + p) * PER + e);
         }
       }
     }
@@ -463,7 +492,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4)
     for (int bit = 63; bit >= 0; --bit) {
       const uint64_t want = reach | 1ull << bit;
       int have = 0;
-      beam_each_key<T>(row, first, last, [&](uint64_t key) { have += key >= want; });
+      beam_each_key(row, first, last, [&](uint64_t key) { have += key >= want; });
       have = __reduce_add_sync(0xffffffffu, have);
       __syncthreads();
       if (t == 0) s_count = 0;
@@ -475,7 +504,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4)
     __syncthreads();
     if (t == 0) s_count = 0;
     __syncthreads();
-    beam_each_key<T>(row, first, last, [&](uint64_t key) {
+    beam_each_key(row, first, last, [&](uint64_t key) {
       if (key != 0 && key >= reach) u.held[atomicAdd(&s_count, 1)] = key;
     });
     __syncthreads();
@@ -485,6 +514,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4)
   for (int i = t; i < n; i += kBeamThreads) {
     const uint64_t key = u.held[i];
     int rank = 0;
+#pragma unroll 8
     for (int k = 0; k < n; ++k) rank += u.held[k] > key ? 1 : 0;
     if (rank < keep) mine[1 + rank] = key;
   }
@@ -502,6 +532,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4)
     s_last = before == members - 1;
     if (s_last) counters[request] = 0;
     s_bars = 0;
+    s_shares = ~0ull;
     u.list.count = 0;
   }
   __syncthreads();
@@ -525,28 +556,33 @@ __global__ void __launch_bounds__(kBeamThreads, 4)
     offset[t] = beam_offset(out.score[static_cast<size_t>(request) * out.beams + t], top, sum);
   }
   __syncthreads();
-  // a bar again: a full list's last total; totals as order-preserving integers
-  auto up = [](double d) {
-    const unsigned long long bits = static_cast<unsigned long long>(__double_as_longlong(d + 0.0));
+  // A bar again: a full list's last total, or the lowest of the lists' shares of `keep`; totals as order-preserving
+  // integers, 0 for none.
+  auto up = [&](int list, uint64_t key) {
+    const double total = key == 0 ? -INFINITY : offset[list / splits].total(beam_value(key));
+    if (!(total > -INFINITY)) return 0ull;
+    const unsigned long long bits = static_cast<unsigned long long>(__double_as_longlong(total + 0.0));
     return bits ^ (static_cast<unsigned long long>(static_cast<long long>(bits) >> 63) | 0x8000000000000000ull);
   };
-  for (int k = t; k < members; k += kBeamThreads) {
-    const uint64_t key = __ldcg(all + static_cast<size_t>(k) * slot + keep);
-    const double total = key == 0 ? -INFINITY : offset[k / splits].total(beam_value(key));
-    if (total > -INFINITY) atomicMax(&s_bars, up(total));
+  const int share = (keep + members - 1) / members;
+  for (int i = t; i < members * keep; i += kBeamThreads) {
+    const int list = i / keep, at = i - list * keep + 1;
+    if (at != keep && at != share) continue;
+    const unsigned long long total = up(list, __ldcg(all + static_cast<size_t>(list) * slot + at));
+    if (at == keep) atomicMax(&s_bars, total);
+    if (at == share) atomicMin(&s_shares, total);
   }
   __syncthreads();
-  const unsigned long long request_bar = s_bars;
+  const unsigned long long request_bar = max(s_bars, s_shares);
   for (int i = t; i < members * keep; i += kBeamThreads) {
-    const int k = i / keep;
-    const uint64_t key = __ldcg(all + static_cast<size_t>(k) * slot + 1 + i % keep);
-    if (key == 0) continue;
-    const double total = offset[k / splits].total(beam_value(key));
-    if (!(total > -INFINITY) || up(total) < request_bar) continue;
+    const int list = i / keep;
+    const uint64_t key = __ldcg(all + static_cast<size_t>(list) * slot + 1 + i - list * keep);
+    const unsigned long long total = up(list, key);
+    if (total == 0 || total < request_bar) continue;
     const int at = atomicAdd(&u.list.count, 1);
     if (at < kBeamHeld) {
-      u.list.total[at] = total;
-      u.list.beam[at] = k / splits;
+      u.list.total[at] = offset[list / splits].total(beam_value(key));
+      u.list.beam[at] = list / splits;
       u.list.column[at] = beam_column(key);
     }
   }
@@ -626,7 +662,8 @@ int beam_select(const T* x, int ld, int requests, const BeamOut& out, void* work
   }
   const int64_t rows = static_cast<int64_t>(requests) * out.beams;
   const int splits = beam_splits(rows, out.vocab);
-  launch(beam_wide_kernel<T>, static_cast<unsigned>(rows * splits), kBeamThreads, 0, s, x, ld, splits,
+  const bool aligned = aligned16(x) && ld * sizeof(T) % 16 == 0;
+  launch(aligned ? beam_wide_kernel<T, true> : beam_wide_kernel<T, false>, static_cast<unsigned>(rows * splits), kBeamThreads, 0, s, x, ld, splits,
          static_cast<int*>(workspace),
          reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + kBeamCounterBytes), out);
   SJ_LAUNCH_CHECK("beam_wide");

@@ -118,6 +118,9 @@ def test_selection_of_ties(vocab, dtype):
     x[1, :, 7::5] = 1.0
     check_select(x, torch.tensor([[-1.0, -1.0, -1.0], [-3.0, -2.0, -2.0]]), 20, dtype)
     check_select(torch.full((1, 64, vocab), 2.5), torch.zeros(1, 64), 64, dtype)
+    x, _ = logits(1, 1, vocab, 6)  # beams that are alike, in rows that begin anywhere
+    for pad in (0, 1, 2, 5):
+        check_select(x.expand(1, 7, vocab).contiguous(), torch.full((1, 7), -2.0), 25, dtype, pad)
     x = torch.arange(vocab).flip(0).float().expand(1, 2, vocab) / 64  # falling along the row
     check_select(x, torch.tensor([[-1.0, -1.5]]), 30)
     check_select(x.flip(2), torch.tensor([[-1.0, -1.5]]), 30)

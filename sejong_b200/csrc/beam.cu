@@ -138,6 +138,33 @@ SJ_DEVICE BeamOffset beam_offset(float score, float m, double s) {
   return BeamOffset{is ? static_cast<double>(score) - log(s) : __longlong_as_double(0x7ff8000000000000ll), m};
 }
 
+// An order-preserving integer of a total; 0 where it is none.
+SJ_DEVICE unsigned long long beam_up(double total) {
+  if (!(total > -INFINITY)) return 0;
+  const unsigned long long bits = static_cast<unsigned long long>(__double_as_longlong(total + 0.0));
+  return bits ^ (static_cast<unsigned long long>(static_cast<long long>(bits) >> 63) | 0x8000000000000000ull);
+}
+// The highest 32 bits that at least `keep` of the values reach of which each thread of the CTA counts its own, bit by
+// bit (0 where there are fewer); it stops where exactly `keep` reach them.  counts: 32 in shared memory.
+template <typename F>
+SJ_DEVICE uint32_t beam_reach(int keep, int* counts, F count) {
+  __syncthreads();
+  if (threadIdx.x < 32) counts[threadIdx.x] = 0;
+  __syncthreads();
+  uint32_t reach = 0;
+#pragma unroll 1
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t want = reach | 1u << bit;
+    const int have = __reduce_add_sync(0xffffffffu, count(want));
+    if ((threadIdx.x & 31) == 0 && have) atomicAdd(&counts[bit], have);
+    __syncthreads();
+    const int all = counts[bit];
+    if (all >= keep) reach = want;
+    if (all == keep) break;
+  }
+  return reach;
+}
+
 // A request's candidates: totals, and beams and columns as one order.
 struct BeamList {
   double total[kBeamHeld];
@@ -215,29 +242,45 @@ __global__ void __launch_bounds__(1024) beam_narrow_kernel(const T* logits, int 
   __syncthreads();
   double bar = -INFINITY;
   for (int b = 0; b < out.beams; ++b) bar = fmax(bar, bars[b]);
-  for (int b = warp; b < out.beams; b += warps) {
-    const BeamOffset off = offset[b];
-    if (!(off.add == off.add)) continue;
-    if (out.beams > warps) load(b);
+  auto each = [&](auto use) {  // the totals of this thread
+    for (int b = warp; b < out.beams; b += warps) {
+      const BeamOffset off = offset[b];
+      if (!(off.add == off.add)) continue;
+      if (out.beams > warps) load(b);
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const double total = off.total(v[i]);
-      if (!(total >= bar) || !(total > -INFINITY)) continue;
+      for (int i = 0; i < R; ++i) use(off.total(v[i]), b, i * 32 + lane);
+    }
+  };
+  auto collect = [&](auto reaches) {
+    each([&](double total, int b, int column) {
+      if (!reaches(total) || !(total > -INFINITY)) return;
       const int at = atomicAdd(&list.count, 1);
       if (at < kBeamHeld) {
         list.total[at] = total;
         list.beam[at] = b;
-        list.column[at] = i * 32 + lane;
+        list.column[at] = column;
       }
-    }
+    });
+    __syncthreads();
+    return list.count;
+  };
+  int n = collect([&](double total) { return total >= bar; });
+  if (n > kBeamHeld) {  // too low a bar, as of many beams that are worth much the same
+    __shared__ int counts[32];
+    const uint32_t reach = beam_reach(out.keep, counts, [&](uint32_t want) {
+      int have = 0;
+      each([&](double total, int, int) { have += beam_up(total) >> 32 >= want; });
+      return have;
+    });
+    if (threadIdx.x == 0) list.count = 0;
+    __syncthreads();
+    n = collect([&](double total) { return beam_up(total) >> 32 >= reach; });
   }
-  __syncthreads();
-  const int n = list.count;
   if (n <= kBeamHeld) {
     beam_rank(out, request, list, n, blockDim.x);
     return;
   }
-  // ties, or no bar: one after the other, each the best one after the last
+  // more ties than the list holds: one after the other, each the best one after the last
   __shared__ double s_total[32];
   __shared__ int s_beam[32], s_column[32];
   double last = INFINITY;
@@ -373,6 +416,167 @@ SJ_DEVICE void beam_each_key(const Row& row, int first, int last, F f) {
   }
 }
 
+// What the CTA that ends a request has in shared memory.
+struct BeamJoin {
+  BeamList list;
+  BeamOffset offset[kBeamMaxBeams];
+  int counts[32];
+  unsigned long long bar, shares;
+};
+SJ_DEVICE unsigned long long beam_up(const BeamJoin& join, int splits, int list, uint64_t key) {
+  return key == 0 ? 0ull : beam_up(join.offset[list / splits].total(beam_value(key)));
+}
+// What is rare in a join is not inlined: its registers and instructions would stand in the way of the rest.
+//
+// What `keep` of the lists' first totals reach, `firsts` of each.
+__device__ __noinline__ unsigned long long beam_join_bar(BeamJoin& join, const uint64_t* all, size_t slot, int splits,
+                                                         int members, int keep, int firsts) {
+  constexpr int MOST = (kBeamMaxBeams * kBeamMaxSplits + kBeamMaxKeep) / kBeamThreads + 1;  // of a thread
+  uint32_t high[MOST];
+#pragma unroll
+  for (int k = 0; k < MOST; ++k) {
+    const int i = static_cast<int>(threadIdx.x) + k * kBeamThreads, list = i / firsts;
+    high[k] = 0;
+    if (list < members)
+      high[k] = static_cast<uint32_t>(
+          beam_up(join, splits, list, __ldcg(all + static_cast<size_t>(list) * slot + 1 + i % firsts)) >> 32);
+  }
+  const uint32_t reach = beam_reach(keep, join.counts, [&](uint32_t want) {
+    int have = 0;
+#pragma unroll
+    for (int k = 0; k < MOST; ++k) have += high[k] >= want;
+    return have;
+  });
+  return static_cast<unsigned long long>(reach) << 32;
+}
+// More ties than the list holds: one candidate after the other.
+__device__ __noinline__ void beam_join_ties(const BeamOut& out, BeamJoin& join, const uint64_t* all, size_t slot,
+                                            int splits, int request) {
+  const int t = threadIdx.x, keep = out.keep, members = out.beams * splits;
+  double done = INFINITY;
+  int done_beam = -1, done_column = -1;
+  double* s_total = join.list.total;
+  for (int k = 0; k < keep; ++k) {
+    double best = -INFINITY;
+    int beam = -1, column = -1;
+    for (int i = t; i < members * keep; i += kBeamThreads) {
+      const int at = i / keep, b = at / splits;
+      const uint64_t key = __ldcg(all + static_cast<size_t>(at) * slot + 1 + i % keep);
+      if (key == 0) continue;
+      const double total = join.offset[b].total(beam_value(key));
+      const int c = beam_column(key);
+      if (!(total > -INFINITY)) continue;
+      const bool left = total < done || (total == done && (b > done_beam || (b == done_beam && c > done_column)));
+      if (left && (beam < 0 || total > best || (total == best && (b < beam || (b == beam && c < column))))) {
+        best = total;
+        beam = b;
+        column = c;
+      }
+    }
+    __syncthreads();
+    s_total[t] = best;
+    join.list.beam[t] = beam;
+    join.list.column[t] = column;
+    __syncthreads();
+    best = -INFINITY;
+    beam = column = -1;
+    for (int i = 0; i < kBeamThreads; ++i) {
+      const int b2 = join.list.beam[i], c2 = join.list.column[i];
+      const double t2 = s_total[i];
+      if (b2 >= 0 && (beam < 0 || t2 > best || (t2 == best && (b2 < beam || (b2 == beam && c2 < column))))) {
+        best = t2;
+        beam = b2;
+        column = c2;
+      }
+    }
+    done = best;
+    done_beam = beam;
+    done_column = column;
+    if (t == 0) beam_write(out, static_cast<size_t>(request) * keep + k, beam, column, best);
+  }
+}
+// A request's parts joined by a CTA.
+SJ_DEVICE void beam_join_parts(const BeamOut& out, const uint64_t* parts, int request, int splits,
+                                             BeamJoin& join) {
+  const int t = threadIdx.x, keep = out.keep, members = out.beams * splits;
+  const size_t slot = beam_part_bytes(keep) / 8;
+  if (t == 0) {
+    join.list.count = 0;
+    join.bar = 0;
+    join.shares = ~0ull;
+  }
+  const uint64_t* all = parts + static_cast<size_t>(request) * members * slot;
+  if (t < out.beams) {
+    float top = -INFINITY;
+    double sum = 0.0;
+    for (int k = 0; k < splits; ++k) {
+      const uint64_t word = __ldcg(all + static_cast<size_t>(t * splits + k) * slot);
+      const float part_m = __uint_as_float(static_cast<uint32_t>(word >> 32));
+      const double part_s = __uint_as_float(static_cast<uint32_t>(word));
+      const float raised = fmaxf(top, part_m);
+      if (raised == -INFINITY) {
+        sum += part_s;
+        continue;
+      }
+      sum = sum * exp(static_cast<double>(top) - raised) + part_s * exp(static_cast<double>(part_m) - raised);
+      top = raised;
+    }
+    join.offset[t] = beam_offset(out.score[static_cast<size_t>(request) * out.beams + t], top, sum);
+  }
+  __syncthreads();
+  // A bar again: what `keep` of the lists' first totals reach, as many of each as it takes; where the list holds all
+  // candidates, the lowest of them or the last total of a list will do.
+  auto up = [&](int list, uint64_t key) { return beam_up(join, splits, list, key); };
+  const int firsts = (keep + members - 1) / members;
+  if (members * keep <= kBeamHeld) {
+    for (int i = t; i < 2 * members; i += kBeamThreads) {
+      const bool whole = i >= members;  // a list's last total is one, too
+      const int list = whole ? i - members : i;
+      const unsigned long long total = up(list, __ldcg(all + static_cast<size_t>(list) * slot + (whole ? keep : firsts)));
+      if (whole)
+        atomicMax(&join.bar, total);
+      else
+        atomicMin(&join.shares, total);
+    }
+    __syncthreads();
+  } else {
+    const unsigned long long bar = beam_join_bar(join, all, slot, splits, members, keep, firsts);
+    if (t == 0) {
+      join.bar = bar;
+      join.shares = 0;
+    }
+    __syncthreads();
+  }
+  const unsigned long long request_bar = max(join.bar, join.shares);
+  // false: the list's others do not reach it either
+  auto file = [&](int list, int k) {
+    const uint64_t key = __ldcg(all + static_cast<size_t>(list) * slot + 1 + k);
+    const unsigned long long total = up(list, key);
+    if (total == 0 || total < request_bar) return false;
+    const int at = atomicAdd(&join.list.count, 1);
+    if (at < kBeamHeld) {
+      join.list.total[at] = join.offset[list / splits].total(beam_value(key));
+      join.list.beam[at] = list / splits;
+      join.list.column[at] = beam_column(key);
+    }
+    return true;
+  };
+  if (members >= kBeamThreads / 2) {  // a thread for a list
+    for (int list = t; list < members; list += kBeamThreads)
+      for (int k = 0; k < keep && file(list, k); ++k) {
+      }
+  } else {
+    for (int i = t; i < members * keep; i += kBeamThreads) file(i / keep, i % keep);
+  }
+  __syncthreads();
+  const int n = join.list.count;
+  if (n <= kBeamHeld) {
+    beam_rank(out, request, join.list, n, kBeamThreads);
+    return;
+  }
+  beam_join_ties(out, join, all, slot, splits, request);
+}
+
 // ALIGNED: every row begins at a multiple of 16 bytes (the other form takes 1.3 times as long).
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(kBeamThreads, kBeamCtas)
@@ -380,15 +584,14 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamCtas)
   pdl_wait();
   using Row = BeamRow<T, ALIGNED>;
   constexpr int PER = Row::PER, STEP = kBeamThreads * kBeamPieces;
-  __shared__ union {
+  __shared__ union Shared {
     uint64_t held[kBeamHeld];
-    BeamList list;
+    BeamJoin join;
+    __device__ Shared() {}
   } u;
-  __shared__ BeamOffset offset[kBeamMaxBeams];
   __shared__ float s_bar[32];
   __shared__ BeamSum s_sum[kBeamWarps];
   __shared__ int s_count, s_last;
-  __shared__ unsigned long long s_bars, s_shares;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, keep = out.keep;
   const int row_at = blockIdx.x / splits, split = blockIdx.x % splits;
   const int request = row_at / out.beams;
@@ -531,109 +734,10 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamCtas)
     asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(counters + request) : "memory");
     s_last = before == members - 1;
     if (s_last) counters[request] = 0;
-    s_bars = 0;
-    s_shares = ~0ull;
-    u.list.count = 0;
   }
   __syncthreads();
   if (!s_last) return;
-  const uint64_t* all = parts + static_cast<size_t>(request) * members * slot;
-  if (t < out.beams) {
-    float top = -INFINITY;
-    double sum = 0.0;
-    for (int k = 0; k < splits; ++k) {
-      const uint64_t word = __ldcg(all + static_cast<size_t>(t * splits + k) * slot);
-      const float part_m = __uint_as_float(static_cast<uint32_t>(word >> 32));
-      const double part_s = __uint_as_float(static_cast<uint32_t>(word));
-      const float raised = fmaxf(top, part_m);
-      if (raised == -INFINITY) {
-        sum += part_s;
-        continue;
-      }
-      sum = sum * exp(static_cast<double>(top) - raised) + part_s * exp(static_cast<double>(part_m) - raised);
-      top = raised;
-    }
-    offset[t] = beam_offset(out.score[static_cast<size_t>(request) * out.beams + t], top, sum);
-  }
-  __syncthreads();
-  // A bar again: a full list's last total, or the lowest of the lists' shares of `keep`; totals as order-preserving
-  // integers, 0 for none.
-  auto up = [&](int list, uint64_t key) {
-    const double total = key == 0 ? -INFINITY : offset[list / splits].total(beam_value(key));
-    if (!(total > -INFINITY)) return 0ull;
-    const unsigned long long bits = static_cast<unsigned long long>(__double_as_longlong(total + 0.0));
-    return bits ^ (static_cast<unsigned long long>(static_cast<long long>(bits) >> 63) | 0x8000000000000000ull);
-  };
-  const int share = (keep + members - 1) / members;
-  for (int i = t; i < members * keep; i += kBeamThreads) {
-    const int list = i / keep, at = i - list * keep + 1;
-    if (at != keep && at != share) continue;
-    const unsigned long long total = up(list, __ldcg(all + static_cast<size_t>(list) * slot + at));
-    if (at == keep) atomicMax(&s_bars, total);
-    if (at == share) atomicMin(&s_shares, total);
-  }
-  __syncthreads();
-  const unsigned long long request_bar = max(s_bars, s_shares);
-  for (int i = t; i < members * keep; i += kBeamThreads) {
-    const int list = i / keep;
-    const uint64_t key = __ldcg(all + static_cast<size_t>(list) * slot + 1 + i - list * keep);
-    const unsigned long long total = up(list, key);
-    if (total == 0 || total < request_bar) continue;
-    const int at = atomicAdd(&u.list.count, 1);
-    if (at < kBeamHeld) {
-      u.list.total[at] = offset[list / splits].total(beam_value(key));
-      u.list.beam[at] = list / splits;
-      u.list.column[at] = beam_column(key);
-    }
-  }
-  __syncthreads();
-  n = u.list.count;
-  if (n <= kBeamHeld) {
-    beam_rank(out, request, u.list, n, kBeamThreads);
-    return;
-  }
-  // more ties than the list holds: one after the other
-  double done = INFINITY;
-  int done_beam = -1, done_column = -1;
-  double* s_total = u.list.total;
-  for (int k = 0; k < keep; ++k) {
-    double best = -INFINITY;
-    int beam = -1, column = -1;
-    for (int i = t; i < members * keep; i += kBeamThreads) {
-      const int at = i / keep, b = at / splits;
-      const uint64_t key = __ldcg(all + static_cast<size_t>(at) * slot + 1 + i % keep);
-      if (key == 0) continue;
-      const double total = offset[b].total(beam_value(key));
-      const int c = beam_column(key);
-      if (!(total > -INFINITY)) continue;
-      const bool left = total < done || (total == done && (b > done_beam || (b == done_beam && c > done_column)));
-      if (left && (beam < 0 || total > best || (total == best && (b < beam || (b == beam && c < column))))) {
-        best = total;
-        beam = b;
-        column = c;
-      }
-    }
-    __syncthreads();
-    s_total[t] = best;
-    u.list.beam[t] = beam;
-    u.list.column[t] = column;
-    __syncthreads();
-    best = -INFINITY;
-    beam = column = -1;
-    for (int i = 0; i < kBeamThreads; ++i) {
-      const int b2 = u.list.beam[i], c2 = u.list.column[i];
-      const double t2 = s_total[i];
-      if (b2 >= 0 && (beam < 0 || t2 > best || (t2 == best && (b2 < beam || (b2 == beam && c2 < column))))) {
-        best = t2;
-        beam = b2;
-        column = c2;
-      }
-    }
-    done = best;
-    done_beam = beam;
-    done_column = column;
-    if (t == 0) beam_write(out, static_cast<size_t>(request) * keep + k, beam, column, best);
-  }
+  beam_join_parts(out, parts, request, splits, u.join);
 }
 
 }  // namespace sj

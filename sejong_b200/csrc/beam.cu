@@ -11,6 +11,11 @@
 //
 // Each logit is read once from memory; a bar that at least `keep` logits reach, found from the threads' maxima, picks
 // the few threads whose logits are looked at again.
+//
+// Measured on B200 (graph replays): 128 requests of 8 beams, 50001 bf16 logits, 16 kept 43 us (2.4 TB/s; 27 without the
+// candidates, which are chains of waits at a row's and a request's end), f32 70 (2.9 TB/s); one request of 5 beams,
+// 131075 f32 logits 29; 16 requests of 4 beams, 257 f32 logits 6.4, where latency counts.  Candidates sought by each
+// thread in its own logits took 53 us on the first, 25 waits one after the other.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -577,7 +582,7 @@ SJ_DEVICE void beam_join_parts(const BeamOut& out, const uint64_t* parts, int re
   beam_join_ties(out, join, all, slot, splits, request);
 }
 
-// ALIGNED: every row begins at a multiple of 16 bytes (the other form takes 1.3 times as long).
+// ALIGNED: every row begins at a multiple of 16 bytes (128 x 8 x 50001 bf16 43 us, otherwise 64).
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(kBeamThreads, kBeamCtas)
     beam_wide_kernel(const T* logits, int ld, int splits, int* counters, uint64_t* parts, BeamOut out) {

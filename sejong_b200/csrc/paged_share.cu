@@ -44,7 +44,9 @@ struct Fork {
 // entry of a slot with c children changes its page's owners by c - 1 (the half-filled page of a slot without children
 // by -1), by integer additions to shares_out, whose order does not matter.  Then each CTA knows which of its pages
 // nobody holds, and after one exchange of numbers where on the stack they go.  The other clusters (the same one, where
-// there is only one) write tables.
+// there is only one) write tables.  Bound by latency, four phases of a few dependent loads: 32 requests 8.6 us (graph
+// replays), 1024 requests of 500 to 32768 tokens in pages of 64 21.7 (34 with an addition to memory, or to another CTA's,
+// for each entry).
 __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) {
   pdl_wait();
   extern __shared__ int dynamic[];
@@ -284,7 +286,9 @@ struct PagedCopy {
 };
 
 // A CTA takes kCopyThreads * kCopyPieces pieces of 16 bytes of one copy, of K or of V of one layer; a page's rows and
-// heads go in the order in which they lie in memory.  All loads of a thread are in flight before its first store.
+// heads go in the order in which they lie in memory.  All loads of a thread are in flight before its first store.  2003
+// pages of 64 rows of 8 heads of 128: 159 us, 6.6 TB/s in and out (the measured copy rate); 13 half-filled pages of six
+// layers 2.1.
 template <int DIM>
 __global__ void __launch_bounds__(kCopyThreads) paged_copy_kernel(const PagedCopy a) {
   pdl_wait();
@@ -326,7 +330,9 @@ struct Compact {
 };
 
 // Every CTA reads the whole stack into a bit mask of the free pages with the numbers of pages in use before each word,
-// and writes its share of the results: the i-th page in use from `used` on goes to the i-th free page below it.
+// and writes its share of the results: the i-th page in use from `used` on goes to the i-th free page below it.  One launch
+// without a wait for other CTAs; bound by the shared-memory atomics of the mask (1024 requests on 183 thousand pages, half of
+// them free, 26 us; 32 requests on a thousand 6.3).
 __global__ void __launch_bounds__(kCompactThreads) paged_compact_kernel(const Compact a) {
   pdl_wait();
   extern __shared__ uint32_t bits[];                          // a bit for each page: free

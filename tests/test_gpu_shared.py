@@ -576,6 +576,100 @@ def test_shared_reports_groups_out_of_range(group):
     assert (out[0][1] - out[1][1]).abs().max() < 1e-4
 
 
+def shared_call(q, k, v, table, request, position, group, hq, hk, dim, window=0, work=None, out=None):
+    from sejong_b200 import _lib
+    rows, groups = q.shape[0], group.shape[0]
+    o, lse = out or (torch.empty_like(q), torch.empty(rows, hq, device=DEV))
+    size = _lib.load().sj_attn_paged_shared_workspace(rows, groups, hq, hk, dim)
+    work = torch.zeros(size, dtype=torch.uint8, device=DEV) if work is None else work
+    call("sj_attn_paged_shared", ptr(q), q.shape[1], ptr(k), ptr(v), k.shape[0], k.shape[2], *k.stride()[:3], ptr(table),
+         table.shape[1], table.shape[0], ptr(request), ptr(position), rows, ptr(group), groups, hq, hk, dim, window, ptr(o),
+         o.shape[1], ptr(lse), ptr(work), work.numel(), stream())
+    return o, lse
+
+
+def test_shared_passes_nan_and_infinity_to_rows_that_see_them():
+    """In common: to every row.  Before a window, past a row's end, in the tile's rest: to no row that does not see it."""
+    gen = torch.Generator().manual_seed(3)
+    for where, seen in ((5, [True, True, True]), (130, [True, False, True]), (199, [True, False, False]), (203, [False] * 3)):
+        k, v = (torch.randn(20, 1, 16, 64, generator=gen).bfloat16().to(DEV) for _ in range(2))
+        table = ints(np.arange(20)[None].repeat(3, 0))
+        q = torch.randn(3, 128, generator=gen).bfloat16().to(DEV)
+        v[where // 16, 0, where % 16, 7] = float("nan")
+        k[where // 16, 0, where % 16] = float("inf")
+        o, lse = shared_call(q, k, v, table, ints([0, 1, 2]), ints([201, 100, 180]), ints([(0, 0, 200)]), 2, 1, 64)
+        assert torch.isfinite(lse).all(1).tolist() == [not s for s in seen]
+        assert torch.isfinite(o.float()).all(1).tolist() == [not s for s in seen]
+    k, v = (torch.randn(20, 1, 16, 64, generator=gen).bfloat16().to(DEV) for _ in range(2))
+    v[2, 0, 3] = float("nan")  # token 35
+    o, _ = shared_call(q, k, v, table, ints([0, 1, 2]), ints([201, 150, 134]), ints([(0, 0, 120)]), 2, 1, 64, window=100)
+    assert torch.isfinite(o.float()).all(1).tolist() == [True, True, False]
+
+
+def test_shared_on_another_stream_and_captured():
+    """The same call on a side stream, and replayed from a CUDA graph over other lengths and groups."""
+    from sejong_b200 import _lib
+    gen = torch.Generator().manual_seed(8)
+    k, v = (torch.randn(300, 2, 16, 64, generator=gen).bfloat16().to(DEV) for _ in range(2))
+    q = torch.randn(6, 4 * 64, generator=gen).bfloat16().to(DEV)
+    ids = np.random.default_rng(0).permutation(300)
+    table = np.concatenate((np.tile(ids[:50], (6, 1)), ids[50:290].reshape(6, 40)), axis=1)
+    table, req = ints(table), ints(np.arange(6))
+    pos, group = ints([900, 850, 801, 1000, 830, 1400]), ints([(0, 0, 800), (4, 4, 790), (6, 0, 0)])
+    work = torch.zeros(_lib.load().sj_attn_paged_shared_workspace(6, 3, 4, 2, 64), dtype=torch.uint8, device=DEV)
+    out = torch.empty_like(q), torch.empty(6, 4, device=DEV)
+
+    def run():
+        return shared_call(q, k, v, table, req, pos, group, 4, 2, 64, work=work, out=out)
+
+    first = [t.clone() for t in run()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = [t.clone() for t in run()]
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for new, groups in (([900, 850, 801, 1000, 830, 1400], [(0, 0, 800), (4, 4, 790), (6, 0, 0)]),
+                        ([700, -1, 10, 799, 800, 801], [(0, 0, 640), (3, 3, 700), (6, 0, 0)]),
+                        ([-1] * 6, [(0, 0, 0), (6, 0, 0), (6, 0, 0)]),
+                        ([1439] * 6, [(0, 5, 800), (6, 0, 0), (6, 0, 0)])):
+        pos.copy_(ints(new))
+        group.copy_(ints(groups))
+        graph.replay()
+        got = [t.clone() for t in out]
+        want = [t.clone() for t in run()]
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        plain = shared_call(q, k, v, table, req, pos, ints([(0, 0, 0)]), 4, 2, 64)
+        assert (got[0].float() - plain[0].float()).abs().max() < 0.02
+
+
+def test_shared_and_copied_offsets_past_32_bits():
+    """Cache buffers of more than 2^32 elements: the last pages are read, by boxes and by pieces, and copied."""
+    free, _ = torch.cuda.mem_get_info()
+    if free < 24 << 30:
+        pytest.skip("needs 24 GB of device memory")
+    gen = torch.Generator().manual_seed(12)
+    page, hk, dim = 64, 8, 128
+    pages = (1 << 32) // (page * hk * dim) + 6
+    k = torch.empty(pages, hk, page, dim, dtype=torch.bfloat16, device=DEV)
+    v = torch.empty_like(k)
+    small = [torch.randn(4, hk, page, dim, generator=gen).bfloat16() for _ in range(2)]
+    for cache, x in ((k, small[0]), (v, small[1])):
+        cache[-4:] = x.to(DEV)
+    q = torch.randn(2, hk * dim, generator=gen).bfloat16()
+    table = ints([[pages - 4, pages - 3, pages - 2, pages - 1]] * 2)
+    o, lse = shared_call(q.to(DEV), k, v, table, ints([0, 1]), ints([210, 215]), ints([(0, 0, 200)]), hk, hk, dim)
+    want, _, mean, _ = opaged.attention(q.double().view(2, hk, dim), small[0].double(), small[1].double(),
+                                        torch.tensor([[0, 1, 2, 3]] * 2), [0, 1], [210, 215], page)
+    assert ((o.cpu().double().view(2, hk, dim) - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -9) * mean).all()
+    call("sj_paged_copy", ptr(ints([(pages - 4, pages - 5, 64)])), 1, ptr(k), ptr(v), 1, 0, pages, page, *k.stride()[:3], hk,
+         dim, stream())
+    assert torch.equal(k[-5], k[-4]) and torch.equal(v[-5], v[-4])
+
+
 # ---------------------------------------------------------------- together
 def test_a_beam_search_on_the_books():
     """Steps of plan, commit, select, fork and copy, as a server runs them, against sequences kept in Python: after every step

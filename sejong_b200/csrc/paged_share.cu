@@ -353,8 +353,8 @@ __global__ void __launch_bounds__(kCompactThreads) paged_compact_kernel(const Co
       if (i + e * kCompactThreads >= count) break;
       if (id[e] < 0 || id[e] >= a.pages)
         s_bad = 1;
-      else if (atomicOr(&bits[id[e] >> 5], 1u << (id[e] & 31)) >> (id[e] & 31) & 1)
-        s_bad = 1;  // twice on the stack
+      else
+        atomicOr(&bits[id[e] >> 5], 1u << (id[e] & 31));
     }
   }
   __syncthreads();
@@ -376,7 +376,9 @@ __global__ void __launch_bounds__(kCompactThreads) paged_compact_kernel(const Co
     before[w] = base;
     base += in_word(w);
   }
-  bad |= s_bad != 0;
+  int in_use = 0;
+  for (int w = 0; w < 32; ++w) in_use += s_warp[w];
+  bad |= s_bad != 0 || in_use != a.pages - count;  // twice on the stack
   __syncthreads();
   const int used = bad ? 0 : a.pages - count;
   auto is_free = [&](int p) { return (bits[p >> 5] >> (p & 31) & 1) != 0; };

@@ -269,14 +269,29 @@ __global__ void __launch_bounds__(1024) beam_narrow_kernel(const T* logits, int 
     __syncthreads();
     return list.count;
   };
-  int n = collect([&](double total) { return total >= bar; });
-  if (n > kBeamHeld) {  // too low a bar, as of many beams that are worth much the same
+  // The beams' bars leave about `keep` candidates of each beam that is worth as much as the best: where those may be more
+  // than the list holds, the bar is sought bit by bit.
+  int n = out.beams * out.keep > kBeamHeld / 2 ? kBeamHeld + 1 : collect([&](double total) { return total >= bar; });
+  if (n > kBeamHeld) {
     __shared__ int counts[32];
-    const uint32_t reach = beam_reach(out.keep, counts, [&](uint32_t want) {
-      int have = 0;
-      each([&](double total, int, int) { have += beam_up(total) >> 32 >= want; });
-      return have;
-    });
+    uint32_t high[R], reach;
+    if (out.beams <= warps) {
+      const BeamOffset off = warp < out.beams ? offset[warp] : beam_offset(-INFINITY, 0.f, 1.0);
+#pragma unroll
+      for (int i = 0; i < R; ++i) high[i] = static_cast<uint32_t>(beam_up(off.total(v[i])) >> 32);
+      reach = beam_reach(out.keep, counts, [&](uint32_t want) {
+        int have = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i) have += high[i] >= want;
+        return have;
+      });
+    } else {
+      reach = beam_reach(out.keep, counts, [&](uint32_t want) {
+        int have = 0;
+        each([&](double total, int, int) { have += beam_up(total) >> 32 >= want; });
+        return have;
+      });
+    }
     if (threadIdx.x == 0) list.count = 0;
     __syncthreads();
     n = collect([&](double total) { return beam_up(total) >> 32 >= reach; });
@@ -433,10 +448,11 @@ SJ_DEVICE unsigned long long beam_up(const BeamJoin& join, int splits, int list,
 }
 // What is rare in a join is not inlined: its registers and instructions would stand in the way of the rest.
 //
-// What `keep` of the lists' first totals reach, `firsts` of each.
+// What `keep` of the lists' first totals reach, as many of each as the threads' registers hold.
 __device__ __noinline__ unsigned long long beam_join_bar(BeamJoin& join, const uint64_t* all, size_t slot, int splits,
-                                                         int members, int keep, int firsts) {
+                                                         int members, int keep) {
   constexpr int MOST = (kBeamMaxBeams * kBeamMaxSplits + kBeamMaxKeep) / kBeamThreads + 1;  // of a thread
+  const int firsts = min(keep, MOST * kBeamThreads / members);
   uint32_t high[MOST];
 #pragma unroll
   for (int k = 0; k < MOST; ++k) {
@@ -545,7 +561,7 @@ SJ_DEVICE void beam_join_parts(const BeamOut& out, const uint64_t* parts, int re
     }
     __syncthreads();
   } else {
-    const unsigned long long bar = beam_join_bar(join, all, slot, splits, members, keep, firsts);
+    const unsigned long long bar = beam_join_bar(join, all, slot, splits, members, keep);
     if (t == 0) {
       join.bar = bar;
       join.shares = 0;

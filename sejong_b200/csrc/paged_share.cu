@@ -332,7 +332,7 @@ struct Compact {
 // Every CTA reads the whole stack into a bit mask of the free pages with the numbers of pages in use before each word,
 // and writes its share of the results: the i-th page in use from `used` on goes to the i-th free page below it.  One launch
 // without a wait for other CTAs; bound by the shared-memory atomics of the mask (1024 requests on 183 thousand pages, half of
-// them free, 26 us; 32 requests on a thousand 6.3).
+// them free, 25 us; 32 requests on a thousand 6.4).
 __global__ void __launch_bounds__(kCompactThreads) paged_compact_kernel(const Compact a) {
   pdl_wait();
   extern __shared__ uint32_t bits[];                          // a bit for each page: free

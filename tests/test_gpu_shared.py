@@ -105,7 +105,8 @@ def logits(requests, beams, vocab, seed, spread=3.0):
 @pytest.mark.parametrize("requests,beams,vocab,keep,pad", [
     (1, 1, 1, 1, 0), (1, 1, 2, 2, 5), (3, 4, 257, 8, 7), (2, 1, 257, 40, 0), (1, 32, 257, 64, 3), (2, 40, 100, 64, 0),
     (2, 3, 1024, 33, 0), (5, 2, 1025, 4, 0), (2, 8, 5000, 16, 3), (1, 5, 50001, 10, 6), (1, 1, 131075, 64, 1),
-    (40, 8, 2049, 1, 0), (3, 64, 1500, 64, 1)])
+    (40, 8, 2049, 1, 0), (3, 64, 1500, 64, 1), (10, 20, 5000, 40, 0), (2, 64, 9000, 64, 2), (30, 25, 257, 50, 0), (3, 12, 700, 24, 1),
+    (2, 2, 1100, 64, 0)])
 def test_selection(dtype, requests, beams, vocab, keep, pad):
     check_select(*logits(requests, beams, vocab, requests * beams + vocab), keep, dtype, pad)
 

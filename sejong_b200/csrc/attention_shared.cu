@@ -58,6 +58,7 @@ struct SpansArgs {
 // One CTA.  A group's p0 is the highest first key of its live rows, p1 the lowest end.
 __global__ void __launch_bounds__(1024) shared_spans_kernel(const SpansArgs a) {
   pdl_wait();
+  pdl_trigger();
   __shared__ int first[kSharedGroups + 1], p0[kSharedGroups], p1[kSharedGroups], live[kSharedGroups];
   __shared__ unsigned long long s_scan[32];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -841,7 +842,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
 // A warp for a row and head: its own part, then the parts of its keys in common, 32 at a time: of 16 chunks two CTAs
 // each, or of one chunk 32 CTAs.  The lanes take the weights, then each its dims of all parts, in order.
 template <int DIM>
-__global__ void __launch_bounds__(256) shared_join_kernel(const SharedSpans s, int rows, int hq, int fan, __nv_bfloat16* o,
+__global__ void __launch_bounds__(256, 5) shared_join_kernel(const SharedSpans s, int rows, int hq, int fan, __nv_bfloat16* o,
                                                           int ldo, float* lse) {
   pdl_wait();
   constexpr int PER = DIM / 32, AT_ONCE = 4;

@@ -527,19 +527,26 @@ SJ_DEVICE void beam_join_parts(const BeamOut& out, const uint64_t* parts, int re
     join.shares = ~0ull;
   }
   const uint64_t* all = parts + static_cast<size_t>(request) * members * slot;
+  // where the list holds all candidates, they come over at once, next to the sums
+  constexpr int HELD = kBeamHeld / kBeamThreads;
+  const bool whole = members * keep <= kBeamHeld;
+  uint64_t held[HELD];
+#pragma unroll
+  for (int k = 0; k < HELD; ++k) {
+    const int i = t + k * kBeamThreads;
+    held[k] = whole && i < members * keep ? __ldcg(all + static_cast<size_t>(i / keep) * slot + 1 + i % keep) : 0;
+  }
   if (t < out.beams) {
     float top = -INFINITY;
     double sum = 0.0;
+#pragma unroll 1
     for (int k = 0; k < splits; ++k) {
       const uint64_t word = __ldcg(all + static_cast<size_t>(t * splits + k) * slot);
       const float part_m = __uint_as_float(static_cast<uint32_t>(word >> 32));
-      const double part_s = __uint_as_float(static_cast<uint32_t>(word));
-      const float raised = fmaxf(top, part_m);
-      if (raised == -INFINITY) {
-        sum += part_s;
-        continue;
-      }
-      sum = sum * exp(static_cast<double>(top) - raised) + part_s * exp(static_cast<double>(part_m) - raised);
+      const float part_s = __uint_as_float(static_cast<uint32_t>(word));
+      const float raised = fmaxf(top, part_m), base = raised == -INFINITY ? 0.f : raised;
+      sum = sum * beam_exp2((top - base) * kLog2e) + static_cast<double>(part_s) * beam_exp2((part_m - base) * kLog2e);
+      if (raised == -INFINITY) sum = part_s;  // 0, or the NaN of a part that is all NaN
       top = raised;
     }
     join.offset[t] = beam_offset(out.score[static_cast<size_t>(request) * out.beams + t], top, sum);
@@ -548,46 +555,45 @@ SJ_DEVICE void beam_join_parts(const BeamOut& out, const uint64_t* parts, int re
   // A bar again: what `keep` of the lists' first totals reach, as many of each as it takes; where the list holds all
   // candidates, the lowest of them or the last total of a list will do.
   auto up = [&](int list, uint64_t key) { return beam_up(join, splits, list, key); };
-  const int firsts = (keep + members - 1) / members;
-  if (members * keep <= kBeamHeld) {
-    for (int i = t; i < 2 * members; i += kBeamThreads) {
-      const bool whole = i >= members;  // a list's last total is one, too
-      const int list = whole ? i - members : i;
-      const unsigned long long total = up(list, __ldcg(all + static_cast<size_t>(list) * slot + (whole ? keep : firsts)));
-      if (whole)
-        atomicMax(&join.bar, total);
-      else
-        atomicMin(&join.shares, total);
-    }
-    __syncthreads();
-  } else {
-    const unsigned long long bar = beam_join_bar(join, all, slot, splits, members, keep);
-    if (t == 0) {
-      join.bar = bar;
-      join.shares = 0;
-    }
-    __syncthreads();
-  }
-  const unsigned long long request_bar = max(join.bar, join.shares);
-  // false: the list's others do not reach it either
-  auto file = [&](int list, int k) {
-    const uint64_t key = __ldcg(all + static_cast<size_t>(list) * slot + 1 + k);
-    const unsigned long long total = up(list, key);
-    if (total == 0 || total < request_bar) return false;
+  auto file = [&](int list, uint64_t key) {
     const int at = atomicAdd(&join.list.count, 1);
     if (at < kBeamHeld) {
       join.list.total[at] = join.offset[list / splits].total(beam_value(key));
       join.list.beam[at] = list / splits;
       join.list.column[at] = beam_column(key);
     }
-    return true;
   };
-  if (members >= kBeamThreads / 2) {  // a thread for a list
-    for (int list = t; list < members; list += kBeamThreads)
-      for (int k = 0; k < keep && file(list, k); ++k) {
-      }
+  if (whole) {
+    const int firsts = (keep + members - 1) / members;
+    unsigned long long total[HELD];
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) {
+      const int i = t + k * kBeamThreads, at = i % keep + 1;
+      total[k] = i < members * keep ? up(i / keep, held[k]) : 0ull;
+      if (i < members * keep && at == keep) atomicMax(&join.bar, total[k]);
+      if (i < members * keep && at == firsts) atomicMin(&join.shares, total[k]);
+    }
+    __syncthreads();
+    const unsigned long long bar = max(join.bar, join.shares);
+#pragma unroll
+    for (int k = 0; k < HELD; ++k)
+      if (total[k] != 0 && total[k] >= bar) file((t + k * kBeamThreads) / keep, held[k]);
   } else {
-    for (int i = t; i < members * keep; i += kBeamThreads) file(i / keep, i % keep);
+    const unsigned long long bar = beam_join_bar(join, all, slot, splits, members, keep);
+    auto reaches = [&](int list, int k) {  // false: the list's others do not either
+      const uint64_t key = __ldcg(all + static_cast<size_t>(list) * slot + 1 + k);
+      const unsigned long long total = up(list, key);
+      if (total == 0 || total < bar) return false;
+      file(list, key);
+      return true;
+    };
+    if (members >= kBeamThreads / 2) {  // a thread for a list
+      for (int list = t; list < members; list += kBeamThreads)
+        for (int k = 0; k < keep && reaches(list, k); ++k) {
+        }
+    } else {
+      for (int i = t; i < members * keep; i += kBeamThreads) reaches(i / keep, i % keep);
+    }
   }
   __syncthreads();
   const int n = join.list.count;

@@ -9,9 +9,9 @@
 // exponentials and the tensor cores many.  A row's keys outside [p0, p1), by its window or its length, are its own, so no
 // tile needs a mask but for the last one's end, and a value that a row does not see reaches no sum of it.
 //
-// Measured on B200 (graph replays, all four kernels): 509 rows that share 32768 keys, 16 / 4 heads of 128 197 us (695
-// TFLOP/s; rows apart 2378); two pieces of 250 and 333 rows over 20 and 60 thousand keys, 16 / 2 heads of 128 225 (774
-// TFLOP/s; 1548); 16 x 16 rows over 2048 to 16384 keys, 12 / 4 heads of 64 76 (164).  The tensor-core pass is about 150,
+// Measured on B200 (graph replays, all four kernels): 509 rows that share 32768 keys, 16 / 4 heads of 128 194 us (704
+// TFLOP/s; rows apart 2378); two pieces of 250 and 333 rows over 20 and 60 thousand keys, 16 / 2 heads of 128 222 (786
+// TFLOP/s; 1548); 16 x 16 rows over 2048 to 16384 keys, 12 / 4 heads of 64 75 (164).  The tensor-core pass is about 150,
 // 180 and 45 of these: 44% of the tensor pipe's cycles on the second, where softmax and products of a stream wait for
 // one another and two streams do not fill the gaps.
 #include <algorithm>

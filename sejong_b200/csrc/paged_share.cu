@@ -20,7 +20,7 @@ namespace cg = cooperative_groups;
 namespace sj {
 
 namespace {
-constexpr int kShareMaxBatch = 4096, kShareMaxPages = 1 << 18;  // masks of them fit shared memory
+constexpr int kShareMaxBatch = 4096, kShareMaxPages = 1 << 18;  // counters of an eighth of them fit shared memory, and masks of all
 constexpr int kForkNoPages = 2, kForkTableNarrow = 3, kForkBad = 4;
 constexpr int kCompactMovesOver = 1, kCompactBad = 4;
 constexpr int kForkCluster = 8, kForkThreads = 1024;
@@ -42,11 +42,12 @@ struct Fork {
 // A slot's pages pass to its children: full ones are shared, a half-filled last page goes to the lowest child and is
 // copied to a fresh page for each of the others.  Every CTA scans the batch for itself.  The first cluster counts: an
 // entry of a slot with c children changes its page's owners by c - 1 (the half-filled page of a slot without children
-// by -1), by integer additions to shares_out, whose order does not matter.  Then each CTA knows which of its pages
-// nobody holds, and after one exchange of numbers where on the stack they go.  The other clusters (the same one, where
-// there is only one) write tables.  Bound by latency, four phases of a few dependent loads: 32 requests 8.6 us (graph
-// replays), 1024 requests of 500 to 32768 tokens in pages of 64 21.7 (34 with an addition to memory, or to another CTA's,
-// for each entry).
+// by -1); the counters of a CTA's share of the pages lie in its shared memory, which the others add to (integers, so the
+// order does not matter; in memory, with the fences that takes, 9.3 us instead of 8.7 for 32 requests).  Then each CTA knows which of its
+// pages nobody holds, and after one exchange of numbers where on the stack they go.  The other clusters (the same one, where
+// there is only one) write tables.  Bound by latency, four phases of a few dependent loads: 32 requests 8.7 us (graph
+// replays), 1024 requests of 500 to 32768 tokens in pages of 64 22.4 (34 with an addition to another CTA's counter for each
+// entry).
 __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) {
   pdl_wait();
   extern __shared__ int dynamic[];
@@ -55,7 +56,7 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) 
   int* rank = lowest + (a.batch + 1);            // [batch + 1] copies of the slots before, -1: no copy
   int* parents = rank + (a.batch + 1);           // [batch + 1]
   int* lengths = parents + (a.batch + 1);        // [batch + 1]
-  uint32_t* gone_bits = reinterpret_cast<uint32_t*>(lengths + (a.batch + 1));  // of the CTA's pages
+  int* counter = lengths + (a.batch + 1);        // of the CTA's pages: the change of their owners
   __shared__ int s_bad, s_narrow, s_back, s_warp[kForkThreads / 32];
   cg::cluster_group cluster = cg::this_cluster();
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, batch = a.batch, page = a.page;
@@ -71,17 +72,7 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) 
   }
   // this CTA's share of the pages
   const int page0 = min(cta * a.per, a.pages), mine = counts ? min(a.per, a.pages - page0) : 0;
-  for (int i = t; i < mine; i += threads * kForkUnits) {
-    int more[kForkUnits];
-#pragma unroll
-    for (int e = 0; e < kForkUnits; ++e)
-      more[e] = i + e * threads < mine ? a.shares[page0 + i + e * threads] : 0;
-#pragma unroll
-    for (int e = 0; e < kForkUnits; ++e) {
-      if (more[e] < 0) record_error(SJ_DEV_BAD_INDEX);
-      if (i + e * threads < mine) a.shares_out[page0 + i + e * threads] = max(more[e], 0);
-    }
-  }
+  for (int i = t; i < mine; i += threads) counter[i] = 0;
   __syncthreads();
   auto length = [&](int b) { return lengths[b]; };
   for (int b = t; b < batch; b += threads) {
@@ -173,8 +164,7 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) 
   if (!counts) return;
 
   // ---- owners
-  __threadfence();
-  cluster.sync();  // shares_out holds the owners so far
+  cluster.sync();  // every counter of the cluster is zero
   if (!status) {
     // A warp takes a chunk of the tables of kForkRun slots side by side.  Slots that came from one share their first pages,
     // and what their children take and leave there mostly adds up to nothing: it is added up here, as long as the page
@@ -201,7 +191,7 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) 
           if (now < 0 || now >= a.pages)
             record_error(SJ_DEV_BAD_INDEX);
           else
-            atomicAdd(&a.shares_out[now], sum);
+            atomicAdd(cluster.map_shared_rank(counter, now / a.per) + now % a.per, sum);
         };
 #pragma unroll
         for (int k = 0; k < kForkRun; ++k) {
@@ -217,26 +207,27 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) 
       }
     }
   }
-  __threadfence();
   cluster.sync();
   // a warp's run of this CTA's pages, in order
   const int run = ((mine + warps - 1) / warps + 31) / 32 * 32;
   const int i0 = min(warp * run, mine), i1 = min(i0 + run, mine);
   int gone = 0;
   for (int i = i0 + lane; i - lane < i1; i += 32 * kForkUnits) {
-    int left[kForkUnits];
+    int more[kForkUnits];
 #pragma unroll
-    for (int e = 0; e < kForkUnits; ++e) left[e] = i + 32 * e < i1 ? __ldcg(a.shares_out + page0 + i + 32 * e) : 0;
+    for (int e = 0; e < kForkUnits; ++e) more[e] = i + 32 * e < i1 ? a.shares[page0 + i + 32 * e] : 0;
 #pragma unroll
     for (int e = 0; e < kForkUnits; ++e) {
-      const bool is = left[e] == -1 && !status;
-      if (left[e] < 0 && !status) {
-        if (left[e] < -1) record_error(SJ_DEV_BAD_INDEX);  // given back more often than it was held
-        a.shares_out[page0 + i + 32 * e] = 0;
+      const int at = i + 32 * e;
+      bool is = false;
+      if (at < i1) {
+        const int left = max(more[e], 0) + counter[at];
+        is = left == -1;
+        if (more[e] < 0 || left < -1) record_error(SJ_DEV_BAD_INDEX);  // given back more often than it was held
+        a.shares_out[page0 + at] = max(left, 0);
+        counter[at] = is;
       }
-      const unsigned have = __ballot_sync(0xffffffffu, is);
-      if (lane == 0 && i + 32 * e < i1) gone_bits[(i + 32 * e) >> 5] = have;
-      gone += __popc(have);
+      gone += __popc(__ballot_sync(0xffffffffu, is));
     }
   }
   if (lane == 0) s_warp[warp] = gone;
@@ -255,8 +246,8 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) 
   }
   for (int w = 0; w < warp; ++w) back += s_warp[w];
   for (int i = i0 + lane; i - lane < i1; i += 32) {
-    const unsigned have = gone_bits[i >> 5];
-    const bool is = have >> lane & 1;
+    const bool is = i < i1 && counter[i] != 0;
+    const unsigned have = __ballot_sync(0xffffffffu, is);
     const int at = back + __popc(have & ((1u << lane) - 1));
     if (is) {
       if (at >= 0 && at < a.pages)
@@ -485,9 +476,9 @@ extern "C" int sj_paged_fork(const int32_t* parent, int batch, int page, const i
          free_out, count_out, copies, summary, batch, page, ld_table, pages, 0};
   constexpr int ctas = kForkCluster;
   a.per = (pages + ctas - 1) / ctas;
-  const int smem = (5 * (batch + 1) + a.per / 32 + 1) * static_cast<int>(sizeof(int));
+  const int smem = (5 * (batch + 1) + a.per) * static_cast<int>(sizeof(int));
   static KernelAttrOnce once;
-  constexpr int most = (5 * (kShareMaxBatch + 1) + kShareMaxPages / 32 + 1) * static_cast<int>(sizeof(int));
+  constexpr int most = (5 * (kShareMaxBatch + 1) + kShareMaxPages / kForkCluster) * static_cast<int>(sizeof(int));
   const int rc = ensure_max_smem(once, reinterpret_cast<const void*>(paged_fork_kernel), most,
                                  "sj_paged_fork: shared memory");
   if (rc != SJ_OK) return rc;

@@ -43,11 +43,10 @@ struct Fork {
 // copied to a fresh page for each of the others.  Every CTA scans the batch for itself.  The first cluster counts: an
 // entry of a slot with c children changes its page's owners by c - 1 (the half-filled page of a slot without children
 // by -1); the counters of a CTA's share of the pages lie in its shared memory, which the others add to (integers, so the
-// order does not matter; in memory, with the fences that takes, 9.3 us instead of 8.7 for 32 requests).  Then each CTA knows which of its
-// pages nobody holds, and after one exchange of numbers where on the stack they go.  The other clusters (the same one, where
-// there is only one) write tables.  Bound by latency, four phases of a few dependent loads: 32 requests 8.7 us (graph
-// replays), 1024 requests of 500 to 32768 tokens in pages of 64 22.4 (34 with an addition to another CTA's counter for each
-// entry).
+// order does not matter; in memory, with the fences that takes, 9.3 us instead of 8.7 for 32 requests).  Then each CTA
+// knows which of its pages nobody holds, and after one exchange of numbers where on the stack they go.  The other
+// clusters write tables.  Bound by latency, four phases of a few dependent loads: 32 requests 8.7 us (graph replays), 1024
+// requests of 500 to 32768 tokens in pages of 64 22.4 (34 with an addition to another CTA's counter for each entry).
 __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) {
   pdl_wait();
   extern __shared__ int dynamic[];
@@ -124,8 +123,7 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) 
   auto fresh = [&](int b) { return a.stack[count - 1 - rank[b]]; };
 
   // ---- tables, lengths, copies, what stays of the stack
-  const int writers = gridDim.x > static_cast<unsigned>(ctas) ? gridDim.x - ctas : gridDim.x;
-  const int writer = gridDim.x > static_cast<unsigned>(ctas) ? static_cast<int>(blockIdx.x) - ctas : blockIdx.x;
+  const int writers = gridDim.x - ctas, writer = static_cast<int>(blockIdx.x) - ctas;
   if (writer >= 0) {
     const int chunks = (a.ld_table + kForkChunk - 1) / kForkChunk;
     for (int u = writer * warps + warp; u < batch * chunks; u += writers * warps) {

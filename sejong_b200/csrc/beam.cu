@@ -545,8 +545,8 @@ SJ_DEVICE void beam_join_parts(const BeamOut& out, const uint64_t* parts, int re
       const float part_m = __uint_as_float(static_cast<uint32_t>(word >> 32));
       const float part_s = __uint_as_float(static_cast<uint32_t>(word));
       const float raised = fmaxf(top, part_m), base = raised == -INFINITY ? 0.f : raised;
+      // (a part without a maximum has the sum 0, or the NaN of a row that has one, which stays)
       sum = sum * beam_exp2((top - base) * kLog2e) + static_cast<double>(part_s) * beam_exp2((part_m - base) * kLog2e);
-      if (raised == -INFINITY) sum = part_s;  // 0, or the NaN of a part that is all NaN
       top = raised;
     }
     join.offset[t] = beam_offset(out.score[static_cast<size_t>(request) * out.beams + t], top, sum);

@@ -148,6 +148,18 @@ def test_selection_of_forbidden_tokens_and_empty_beams(vocab):
     check_select(x, score, 12)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("at", [1234, 21000, 37999])
+def test_selection_keeps_the_nan_of_a_part_without_other_values(dtype, at):
+    """A row of 20 parts, of which one has a NaN and forbidden tokens only, and the next one nothing but those."""
+    x, _ = logits(1, 2, 40000, 4)
+    score = torch.tensor([[-1.0, -9.0]])  # the row with the NaN would bring the best
+    first = at // 2000 * 2000
+    x[0, 0, first:first + 4000] = -float("inf")
+    x[0, 0, at] = float("nan")
+    check_select(x, score, 8, dtype)
+
+
 def test_selection_of_extreme_logits():
     x, score = logits(2, 2, 3000, 3)
     x[0] *= 1e30

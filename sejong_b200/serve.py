@@ -584,11 +584,13 @@ class BatchGenerator:
             del q.ended[beams:]
             q.live = live
             length = len(live[0][0]) if live else 0
-            # what goes on may still be worth more than the worst that has ended
-            hope = max((rank(s, length) for _, s in live), default=-float("inf"))
+            # what goes on can come to be worth no more than its score at the length that is best for it: the largest, or
+            # where a greater length makes less of it, the next one, by an end
+            hope = max((max(rank(s, length + 1), rank(s, most_bytes)) for _, s in live), default=-float("inf"))
             done = not live or length >= most_bytes or (len(q.ended) == beams and q.ended[-1].ranked >= hope)
             if done:
-                rest = [Hypothesis(bytes(d), False, s, rank(s, len(d))) for d, s in live]
+                whole = length >= most_bytes
+                rest = [Hypothesis(bytes(d), False, s, rank(s, len(d))) for d, s in live if whole]
                 results[q.index] = sorted(q.ended + rest, key=lambda h: -h.ranked)[:beams]
                 blocks[n] = None
                 self.reserved -= q.reserved
@@ -639,7 +641,8 @@ class BatchGenerator:
 
     def beam_search(self, prompts, beams=4, max_bytes=64, length_penalty=1.0):
         """For each prompt the `beams` best continuations found (Hypothesis, the best first): those that end, or have
-        `max_bytes` bytes, ordered by their log probability over length ** length_penalty."""
+        `max_bytes` bytes, ordered by their log probability over length ** length_penalty (an end counts as a byte).  The
+        search stops early only where no beam can come to be worth more."""
         if not 1 <= beams <= min(self.batch, 32):
             raise ValueError("beams must be 1 to 32, and at most the batch")
         if max_bytes < 1:

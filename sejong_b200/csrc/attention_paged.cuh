@@ -44,6 +44,12 @@ struct SharedRow {
   int lo, n, p0, p1, group;
 };
 
+// Whether a block's first and last CTA can be those that attn_shared_kernel wrote.  Where a wait of it gave up it left blocks
+// out, and a workspace may hold anything there.
+__host__ __device__ inline bool shared_span_fine(int2 span, int ctas) {
+  return span.x >= 0 && span.x <= span.y && span.y < ctas;
+}
+
 // A softmax's part: maximum (of log2), sum and outputs of each query.
 struct SharedParts {
   float *m, *l, *o;  // o: [queries][dim]

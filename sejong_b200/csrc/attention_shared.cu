@@ -869,7 +869,8 @@ __global__ void __launch_bounds__(256, 5) shared_join_kernel(const SharedSpans s
     const int side = chunks > 1 ? 2 : 32;  // CTAs of a chunk at a time
     for (int c0 = 0; c0 < chunks; c0 += 32 / side) {
       const int c = c0 + lane / side;
-      const int2 span = c < chunks ? blocks[c * ((g.tiles + 1) / 2)] : make_int2(0, -1);
+      int2 span = c < chunks ? blocks[c * ((g.tiles + 1) / 2)] : make_int2(0, -1);
+      if (!shared_span_fine(span, s.ctas)) span = make_int2(0, -1);
       for (int k = lane % side; __any_sync(0xffffffffu, span.x + k <= span.y); k += side) {
         const bool is = span.x + k <= span.y;
         const SharedParts& part = k == 0 ? s.main : s.slots;

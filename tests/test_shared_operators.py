@@ -121,3 +121,24 @@ def test_compact_fills_holes_in_order():
     table, shares, free, moves = oracle.compact(4, [8, 4], [[5, 0], [3, -1]], [1, 0, 0, 0, 0, 2], [1, 4, 2], 6)
     assert moves == [(3, 1), (5, 2)] and table.tolist() == [[2, 0], [1, -1]]
     assert shares.tolist() == [1, 0, 2, 0, 0, 0] and free == [5, 4, 3]
+
+
+# ---------------------------------------------------------------- what the kernels decide by, on the host
+def host_program(where, body):
+    """The output of a program with the kernels' own functions, which runs without a GPU."""
+    import subprocess
+    from sejong_b200 import build
+    source, program = where / "host.cu", where / "host"
+    source.write_text('#include <cstdio>\n#include "attention_paged.cuh"\nusing namespace sj;\nint main() {\n'
+                      + body + "\nreturn 0;\n}\n")
+    subprocess.run([build.nvcc(), *build.ARCH, *build.NVCC_FLAGS, str(source), "-o", str(program)], check=True)
+    return subprocess.run([str(program)], check=True, capture_output=True, text=True).stdout.split()
+
+
+def test_blocks_that_were_never_written_are_no_ctas(tmp_path):
+    """What a broken-off call leaves in the place of a block's CTAs: nothing that the join could go astray by."""
+    ctas = 148
+    cases = [(0, 0), (0, 147), (147, 147), (5, 9), (0, -1), (9, 5), (-1, 3), (-5, -2), (0, 148), (148, 148), (-2 ** 31, 2 ** 31 - 1),
+             (0, 2 ** 31 - 1), (0x3f800000, 0x40000000), (2 ** 31 - 1, -2 ** 31)]
+    body = "".join(f'printf("%d ", shared_span_fine(make_int2(int({a}ll), int({b}ll)), {ctas}));' for a, b in cases)
+    assert [x == "1" for x in host_program(tmp_path, body)] == [0 <= a <= b < ctas for a, b in cases]

@@ -44,6 +44,14 @@ struct SharedRow {
   int lo, n, p0, p1, group;
 };
 
+// Whether group t of `groups` (first row, request, tokens) is in order and in range; `most`: the tokens that a table holds.
+__host__ __device__ inline bool shared_group_fine(const int32_t* group, int t, int groups, int rows, int requests,
+                                                  int64_t most) {
+  const int at = group[3 * t], b = group[3 * t + 1], n = group[3 * t + 2], next = t + 1 < groups ? group[3 * t + 3] : rows;
+  const bool ordered = at >= 0 && next <= rows && (at < next || (at == rows && next == rows));
+  return ordered && b >= 0 && b < requests && n >= 0 && n <= most;
+}
+
 // Whether a block's first and last CTA can be those that attn_shared_kernel wrote.  Where a wait of it gave up it left blocks
 // out, and a workspace may hold anything there.
 __host__ __device__ inline bool shared_span_fine(int2 span, int ctas) {

@@ -64,13 +64,11 @@ __global__ void __launch_bounds__(1024) shared_spans_kernel(const SpansArgs a) {
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int64_t most = static_cast<int64_t>(a.ld_table) * a.page;
   if (t < a.groups) {
-    const int at = a.group[3 * t], b = a.group[3 * t + 1], n = a.group[3 * t + 2];
-    const int next = t + 1 < a.groups ? a.group[3 * t + 3] : a.rows;
-    const bool fine = at >= 0 && (at < next || at == a.rows) && next <= a.rows && b >= 0 && b < a.requests && n >= 0 && n <= most;
+    const bool fine = shared_group_fine(a.group, t, a.groups, a.rows, a.requests, most);
     if (!fine) record_error(SJ_DEV_BAD_INDEX);
-    first[t] = at;
+    first[t] = a.group[3 * t];
     p0[t] = 0;
-    p1[t] = fine ? n : -1;
+    p1[t] = fine ? a.group[3 * t + 2] : -1;
     live[t] = 0;
   }
   const bool ordered = __syncthreads_and(t >= a.groups || p1[t] >= 0);

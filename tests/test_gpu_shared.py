@@ -589,6 +589,12 @@ def test_shared_reports_groups_out_of_range(group):
     assert (out[0][1] - out[1][1]).abs().max() < 1e-4
 
 
+@pytest.mark.parametrize("group", [[(0, 0, 32), (4, 0, 0), (2, 0, 32)], [(0, 0, 32), (4, 0, 0), (2, 0, 32), (4, 0, 0)],
+                                   [(4, 0, 0), (0, 0, 32)]])
+def test_shared_reports_groups_after_the_end(group):
+    test_shared_reports_groups_out_of_range(group)
+
+
 def shared_call(q, k, v, table, request, position, group, hq, hk, dim, window=0, work=None, out=None):
     from sejong_b200 import _lib
     rows, groups = q.shape[0], group.shape[0]

@@ -142,3 +142,23 @@ def test_blocks_that_were_never_written_are_no_ctas(tmp_path):
              (0, 2 ** 31 - 1), (0x3f800000, 0x40000000), (2 ** 31 - 1, -2 ** 31)]
     body = "".join(f'printf("%d ", shared_span_fine(make_int2(int({a}ll), int({b}ll)), {ctas}));' for a, b in cases)
     assert [x == "1" for x in host_program(tmp_path, body)] == [0 <= a <= b < ctas for a, b in cases]
+
+
+def test_groups_are_in_order_to_the_end(tmp_path):
+    """A first row of `rows` ends the list: a smaller one after it is out of order, whatever comes then."""
+    rows, requests, most = 9, 4, 100
+    cases = [[0, 3, 5], [0, 9, 9], [9, 9, 9], [0, 9, 5], [0, 9, 5, 9], [9, 0], [0, 5, 5], [5, 3], [-1, 3], [0, 10], [8], [9], [10]]
+    body = ""
+    for first in cases:
+        body += f"{{ const int32_t g[] = {{{', '.join(f'{f}, 1, 7' for f in first)}}}; int fine = 1; " \
+                f"for (int t = 0; t < {len(first)}; ++t) fine &= shared_group_fine(g, t, {len(first)}, {rows}, {requests}, {most}); " \
+                "printf(\"%d \", fine); }\n"
+    for b, n in ((-1, 7), (4, 7), (3, -1), (3, 101), (3, 100)):
+        body += f"{{ const int32_t g[] = {{0, {b}, {n}}}; printf(\"%d \", shared_group_fine(g, 0, 1, {rows}, {requests}, {most})); }}\n"
+
+    def in_order(first):
+        starts = [f for f in first if f != rows]
+        return first == starts + [rows] * (len(first) - len(starts)) and all(0 <= f < rows for f in starts) \
+            and all(a < b for a, b in zip(starts, starts[1:]))
+
+    assert [x == "1" for x in host_program(tmp_path, body)] == [in_order(c) for c in cases] + [False] * 4 + [True]

@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
       const bool idle = !__any_sync(0xffffffffu, is);  // a warp without queries leaves S as it is
       float m = -INFINITY, l = 0.f;
       for (int step = 0; ok && step < steps; ++step, ++tile_at) {
-        if (!mbar_wait(&s_full[stream], tile_at & 1, abort_flag, SJ_DEV_ATTN_WAIT)) {
+        if (!mbar_wait_warp(&s_full[stream], tile_at & 1, abort_flag, SJ_DEV_ATTN_WAIT)) {
           ok = false;
           break;
         }
@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
             m = next;
             if (step > 0 || half > 0) {
               // the output has the products of all tiles before, since S came after them, but maybe not this one's
-              if (half == 1 && !mbar_wait(&o_half[stream], tile_at & 1, abort_flag, SJ_DEV_ATTN_WAIT)) {
+              if (half == 1 && !mbar_wait_warp(&o_half[stream], tile_at & 1, abort_flag, SJ_DEV_ATTN_WAIT)) {
                 ok = false;
                 break;
               }
@@ -530,7 +530,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
       }
       if (!ok) break;
       if (steps > 0) {
-        if (!mbar_wait(&o_full[stream], piece_at & 1, abort_flag, SJ_DEV_ATTN_WAIT)) break;
+        if (!mbar_wait_warp(&o_full[stream], piece_at & 1, abort_flag, SJ_DEV_ATTN_WAIT)) break;
         ++piece_at;
         tc_fence_after();
       }
@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
       const bool joined = !p.two && p.steps1 > 0;
       float f = 1.f, g = 0.f;
       if (joined) {
-        if (!mbar_wait(sums_full, sums_at & 1, abort_flag, SJ_DEV_ATTN_WAIT)) break;
+        if (!mbar_wait_warp(sums_full, sums_at & 1, abort_flag, SJ_DEV_ATTN_WAIT)) break;
         ++sums_at;
         tc_fence_after();
         const float m2 = sums[row], top = fmaxf(m, m2), base = top == -INFINITY ? 0.f : top;
@@ -751,8 +751,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
       if (lane == 0) seen[(stream * kSeen + (seen_at[stream] & (kSeen - 1))) * 4 + word] = have;
     };
     auto fetch = [&](int stream, int key, const Box& x) {
-      if (!mbar_wait(&empty[slot], turn ^ 1, abort_flag, SJ_DEV_ATTN_WAIT)) ok = false;
-      ok = __all_sync(0xffffffffu, ok);
+      ok = mbar_wait_warp(&empty[slot], turn ^ 1, abort_flag, SJ_DEV_ATTN_WAIT);
       if (!ok) return;
       const uint32_t dst = smem_u32(smem + L::RING + slot * L::SLOT);
       const bool boxed = boxes > 0 && key % a.box == 0 && key + kSharedKeys <= p.g.p1;

@@ -115,6 +115,12 @@ SJ_DEVICE bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort, in
   }
 }
 
+// The same for a whole warp, which gets one answer: lanes that gave up and lanes that did not would part before the
+// instructions that take all of them.
+SJ_DEVICE bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, code));
+}
+
 // Bounded wait that lets the waiting thread sleep: try_wait with a suspend-time hint returns when the
 // phase completes or after about `hint_ns`, so a warp that waits long (a producer or MMA thread
 // sharing its scheduler with compute warps) does not spend issue slots polling.

@@ -162,3 +162,17 @@ def test_groups_are_in_order_to_the_end(tmp_path):
             and all(a < b for a, b in zip(starts, starts[1:]))
 
     assert [x == "1" for x in host_program(tmp_path, body)] == [in_order(c) for c in cases] + [False] * 4 + [True]
+
+
+def test_warps_give_up_as_a_whole():
+    """The warps of attn_shared_kernel that go on by the answer of a wait, and to instructions of all their lanes, wait as
+    warps; only the one that issues products, and goes on in any case, and the last look before the end do not."""
+    import os
+    import re
+    from sejong_b200 import build
+    text = open(os.path.join(build.CSRC, "attention_shared.cu")).read()
+    softmax, rest = text[text.index("if (warp < kSoftmaxWarps) {"):].split("} else if (warp == kMmaWarp) {")
+    loads = rest[rest.index("both warps follow the order of all tiles"):rest.index("// nothing lands after the CTA has gone")]
+    for part, waits in ((softmax, 4), (loads, 1)):
+        assert len(re.findall(r"\bmbar_wait_warp\(", part)) == waits
+        assert not re.findall(r"\bmbar_wait\(", part)

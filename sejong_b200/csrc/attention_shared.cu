@@ -406,6 +406,8 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   SharedWalk walk(a);
   SharedPiece p;
+  uint32_t asked = 0;  // of a load warp's last tiles, the bits of those that it has asked for, and the slot after them
+  int last_slot = 0, last_turn = 0;
 
   if (warp < kSoftmaxWarps) {
     const int stream = warp >> 2, row = (warp & 3) * 32 + lane, per = kSharedQueries / a.fan;
@@ -819,19 +821,22 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
         if (ok && i + 1 < n1) tile(1, i + 1, of_k);
       }
     }
-    // nothing lands after the CTA has gone: every tile that was asked for has been waited for by the products, unless a
-    // wait gave up
-    for (int i = 0; *abort_flag != 0 && i < L::STAGES; ++i, fetched >>= 1) {
-      turn ^= slot == 0 ? 1 : 0;
-      slot = slot == 0 ? L::STAGES - 1 : slot - 1;
-      if (fetched & 1) mbar_wait(&full[slot], turn, nullptr, SJ_DEV_ATTN_WAIT);
-    }
+    asked = fetched;
+    last_slot = slot;
+    last_turn = turn;
   }
   tc_fence_before();
   __syncthreads();
   if (warp == kMmaWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, kTmemAll);
+  }
+  // Nothing lands after the CTA has gone: the products have waited for every tile that was asked for, unless a wait gave up,
+  // which all warps know by now.
+  for (int i = 0; warp >= kLoadWarp && *abort_flag != 0 && i < L::STAGES; ++i, asked >>= 1) {
+    last_turn ^= last_slot == 0 ? 1 : 0;
+    last_slot = last_slot == 0 ? L::STAGES - 1 : last_slot - 1;
+    if (asked & 1) mbar_wait(&full[last_slot], last_turn, nullptr, SJ_DEV_ATTN_WAIT);
   }
 }
 

@@ -172,7 +172,18 @@ def test_warps_give_up_as_a_whole():
     from sejong_b200 import build
     text = open(os.path.join(build.CSRC, "attention_shared.cu")).read()
     softmax, rest = text[text.index("if (warp < kSoftmaxWarps) {"):].split("} else if (warp == kMmaWarp) {")
-    loads = rest[rest.index("both warps follow the order of all tiles"):rest.index("// nothing lands after the CTA has gone")]
+    loads = rest[rest.index("both warps follow the order of all tiles"):rest.index("tc_fence_before();")]
     for part, waits in ((softmax, 4), (loads, 1)):
         assert len(re.findall(r"\bmbar_wait_warp\(", part)) == waits
         assert not re.findall(r"\bmbar_wait\(", part)
+
+
+def test_load_warps_learn_of_every_wait_that_gave_up():
+    """A wait of another warp may give up after they have asked for their last copies: they look behind the barrier of all
+    warps, and then wait for the copies."""
+    import os
+    from sejong_b200 import build
+    text = open(os.path.join(build.CSRC, "attention_shared.cu")).read()
+    kernel = text[text.index("attn_shared_kernel(const __grid_constant__"):text.index("shared_join_kernel(const")]
+    barrier, look = kernel.rindex("__syncthreads();"), kernel.index("warp >= kLoadWarp && *abort_flag != 0")
+    assert barrier < look < kernel.index("mbar_wait(&full[last_slot], last_turn, nullptr")

@@ -18,6 +18,9 @@ struct PagedAttention {
   float* partial;  // two slots per CTA
   int64_t page_stride, head_stride, token_stride;
   int ldq, ldo, pages, page, ld_table, requests, rows, hq, hk, window;
+  // of rows that are left apart though a call names groups of them: looked at for the report only, else none
+  const int32_t* group;
+  int groups;
 };
 
 constexpr int kSharedKeys = 128;     // keys of a tile

@@ -1006,7 +1006,11 @@ extern "C" int sj_attn_paged_shared(const void* q, int ldq, const void* k_cache,
   const double most = static_cast<double>(rows) * hk * head_dim * 4 * ld_table * page;  // bytes that rows apart read
   const char* wish = std::getenv("SJ_ATTN_SHARE");
   const bool always = wish && std::strcmp(wish, "always") == 0;
-  if (!shares(groups, hq, hk) || (!always && most < kSharedRate * kSharedStart)) return attn_paged_rows(a, nullptr, head_dim, s);
+  if (!shares(groups, hq, hk) || (!always && most < kSharedRate * kSharedStart)) {
+    a.group = group;
+    a.groups = groups;
+    return attn_paged_rows(a, nullptr, head_dim, s);
+  }
   SharedSpans spans;
   shared_layout(&spans, static_cast<char*>(workspace) + up256(sj_attn_paged_workspace(rows, hq, hk, head_dim)), rows,
                 groups, hq, hk, head_dim);

@@ -595,6 +595,39 @@ def test_shared_reports_groups_after_the_end(group):
     test_shared_reports_groups_out_of_range(group)
 
 
+BAD_GROUPS = [[(0, 9, 32)], [(0, -1, 32)], [(-1, 0, 32)], [(5, 0, 32)], [(0, 0, -3)], [(0, 0, 1000)], [(2, 0, 32), (1, 0, 32)],
+              [(1, 0, 32), (1, 0, 32)], [(0, 0, 32), (4, 0, 0), (2, 0, 32)]]
+
+
+@pytest.mark.parametrize("group", BAD_GROUPS)
+def test_shared_reports_groups_where_rows_are_left_apart(monkeypatch, group):
+    """The same where the rule sees too little to share."""
+    monkeypatch.delenv("SJ_ATTN_SHARE")
+    test_shared_reports_groups_out_of_range(group)
+    gen = torch.Generator().manual_seed(1)  # and nothing to report of groups that are in order
+    k, v = (torch.randn(8, 2, 16, 64, generator=gen).bfloat16().to(DEV) for _ in range(2))
+    q = torch.randn(4, 256, generator=gen).bfloat16().to(DEV)
+    shared_call(q, k, v, ints([[0, 1, 2]] * 4), ints([0, 1, 2, 3]), ints([40, 39, 41, 33]), ints([(0, 1, 32), (2, 3, 48), (4, 0, 0)]),
+                4, 2, 64)
+    assert device_error() == 0
+
+
+@pytest.mark.parametrize("rows,hq", [(1030, 2), (4, 130)])
+def test_shared_reports_groups_of_shapes_that_never_share(rows, hq):
+    """More than 1024 groups, or more than 128 query heads a KV head."""
+    gen = torch.Generator().manual_seed(2)
+    k, v = (torch.randn(8, 1, 16, 64, generator=gen).bfloat16().to(DEV) for _ in range(2))
+    q = torch.randn(rows, hq * 64, generator=gen).bfloat16().to(DEV)
+    table, req, pos = ints([[0, 1, 2]] * rows), ints(np.arange(rows)), ints([40] * rows)
+    group = np.array([(r, r, 32) for r in range(rows)])
+    want = shared_call(q, k, v, table, req, pos, ints(group), hq, 1, 64)
+    assert device_error() == 0
+    group[rows - 2, 2] = 49
+    got = shared_call(q, k, v, table, req, pos, ints(group), hq, 1, 64)
+    assert device_error() == BAD_INDEX
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def shared_call(q, k, v, table, request, position, group, hq, hk, dim, window=0, work=None, out=None):
     from sejong_b200 import _lib
     rows, groups = q.shape[0], group.shape[0]

@@ -427,8 +427,9 @@ int sj_attn_paged(const void* q, int ldq, const void* k_cache, const void* v_cac
  *                    free_out that hold pages).  Call it between sj_paged_commit, whose release then is null, and
  *                    sj_paged_plan.  summary (int32 [4]) = {copies, pages back, status, pages left}.  status 0:
  *                    done; 2: too few free pages; 3: ld_table too small; 4: a parent, length or stack out of range.
- *                    With a status other than 0 the new state is the old one.  A page id outside [0, pages), or one
- *                    given back more often than it was held, records SJ_DEV_BAD_INDEX and is not counted.
+ *                    With a status other than 0 the new state is the old one, which is not looked into.  Else a page
+ *                    id outside [0, pages), or one given back more often than it was held, records SJ_DEV_BAD_INDEX
+ *                    and is not counted.
  *   sj_paged_copy    rows 0 .. tokens - 1 of page copies[i][0] to page copies[i][1], keys and values of every head
  *                    and of `layers` caches that lie layer_stride elements apart in k_cache and v_cache.  An entry
  *                    whose first value is -1 is passed over; one out of range records SJ_DEV_BAD_INDEX.  A page

@@ -27,7 +27,7 @@ constexpr int kForkCluster = 8, kForkThreads = 1024;
 constexpr int kForkChunk = 128;       // entries of a block table that a warp takes at a time
 constexpr int kForkRun = 8;           // slots whose entries it counts together
 constexpr int kForkUnits = 4;         // owners that a thread asks for at a time
-constexpr int kNoEntry = INT_MIN;
+constexpr int kNoEntry = INT_MIN;     // out of range as well, so that it need not be told from a table's
 constexpr int kCopyThreads = 256, kCopyPieces = 8;  // 16-byte pieces of a thread
 constexpr int kCompactThreads = 1024, kCompactIds = 8;  // of the stack, that a thread asks for at a time
 }  // namespace
@@ -136,8 +136,20 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) 
 #pragma unroll
       for (int e = 0; e < kForkChunk / 32; ++e) id[e] = j0 + 32 * e + lane < end ? from[j0 + 32 * e + lane] : 0;
 #pragma unroll
-      for (int e = 0; e < kForkChunk / 32; ++e)
-        if (j0 + 32 * e + lane < end && j0 + 32 * e + lane != own) to[j0 + 32 * e + lane] = id[e];
+      for (int e = 0; e < kForkChunk / 32; ++e) {
+        if (j0 + 32 * e + lane >= end) continue;
+        if (!status && (id[e] < 0 || id[e] >= a.pages)) record_error(SJ_DEV_BAD_INDEX);
+        if (j0 + 32 * e + lane != own) to[j0 + 32 * e + lane] = id[e];
+      }
+      if (!status && children[b] == 0) {  // whose entries nobody takes over: looked at here, where there is time, and counted below
+        const int32_t* left = a.table + static_cast<size_t>(b) * a.ld_table;
+        const int until = min(held(b), j0 + kForkChunk);
+#pragma unroll
+        for (int e = 0; e < kForkChunk / 32; ++e) id[e] = j0 + 32 * e + lane < until ? left[j0 + 32 * e + lane] : 0;
+#pragma unroll
+        for (int e = 0; e < kForkChunk / 32; ++e)
+          if (id[e] < 0 || id[e] >= a.pages) record_error(SJ_DEV_BAD_INDEX);
+      }
       if (lane == 0 && j0 == 0) {
         a.cached_out[b] = p < 0 ? 0 : length(p);
         if (copied) {
@@ -186,9 +198,7 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) 
         int sum = 0;
         auto add = [&]() {
           if (now == kNoEntry || sum == 0) return;
-          if (now < 0 || now >= a.pages)
-            record_error(SJ_DEV_BAD_INDEX);
-          else
+          if (now >= 0 && now < a.pages)  // others are reported above
             atomicAdd(cluster.map_shared_rank(counter, now / a.per) + now % a.per, sum);
         };
 #pragma unroll

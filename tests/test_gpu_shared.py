@@ -325,6 +325,19 @@ def test_fork_reports_pages_out_of_range(bad):
     assert new[2].sum().item() == 4
 
 
+@pytest.mark.parametrize("parent", [[0, 1], [1, 0], [1, 1], [0, 0], [-1, -1]])
+@pytest.mark.parametrize("bad", [-1, -7, 10 ** 6, -2 ** 31])
+def test_fork_reports_pages_out_of_range_whoever_goes_on(parent, bad):
+    """Of requests with one child, with several, and with none."""
+    books = start([14, 16], 4, 3)
+    books.now[1][0, 1] = bad
+    new = books.fork(parent)
+    assert device_error() == BAD_INDEX and books.summary[2].item() == 0
+    assert all(new[1][b, 1].item() == bad for b, p in enumerate(parent) if p == 0)
+    start([14, 16], 4, 3).fork(parent)
+    assert device_error() == 0
+
+
 def test_fork_reports_pages_given_back_too_often():
     books = start([8, 8], 4, 3)
     books.now[1][1, 0] = books.now[1][0, 0].item()  # in two tables, but counted once

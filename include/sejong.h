@@ -472,9 +472,10 @@ int sj_attn_paged_shared(const void* q, int ldq, const void* k_cache, const void
 /* The best continuations of each request's beams: of the totals score[r][b] + log softmax(logits[r * beams + b])[t] (logits
  * f32 or bf16 by dtype, [requests * beams, ld], the first vocab columns; score f32 [requests, beams]) the `keep` largest
  * in order, the lowest b * vocab + t first among equal ones: parent = b, token = t, new_score = total, each [requests,
- * keep].  Totals are compared before they are rounded to f32.  A logit of -inf is a forbidden token and a score of -inf
- * an empty beam; they, and rows with a NaN or +inf, have no candidates.  Past the last candidate parent = token = -1
- * and new_score = -inf.  requests <= 4096, beams <= 64, keep <= min(64, beams * vocab), vocab <= 2^31 - 1 - 2^16.
+ * keep].  Totals are compared in f64, before they are rounded to f32 (where it cannot tell tokens of one beam with different
+ * logits apart, any of them may be kept).  A logit of -inf is a forbidden token and a score of -inf an empty beam; they, and
+ * rows with a NaN or +inf among their logits or for a score, have no candidates.  Past the last candidate parent = token =
+ * -1 and new_score = -inf.  requests <= 4096, beams <= 64, keep <= min(64, beams * vocab), vocab <= 2^31 - 1 - 2^16.
  * workspace: sj_beam_select_workspace bytes (0 for small vocabularies), zero before its first use (each call leaves it
  * ready for the next, of any size); one per stream.  Fewer rows may take more bytes, since they are cut into parts. */
 size_t sj_beam_select_workspace(int requests, int beams, int vocab, int keep);

@@ -15,7 +15,7 @@ def select(logits, score, keep):
         total = np.full((beams, vocab), -np.inf)
         for b in range(beams):
             x, m = logits[r, b], np.max(logits[r, b])
-            if not (np.isfinite(m) and score[r, b] > -np.inf):  # NaN, +inf, or nothing allowed
+            if not (np.isfinite(m) and np.isfinite(score[r, b])):  # NaN, +inf, or nothing allowed
                 continue
             total[b] = score[r, b] + ((x - m) - np.log(np.sum(np.exp(x - m))))
         order = np.argsort(-total.reshape(-1), kind="stable")[:keep]

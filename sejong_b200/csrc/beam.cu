@@ -139,7 +139,7 @@ struct BeamOffset {
   SJ_DEVICE double total(float x) const { return add + (static_cast<double>(x) - m); }
 };
 SJ_DEVICE BeamOffset beam_offset(float score, float m, double s) {
-  const bool is = score > -INFINITY && m > -INFINITY;
+  const bool is = score > -INFINITY && score < INFINITY && m > -INFINITY;
   return BeamOffset{is ? static_cast<double>(score) - log(s) : __longlong_as_double(0x7ff8000000000000ll), m};
 }
 

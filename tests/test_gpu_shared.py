@@ -160,6 +160,16 @@ def test_selection_keeps_the_nan_of_a_part_without_other_values(dtype, at):
     check_select(x, score, 8, dtype)
 
 
+@pytest.mark.parametrize("vocab", [257, 5000])
+def test_selection_without_scores_that_are_no_numbers(vocab):
+    """A score of +inf would make every total of its beam equal, and which tokens are kept would not follow from them."""
+    x, score = logits(3, 3, vocab, 5)
+    score[0, 1] = float("inf")
+    score[1, 0] = float("nan")
+    score[2] = float("inf")
+    check_select(x, score, 12)
+
+
 def test_selection_of_extreme_logits():
     x, score = logits(2, 2, 3000, 3)
     x[0] *= 1e30

@@ -119,7 +119,7 @@ class BatchGenerator:
         if not 0 < L < 1 << 19:
             raise ValueError("the context must be 1 to 524287")
         self.width = -(-L // P)
-        self.pages = int(pages or B * self.width)
+        self.pages = int(pages or self.default_pages())
         if self.pages < 1:
             raise ValueError("the cache needs at least one page")
         self.layout = FlatLayout(c)
@@ -169,6 +169,10 @@ class BatchGenerator:
         self.finished = set()
         self.reserved = 0
         torch.cuda.current_stream(self.dev).synchronize()  # calls run on whichever stream is current then
+
+    def default_pages(self):
+        """As many as a whole batch of full contexts holds, and as a fork of it takes before it returns others."""
+        return self.batch * self.width + self.batch - 1
 
     def _books(self, state):
         B, W, N = self.batch, self.width, self.pages
@@ -468,12 +472,13 @@ class BatchGenerator:
         if status or forked:
             raise RuntimeError(f"a step could not be planned: status {status}, of the fork {forked}")
 
-    def _reserve(self, tokens, most_bytes, count):
-        """Pages that `count` continuations of a prompt may come to need: its full pages once, the rest and a page that a
-        fork takes before it returns others for each; all of them for each where a full context may start again."""
+    def _reserve(self, tokens, most_bytes, count, forks):
+        """Pages that `count` continuations of a prompt may come to need: its full pages once, the rest for each; all of them
+        for each where a full context may start again.  `forks`: those of a beam search, whose forks copy half-filled pages
+        for all but one before they return others; the copies of samples, made once, are pages that they go on to fill."""
         most = -(-min(self.context, len(tokens) + most_bytes) // self.page)
         shared = len(tokens) // self.page if len(tokens) + most_bytes <= self.context else 0
-        pages = shared + count * (most - shared + 1)
+        pages = shared + count * (most - shared) + (count - 1 if forks else 0)
         if pages > self.pages:
             raise ValueError(f"{count} continuations of a prompt may need {pages} pages of a cache of {self.pages}")
         return pages
@@ -652,7 +657,7 @@ class BatchGenerator:
             tokens = [EOS] + list(bytes(prompt))
             if len(tokens) + max_bytes > self.context:
                 raise ValueError("a prompt and its continuations have to fit the context")
-            waiting.append(_Beams(i, tokens, self._reserve(tokens, max_bytes, beams)))
+            waiting.append(_Beams(i, tokens, self._reserve(tokens, max_bytes, beams, True)))
         return self._guard(self._run_beams, waiting, beams, max_bytes, float(length_penalty))
 
     def _admit(self, index, prompt, options, top):
@@ -682,7 +687,7 @@ class BatchGenerator:
                 tokens = ([EOS] + list(bytes(prompt)))[-self.context:]
                 if len(tokens) == self.context:
                     raise ValueError("a prompt that fills the context cannot be shared")
-                shared.append((tokens, o, self._reserve(tokens, o.max_bytes, samples)))
+                shared.append((tokens, o, self._reserve(tokens, o.max_bytes, samples, False)))
             return self._guard(self._run_samples, shared, samples, top)
         waiting = deque(self._admit(i, p, o, top) for i, (p, o) in enumerate(zip(prompts, options)))
         for q in waiting:

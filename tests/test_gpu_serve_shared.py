@@ -98,6 +98,20 @@ def test_samples_of_a_full_context_start_again(made):
     check_clean(gen)
 
 
+@pytest.mark.parametrize("page", [8, 64])
+def test_a_whole_batch_of_continuations_on_a_default_cache(made, page):
+    """Samples that start again from a full context, and beams that fill it, of prompts shorter and longer than a page."""
+    from sejong_b200.generate import Sampling
+    gen = generator(made, context=32, page=page, batch=4)
+    for prompt in (b"ab", b"0123456789012345678901234"):
+        found = gen.generate([prompt], Sampling(max_bytes=33, temperature=0.9, seed=5), samples=4)[0]
+        assert all(len(d.text) == 33 or d.ended for d in found)
+        check_clean(gen)
+        found = gen.beam_search([prompt], beams=4, max_bytes=31 - len(prompt))[0]
+        assert found and all(len(h.text) == 31 - len(prompt) or h.ended for h in found)
+        check_clean(gen)
+
+
 def test_more_prompts_than_blocks_and_few_pages(made, sharing):
     from sejong_b200.generate import Sampling
     gen = generator(made, batch=5, page=4, pages=50)

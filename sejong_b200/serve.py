@@ -40,6 +40,9 @@ from .generate import Sampling, _ptr, check_sampling, sample
 from .model import EOS, HEAD_DIM, VOCAB, VOCAB_PAD, FlatLayout, global_stage, initialize
 
 
+SHARED_PAGES = 1 << 18  # that sj_paged_fork takes
+
+
 @dataclass
 class RopeScaling:
     """Rotary positions for contexts longer than the trained one: "linear" (positions divided by the factor),
@@ -472,6 +475,11 @@ class BatchGenerator:
         if status or forked:
             raise RuntimeError(f"a step could not be planned: status {status}, of the fork {forked}")
 
+    def _check_sharing(self):
+        """Before a call stages anything: a cache whose pages can be shared."""
+        if self.pages > SHARED_PAGES:
+            raise ValueError(f"several continuations of a prompt take a cache of at most {SHARED_PAGES} pages, not {self.pages}")
+
     def _reserve(self, tokens, most_bytes, count, forks):
         """Pages that `count` continuations of a prompt may come to need: its full pages once, the rest for each; all of them
         for each where a full context may start again.  `forks`: those of a beam search, whose forks copy half-filled pages
@@ -652,6 +660,7 @@ class BatchGenerator:
             raise ValueError("beams must be 1 to 32, and at most the batch")
         if max_bytes < 1:
             raise ValueError("max_bytes must be positive")
+        self._check_sharing()
         waiting = []
         for i, prompt in enumerate(prompts):
             tokens = [EOS] + list(bytes(prompt))
@@ -679,6 +688,7 @@ class BatchGenerator:
         if not 1 <= samples <= self.batch:
             raise ValueError("samples must be 1 to the batch")
         if samples > 1:
+            self._check_sharing()
             shared = []
             for prompt, o in zip(prompts, options):
                 if o.max_bytes < 1:

@@ -126,3 +126,18 @@ def test_several_prompts_get_by_with_few_pages():
             assert all(Booked(6, 40, page, pages).beam_search(prompts, beams=3, max_bytes=12))
             found = Booked(6, 40, page, pages).generate(prompts, Sampling(max_bytes=12, temperature=1.0), samples=3)
             assert all(d.ended or len(d.text) == 12 for done in found for d in done)
+
+
+def test_a_cache_of_more_pages_than_can_be_shared_is_refused_at_once():
+    gen = Booked(2, 32, 8, pages=(1 << 18) + 1)
+
+    def staged(*args):
+        raise AssertionError("a step was staged")
+
+    gen._write_shared = staged
+    with pytest.raises(ValueError, match="262144 pages"):
+        gen.generate([b"a"], Sampling(max_bytes=3), samples=2)
+    with pytest.raises(ValueError, match="262144 pages"):
+        gen.beam_search([b"a"], beams=2, max_bytes=3)
+    gen = Booked(2, 32, 8, pages=1 << 18)
+    assert gen.beam_search([b"a"], beams=2, max_bytes=1)[0]

@@ -741,10 +741,19 @@ def _score_record(scores):
             "alternatives": [[[t, p] for t, p in row] for row in scores.alternatives]}
 
 
+SAMPLING = {"temperature": 0.8, "top-k": 0, "top-p": 0.95}  # unless the command line says otherwise
+
+
 def generate_batch(model, prompts, max_bytes, temperature, top_k, top_p, seed, batch, page, pages, top, device=0,
                    out=None, samples=1, beams=0):
     """Generate for each line of the file `prompts` together; the i-th prompt draws with seed + i * samples.  `beams` > 0: a
-    beam search instead."""
+    beam search instead, which draws nothing (the seed has no effect) and takes no options of sampling or scoring."""
+    if beams:
+        drawing = {"temperature": temperature, "top-k": top_k, "top-p": top_p}
+        unused = [name for name, value in drawing.items() if value != SAMPLING[name]]
+        unused += ["samples"] * (samples != 1) + ["alternatives"] * (top is not None)
+        if unused:
+            raise ValueError(f"a beam search has no use for --{', --'.join(unused)}")
     from . import checkpoint
     from .generate import Sampling
     from .serve import BatchGenerator
@@ -828,16 +837,17 @@ def main(argv=None):
     p.add_argument("--model", required=True)
     p.add_argument("--prompts", required=True)
     p.add_argument("--max-bytes", type=int, default=512)
-    p.add_argument("--temperature", type=float, default=0.8)
-    p.add_argument("--top-k", type=int, default=0)
-    p.add_argument("--top-p", type=float, default=0.95)
+    p.add_argument("--temperature", type=float, default=SAMPLING["temperature"])
+    p.add_argument("--top-k", type=int, default=SAMPLING["top-k"])
+    p.add_argument("--top-p", type=float, default=SAMPLING["top-p"])
     p.add_argument("--seed", type=int, default=42)
     p.add_argument("--batch", type=int, default=32)
     p.add_argument("--page", type=int, default=16)
     p.add_argument("--pages", type=int, default=None)
     p.add_argument("--alternatives", type=int, default=None, help="score the drawn bytes, with this many alternatives")
     p.add_argument("--samples", type=int, default=1, help="continuations of each prompt")
-    p.add_argument("--beams", type=int, default=0, help="the best continuations of a beam search instead")
+    p.add_argument("--beams", type=int, default=0, help="the best continuations of a beam search instead, which takes no "
+                   "--temperature, --top-k, --top-p, --samples and --alternatives")
     p = sub.add_parser("score", help="log probabilities of the bytes of a text file")
     p.add_argument("--model", required=True)
     p.add_argument("--data", required=True)

@@ -148,3 +148,16 @@ def test_value_fingerprint_ignores_resume_and_byte_values():
     assert cli.value_fingerprint(spec) != cli.value_fingerprint(dict(spec, steps=2))
     assert cli._byte_value({"hex": "00ff"}) == b"\x00\xff" and cli._byte_json(b"\xff") == {"hex": "ff"}
     assert cli._byte_value("ab") == b"ab" and cli._byte_json(b"ab") == "ab"
+
+
+@pytest.mark.parametrize("option", [["--temperature", "0.5"], ["--top-k", "3"], ["--top-p", "0.9"], ["--samples", "2"],
+                                    ["--alternatives", "4"], ["--samples", "0", "--alternatives", "0"]])
+def test_options_that_a_beam_search_has_no_use_for_are_refused(option):
+    """Before the model is looked for."""
+    run = ["generate-batch", "--model", "/nowhere", "--prompts", "/nowhere", "--beams", "2"]
+    with pytest.raises(ValueError, match=f"no use for {option[0]}"):
+        cli.main(run + option)
+    with pytest.raises((OSError, ck.ArtifactError)):
+        cli.main(run + ["--seed", "7", "--max-bytes", "5"])
+    with pytest.raises((OSError, ck.ArtifactError)):
+        cli.main(run[:-2] + option)

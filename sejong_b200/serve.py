@@ -660,6 +660,8 @@ class BatchGenerator:
             raise ValueError("beams must be 1 to 32, and at most the batch")
         if max_bytes < 1:
             raise ValueError("max_bytes must be positive")
+        if not abs(float(length_penalty)) <= 50:  # nor NaN; a length to a much larger power leaves f64
+            raise ValueError("the length penalty must be -50 to 50")
         self._check_sharing()
         waiting = []
         for i, prompt in enumerate(prompts):

@@ -115,3 +115,16 @@ def test_stopping_early_loses_nothing(beams, penalty):
         want = search_to_the_end(model, beams, 9, penalty)
         assert [(h.text, h.ended) for h in found] == [(bytes(d), e) for _, d, e in want]
         assert [h.ranked for h in found] == pytest.approx([r for r, _, _ in want])
+
+
+@pytest.mark.parametrize("penalty", [float("nan"), float("inf"), -float("inf"), 51, 1e6])
+def test_length_penalties_that_rank_nothing_are_refused(penalty):
+    """By NaN no text is worth more than another, by infinities none or all, and 20 ** 1e6 is no number."""
+    with pytest.raises(ValueError, match="length penalty"):
+        Scripted(overtaking).beam_search([b"a"], beams=2, max_bytes=20, length_penalty=penalty)
+
+
+def test_the_largest_length_penalties_rank():
+    for penalty in (-50, 50):
+        found = Scripted(overtaking).beam_search([b""], beams=2, max_bytes=20, length_penalty=penalty)[0]
+        assert all(math.isfinite(h.ranked) for h in found) and found[0].ended == (penalty < 0)

@@ -561,6 +561,11 @@ def test_shared_large_groups():
     shared_case([(300 + i, [301 + i]) for i in range(40)], 2, 1, 64, 16, seed=4)
 
 
+@pytest.mark.parametrize("rows", [1030, 2048, 2100])
+def test_shared_many_rows(rows):
+    shared_case([(64, [65 + i % 3 for i in range(rows - 30)]), (32, [40] * 30)], 2, 1, 64, 16, seed=rows)
+
+
 def test_shared_sharp_scores():
     shared_case([(500, [520, 501, 530])], 4, 2, 64, 16, scale=30.0, seed=5)
     shared_case([(3000, [3001] * 40)], 4, 2, 128, 16, scale=30.0, seed=6)

@@ -580,20 +580,15 @@ SJ_DEVICE void beam_join_parts(const BeamOut& out, const uint64_t* parts, int re
       if (total[k] != 0 && total[k] >= bar) file((t + k * kBeamThreads) / keep, held[k]);
   } else {
     const unsigned long long bar = beam_join_bar(join, all, slot, splits, members, keep);
-    auto reaches = [&](int list, int k) {  // false: the list's others do not either
-      const uint64_t key = __ldcg(all + static_cast<size_t>(list) * slot + 1 + k);
-      const unsigned long long total = up(list, key);
-      if (total == 0 || total < bar) return false;
-      file(list, key);
-      return true;
-    };
-    if (members >= kBeamThreads / 2) {  // a thread for a list
-      for (int list = t; list < members; list += kBeamThreads)
-        for (int k = 0; k < keep && reaches(list, k); ++k) {
-        }
-    } else {
-      for (int i = t; i < members * keep; i += kBeamThreads) reaches(i / keep, i % keep);
-    }
+    // a thread for a list, until one of its totals does not reach the bar (a thread for an entry reads them all: 10 x 20 x 5000
+    // with 40 kept 38.5 us instead of 36.1, 1 x 32 x 131072 with 64 kept 229 instead of 62)
+    for (int list = t; list < members; list += kBeamThreads)
+      for (int k = 0; k < keep; ++k) {
+        const uint64_t key = __ldcg(all + static_cast<size_t>(list) * slot + 1 + k);
+        const unsigned long long total = up(list, key);
+        if (total == 0 || total < bar) break;
+        file(list, key);
+      }
   }
   __syncthreads();
   const int n = join.list.count;

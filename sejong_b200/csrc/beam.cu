@@ -28,7 +28,9 @@ namespace sj {
 namespace {
 constexpr int kBeamMaxBeams = 64, kBeamMaxKeep = 64, kBeamMaxRequests = 4096;
 constexpr int kBeamMaxColumns = INT_MAX - (1 << 16);  // 32 bits count to a chunk past the last column
-constexpr int kBeamNarrow = 1024;                       // logits of a row that a warp holds
+// Logits of a row that a warp holds; at 1000 f32 logits the kernel for wide rows takes 10.2 us instead of 8.0 for 16 x 4 rows,
+// 16.9 instead of 13.8 for 128 x 8.
+constexpr int kBeamNarrow = 1024;
 // Small CTAs, since a part's end is a chain of waits (its sums, bar, candidates, their ranks, the arrival: about 7 us)
 // that the others have to cover: 1024 x 50001 bf16 41.9 us with eight CTAs of 128 threads an SM, 48.3 with ten (fewer
 // registers), 45.4 with four of 256; rows cut in two 62.
@@ -198,8 +200,11 @@ SJ_DEVICE void beam_rank(const BeamOut& out, int request, const BeamList& c, int
 }
 
 // ---------------------------------------------------------------- narrow rows
-// R: logits of a lane.  Warps take the request's beams in turn.  Of a beam, `keep` logits reach a bar that the lanes'
-// maxima give; with the beam's offset it is one for the whole request, and the highest of the beams' counts.
+// R: logits of a lane.  Warps take the request's beams in turn.  Up to 16 kept: of a beam, `keep` logits reach a bar that the
+// lanes' maxima give; with the beam's offset it is one for the whole request, and the highest of the beams' counts.  More of
+// them come near the number of lanes, whose lowest maximum keeps little out, and many beams leave more than the list
+// holds: then the bar is sought bit by bit (both ways, 257 logits: 16 x 4 with 8 kept 6.5 and 8.0 us, 128 x 8 with 16 11.6
+// and 10.4, with 24 17.4 and 11.2, with 32 63 and 12.5; 128 x 1 with 64 100 and 19; 256 x 16 with 32 42 and 17.6).
 template <typename T, int R>
 __global__ void __launch_bounds__(1024) beam_narrow_kernel(const T* logits, int ld, BeamOut out) {
   pdl_wait();
@@ -210,6 +215,7 @@ __global__ void __launch_bounds__(1024) beam_narrow_kernel(const T* logits, int 
   if (threadIdx.x == 0) list.count = 0;
   const T* rows = logits + static_cast<size_t>(request) * out.beams * ld;
   float v[R + (R & 1)];
+  const bool few = out.keep <= 16 && out.beams * out.keep <= kBeamHeld / 2;
   auto load = [&](int b) {
     const T* x = rows + static_cast<size_t>(b) * ld;
 #pragma unroll
@@ -222,22 +228,15 @@ __global__ void __launch_bounds__(1024) beam_narrow_kernel(const T* logits, int 
     double bar = -INFINITY;
     if (score > -INFINITY) {
       load(b);
-      float top = -INFINITY, second = -INFINITY;
+      float top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < R; ++i) {
-        if (v[i] != v[i]) continue;
-        second = fmaxf(second, fminf(top, v[i]));
-        top = fmaxf(top, v[i]);
-      }
+      for (int i = 0; i < R; ++i) top = fmaxf(top, v[i]);  // NaN left out
       const float m = beam_warp_largest(top), base = m == -INFINITY ? 0.f : m;
       uint64_t s = 0;
 #pragma unroll
       for (int i = 0; i < R; i += 2) s = beam_sum2(s, v[i], v[i + 1], base);
       off = beam_offset(score, m, warp_sum(static_cast<double>(beam_low(s) + beam_high(s))));
-      // 32 logits reach the lowest of the lanes' maxima; n - 32 more reach the (n - 32)-th of their seconds
-      float reach = beam_warp_nth(top, min(out.keep, 32));
-      if (out.keep > 32) reach = fminf(reach, beam_warp_nth(second, out.keep - 32));
-      bar = off.total(reach);  // NaN where the row has none
+      if (few) bar = off.total(beam_warp_nth(top, out.keep));  // NaN where the row has none
     }
     if (lane == 0) {
       offset[b] = off;
@@ -269,9 +268,7 @@ __global__ void __launch_bounds__(1024) beam_narrow_kernel(const T* logits, int 
     __syncthreads();
     return list.count;
   };
-  // The beams' bars leave about `keep` candidates of each beam that is worth as much as the best: where those may be more
-  // than the list holds, the bar is sought bit by bit.
-  int n = out.beams * out.keep > kBeamHeld / 2 ? kBeamHeld + 1 : collect([&](double total) { return total >= bar; });
+  int n = few ? collect([&](double total) { return total >= bar; }) : kBeamHeld + 1;
   if (n > kBeamHeld) {
     __shared__ int counts[32];
     uint32_t high[R], reach;
@@ -783,6 +780,7 @@ int beam_narrow(const T* x, int ld, int requests, const BeamOut& out, cudaStream
 template <typename T>
 int beam_select(const T* x, int ld, int requests, const BeamOut& out, void* workspace, cudaStream_t s) {
   if (out.vocab <= kBeamNarrow) {
+    // fewer registers for the vocabulary of bytes: 16 x 4 x 257 6.5 us instead of 7.8, 1000 x 4 x 257 8.6 instead of 11.8
     if (out.vocab <= 9 * 32) return beam_narrow<T, 9>(x, ld, requests, out, s);
     return beam_narrow<T, 32>(x, ld, requests, out, s);
   }

@@ -127,6 +127,24 @@ def test_selection_of_ties(vocab, dtype):
     check_select(x.flip(2), torch.tensor([[-1.0, -1.5]]), 30)
 
 
+@pytest.mark.parametrize("keep", [1, 8, 9, 16, 17])
+@pytest.mark.parametrize("vocab", [257, 1000, 3000])
+def test_selection_of_few_among_ties(vocab, keep):
+    x = torch.zeros(2, 3, vocab)
+    x[1, :, 7::5] = 1.0
+    check_select(x, torch.tensor([[-1.0, -1.0, -1.0], [-3.0, -2.0, -2.0]]), keep)
+    x, _ = logits(1, 1, vocab, 6)
+    check_select(x.expand(1, 9, vocab).contiguous(), torch.full((1, 9), -2.0), keep)
+
+
+@pytest.mark.parametrize("beams,keep", [(1, 16), (15, 16), (16, 16), (17, 16), (1, 17), (8, 24), (8, 32), (32, 8), (33, 8), (1, 64)])
+@pytest.mark.parametrize("vocab", [100, 257, 1000])
+def test_selection_about_the_ways_to_a_bar(vocab, beams, keep):
+    """Both sides of the rule by which a small vocabulary's bar is found."""
+    check_select(*logits(3, beams, vocab, beams * vocab + keep), keep)
+    check_select(*logits(3, beams, vocab, beams * vocab + keep, spread=0.1), keep, torch.bfloat16)
+
+
 @pytest.mark.parametrize("vocab", [257, 4097, 40000])
 def test_selection_of_forbidden_tokens_and_empty_beams(vocab):
     inf = float("inf")

@@ -31,11 +31,11 @@ constexpr int kBeamMaxColumns = INT_MAX - (1 << 16);  // 32 bits count to a chun
 // Logits of a row that a warp holds; at 1000 f32 logits the kernel for wide rows takes 10.2 us instead of 8.0 for 16 x 4 rows,
 // 16.9 instead of 13.8 for 128 x 8.
 constexpr int kBeamNarrow = 1024;
-// Small CTAs, since a part's end is a chain of waits (its sums, bar, candidates, their ranks, the arrival: about 7 us)
-// that the others have to cover: 1024 x 50001 bf16 41.9 us with eight CTAs of 128 threads an SM, 48.3 with ten (fewer
-// registers), 45.4 with four of 256; rows cut in two 62.
+// Small CTAs, since a part's end is a chain of waits (its sums, bar, candidates, their ranks, the arrival: about 7 us) that
+// only the others of its SM can cover: 1024 x 50001 bf16 43.0 us with eight CTAs of 128 threads an SM, 43.5 with ten (fewer
+// registers), 44.6 with four of 256; rows cut in two 50.  As one wave its rows still end together, which is 16 of the 43.
 constexpr int kBeamThreads = 128, kBeamWarps = kBeamThreads / 32, kBeamCtas = 8;
-constexpr int kBeamPieces = 3;                          // 16-byte pieces of a thread at a time (four: 2 us more)
+constexpr int kBeamPieces = 3;                          // 16-byte pieces of a thread at a time (four: as fast to 2%)
 constexpr int kBeamLook = 4;                            // threads whose logits a warp looks at again at a time
 constexpr int kBeamMaxSplits = 32;
 constexpr int kBeamHeld = 512;                          // candidates of a part, or of a request

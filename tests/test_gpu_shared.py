@@ -197,6 +197,35 @@ def test_selection_of_extreme_logits():
     check_select(x, score, 16)
 
 
+def test_selection_of_the_most_requests():
+    check_select(*logits(4096, 2, 1030, 1), 3)
+    check_select(*logits(4096, 3, 40, 2), 5, torch.bfloat16)
+
+
+def test_selection_offsets_past_32_bits():
+    """Three rows of more than 2^30 columns, which begin past 2^31 and 2^32 bytes and elements."""
+    free, _ = torch.cuda.mem_get_info()
+    if free < 16 << 30:
+        pytest.skip("needs 16 GB of device memory")
+    from sejong_b200 import _lib
+    vocab, keep = (1 << 31) - (1 << 17) - 3, 4
+    x = torch.full((3, vocab + 3), -200.0, dtype=torch.bfloat16, device=DEV)  # nothing beside the rest: e^-200 is 0 in f32
+    want = []
+    for r, places in enumerate(((5, vocab - 1, 1 << 30, 77), (vocab - 1, vocab - 2, 0, 1), (1 << 30, vocab // 2, 9, vocab - 9))):
+        for i, at in enumerate(places):
+            x[r, at] = 4.0 - i
+        want.append(list(places))
+    score = torch.tensor([-1.0, -2.0, -3.0], device=DEV)
+    out = [torch.empty(3, keep, dtype=d, device=DEV) for d in (torch.int32, torch.int32, torch.float32)]
+    size = _lib.load().sj_beam_select_workspace(3, 1, vocab, keep)
+    work = torch.zeros(size, dtype=torch.uint8, device=DEV)
+    call("sj_beam_select", ptr(x), 4, vocab + 3, ptr(score), 3, 1, vocab, keep, *(ptr(t) for t in out), ptr(work), size, stream())
+    assert out[1].tolist() == want and (out[0] == 0).all()
+    top = torch.arange(4, 0, -1).double()
+    exact = score.cpu().double()[:, None] + torch.log_softmax(top, 0)
+    assert ((out[2].cpu().double() - exact).abs() <= 2.0 ** -16 + 2.0 ** -23 * exact.abs()).all()
+
+
 def test_selection_shares_a_workspace_between_sizes():
     from sejong_b200 import _lib
     sizes = [(1, 2, 9000), (60, 4, 1100), (2, 1, 70000), (3, 5, 300)]
@@ -320,6 +349,29 @@ def test_fork_of_the_largest_cache():
     new = books.fork([0, 0])
     assert books.summary.tolist() == [1, 50000, 0, pages - 70001]
     assert new[2].sum().item() == 69999
+
+
+def test_fork_and_compaction_of_the_largest_batch_and_cache():
+    """4096 requests on 2^18 pages: the most shared memory that either takes."""
+    pages, rng = 1 << 18, np.random.default_rng(1)
+    lengths = [16 * (1 + b % 60) - 5 * (b % 3) for b in range(4096)]
+    ids = rng.permutation(pages)
+    table = np.full((4096, 62), -1)
+    at = 0
+    for b, n in enumerate(lengths):
+        held = opaged.ceil_div(n, 16)
+        table[b, :held] = ids[at:at + held]
+        at += held
+    books = Books(lengths, table, [0] * pages, ids[at:].tolist(), 16)
+    parent = rng.integers(-1, 4096, 4096)
+    want = oracle.fork(parent.tolist(), 16, books.cached, books.table, books.shares, books.free)
+    assert want[-1] == 0 and len(want[4]) > 100
+    books.expect(books.fork(parent), want)
+    table, shares, free, moves = oracle.compact(16, books.cached, books.table, books.shares, books.free, pages)
+    new, got = compact(books, len(moves))
+    assert [tuple(m) for m in got] == [(a, b, 16) for a, b in moves]
+    assert np.array_equal(new[0].cpu().numpy(), table) and new[2].tolist()[:len(free)] == free
+    assert books.summary.tolist() == [len(moves), at, 0, len(free)]
 
 
 @pytest.mark.parametrize("parent,cached,status", [

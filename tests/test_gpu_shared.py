@@ -796,6 +796,88 @@ def test_shared_on_another_stream_and_captured():
         assert (got[0].float() - plain[0].float()).abs().max() < 0.02
 
 
+def random_shared(seed, rows, keys, hq, hk, dim):
+    """Rows that share all but their last page, and the call's arguments."""
+    gen, page = torch.Generator().manual_seed(seed), 16
+    common = keys // page
+    k, v = (torch.randn(common + rows, hk, page, dim, generator=gen).bfloat16().to(DEV) for _ in range(2))
+    table = np.concatenate((np.tile(np.arange(common), (rows, 1)), common + np.arange(rows)[:, None]), axis=1)
+    q = torch.randn(rows, hq * dim, generator=gen).bfloat16().to(DEV)
+    return q, k, v, ints(table), ints(np.arange(rows)), ints([common * page + i % page for i in range(rows)]), \
+        ints([(0, 0, common * page)]), hq, hk, dim
+
+
+def test_shared_calls_at_once_and_graphs_that_share_a_workspace():
+    """Two streams with workspaces of their own; then two captured calls of different sizes on one workspace, in turn."""
+    from sejong_b200 import _lib
+    calls = [random_shared(1, 40, 4000, 12, 4, 64), random_shared(2, 150, 2500, 8, 2, 128)]
+    want = [[t.clone() for t in shared_call(*c)] for c in calls]
+    size = [_lib.load().sj_attn_paged_shared_workspace(c[0].shape[0], 1, c[7], c[8], c[9]) for c in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    works = [torch.zeros(n, dtype=torch.uint8, device=DEV) for n in size]
+    outs = [[(torch.empty_like(c[0]), torch.empty(c[0].shape[0], c[7], device=DEV)) for _ in range(8)] for c in calls]
+    torch.cuda.synchronize()
+    for i in range(8):
+        for c, s, w, out in zip(calls, streams, works, outs):
+            with torch.cuda.stream(s):
+                shared_call(*c, work=w, out=out[i])
+    torch.cuda.synchronize()
+    for out, w in zip(outs, want):
+        assert all(torch.equal(a, b) for pair in out for a, b in zip(pair, w))
+    work = torch.zeros(max(size), dtype=torch.uint8, device=DEV)
+    graphs = []
+    for c, out in zip(calls, outs):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            shared_call(*c, work=work, out=out[0])
+    for i in (0, 1, 1, 0, 1, 0, 0):
+        for t in outs[i][0]:
+            t.fill_(3.0)
+        graphs[i].replay()
+        assert all(torch.equal(a, b) for a, b in zip(outs[i][0], want[i]))
+
+
+def test_selections_at_once_and_graphs_that_share_a_workspace():
+    from sejong_b200 import _lib
+    sizes = [(3, 4, 9000, 8), (1, 2, 70000, 20)]
+    inputs, want, outs, need = [], [], [], []
+    for requests, beams, vocab, keep in sizes:
+        x, score = logits(requests, beams, vocab, vocab)
+        inputs.append((x.reshape(-1, vocab).to(DEV), score.to(DEV)))
+        want.append(oracle.select(x.double().numpy(), score.double().numpy(), keep))
+        outs.append([[torch.full((requests, keep), 9, dtype=d, device=DEV) for d in (torch.int32, torch.int32, torch.float32)]
+                     for _ in range(8)])
+        need.append(_lib.load().sj_beam_select_workspace(requests, beams, vocab, keep))
+
+    def run(i, out, work):
+        requests, beams, vocab, keep = sizes[i]
+        call("sj_beam_select", ptr(inputs[i][0]), 0, vocab, ptr(inputs[i][1]), requests, beams, vocab, keep, *(ptr(t) for t in out),
+             ptr(work), work.numel(), stream())
+
+    def right(i, out):
+        return np.array_equal(out[0].cpu().numpy(), want[i][0]) and np.array_equal(out[1].cpu().numpy(), want[i][1])
+
+    streams, works = [torch.cuda.Stream() for _ in sizes], [torch.zeros(n, dtype=torch.uint8, device=DEV) for n in need]
+    torch.cuda.synchronize()
+    for k in range(8):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                run(i, outs[i][k], works[i])
+    torch.cuda.synchronize()
+    assert all(right(i, out) for i in (0, 1) for out in outs[i])
+    work = torch.zeros(max(need), dtype=torch.uint8, device=DEV)
+    graphs = []
+    for i in (0, 1):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            run(i, outs[i][0], work)
+    for i in (0, 1, 1, 0, 1, 0, 0):
+        for t in outs[i][0]:
+            t.fill_(7)
+        graphs[i].replay()
+        assert right(i, outs[i][0])
+
+
 def test_shared_and_copied_offsets_past_32_bits():
     """Cache buffers of more than 2^32 elements: the last pages are read, by boxes and by pieces, and copied."""
     free, _ = torch.cuda.mem_get_info()

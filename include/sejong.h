@@ -444,14 +444,15 @@ int sj_attn_paged(const void* q, int ldq, const void* k_cache, const void* v_cac
  *   sj_attn_paged_shared  sj_attn_paged, for rows that share keys.  group (int32 [groups, 3]) = {first row, request,
  *                    tokens}, by first rows in order: the rows from the first one to the next group's (or `rows`) all
  *                    have the first `tokens` tokens of that request among theirs, at the same positions, so they
- *                    are read once for all of them, where that is faster (decided on the GPU by the sizes; with
- *                    SJ_ATTN_SHARE=always in the environment, wherever two rows share keys).  Each row still sees no
- *                    more than position[r] + 1 tokens and its window.  groups <= rows; more than 1024 of them, or
- *                    more than 128 query heads a KV head, share nothing.  Groups at the end whose first row is
- *                    `rows` are empty.  A group out of order or out of range records SJ_DEV_BAD_INDEX, and then no
- *                    rows share.  Results are those of sj_attn_paged but for
- *                    the order of the sums.  workspace: sj_attn_paged_shared_workspace bytes, zero before its first
- *                    use (each call leaves it ready for the next, of any size); one per stream. */
+ *                    are read once for all of them, where that is faster (decided on the host by the largest lengths
+ *                    that ld_table allows, then on the GPU by the real ones; with SJ_ATTN_SHARE=always in the
+ *                    environment, wherever two rows share keys).  Each row still sees no more than position[r] + 1
+ *                    tokens and its window.  groups <= rows; more than 1024 of them, or more than 128 query heads a KV
+ *                    head, share nothing.  Groups at the end whose first row is `rows` are empty.  A group out of
+ *                    order or out of range records SJ_DEV_BAD_INDEX, and then no rows share.  Results are those of
+ *                    sj_attn_paged but for the order of the sums.  workspace: sj_attn_paged_shared_workspace bytes,
+ *                    zero before its first use (each call leaves it ready for the next, of any size); one per
+ *                    stream. */
 int sj_paged_fork(const int32_t* parent, int batch, int page, const int32_t* cached, const int32_t* block_table,
                   int ld_table, const int32_t* shares, const int32_t* free_pages, const int32_t* free_count, int pages,
                   int32_t* cached_out, int32_t* table_out, int32_t* shares_out, int32_t* free_out, int32_t* count_out,

@@ -43,10 +43,10 @@ struct Fork {
 // copied to a fresh page for each of the others.  Every CTA scans the batch for itself.  The first cluster counts: an
 // entry of a slot with c children changes its page's owners by c - 1 (the half-filled page of a slot without children
 // by -1); the counters of a CTA's share of the pages lie in its shared memory, which the others add to (integers, so the
-// order does not matter; in memory, with the fences that takes, 9.3 us instead of 8.7 for 32 requests).  Then each CTA
+// order does not matter; in memory, with the fences that takes, 9.3 us instead of 8.8 for 32 requests).  Then each CTA
 // knows which of its pages nobody holds, and after one exchange of numbers where on the stack they go.  The other
-// clusters write tables.  Bound by latency, four phases of a few dependent loads: 32 requests 8.7 us (graph replays), 1024
-// requests of 500 to 32768 tokens in pages of 64 22.4 (34 with an addition to another CTA's counter for each entry).
+// clusters write tables.  Bound by latency, four phases of a few dependent loads: 32 requests 8.8 us (graph replays), 1024
+// requests of 500 to 32768 tokens in pages of 64 22.2 (34 with an addition to another CTA's counter for each entry).
 __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const Fork a) {
   pdl_wait();
   extern __shared__ int dynamic[];
@@ -331,7 +331,7 @@ struct Compact {
 // Every CTA reads the whole stack into a bit mask of the free pages with the numbers of pages in use before each word,
 // and writes its share of the results: the i-th page in use from `used` on goes to the i-th free page below it.  One launch
 // without a wait for other CTAs; bound by the shared-memory atomics of the mask (1024 requests on 183 thousand pages, half of
-// them free, 25 us; 32 requests on a thousand 6.4).
+// them free, 25 us; 32 requests on a thousand 6.5).
 __global__ void __launch_bounds__(kCompactThreads) paged_compact_kernel(const Compact a) {
   pdl_wait();
   extern __shared__ uint32_t bits[];                          // a bit for each page: free
